@@ -262,6 +262,133 @@ int moe_fp8_ep_peer_combine(const int32_t* topk_idx, int32_t num_tokens, int32_t
                             void* base, void* output, void* stream);
 int moe_fp8_ep_peer_read_error(void* base, void* stream, int32_t* bits);
 
+/* ---- Dense products around the routed experts (the router's gate, the shared
+ * expert), 8-bit activation checkpoints and gradients for training them. No
+ * counterpart in the reference, which holds the routed operator alone. Sizes
+ * are free (m tokens >= 0, k and n >= 1); matrices are row-major with a row
+ * stride in elements and need the alignment of their type only. Every entry
+ * works on the current device, asynchronously on `stream`, and keeps nothing
+ * between calls; `workspace` is device scratch, 256-byte aligned, that calls in
+ * flight on different streams (and different captured graphs) must not share. */
+#define MOE_ACT_NONE 0
+#define MOE_ACT_RELU 1
+#define MOE_ACT_GELU 2     /* exact (erf) form */
+#define MOE_ACT_SILU 3
+#define MOE_ACT_SWIGLU 4   /* z = [a | b], n even: y = a * silu(b), the routed experts' order */
+
+/* y = act(x W^T + bias) + residual; O = n / 2 for MOE_ACT_SWIGLU, n otherwise.
+ * bf16 products are summed in fp32, everything after them is computed in fp32
+ * and rounded once. y may be the residual itself (same pointer and stride); it
+ * must not overlap the other inputs. With z8 / z_scale given, the
+ * pre-activation z = x W^T + bias is also kept as an 8-bit checkpoint (see
+ * moe_checkpoint_activations): [m, n] and [ceil(n / 128), m], or, for
+ * MOE_ACT_SWIGLU, the halves one after the other: [2, m, O] and
+ * [2, ceil(O / 128), m]. */
+typedef struct MoeLinearArgs {
+  const void* x;             /* bf16 [m, k] */
+  const void* weight;        /* bf16 [n, k] */
+  const void* bias;          /* bf16 [n] or NULL */
+  const void* residual;      /* bf16 [m, O] or NULL */
+  void* y;                   /* bf16 (f32 if y_f32) [m, O] */
+  void* z8;                  /* e4m3 or NULL */
+  void* z_scale;             /* e8m0, with z8 */
+  void* workspace;           /* >= moe_linear_workspace_bytes(args); may be NULL if that is 0 */
+  size_t workspace_bytes;
+  int64_t ldx, ldw, ldr, ldy;
+  int32_t m, k, n;
+  int32_t activation;
+  int32_t y_f32;
+} MoeLinearArgs;
+size_t moe_linear_workspace_bytes(const MoeLinearArgs* args);
+int moe_linear_run(const MoeLinearArgs* args, void* stream);
+
+/* Gradients of moe_linear_run from its checkpoints:
+ *   dz = dy * act'(z^),  grad_x = dz W,  grad_weight = dz^T x^,  grad_bias = sum over tokens of dz
+ * with x^, z^ the values the checkpoints stand for (the residual's gradient is
+ * dy). dz is rounded to bf16 for the two products; with grad_f32 it is kept as
+ * the sum of two bf16 terms, so that fp32 gradients are not limited by that
+ * rounding. NULL outputs are not computed. grad_x, grad_weight and grad_bias are
+ * contiguous, bf16 (f32 if grad_f32), and overwritten. Sums run in a fixed
+ * order: repeated calls give the same bits. */
+typedef struct MoeLinearGradArgs {
+  const void* grad_y;        /* bf16 (f32 if grad_y_f32) [m, O] */
+  const void* x8;            /* e4m3 [m, k], contiguous (needed for grad_weight) */
+  const void* x_scale;       /* e8m0 [ceil(k / 128), m] */
+  const void* z8;            /* as moe_linear_run writes it; NULL for MOE_ACT_NONE */
+  const void* z_scale;
+  const void* weight;        /* bf16 [n, k] (needed for grad_x) */
+  void* grad_x;              /* [m, k] or NULL */
+  void* grad_weight;         /* [n, k] or NULL */
+  void* grad_bias;           /* [n] or NULL */
+  void* workspace;           /* >= moe_linear_grad_workspace_bytes(args) */
+  size_t workspace_bytes;
+  int64_t ldg, ldw;
+  int32_t m, k, n;
+  int32_t activation;
+  int32_t grad_y_f32, grad_f32;
+} MoeLinearGradArgs;
+size_t moe_linear_grad_workspace_bytes(const MoeLinearGradArgs* args);
+int moe_linear_grad(const MoeLinearGradArgs* args, void* stream);
+
+/* 8-bit activation checkpoints. x [rows, cols] (bf16, or f32 if !x_is_bf16) ->
+ * q e4m3 [rows, cols] and scale e8m0 [ceil(cols / 128), rows]: per 1x128 block
+ * (the last one of a row may be shorter) the scale is 2^e with the least
+ * e >= -117 for which amax <= 448 * 2^e, and q = e4m3(x / 2^e), round to
+ * nearest even (magnitudes above 240 * 2^120, the largest restored value, are
+ * held there). A block that holds an infinity or a NaN gets the NaN scale and is
+ * restored as NaN. restore: `batch` checkpoints of the same size one after
+ * the other -> out [batch, rows, cols], bf16 or f32, exact (no rounding). */
+int moe_checkpoint_activations(const void* x, int32_t x_is_bf16, int64_t rows, int64_t cols, int64_t ldx, void* q,
+                               void* scale, void* stream);
+int moe_restore_activations(const void* q, const void* scale, int64_t batch, int64_t rows, int64_t cols, void* out,
+                            int32_t out_f32, void* stream);
+
+/* Balance loss of the router with the counts per expert. For every sequence q
+ * (tokens [cu_seqlens[q], cu_seqlens[q + 1]); one sequence of all tokens if
+ * NULL) with T_q tokens, E experts and k picks per token:
+ *   loss = alpha * mean over sequences with T_q > 0 of sum_e f_qe P_qe,
+ *   f_qe = E / (k T_q) * count_qe,   P_qe = 1 / T_q * sum_t p_te,
+ *   p_te = s_te / (sum_j s_tj + 1e-20), s = sigmoid(logit)   (scoring 0), or softmax (scoring 1).
+ * A pick outside [0, E) selects nothing, and a token with no other picks is
+ * padding: it counts in no T_q and no sum. Tokens outside every sequence count
+ * nowhere. Boundaries that decrease or leave [0, T] give a NaN loss. The gradient
+ * treats f as constant. grad_topk_weights adds the gradient of the combine
+ * weights of moe_fp8_route, w_k = s_k / (sum of the picked s + 1e-20) * scale
+ * with s = sigmoid(logit), for every token. Both sums run in a fixed order. */
+typedef struct MoeBalanceArgs {
+  const float* routing_logits;   /* f32 [T, E], contiguous */
+  const int32_t* topk_idx;       /* [T, k] */
+  const int32_t* cu_seqlens;     /* [S + 1] device, or NULL (S = 1) */
+  float* loss;                   /* [1] */
+  int32_t* counts;               /* [S, E] */
+  int32_t* tokens;               /* [S]: T_q */
+  float* mean_scores;            /* [S, E]: P */
+  int32_t* sequences;            /* [1]: sequences with T_q > 0 */
+  void* workspace;               /* >= moe_balance_workspace_bytes(T, E, S) */
+  size_t workspace_bytes;
+  int32_t num_tokens, num_experts, top_k, num_sequences;   /* E <= 1024, k <= 32, S <= 65535 */
+  int32_t scoring;
+  float alpha;
+} MoeBalanceArgs;
+size_t moe_balance_workspace_bytes(int32_t num_tokens, int32_t num_experts, int32_t num_sequences);
+int moe_balance_loss(const MoeBalanceArgs* args, void* stream);
+
+typedef struct MoeBalanceGradArgs {
+  const float* routing_logits;
+  const int32_t* topk_idx;
+  const int32_t* cu_seqlens;
+  const int32_t* counts;            /* as moe_balance_loss wrote them */
+  const int32_t* tokens;
+  const int32_t* sequences;
+  const float* grad_loss;           /* device scalar, or NULL: no loss part (counts .. sequences unused) */
+  const float* grad_topk_weights;   /* f32 [T, k] or NULL */
+  float* grad_logits;               /* f32 [T, E], overwritten */
+  int32_t num_tokens, num_experts, top_k, num_sequences;
+  int32_t scoring;
+  float alpha, routed_scaling_factor;
+} MoeBalanceGradArgs;
+int moe_balance_loss_grad(const MoeBalanceGradArgs* args, void* stream);
+
 /* Text of the last error on the calling thread (the reference raises the
  * equivalent message through TVM_FFI_ICHECK, solution/cuda/main.cpp:20-34). */
 const char* moe_fp8_last_error(void);

@@ -73,6 +73,9 @@ EXPORTED_SYMBOLS = (
     "moe_fp8_ep_peer_buffer_free", "moe_fp8_ep_peer_ipc_handle", "moe_fp8_ep_peer_ipc_open",
     "moe_fp8_ep_peer_ipc_close", "moe_fp8_ep_peer_recv_view", "moe_fp8_ep_peer_dispatch", "moe_fp8_ep_peer_wait",
     "moe_fp8_ep_peer_return", "moe_fp8_ep_peer_combine", "moe_fp8_ep_peer_read_error",
+    "moe_linear_workspace_bytes", "moe_linear_run", "moe_linear_grad_workspace_bytes", "moe_linear_grad",
+    "moe_checkpoint_activations", "moe_restore_activations", "moe_balance_workspace_bytes", "moe_balance_loss",
+    "moe_balance_loss_grad",
 )
 
 _lib = None
@@ -331,3 +334,8 @@ def read_device_error(device=None) -> int:
     if rc not in (MOE_OK, 4):
         _check(rc, "moe_fp8_read_device_error")
     return int(bits.value)
+
+
+# Operators around the routed experts (they load the library through this module).
+from .layer import (BalanceLoss, LinearCheckpoint, LinearGrads, balance_loss, balance_loss_backward,  # noqa: E402,F401
+                    checkpoint_activations, linear, linear_backward, linear_checkpointed, restore_activations)

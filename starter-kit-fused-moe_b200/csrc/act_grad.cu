@@ -1,0 +1,206 @@
+// Gradient of a dense product's pre-activation, dz = dy * act'(z^) with z^ the
+// 8-bit checkpoint of z, and its column sums (the bias gradient).
+//
+//   relu'(z) = [z > 0], silu'(z) = s (1 + z (1 - s)), gelu'(z) = Phi(z) + z phi(z),
+//   SwiGLU y = a silu(b): da = dy silu(b), db = dy a silu'(b), stored as [da | db].
+//
+// dz is computed in fp32 and written in bf16, the operand type of the two
+// gradient products (half a step, at most 2^-8 relative, per value; the products sum
+// many of them in fp32). With `terms` = 2 the remainder dz - bf16(dz) follows as
+// a second bf16 matrix, so fp32 gradients keep about 17 bits of dz.
+//
+// Bound by HBM: dy, one byte per z value, two (or four) written per dz value.
+// 32 threads take 256 columns (8 neighbouring ones each, 16-byte accesses) and
+// 8 thread rows walk a chunk of 64 rows, so a column's sum is in registers until
+// the chunk ends; the chunks' sums are added in order by a second kernel, hence
+// the bias gradient does not depend on the order in which blocks ran.
+#include "train_common.cuh"
+
+namespace moe {
+
+constexpr int kAgRows = 64, kAgCols = 256;
+
+template <int HALVES, bool F32, bool VEC>
+__global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
+  __shared__ float red[8][kAgCols];
+  pdl_wait();
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t r0 = (int64_t)blockIdx.y * kAgRows;
+  const int64_t rend = min(r0 + kAgRows, (int64_t)a.m);
+  const int64_t c0 = (int64_t)blockIdx.x * kAgCols;
+  auto col = [&](int j) -> int64_t { return VEC ? c0 + 8 * tx + j : c0 + tx + 32 * j; };
+  const int64_t nb = (O + 127) / 128;
+  __nv_bfloat16* dz = static_cast<__nv_bfloat16*>(a.dz);
+  const int64_t term = (int64_t)a.m * a.ldz;
+  float sum[HALVES][8];
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[h][j] = 0.f;
+
+#pragma unroll 2
+  for (int64_t row = r0 + ty; row < rend; row += 8) {
+    float dy[8], z[HALVES][8];
+    if constexpr (VEC) {
+      const bool in = col(0) < O;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dy[j] = 0.f;
+      if (in) {
+        if constexpr (F32) {
+          const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.dy) + row * a.ldg + col(0));
+          const float4 u = __ldg(p), v = __ldg(p + 1);
+          dy[0] = u.x; dy[1] = u.y; dy[2] = u.z; dy[3] = u.w;
+          dy[4] = v.x; dy[5] = v.y; dy[6] = v.z; dy[7] = v.w;
+        } else {
+          const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.dy) + row * a.ldg + col(0)));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack_bf16(w[j]);
+            dy[2 * j] = f.x;
+            dy[2 * j + 1] = f.y;
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        dy[j] = 0.f;
+        if (col(j) < O)
+          dy[j] = F32 ? static_cast<const float*>(a.dy)[row * a.ldg + col(j)]
+                      : (float)static_cast<const __nv_bfloat16*>(a.dy)[row * a.ldg + col(j)];
+      }
+    }
+    if (a.z8 != nullptr) {
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        const uint8_t* zr = a.z8 + ((int64_t)h * a.m + row) * O;
+        const uint8_t* sr = a.z_scale + (int64_t)h * nb * a.m + row;
+        if constexpr (VEC) {
+          uint2 raw = make_uint2(0, 0);
+          float s = 1.f;
+          if (col(0) < O) {
+            raw = __ldg(reinterpret_cast<const uint2*>(zr + col(0)));
+            s = e8m0_value(sr[(col(0) >> 7) * a.m]);       // 8 aligned columns share a block
+          }
+          const float2 p0 = e4m3x2_value(raw.x & 0xffffu), p1 = e4m3x2_value(raw.x >> 16);
+          const float2 p2 = e4m3x2_value(raw.y & 0xffffu), p3 = e4m3x2_value(raw.y >> 16);
+          z[h][0] = p0.x * s; z[h][1] = p0.y * s; z[h][2] = p1.x * s; z[h][3] = p1.y * s;
+          z[h][4] = p2.x * s; z[h][5] = p2.y * s; z[h][6] = p3.x * s; z[h][7] = p3.y * s;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            z[h][j] = col(j) < O ? e4m3_value(zr[col(j)]) * e8m0_value(sr[(col(j) >> 7) * a.m]) : 0.f;
+        }
+      }
+      if constexpr (HALVES == 2) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float b = z[1][j], s = sigmoid_f(b), av = z[0][j];
+          // __fmul_rn: dz is a rounded value, never the inside of an FMA, so the sums do not
+          // depend on which outputs are asked for
+          z[0][j] = __fmul_rn(dy[j], b * s);
+          z[1][j] = __fmul_rn(dy[j] * av, s * (1.0f + b * (1.0f - s)));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[0][j] = __fmul_rn(dy[j], act_slope(z[0][j], a.act));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[0][j] = dy[j];
+    }
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[h][j] += z[h][j];
+      if (dz == nullptr) continue;
+      __nv_bfloat16* out = dz + row * a.ldz + (int64_t)h * O;
+      float lo[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float hi = __bfloat162float(__float2bfloat16_rn(z[h][j]));
+        lo[j] = isfinite(hi) ? z[h][j] - hi : 0.f;       // a non-finite value is whole in the first term
+      }
+      if constexpr (VEC) {
+        if (col(0) < O) {
+          *reinterpret_cast<uint4*>(out + col(0)) = make_uint4(pack_bf16(z[h][0], z[h][1]), pack_bf16(z[h][2], z[h][3]),
+                                                               pack_bf16(z[h][4], z[h][5]), pack_bf16(z[h][6], z[h][7]));
+          if (a.terms == 2)
+            *reinterpret_cast<uint4*>(out + term + col(0)) =
+                make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col(j) < O) {
+            out[col(j)] = __float2bfloat16_rn(z[h][j]);
+            if (a.terms == 2) out[term + col(j)] = __float2bfloat16_rn(lo[j]);
+          }
+      }
+    }
+  }
+  if (a.colsum == nullptr) return;
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[ty][VEC ? 8 * tx + j : tx + 32 * j] = sum[h][j];
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x];
+    if (c0 + threadIdx.x < O) a.colsum[(int64_t)blockIdx.y * a.n + (int64_t)h * O + c0 + threadIdx.x] = t;
+  }
+}
+
+// Sums of the chunks' column sums, 32 columns per block, 8 interleaved chunk
+// groups; fp64 because a long batch adds hundreds of chunks.
+__global__ void __launch_bounds__(256) colsum_finish_kernel(const float* __restrict__ colsum, int chunks, int n,
+                                                            void* __restrict__ out, int f32) {
+  __shared__ double red[8][32];
+  pdl_wait();
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+  double t = 0.0;
+  if (c < n)
+    for (int i = ty; i < chunks; i += 8) t += (double)colsum[(int64_t)i * n + c];
+  red[ty][tx] = t;
+  __syncthreads();
+  if (ty == 0 && c < n) {
+    for (int i = 1; i < 8; ++i) t += red[i][tx];
+    if (f32) static_cast<float*>(out)[c] = (float)t;
+    else static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn((float)t);
+  }
+}
+
+int act_grad_chunks(int m, int) { return ceil_div(m, kAgRows); }
+
+static bool al(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+cudaError_t launch_act_grad(const ActGradArgs& a, cudaStream_t st) {
+  if (a.m == 0 || a.n == 0) return cudaSuccess;
+  const bool two = a.act == kActSwiglu;
+  const int O = two ? a.n / 2 : a.n;
+  const bool vec = al(a.dy, 16) && a.ldg % (a.dy_f32 ? 4 : 8) == 0 && O % 8 == 0 && (!a.z8 || al(a.z8, 8)) &&
+                   (!a.dz || (al(a.dz, 16) && a.ldz % 8 == 0));
+  const dim3 grid((unsigned)ceil_div(O, kAgCols), (unsigned)act_grad_chunks(a.m, a.n));
+#define MOE_AG(H, F, V) act_grad_kernel<H, F, V><<<grid, 256, 0, st>>>(a, O)
+  if (two) {
+    if (a.dy_f32) { if (vec) MOE_AG(2, true, true); else MOE_AG(2, true, false); }
+    else { if (vec) MOE_AG(2, false, true); else MOE_AG(2, false, false); }
+  } else {
+    if (a.dy_f32) { if (vec) MOE_AG(1, true, true); else MOE_AG(1, true, false); }
+    else { if (vec) MOE_AG(1, false, true); else MOE_AG(1, false, false); }
+  }
+#undef MOE_AG
+  return cudaGetLastError();
+}
+
+cudaError_t launch_colsum_finish(const float* colsum, int chunks, int n, void* out, bool f32, cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  colsum_finish_kernel<<<ceil_div(n, 32), 256, 0, st>>>(colsum, chunks, n, out, f32);
+  return cudaGetLastError();
+}
+
+}  // namespace moe

@@ -1,0 +1,393 @@
+// The router's balance loss with its per-expert counts, and the gradient of the
+// routing logits.
+//
+// For every sequence q (tokens [cu[q], cu[q+1])), with T_q its tokens that
+// select at least one expert, E experts and k picks per token:
+//   p_te    = s_te / (sum_j s_tj + 1e-20), s = sigmoid(logit)   (or softmax)
+//   f_qe    = E / (k T_q) * (times expert e was picked in q)
+//   P_qe    = 1 / T_q * sum_t p_te
+//   loss    = alpha * mean over non-empty sequences of sum_e f_qe P_qe
+// A pick outside [0, E) selects nothing; a token all of whose picks do so is
+// padding (the exchange buffers of expert parallelism mark rows past a rank's
+// tokens this way) and counts nowhere, whatever its logits hold. Gradient
+// (f does not depend on the logits):
+//   c_e = g alpha E / (k n_seq T_q^2) * count_qe
+//   d loss / d logit_te = (c_e - sum_j c_j p_tj) / (sum_j s_tj + 1e-20) * s_te (1 - s_te)
+//   (softmax: p_te (c_e - sum_j c_j p_tj)),
+// and, with the gradient dw of the combine weights w_k = s_k / (sum_sel s + 1e-20) * scale,
+//   d / d logit_k += (dw_k scale - sum_j dw_j scale s_j / S) / S * s_k (1 - s_k), S = sum_sel s + 1e-20.
+//
+// Forward: blocks of consecutive tokens, a warp per token, the sums of a
+// (block, sequence) pair in registers and shared memory, stored to slot
+// block + sequence (unique: along the tokens one of the two grows with every
+// new pair, so no list is needed and nothing is added atomically); a second
+// kernel adds a sequence's slots in order, fp64, one block per sequence and 32
+// experts, and its last block adds up the loss in order. The result does not
+// depend on the order in which blocks run. Backward: one pass, a warp per
+// token. Both read the logits once and are bound by latency at a few hundred
+// tokens and by HBM (or L2, which holds the logits of 16k tokens) above.
+#include "train_common.cuh"
+
+namespace moe {
+
+constexpr int kBalWarps = 8;
+constexpr float kScoreEps = 1e-20f;
+
+static int balance_chunk(int t) {   // tokens per block: about two blocks per SM, a multiple of the warps
+  const int c = align_up(ceil_div(t, 2 * 148), kBalWarps);
+  return c < kBalWarps ? kBalWarps : c;
+}
+
+struct BalanceWs {
+  float* p;        // [blocks + s, e]
+  int32_t* c;      // [blocks + s, e]
+  int32_t* t;      // [blocks + s]
+  double* loss;    // [s * groups]
+  int32_t* state;  // [1]: finished blocks of the second kernel
+};
+static size_t up(size_t x) { return (x + 255) & ~size_t(255); }
+static size_t balance_ws(int t, int e, int s, uint8_t* base, BalanceWs* w) {
+  const size_t slots = (size_t)ceil_div(t, balance_chunk(t)) + s;
+  size_t o = 0;
+  auto take = [&](size_t bytes) { const size_t at = o; o += up(bytes); return base + at; };
+  uint8_t* p = take(slots * e * 4);
+  uint8_t* c = take(slots * e * 4);
+  uint8_t* tt = take(slots * 4);
+  uint8_t* l = take((size_t)s * ceil_div(e, 32) * 8);
+  uint8_t* st = take(4);
+  if (w) *w = {reinterpret_cast<float*>(p), reinterpret_cast<int32_t*>(c), reinterpret_cast<int32_t*>(tt),
+               reinterpret_cast<double*>(l), reinterpret_cast<int32_t*>(st)};
+  return o;
+}
+size_t balance_workspace_bytes(int t, int e, int s) { return balance_ws(t, e, s, nullptr, nullptr); }
+
+// Bounds of sequence q, held inside [0, t] whatever cu contains.
+__device__ __forceinline__ void seq_bounds(const int32_t* cu, int q, int t, int& a, int& b) {
+  if (cu == nullptr) {
+    a = 0;
+    b = t;
+    return;
+  }
+  a = min(max(__ldg(cu + q), 0), t);
+  b = min(max(__ldg(cu + q + 1), a), t);
+}
+// The last sequence that starts at or before token x (0 if none does).
+__device__ __forceinline__ int seq_of(const int32_t* cu, int s, int x) {
+  if (cu == nullptr) return 0;
+  int lo = 0, hi = s - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(cu + mid) <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <int ITEMS>
+__device__ __forceinline__ void load_logits(const float* row, int e, int lane, float* x) {
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) x[j] = lane + 32 * j < e ? __ldg(row + lane + 32 * j) : -INFINITY;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+
+// Unnormalised scores of a token (experts past E: 0) and the inverse of their sum.
+template <int ITEMS>
+__device__ __forceinline__ float scores(const float* x, int scoring, float* s) {
+  float sum = 0.f;
+  if (scoring == 0) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      s[j] = sigmoid_f(x[j]);
+      sum += s[j];
+    }
+    return 1.0f / (warp_sum(sum) + kScoreEps);
+  }
+  float m = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    m = fmaxf(m, x[j]);
+    nan |= x[j] != x[j];
+  }
+  m = warp_max(m);
+  if (__any_sync(0xffffffffu, nan)) m = NAN;
+  if (m == -INFINITY) {          // nothing to choose from: no scores
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) s[j] = 0.f;
+    return 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    s[j] = expf(x[j] - m);
+    sum += s[j];
+  }
+  return 1.0f / warp_sum(sum);
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(BalanceArgs a, BalanceWs w, int chunk) {
+  __shared__ float psum[kBalWarps][32 * ITEMS > 256 ? 256 : 32 * ITEMS];
+  __shared__ int hist[32 * ITEMS];
+  __shared__ int tok;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *w.state = 0;
+  const int b0 = blockIdx.x * chunk, b1 = min(b0 + chunk, a.t);
+  for (int q = seq_of(a.cu, a.s, b0); q < a.s; ++q) {
+    int qa, qb;
+    seq_bounds(a.cu, q, a.t, qa, qb);
+    if (qa >= b1) break;
+    const int s0 = max(qa, b0), s1 = min(qb, b1);
+    if (s0 >= s1) continue;                                  // block-uniform
+    for (int i = threadIdx.x; i < a.e; i += blockDim.x) hist[i] = 0;
+    if (threadIdx.x == 0) tok = 0;
+    __syncthreads();
+    float acc[ITEMS];
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) acc[j] = 0.f;
+    int mine = 0;
+    for (int t = s0 + warp; t < s1; t += kBalWarps) {
+      const int id = lane < a.k ? __ldg(a.idx + (int64_t)t * a.k + lane) : -1;
+      float x[ITEMS], s[ITEMS];
+      load_logits<ITEMS>(a.logits + (int64_t)t * a.e, a.e, lane, x);
+      const bool hit = id >= 0 && id < a.e;
+      if (!__any_sync(0xffffffffu, hit)) continue;           // padding
+      if (hit) atomicAdd(&hist[id], 1);
+      ++mine;
+      const float inv = scores<ITEMS>(x, a.scoring, s);
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j) acc[j] += s[j] * inv;
+    }
+    if (lane == 0) atomicAdd(&tok, mine);
+    const int64_t slot = (int64_t)blockIdx.x + q;
+    // 8 experts' columns (256 experts) at a time through shared memory
+#pragma unroll
+    for (int j0 = 0; j0 < ITEMS; j0 += 8) {
+      __syncthreads();
+#pragma unroll
+      for (int j = j0; j < j0 + 8 && j < ITEMS; ++j) psum[warp][lane + 32 * (j - j0)] = acc[j];
+      __syncthreads();
+      const int i = threadIdx.x, e = 32 * j0 + i;
+      if (i < 32 * ITEMS && e < a.e) {
+        float t = 0.f;
+#pragma unroll
+        for (int v = 0; v < kBalWarps; ++v) t += psum[v][i];
+        w.p[slot * a.e + e] = t;
+        w.c[slot * a.e + e] = hist[e];
+      }
+    }
+    if (threadIdx.x == 0) w.t[slot] = tok;
+    __syncthreads();                                         // hist, tok and psum are reused
+  }
+}
+
+__global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, BalanceWs w, int chunk) {
+  __shared__ double rp[8][32];
+  __shared__ int rc[8][32];
+  __shared__ int rt[256];
+  __shared__ double rl[256];
+  __shared__ int last;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int groups = gridDim.x, g = blockIdx.x;
+  const int q = blockIdx.y;
+  const int e = 32 * g + tx;
+  int qa, qb;
+  seq_bounds(a.cu, q, a.t, qa, qb);
+  // a decreasing or out-of-range boundary is reported as a NaN loss
+  bool bad = false;
+  if (a.cu != nullptr) {
+    const int c0 = __ldg(a.cu + q), c1 = __ldg(a.cu + q + 1);
+    bad = c0 < 0 || c1 < c0 || c1 > a.t;
+  }
+  const int blo = qa / chunk, bhi = qb > qa ? (qb - 1) / chunk + 1 : blo;
+  double p = 0.0;
+  int c = 0, n = 0;
+  if (!bad) {
+    for (int b = blo + ty; b < bhi; b += 8)
+      if (e < a.e) {
+        const int64_t slot = (int64_t)b + q;
+        p += (double)w.p[slot * a.e + e];
+        c += w.c[slot * a.e + e];
+      }
+    for (int b = blo + (int)threadIdx.x; b < bhi; b += 256) n += w.t[(int64_t)b + q];
+  }
+  rp[ty][tx] = p;
+  rc[ty][tx] = c;
+  rt[threadIdx.x] = n;
+  __syncthreads();
+  for (int d = 128; d >= 1; d >>= 1) {
+    if (threadIdx.x < d) rt[threadIdx.x] += rt[threadIdx.x + d];
+    __syncthreads();
+  }
+  const int tq = rt[0];
+  double term = 0.0;
+  if (ty == 0) {
+    for (int i = 1; i < 8; ++i) {
+      p += rp[i][tx];
+      c += rc[i][tx];
+    }
+    if (e < a.e) {
+      const double mean = tq > 0 ? p / tq : 0.0;
+      a.mean_scores[(int64_t)q * a.e + e] = bad ? NAN : (float)mean;
+      a.counts[(int64_t)q * a.e + e] = c;
+      if (tq > 0) term = mean * ((double)c * a.e / ((double)a.k * tq));
+    }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) term += __shfl_xor_sync(0xffffffffu, term, d);
+    if (tx == 0) {
+      w.loss[(int64_t)q * groups + g] = bad ? (double)NAN : term;
+      if (g == 0) a.tokens[q] = tq;
+      __threadfence();
+      last = atomicAdd(w.state, 1) == (int)(gridDim.x * gridDim.y) - 1;
+    }
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double l = 0.0;
+  int live = 0;
+  const int64_t parts = (int64_t)a.s * groups;
+  for (int64_t i = threadIdx.x; i < parts; i += 256) l += __ldcg(w.loss + i);
+  for (int i = threadIdx.x; i < a.s; i += 256) live += __ldcg(a.tokens + i) > 0;
+  rl[threadIdx.x] = l;
+  rt[threadIdx.x] = live;
+  __syncthreads();
+  for (int d = 128; d >= 1; d >>= 1) {
+    if (threadIdx.x < d) {
+      rl[threadIdx.x] += rl[threadIdx.x + d];
+      rt[threadIdx.x] += rt[threadIdx.x + d];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    *a.loss = (float)(rt[0] > 0 ? (double)a.alpha * rl[0] / rt[0] : rl[0]);   // rl is 0 (or NaN) without sequences
+    *a.live = rt[0];
+  }
+}
+
+// t = 0: no tokens anywhere.
+__global__ void balance_empty_kernel(BalanceArgs a) {
+  for (int64_t i = threadIdx.x; i < (int64_t)a.s * a.e; i += blockDim.x) {
+    a.counts[i] = 0;
+    a.mean_scores[i] = 0.f;
+  }
+  for (int i = threadIdx.x; i < a.s; i += blockDim.x) a.tokens[i] = 0;
+  if (threadIdx.x == 0) {
+    *a.loss = 0.f;
+    *a.live = 0;
+  }
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGradArgs a, int per_warp) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t t0 = ((int64_t)blockIdx.x * kBalWarps + warp) * per_warp;
+  if (t0 >= a.t) return;
+  const int t1 = (int)min(t0 + per_warp, (int64_t)a.t);
+  const float g = a.grad_loss != nullptr ? __ldg(a.grad_loss) : 0.f;
+  const int live = a.grad_loss != nullptr ? __ldg(a.live) : 0;
+  int q = -1, qa = 0, qb = 0;
+  float coef[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) coef[j] = 0.f;
+  for (int t = (int)t0; t < t1; ++t) {
+    const int id = lane < a.k ? __ldg(a.idx + (int64_t)t * a.k + lane) : -1;
+    float x[ITEMS], s[ITEMS], dx[ITEMS];
+    load_logits<ITEMS>(a.logits + (int64_t)t * a.e, a.e, lane, x);
+    const bool hit = id >= 0 && id < a.e;
+    const bool token = __any_sync(0xffffffffu, hit);
+    // the token's sequence and its coefficients (t == qa: the first sequence may start after a gap)
+    if (a.grad_loss != nullptr && (q < 0 || t >= qb || t == qa)) {
+      q = seq_of(a.cu, a.s, t);
+      seq_bounds(a.cu, q, a.t, qa, qb);
+      const int tq = t >= qa && t < qb ? __ldg(a.tokens + q) : 0;   // 0: in no sequence
+      const double f = tq > 0 && live > 0 ? (double)g * a.alpha * a.e / ((double)a.k * live * tq * tq) : 0.0;
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j)
+        coef[j] = tq > 0 && lane + 32 * j < a.e ? (float)(f * __ldg(a.counts + (int64_t)q * a.e + lane + 32 * j)) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) dx[j] = 0.f;
+    if (token && a.grad_loss != nullptr) {
+      const float inv = scores<ITEMS>(x, a.scoring, s);
+      float inner = 0.f;
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j) inner += coef[j] * s[j];
+      inner = warp_sum(inner) * inv;
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j) {
+        const float d = (coef[j] - inner) * inv;
+        dx[j] = d * (a.scoring == 0 ? s[j] * sigmoid_f(-x[j]) : s[j]);
+      }
+    }
+    if (token && a.grad_weights != nullptr) {
+      const float xs = hit ? __ldg(a.logits + (int64_t)t * a.e + id) : 0.f;
+      const float top = hit ? sigmoid_f(xs) : 0.f;
+      const float dw = hit ? __ldg(a.grad_weights + (int64_t)t * a.k + lane) * a.route_scale : 0.f;
+      const float total = warp_sum(top) + kScoreEps;
+      const float dot = warp_sum(dw * top);
+      const float d = hit ? (dw - dot / total) / total * (top * sigmoid_f(-xs)) : 0.f;
+      for (int i = 0; i < a.k; ++i) {                        // in pick order; a repeated pick adds up
+        const int ie = __shfl_sync(0xffffffffu, hit ? id : -1, i);
+        const float id_d = __shfl_sync(0xffffffffu, d, i);
+        if (ie >= 0 && (ie & 31) == lane) {
+#pragma unroll
+          for (int j = 0; j < ITEMS; ++j)
+            if (j == ie >> 5) dx[j] += id_d;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (lane + 32 * j < a.e) a.grad_logits[(int64_t)t * a.e + lane + 32 * j] = dx[j];
+  }
+}
+
+cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
+  if (a.t == 0) {
+    balance_empty_kernel<<<1, 256, 0, st>>>(a);
+    return cudaGetLastError();
+  }
+  BalanceWs w;
+  balance_ws(a.t, a.e, a.s, static_cast<uint8_t*>(a.workspace), &w);
+  const int chunk = balance_chunk(a.t), grid = ceil_div(a.t, chunk);
+#define MOE_BAL(I) balance_partial_kernel<I><<<grid, kBalWarps * 32, 0, st>>>(a, w, chunk)
+  if (a.e <= 32) MOE_BAL(1);
+  else if (a.e <= 64) MOE_BAL(2);
+  else if (a.e <= 128) MOE_BAL(4);
+  else if (a.e <= 256) MOE_BAL(8);
+  else if (a.e <= 512) MOE_BAL(16);
+  else MOE_BAL(32);
+#undef MOE_BAL
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  balance_reduce_kernel<<<dim3((unsigned)ceil_div(a.e, 32), (unsigned)a.s), 256, 0, st>>>(a, w, chunk);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_balance_grad(const BalanceGradArgs& a, cudaStream_t st) {
+  if (a.t == 0) return cudaSuccess;
+  int per = ceil_div(a.t, 148 * 8 * kBalWarps);
+  if (per < 1) per = 1;
+  const int grid = ceil_div(a.t, (int64_t)per * kBalWarps);
+#define MOE_BALG(I) balance_grad_kernel<I><<<grid, kBalWarps * 32, 0, st>>>(a, per)
+  if (a.e <= 32) MOE_BALG(1);
+  else if (a.e <= 64) MOE_BALG(2);
+  else if (a.e <= 128) MOE_BALG(4);
+  else if (a.e <= 256) MOE_BALG(8);
+  else if (a.e <= 512) MOE_BALG(16);
+  else MOE_BALG(32);
+#undef MOE_BALG
+  return cudaGetLastError();
+}
+
+}  // namespace moe

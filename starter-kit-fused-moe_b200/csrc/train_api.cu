@@ -1,0 +1,243 @@
+// C-ABI layer of the dense products, 8-bit activation checkpoints, gradients
+// and the balance loss: argument checks, workspace carving, launches. Nothing
+// here allocates, synchronises or keeps state between calls.
+#include <cstdio>
+
+#include "moe_fp8.h"
+#include "moe_kernels.h"
+#include "train_kernels.h"
+
+namespace {
+
+int bad(const char* msg) {
+  moe::set_last_error(msg);
+  return MOE_ERR_INVALID_ARGUMENT;
+}
+int workspace_error(const char* what, size_t need, size_t got) {
+  char buf[160];
+  snprintf(buf, sizeof(buf), "%s: workspace missing, misaligned or too small (need %zu bytes, got %zu)", what, need, got);
+  moe::set_last_error(buf);
+  return MOE_ERR_WORKSPACE;
+}
+int done(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return MOE_OK;
+  char buf[160];
+  snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
+  moe::set_last_error(buf);
+  return MOE_ERR_CUDA;
+}
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+int64_t up8(int64_t x) { return (x + 7) & ~int64_t(7); }
+
+constexpr int64_t kMaxDim = 1 << 30;
+
+int check_sizes(int64_t m, int64_t k, int64_t n, int act) {
+  if (m < 0 || k < 1 || n < 1 || m > kMaxDim || k > kMaxDim || n > kMaxDim)
+    return bad("m must be in [0, 2^30], k and n in [1, 2^30]");
+  if (act < MOE_ACT_NONE || act > MOE_ACT_SWIGLU) return bad("unknown activation");
+  if (act == MOE_ACT_SWIGLU && n % 2) return bad("SwiGLU needs an even n");
+  return MOE_OK;
+}
+
+// Workspace of the gradient entry.
+struct GradPlan {
+  bool need_dz, two_terms;
+  int chunks;
+  int64_t ldz, ldk;
+  size_t dz, xhat, colsum, tmp, total;
+};
+GradPlan grad_plan(const MoeLinearGradArgs& a) {
+  GradPlan p{};
+  p.ldz = up8(a.n);
+  p.ldk = up8(a.k);
+  p.two_terms = a.grad_f32 && (a.activation != MOE_ACT_NONE || a.grad_y_f32);
+  p.need_dz = a.grad_x || a.grad_weight;
+  p.chunks = moe::act_grad_chunks(a.m, a.n);
+  size_t o = 0;
+  p.dz = o;
+  if (p.need_dz) o += up256((size_t)a.m * p.ldz * 2 * (p.two_terms ? 2 : 1));
+  p.xhat = o;
+  if (a.grad_weight) o += up256((size_t)a.m * p.ldk * 2);
+  p.colsum = o;
+  if (a.grad_bias) o += up256((size_t)p.chunks * a.n * 4);
+  p.tmp = o;
+  o += up256((size_t)(a.grad_x ? a.m : 0) * a.k * 4) + up256((size_t)(a.grad_weight ? a.n : 0) * a.k * 4);
+  p.total = o;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t moe_linear_workspace_bytes(const MoeLinearArgs* a) {
+  if (!a || a->m <= 0 || a->n <= 0) return 0;
+  return up256((size_t)a->m * a->n * 4);
+}
+
+int moe_linear_run(const MoeLinearArgs* a, void* stream) {
+  if (!a) return bad("args is NULL");
+  if (int rc = check_sizes(a->m, a->k, a->n, a->activation)) return rc;
+  if (a->m == 0) return MOE_OK;
+  const int64_t O = a->activation == MOE_ACT_SWIGLU ? a->n / 2 : a->n;
+  if (!a->x || !a->weight || !a->y) return bad("linear: x, weight and y must not be NULL");
+  if ((a->z8 == nullptr) != (a->z_scale == nullptr)) return bad("linear: z8 and z_scale go together");
+  if (!aligned(a->x, 2) || !aligned(a->weight, 2) || !aligned(a->bias, 2) || !aligned(a->residual, 2) ||
+      !aligned(a->y, a->y_f32 ? 4 : 2))
+    return bad("linear: a pointer is not aligned to its type");
+  if (a->ldx < a->k || a->ldw < a->k || a->ldy < O || (a->residual && a->ldr < 0))
+    return bad("linear: a row stride is smaller than the row");
+  const size_t need = moe_linear_workspace_bytes(a);
+  if (need && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need))
+    return workspace_error("linear", need, a->workspace_bytes);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* z = static_cast<float*>(a->workspace);
+  cudaError_t e = moe::launch_simple_gemm(a->x, a->ldx, 1, a->weight, a->ldw, 1, a->m, a->n, a->k, false, z, st);
+  if (e != cudaSuccess) return done(e, "linear product");
+  moe::LinearEpilogue ep{a->bias, a->residual, a->y, static_cast<uint8_t*>(a->z8), static_cast<uint8_t*>(a->z_scale),
+                         a->ldr, a->ldy, a->activation, a->y_f32};
+  return done(moe::launch_simple_epilogue(z, a->m, a->n, ep, st), "linear epilogue");
+}
+
+size_t moe_linear_grad_workspace_bytes(const MoeLinearGradArgs* a) {
+  if (!a || a->m <= 0 || a->n <= 0 || a->k <= 0) return 0;
+  return grad_plan(*a).total;
+}
+
+int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
+  if (!a) return bad("args is NULL");
+  if (int rc = check_sizes(a->m, a->k, a->n, a->activation)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t gsize = a->grad_f32 ? 4 : 2;
+  if (!aligned(a->grad_x, gsize) || !aligned(a->grad_weight, gsize) || !aligned(a->grad_bias, gsize))
+    return bad("linear gradient: a pointer is not aligned to its type");
+  if (a->m == 0) {           // sums over no tokens
+    cudaError_t e = cudaSuccess;
+    if (a->grad_weight) e = cudaMemsetAsync(a->grad_weight, 0, (size_t)a->n * a->k * gsize, st);
+    if (e == cudaSuccess && a->grad_bias) e = cudaMemsetAsync(a->grad_bias, 0, (size_t)a->n * gsize, st);
+    return done(e, "clearing the gradients");
+  }
+  if (!a->grad_x && !a->grad_weight && !a->grad_bias) return MOE_OK;
+  const int64_t O = a->activation == MOE_ACT_SWIGLU ? a->n / 2 : a->n;
+  const bool act = a->activation != MOE_ACT_NONE;
+  if (!a->grad_y || (act && (!a->z8 || !a->z_scale)) || (a->grad_x && !a->weight) ||
+      (a->grad_weight && (!a->x8 || !a->x_scale)))
+    return bad("linear gradient: an input that the requested gradients need is NULL");
+  if (!aligned(a->grad_y, a->grad_y_f32 ? 4 : 2) || !aligned(a->weight, 2))
+    return bad("linear gradient: a pointer is not aligned to its type");
+  if (a->ldg < 0 || (a->grad_x && a->ldw < a->k)) return bad("linear gradient: a row stride is smaller than the row");
+  const GradPlan p = grad_plan(*a);
+  if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < p.total)
+    return workspace_error("linear gradient", p.total, a->workspace_bytes);
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  const int terms = p.two_terms ? 2 : 1;
+  moe::ActGradArgs g{};
+  g.dy = a->grad_y;
+  g.z8 = act ? static_cast<const uint8_t*>(a->z8) : nullptr;
+  g.z_scale = static_cast<const uint8_t*>(a->z_scale);
+  g.dz = p.need_dz ? ws + p.dz : nullptr;
+  g.colsum = a->grad_bias ? reinterpret_cast<float*>(ws + p.colsum) : nullptr;
+  g.ldg = a->ldg;
+  g.ldz = p.ldz;
+  g.m = a->m;
+  g.n = a->n;
+  g.act = a->activation;
+  g.dy_f32 = a->grad_y_f32;
+  g.terms = terms;
+  cudaError_t e = moe::launch_act_grad(g, st);
+  if (e != cudaSuccess) return done(e, "activation gradient");
+  if (a->grad_bias) {
+    e = moe::launch_colsum_finish(g.colsum, p.chunks, a->n, a->grad_bias, a->grad_f32 != 0, st);
+    if (e != cudaSuccess) return done(e, "bias gradient");
+  }
+  float* tmp = reinterpret_cast<float*>(ws + p.tmp);
+  const uint16_t* dz = reinterpret_cast<const uint16_t*>(ws + p.dz);
+  if (a->grad_x) {
+    for (int t = 0; t < terms && e == cudaSuccess; ++t)
+      e = moe::launch_simple_gemm(dz + (size_t)t * a->m * p.ldz, p.ldz, 1, a->weight, 1, a->ldw, a->m, a->k, a->n, t > 0,
+                                  tmp, st);
+    if (e == cudaSuccess) e = moe::launch_simple_store(tmp, (int64_t)a->m * a->k, a->grad_x, a->grad_f32 != 0, st);
+    if (e != cudaSuccess) return done(e, "input gradient");
+    tmp += up256((size_t)a->m * a->k * 4) / 4;
+  }
+  if (a->grad_weight) {
+    e = moe::launch_restore(static_cast<const uint8_t*>(a->x8), static_cast<const uint8_t*>(a->x_scale), 1, a->m, a->k,
+                            ws + p.xhat, false, p.ldk, st);
+    for (int t = 0; t < terms && e == cudaSuccess; ++t)
+      e = moe::launch_simple_gemm(dz + (size_t)t * a->m * p.ldz, 1, p.ldz, ws + p.xhat, 1, p.ldk, a->n, a->k, a->m, t > 0,
+                                  tmp, st);
+    if (e == cudaSuccess) e = moe::launch_simple_store(tmp, (int64_t)a->n * a->k, a->grad_weight, a->grad_f32 != 0, st);
+    if (e != cudaSuccess) return done(e, "weight gradient");
+  }
+  return MOE_OK;
+}
+
+int moe_checkpoint_activations(const void* x, int32_t x_is_bf16, int64_t rows, int64_t cols, int64_t ldx, void* q,
+                               void* scale, void* stream) {
+  if (rows < 0 || cols < 0 || rows > kMaxDim || cols > (int64_t)65535 * 1024)
+    return bad("checkpoint: rows must be in [0, 2^30], cols in [0, 65535 * 1024]");
+  if (rows == 0 || cols == 0) return MOE_OK;
+  if (!x || !q || !scale || !aligned(x, x_is_bf16 ? 2 : 4)) return bad("checkpoint: NULL or misaligned pointer");
+  if (ldx < 0) return bad("checkpoint: negative row stride");
+  return done(moe::launch_checkpoint(x, x_is_bf16 != 0, rows, cols, ldx, static_cast<uint8_t*>(q),
+                                     static_cast<uint8_t*>(scale), static_cast<cudaStream_t>(stream)),
+              "checkpoint");
+}
+
+int moe_restore_activations(const void* q, const void* scale, int64_t batch, int64_t rows, int64_t cols, void* out,
+                            int32_t out_f32, void* stream) {
+  if (batch < 0 || batch > 65535 || rows < 0 || cols < 0 || rows > kMaxDim || cols > (int64_t)65535 * 1024)
+    return bad("restore: batch must be in [0, 65535], rows in [0, 2^30], cols in [0, 65535 * 1024]");
+  if (batch == 0 || rows == 0 || cols == 0) return MOE_OK;
+  if (!q || !scale || !out || !aligned(out, out_f32 ? 4 : 2)) return bad("restore: NULL or misaligned pointer");
+  return done(moe::launch_restore(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), batch, rows, cols,
+                                  out, out_f32 != 0, cols, static_cast<cudaStream_t>(stream)),
+              "restore");
+}
+
+static int check_balance(int t, int e, int k, int s, int scoring) {
+  if (t < 0 || t > kMaxDim || e < 1 || e > 1024 || k < 1 || k > 32 || s < 1 || s > 65535)
+    return bad("balance: need T in [0, 2^30], E in [1, 1024], k in [1, 32], S in [1, 65535]");
+  if (scoring != 0 && scoring != 1) return bad("balance: scoring must be 0 (sigmoid) or 1 (softmax)");
+  return MOE_OK;
+}
+
+size_t moe_balance_workspace_bytes(int32_t t, int32_t e, int32_t s) {
+  if (t <= 0 || e < 1 || e > 1024 || s < 1 || s > 65535) return 0;
+  return moe::balance_workspace_bytes(t, e, s);
+}
+
+int moe_balance_loss(const MoeBalanceArgs* a, void* stream) {
+  if (!a) return bad("args is NULL");
+  if (int rc = check_balance(a->num_tokens, a->num_experts, a->top_k, a->num_sequences, a->scoring)) return rc;
+  if (!a->loss || !a->counts || !a->tokens || !a->mean_scores || !a->sequences) return bad("balance: an output is NULL");
+  if (a->num_tokens > 0 && (!a->routing_logits || !a->topk_idx || !aligned(a->routing_logits, 4) || !aligned(a->topk_idx, 4)))
+    return bad("balance: NULL or misaligned input");
+  if (!a->cu_seqlens && a->num_sequences != 1) return bad("balance: one sequence without cu_seqlens");
+  const size_t need = moe_balance_workspace_bytes(a->num_tokens, a->num_experts, a->num_sequences);
+  if (need && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need))
+    return workspace_error("balance", need, a->workspace_bytes);
+  moe::BalanceArgs b{a->routing_logits, a->topk_idx, a->cu_seqlens, a->num_tokens, a->num_experts, a->top_k,
+                     a->num_sequences, a->scoring, a->alpha, a->loss, a->counts, a->tokens, a->mean_scores,
+                     a->sequences, a->workspace};
+  return done(moe::launch_balance(b, static_cast<cudaStream_t>(stream)), "balance loss");
+}
+
+int moe_balance_loss_grad(const MoeBalanceGradArgs* a, void* stream) {
+  if (!a) return bad("args is NULL");
+  if (int rc = check_balance(a->num_tokens, a->num_experts, a->top_k, a->num_sequences, a->scoring)) return rc;
+  if (a->num_tokens == 0) return MOE_OK;
+  if (!a->routing_logits || !a->topk_idx || !a->grad_logits || !aligned(a->routing_logits, 4) ||
+      !aligned(a->topk_idx, 4) || !aligned(a->grad_logits, 4) || !aligned(a->grad_topk_weights, 4))
+    return bad("balance gradient: NULL or misaligned pointer");
+  if (a->grad_loss && (!a->counts || !a->tokens || !a->sequences))
+    return bad("balance gradient: grad_loss needs counts, tokens and sequences");
+  if (!a->cu_seqlens && a->num_sequences != 1) return bad("balance gradient: one sequence without cu_seqlens");
+  moe::BalanceGradArgs b{a->routing_logits, a->topk_idx, a->cu_seqlens, a->num_tokens, a->num_experts, a->top_k,
+                         a->num_sequences, a->scoring, a->alpha, a->routed_scaling_factor, a->counts, a->tokens,
+                         a->sequences, a->grad_loss, a->grad_topk_weights, a->grad_logits};
+  return done(moe::launch_balance_grad(b, static_cast<cudaStream_t>(stream)), "balance gradient");
+}
+
+}  // extern "C"

@@ -1,0 +1,86 @@
+// Device helpers of the dense products, their checkpoints and gradients:
+// activations, e4m3 / e8m0 conversion.
+//
+// An 8-bit checkpoint keeps a row in blocks of 128 values: e4m3 bytes and one
+// e8m0 scale per block, a power of two 2^e with the least e for which
+// amax <= 448 * 2^e (and e >= -117). Scaling by a power of two is exact, so the
+// only rounding is the e4m3 one (half a step: 2^-4 relative above the
+// subnormals), and every restored value q * 2^e (four significant bits, least
+// magnitude 2^-126) is a bf16 number: the backward's bf16 matrix products see
+// the checkpoint exactly. In a block of the largest scale, 2^120, magnitudes are
+// held at 240 * 2^120 (256 * 2^120 would be infinite). A block holding an infinity or NaN gets the e8m0 NaN
+// code and comes back as NaN throughout.
+#pragma once
+
+#include "moe_common.cuh"
+#include "train_kernels.h"
+
+namespace moe {
+
+constexpr int kMinScaleExp = -117;
+
+// e8m0 code of a block from its largest magnitude (bits of a non-negative
+// float; NaN and infinity compare above every finite value as integers).
+__device__ __forceinline__ uint32_t e8m0_of_amax(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return 255u;
+  // amax = 1.f * 2^p: 448 = 1.75 * 2^8, so e = p - 8 while the significand is at most 1.75
+  const int p = (int)(amax_bits >> 23) - 127;
+  const int e = p - ((amax_bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
+  return (uint32_t)((e < kMinScaleExp ? kMinScaleExp : e) + 127);
+}
+// Scaled values of a block, held below infinity (a rare, block-uniform branch).
+constexpr uint32_t kTopScaleCode = 120 + 127;
+__device__ __forceinline__ float hold_finite(float v) { return fminf(fmaxf(v, -240.f), 240.f); }
+// 2^-e for a code made above (e in [-117, 120]); NaN for the NaN code.
+__device__ __forceinline__ float e8m0_inverse(uint32_t code) {
+  return code == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float((254u - code) << 23);
+}
+// 2^e for any code a caller may hand over.
+__device__ __forceinline__ float e8m0_value(uint32_t code) {
+  return code == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(code ? code << 23 : 0x00400000u);
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+__device__ __forceinline__ float2 e4m3x2_value(uint32_t v16) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v16, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ float e4m3_value(uint8_t v) { return e4m3x2_value(v).x; }
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_bf16(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+
+__device__ __forceinline__ float sigmoid_f(float z) { return 1.0f / (1.0f + expf(-z)); }
+
+// Single-input activations (codes 0..3); SwiGLU is first * silu(second).
+__device__ __forceinline__ float act_value(float z, int act) {
+  switch (act) {
+    case kActRelu: return z < 0.f ? 0.f : z;              // NaN stays
+    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case kActSilu: return z / (1.0f + expf(-z));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+  switch (act) {
+    case kActRelu: return z > 0.f ? 1.f : 0.f;
+    case kActGelu:
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case kActSilu: {
+      const float s = sigmoid_f(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    default: return 1.f;
+  }
+}
+
+}  // namespace moe

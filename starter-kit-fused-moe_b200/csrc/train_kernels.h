@@ -1,0 +1,78 @@
+// Launchers of the kernels around the routed experts: dense products, 8-bit
+// activation checkpoints, gradients, and the router's balance loss.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace moe {
+
+// activation codes (MOE_ACT_* of moe_fp8.h)
+constexpr int kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActSwiglu = 4;
+
+inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Epilogue of a dense product z = x W^T: y = act(z + b) + r, optionally with the
+// pre-activation kept in 8 bits. O = n / 2 for SwiGLU, n otherwise.
+struct LinearEpilogue {
+  const void* bias;        // bf16 [n] or NULL
+  const void* residual;    // bf16 [m, O] or NULL, row stride ldr
+  void* y;                 // bf16 / f32 [m, O], row stride ldy
+  uint8_t* z8;             // e4m3 [m, n] ([2, m, O] for SwiGLU) or NULL
+  uint8_t* z_scale;        // e8m0 [ceil(n / 128), m] ([2, ceil(O / 128), m])
+  int64_t ldr, ldy;
+  int act;
+  int y_f32;
+};
+
+cudaError_t launch_checkpoint(const void* x, bool bf16, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q,
+                              uint8_t* scale, cudaStream_t st);
+cudaError_t launch_restore(const uint8_t* q, const uint8_t* scale, int64_t batch, int64_t rows, int64_t cols, void* out,
+                           bool f32, int64_t ldo, cudaStream_t st);
+
+// z[m, n] = sum_k A(m, k) B(n, k) with arbitrary element strides, f32 out (row stride n).
+cudaError_t launch_simple_gemm(const void* A, int64_t am, int64_t ak, const void* B, int64_t bn, int64_t bk, int m,
+                               int n, int k, bool accumulate, float* out, cudaStream_t st);
+cudaError_t launch_simple_epilogue(const float* z, int m, int n, const LinearEpilogue& ep, cudaStream_t st);
+cudaError_t launch_simple_store(const float* z, int64_t count, void* out, bool f32, cudaStream_t st);
+
+// Gradient of the pre-activation: dz = dy * act'(z), written as bf16 [terms][m][ldz]
+// (terms = 2: the rounding's remainder follows), and per-chunk column sums.
+struct ActGradArgs {
+  const void* dy;          // bf16 / f32 [m, O], row stride ldg
+  const uint8_t* z8;       // as LinearEpilogue; NULL when act is none
+  const uint8_t* z_scale;
+  void* dz;                // NULL: column sums only
+  float* colsum;           // [chunks, n] or NULL
+  int64_t ldg, ldz;
+  int m, n, act, dy_f32, terms;
+};
+int act_grad_chunks(int m, int n);
+cudaError_t launch_act_grad(const ActGradArgs& a, cudaStream_t st);
+cudaError_t launch_colsum_finish(const float* colsum, int chunks, int n, void* out, bool f32, cudaStream_t st);
+
+struct BalanceArgs {
+  const float* logits;     // [t, e]
+  const int32_t* idx;      // [t, k]
+  const int32_t* cu;       // [s + 1] or NULL (one sequence)
+  int t, e, k, s, scoring; // scoring 0 sigmoid, 1 softmax
+  float alpha;
+  float* loss; int32_t* counts; int32_t* tokens; float* mean_scores; int32_t* live;
+  void* workspace;
+};
+size_t balance_workspace_bytes(int t, int e, int s);
+cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st);
+
+struct BalanceGradArgs {
+  const float* logits; const int32_t* idx; const int32_t* cu;
+  int t, e, k, s, scoring;
+  float alpha, route_scale;
+  const int32_t* counts; const int32_t* tokens; const int32_t* live;
+  const float* grad_loss;      // device scalar or NULL (0: no balance part)
+  const float* grad_weights;   // [t, k] or NULL
+  float* grad_logits;          // [t, e]
+};
+cudaError_t launch_balance_grad(const BalanceGradArgs& a, cudaStream_t st);
+
+}  // namespace moe

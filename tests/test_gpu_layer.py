@@ -1,0 +1,452 @@
+"""GPU: dense products, 8-bit checkpoints and gradients against 64-bit forms.
+
+Tolerances. A product summed in fp32 is off by at most K * 2^-23 * sum |x||w|
+(an addition that truncates loses up to 2^-23 of the running sum); rounding to
+bf16 loses at most 2^-8 of the value, to e4m3 2^-4 of it (2^-10 of the block's
+scale below the normal numbers). The activations' slopes are at most 1.13 and
+their own fp32 evaluation is good to 2^-20 of 1 + |z|."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+ACTS = ("none", "relu", "gelu", "silu", "swiglu")
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def randn(*shape, seed=0, scale=1.0, dtype=BF):
+    g = torch.Generator(device="cuda").manual_seed(seed + 1000 * sum(shape))
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def act64(z, act):
+    if act == "none":
+        return z
+    if act == "relu":
+        return z.clamp(min=0)
+    if act == "gelu":
+        return z * 0.5 * torch.erfc(-z / math.sqrt(2))
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    a, b = z.chunk(2, dim=-1)
+    return a * b * torch.sigmoid(b)
+
+
+def dense64(x, w, b=None):
+    z = x.double() @ w.double().t()
+    mag = x.double().abs() @ w.double().abs().t()
+    if b is not None:
+        z, mag = z + b.double(), mag + b.double().abs()
+    return z, mag * ((x.shape[1] + 2) * 2.0 ** -23) + 1e-30
+
+
+def tol_act(z, tz, act):
+    """Error of act(z) in fp32 from an error tz of z."""
+    if act == "swiglu":
+        a, b = z.chunk(2, dim=-1)
+        ta, tb = tz.chunk(2, dim=-1)
+        return ta * (b.abs() + 1) + (a.abs() + ta) * 1.13 * tb + 2.0 ** -20 * (1 + b.abs()) * a.abs()
+    return 1.13 * tz + (2.0 ** -20 * (1 + z.abs()) if act != "none" else 0)
+
+
+def check(got, ref, tol, what):
+    got = got.double()
+    assert got.shape == ref.shape, what
+    bad = ~((got - ref).abs() <= tol)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst "
+                           f"{float(((got - ref).abs() - tol).max()):.3e} over, first at {bad.nonzero()[0].tolist()}")
+
+
+def rounded(ref, tol, dtype):
+    return tol + (ref.abs() + tol) * (2.0 ** -8 if dtype == BF else 2.0 ** -23) + 1e-38
+
+
+def linear_case(pkg, m, k, n, act="none", bias=False, res=False, dtype=BF, x=None, w=None):
+    x = randn(m, k, seed=1) if x is None else x
+    w = randn(n, k, seed=2, scale=k ** -0.5) if w is None else w
+    b = randn(n, seed=3, scale=0.3) if bias else None
+    o = n // 2 if act == "swiglu" else n
+    r = randn(m, o, seed=4) if res else None
+    y = pkg.linear(x, w, bias=b, residual=r, activation=act, out_dtype=dtype)
+    z, tz = dense64(x, w, b)
+    ref, tol = act64(z, act), tol_act(z, tz, act)
+    if res:
+        ref = ref + r.double()
+        tol = tol + ref.abs() * 2.0 ** -23
+    assert y.dtype == dtype
+    check(y, ref, rounded(ref, tol, dtype), f"linear {m}x{k}x{n} {act}")
+    return y
+
+
+SIZES = [(1, 7168, 256), (1, 8, 1), (2, 64, 16), (3, 72, 130), (7, 7168, 64), (8, 2048, 512), (9, 128, 264), (16, 256, 48),
+         (17, 320, 96), (32, 512, 128), (33, 512, 128), (64, 7168, 512), (127, 64, 256), (128, 192, 256), (129, 200, 264),
+         (255, 640, 96), (256, 64, 512), (257, 72, 520), (300, 7168, 256), (600, 2048, 1032), (1000, 136, 2050)]
+
+
+@pytest.mark.parametrize("m, k, n", SIZES)
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+def test_linear_sizes(pkg, m, k, n, act):
+    if act == "swiglu" and n % 2:
+        n += 1
+    linear_case(pkg, m, k, n, act)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m, k, n", [(5, 96, 80), (40, 96, 80), (300, 520, 390), (520, 1024, 768)])
+def test_linear_epilogues(pkg, m, k, n, act):
+    for bias, res, dtype in ((True, False, BF), (False, True, BF), (True, True, F32), (False, False, F32)):
+        linear_case(pkg, m, k, n, act, bias, res, dtype)
+
+
+@pytest.mark.parametrize("m", [1, 6, 31, 70, 400])
+@pytest.mark.parametrize("k, n", [(1, 1), (7, 3), (65, 33), (129, 257), (1001, 130)])
+def test_linear_odd_sizes(pkg, m, k, n):
+    linear_case(pkg, m, k, n, "gelu", True, True)
+    linear_case(pkg, m, k, 2 * n, "swiglu", True, True, F32)
+
+
+@pytest.mark.parametrize("m", [4, 50, 300])
+def test_linear_strides_and_offsets(pkg, m):
+    """Row strides, misaligned bases, transposed and expanded inputs."""
+    big = randn(m + 1, 300, seed=5)
+    wbig = randn(200, 300, seed=6, scale=0.1)
+    for c0, k in ((0, 128), (8, 128), (1, 128), (3, 77)):
+        linear_case(pkg, m, k, 96, "silu", x=big[1:, c0:c0 + k], w=wbig[7:103, c0:c0 + k])
+    linear_case(pkg, m, 64, 96, x=randn(64, m, seed=7).t(), w=randn(64, 96, seed=8).t())
+    linear_case(pkg, m, 64, 96, x=randn(1, 64, seed=9).expand(m, 64))
+    x, w = randn(m, 64, seed=10), randn(96, 64, seed=11)
+    r = randn(1, 96, seed=12).expand(m, 96)
+    wide = randn(m, 200, seed=13)
+    for out in (None, torch.empty(m, 96, dtype=BF, device="cuda"), wide[:, 3:99], torch.empty(96, m, dtype=BF, device="cuda").t()):
+        before = wide.clone()
+        y = pkg.linear(x, w, residual=r, output=out)
+        z, tz = dense64(x, w)
+        check(y, z + r.double(), rounded(z + r.double(), tz * 2, BF), "strided")
+        if out is not None:
+            assert y is out
+        assert torch.equal(wide[:, :3], before[:, :3]) and torch.equal(wide[:, 99:], before[:, 99:])
+
+
+@pytest.mark.parametrize("m", [5, 200])
+def test_linear_in_place_residual(pkg, m):
+    x, w, r = randn(m, 256, seed=1), randn(128, 256, seed=2, scale=0.06), randn(m, 128, seed=3)
+    want = pkg.linear(x, w, residual=r)
+    got = pkg.linear(x, w, residual=r, output=r)
+    assert got is r and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m", [1, 12, 90, 700])
+def test_linear_non_finite(pkg, m):
+    """A NaN or infinity stays in its row (x) or column (weight); rows past the matrix do not leak in."""
+    x, w = randn(m, 192, seed=1), randn(80, 192, seed=2)
+    clean = pkg.linear(x, w)
+    x2 = x.clone()
+    x2[m // 2, 100] = float("nan")
+    y = pkg.linear(x2, w)
+    assert torch.isnan(y[m // 2]).all()
+    keep = torch.arange(m, device="cuda") != m // 2
+    assert torch.equal(y[keep], clean[keep])
+    w2 = w.clone()
+    w2[11, 3] = float("inf")
+    y = pkg.linear(x, w2)
+    cols = torch.arange(80, device="cuda") != 11
+    assert torch.equal(y[:, cols], clean[:, cols]) and not torch.isfinite(y[:, 11]).any()
+    big = torch.full((m, 192), float("nan"), dtype=BF, device="cuda")
+    xs = torch.cat([x, big])[:m]                   # NaN rows lie right behind the last one
+    assert torch.equal(pkg.linear(xs, w), clean)
+
+
+def test_linear_empty_and_refusals(pkg):
+    x, w = randn(4, 64), randn(32, 64)
+    assert pkg.linear(x[:0], w).shape == (0, 32)
+    bad = [dict(x=x[0]), dict(x=x.float()), dict(weight=w[:, :32]), dict(weight=w.float()), dict(weight=w.cpu()),
+           dict(bias=randn(31)), dict(bias=randn(32).float()), dict(residual=randn(4, 31)), dict(residual=randn(4, 32).float()),
+           dict(activation="tanh"), dict(weight=randn(31, 64), activation="swiglu"), dict(out_dtype=torch.float16),
+           dict(output=torch.empty(4, 31, dtype=BF, device="cuda")), dict(output=torch.empty(4, 32, device="cuda")),
+           dict(output=torch.empty(4, 32, dtype=BF)), dict(weight=w[:0]), dict(x=x[:, :0], weight=w[:, :0])]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            pkg.linear(**{"x": x, "weight": w, **kw})
+    sq = randn(64, 64)
+    with pytest.raises(ValueError, match="overlaps x"):
+        pkg.linear(sq, sq.clone(), output=sq)
+    r = randn(9, 64)
+    with pytest.raises(ValueError, match="residual"):
+        pkg.linear(sq[:8], sq, residual=r[:8], output=r[1:])
+
+
+# --------------------------------------------------------------------------------- checkpoints
+def quantize64(x):
+    """(values, codes) of the format, element by element in 64 bits."""
+    t, k = x.shape
+    v = torch.nn.functional.pad(x.double(), (0, -k % 128)).view(t, -1, 128)
+    amax = v.abs().amax(-1, keepdim=True)
+    e = torch.full_like(amax, -117.0)
+    for p in range(-116, 121):                      # the least e with amax <= 448 * 2^e
+        e = torch.where(amax > 448.0 * 2.0 ** (p - 1), torch.full_like(e, p), e)
+    s = v / torch.exp2(e)
+    s = torch.where(e == 120, s.clamp(-240, 240), s)          # 256 * 2^120 would be infinite
+    ex = torch.floor(torch.log2(s.abs().clamp(min=2.0 ** -30))).clamp(min=-6)
+    step = torch.exp2(ex - 3)
+    out = torch.round(s / step) * step * torch.exp2(e)
+    return out.flatten(1)[:, :k], (e.squeeze(-1).t() + 127).to(torch.uint8)
+
+
+@pytest.mark.parametrize("t, k", [(1, 1), (1, 128), (2, 7168), (3, 129), (31, 1000), (33, 136), (64, 7168), (65, 2047),
+                                  (513, 1024), (4099, 264)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_checkpoint_round_trip(pkg, t, k, dtype):
+    x = randn(t, k, dtype=F32)
+    x = (x * torch.exp(2 * randn(1, k, seed=5, dtype=F32)) * torch.exp2(randn(t, 1, seed=6, dtype=F32) * 20)).to(dtype)
+    x[0, : k // 2] = 0
+    q, s = pkg.checkpoint_activations(x)
+    assert q.dtype == torch.float8_e4m3fn and s.dtype == torch.float8_e8m0fnu and s.shape == (-(-k // 128), t)
+    want, codes = quantize64(x)
+    assert torch.equal(s.view(torch.uint8), codes)
+    for out in (BF, F32):
+        r = pkg.restore_activations(q, s, out)
+        assert r.dtype == out and torch.equal(r.double(), want)
+    assert ((want - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + torch.exp2(
+        codes.double() - 127 - 10).t().repeat_interleave(128, 1)[:, :k]).all()
+
+
+def test_checkpoint_edges(pkg):
+    """Borders of the scale (448 * 2^e and its neighbours), the smallest and largest values, zero blocks, NaN and infinity."""
+    tops = []
+    for e in (-140, -126, -125, -117, -100, -3, 0, 5, 90, 118, 119):
+        v = 448.0 * 2.0 ** e
+        tops += [v, v * (1 + 2.0 ** -7), v * (1 - 2.0 ** -8), v / 1.75, v / 1.75 * (2 - 2.0 ** -7)]
+    tops += [0.0, 1e-45, 1.1754944e-38, 3.38e38]
+    x = torch.zeros(len(tops), 128, device="cuda", dtype=F32)
+    x[:, 17] = torch.tensor(tops, dtype=torch.float64).to(F32)
+    x[:, 18] = -x[:, 17] / 3
+    x[:, 19] = x[:, 17] * 2.0 ** -17
+    q, s = pkg.checkpoint_activations(x)
+    want, codes = quantize64(x)
+    assert torch.equal(s.view(torch.uint8), codes)
+    assert torch.equal(pkg.restore_activations(q, s).double(), want)
+    y = randn(4, 300)
+    clean = pkg.restore_activations(*pkg.checkpoint_activations(y))
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        z = y.clone()
+        z[2, 140] = bad
+        got = pkg.restore_activations(*pkg.checkpoint_activations(z))
+        assert torch.isnan(got[2, 128:256]).all()
+        got[2, 128:256] = clean[2, 128:256]
+        assert torch.equal(got, clean)
+
+
+def test_checkpoint_strides_batch_and_refusals(pkg):
+    x = randn(40, 700)
+    for v in (x[3:30, 5:400], x[::2, 8:264], x.t(), x[:1, 1:129]):
+        q, s = pkg.checkpoint_activations(v)
+        q2, s2 = pkg.checkpoint_activations(v.contiguous())
+        assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s.view(torch.uint8), s2.view(torch.uint8))
+    a, b = pkg.checkpoint_activations(x), pkg.checkpoint_activations(-x)
+    q, s = torch.stack([a[0].view(torch.uint8), b[0].view(torch.uint8)]), torch.stack([a[1].view(torch.uint8), b[1].view(torch.uint8)])
+    r = pkg.restore_activations(q.view(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu))
+    assert torch.equal(r[0], pkg.restore_activations(*a)) and torch.equal(r[1], -r[0])
+    q, s = pkg.checkpoint_activations(x[:0])
+    assert q.shape == (0, 700) and pkg.restore_activations(q, s).shape == (0, 700)
+    for bad in (lambda: pkg.checkpoint_activations(x.half()), lambda: pkg.checkpoint_activations(x.cpu()),
+                lambda: pkg.restore_activations(a[0], a[1][1:]), lambda: pkg.restore_activations(x, a[1]),
+                lambda: pkg.restore_activations(a[0], a[1], torch.float16), lambda: pkg.restore_activations(a[0], a[1].cpu())):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# --------------------------------------------------------------------------------- training pass
+def act_slope64(z, act):
+    if act == "relu":
+        return (z > 0).double()
+    s = torch.sigmoid(z)
+    if act == "silu":
+        return s * (1 + z * (1 - s))
+    return 0.5 * torch.erfc(-z / math.sqrt(2)) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+
+
+def grads64(pkg, dy, ck, w):
+    """64-bit gradients from the checkpoint's values, with the magnitudes the tolerances need."""
+    x = pkg.restore_activations(ck.x, ck.x_scale, F32).double()
+    dz = dy.double()
+    if ck.activation == "swiglu":
+        a, b = pkg.restore_activations(ck.z, ck.z_scale, F32).double()
+        s = torch.sigmoid(b)
+        dz = torch.cat([dz * b * s, dz * a * (s + b * s * (1 - s))], 1)
+    elif ck.activation != "none":
+        dz = dz * act_slope64(pkg.restore_activations(ck.z, ck.z_scale, F32).double(), ck.activation)
+    return x, dz
+
+
+TRAIN = [(1, 64, 32), (3, 8, 2), (30, 200, 130), (64, 128, 256), (130, 96, 264), (300, 1000, 390), (513, 512, 512),
+         (600, 7168, 256), (1100, 264, 1040)]
+
+
+@pytest.mark.parametrize("m, k, n", TRAIN)
+@pytest.mark.parametrize("act", ACTS)
+def test_linear_checkpointed(pkg, m, k, n, act):
+    x, w, b = randn(m, k, seed=1), randn(n, k, seed=2, scale=k ** -0.5), randn(n, seed=3)
+    y, ck = pkg.linear_checkpointed(x, w, bias=b, activation=act)
+    z, tz = dense64(x, w, b)
+    ref = act64(z, act)
+    check(y, ref, rounded(ref, tol_act(z, tz, act), BF), "y")
+    q, s = pkg.checkpoint_activations(x)
+    assert torch.equal(ck.x.view(torch.uint8), q.view(torch.uint8)) and torch.equal(ck.x_scale.view(torch.uint8), s.view(torch.uint8))
+    assert ck.activation == act
+    if act == "none":
+        assert ck.z is None and ck.z_scale is None
+        return
+    zs = z.chunk(2, 1) if act == "swiglu" else (z,)
+    ts = tz.chunk(2, 1) if act == "swiglu" else (tz,)
+    got = pkg.restore_activations(ck.z, ck.z_scale, F32)
+    got = got if act == "swiglu" else got[None]
+    codes = ck.z_scale.view(torch.uint8)
+    codes = codes if act == "swiglu" else codes[None]
+    for h, (zz, tt) in enumerate(zip(zs, ts)):
+        scale = torch.exp2(codes[h].double() - 127).t().repeat_interleave(128, 1)[:, : zz.shape[1]]
+        check(got[h], zz, 2.0 ** -4 * (zz.abs() + tt) + 2.0 ** -10 * scale + tt, "z")
+        # the scale is the least that holds the block, up to the error of its largest value
+        amax = torch.nn.functional.pad(zz.abs(), (0, -zz.shape[1] % 128)).unflatten(1, (-1, 128)).amax(-1).t()
+        slack = torch.nn.functional.pad(tt, (0, -tt.shape[1] % 128)).unflatten(1, (-1, 128)).amax(-1).t()
+        sc = torch.exp2(codes[h].double() - 127)
+        assert (amax - slack <= 448 * sc).all() and ((amax + slack > 224 * sc) | (codes[h] == 10)).all()
+
+
+@pytest.mark.parametrize("m, k, n", TRAIN)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("gin, gout", [(BF, BF), (F32, F32), (F32, BF), (BF, F32)])
+def test_linear_backward(pkg, m, k, n, act, gin, gout):
+    x, w = randn(m, k, seed=1), randn(n, k, seed=2, scale=k ** -0.5)
+    y, ck = pkg.linear_checkpointed(x, w, activation=act)
+    dy = randn(m, y.shape[1], seed=5, dtype=gin)
+    g = pkg.linear_backward(dy, ck, w, need_bias=True, grad_dtype=gout)
+    xr, dz = grads64(pkg, dy, ck, w)
+    # dz: fp32 evaluation (2^-20 of its factors), then bf16 (2^-8), or two bf16 terms (2^-16)
+    exact = act == "none" and gin == BF
+    rel = (0 if act == "none" else 2.0 ** -19) + (0 if exact else 2.0 ** -8 if gout == BF else 2.0 ** -16)
+    mag = dz.abs() + 2.0 ** -6 * dy.double().abs().repeat(1, 2 if act == "swiglu" else 1) * (act != "none")
+    zmag = 1.0
+    if act == "swiglu":
+        zr = pkg.restore_activations(ck.z, ck.z_scale, F32).double().abs()
+        zmag = 1 + torch.cat([zr[1], zr[0]], 1)
+    ez = mag * rel + (2.0 ** -19 * dy.double().abs().repeat(1, 2 if act == "swiglu" else 1) * zmag if act != "none" else 0)
+    ww = w.double()
+    ref = dz @ ww
+    check(g.x, ref, rounded(ref, ez @ ww.abs() + 2 * (n + 2) * 2.0 ** -23 * (dz.abs() @ ww.abs()) + 1e-30, gout), "grad_x")
+    ref = dz.t() @ xr
+    check(g.weight, ref, rounded(ref, ez.t() @ xr.abs() + 2 * (m + 2) * 2.0 ** -23 * (dz.abs().t() @ xr.abs()) + 1e-30, gout), "grad_weight")
+    ref = dz.sum(0)
+    eb = (mag * (0 if act == "none" else 2.0 ** -19)).sum(0) + (ez.sum(0) if act == "swiglu" else 0) + (m + 2) * 2.0 ** -23 * dz.abs().sum(0)
+    eb = eb + (2.0 ** -19 * dy.double().abs().sum(0) if act not in ("none", "swiglu") else 0)
+    check(g.bias, ref, rounded(ref, eb + 1e-30, gout), "grad_bias")
+    assert g.x.dtype == g.weight.dtype == g.bias.dtype == gout
+    again = pkg.linear_backward(dy, ck, w, need_bias=True, grad_dtype=gout)
+    assert all(torch.equal(a, b) for a, b in zip(g, again))
+    only = pkg.linear_backward(dy, ck, w, need_x=False, need_weight=False, need_bias=True, grad_dtype=gout)
+    assert only.x is None and only.weight is None and torch.equal(only.bias, g.bias)
+    assert torch.equal(pkg.linear_backward(dy, ck, w, need_weight=False, grad_dtype=gout).x, g.x)
+    assert torch.equal(pkg.linear_backward(dy, ck, w, need_x=False, grad_dtype=gout).weight, g.weight)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_backward_against_differences(pkg, act):
+    """The gradients are those of the forward: with inputs whose checkpoints are exact (few-bit values, one
+    scale), a central difference of sum(y * dy) in 64 bits agrees to the difference's own error."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    m, k, n = 5, 16, 8
+    x = torch.randint(-4, 5, (m, k), generator=g, device="cuda").double() / 4
+    w = torch.randint(-4, 5, (n, k), generator=g, device="cuda").double() / 8
+    x8, xs = pkg.checkpoint_activations(x.to(BF))
+    assert torch.equal(pkg.restore_activations(x8, xs).double(), x)
+    z = x @ w.t()
+    if act == "relu":
+        z = torch.where(z == 0, z + 0.5, z)
+    zq = torch.stack(z.chunk(2, 1)) if act == "swiglu" else z
+    pairs = [pkg.checkpoint_activations(h.float().contiguous()) for h in (zq if act == "swiglu" else zq[None])]
+    st = lambda i, d: torch.stack([p[i].view(torch.uint8) for p in pairs]).view(d)  # noqa: E731
+    z8, zs = st(0, torch.float8_e4m3fn), st(1, torch.float8_e8m0fnu)
+    zr = pkg.restore_activations(z8, zs, F32).double()
+    zr = torch.cat(list(zr), 1) if act == "swiglu" else zr[0]
+    ck = pkg.LinearCheckpoint(x8, xs, None if act == "none" else z8 if act == "swiglu" else z8[0],
+                              None if act == "none" else zs if act == "swiglu" else zs[0], act)
+    if act == "none":
+        zr = z
+    o = n // 2 if act == "swiglu" else n
+    dy = torch.randint(-8, 9, (m, o), generator=g, device="cuda").double() / 8
+    got = pkg.linear_backward(dy.float(), ck, w.to(BF), need_bias=True, grad_dtype=F32)
+    h = 1e-4
+
+    def f(dz):      # the loss along a change of the pre-activation, from the checkpoint's own point
+        return (act64(zr + dz, act) * dy).sum()
+
+    for name, grad, shape, change in (("x", got.x, (m, k), lambda d: d @ w.t()), ("weight", got.weight, (n, k), lambda d: x @ d.t()),
+                                      ("bias", got.bias, (n,), lambda d: d.expand(m, n))):
+        for t in range(6):
+            d = torch.randn(shape, generator=g, device="cuda", dtype=torch.float64)
+            dz = change(d)
+            diff = (f(h * dz) - f(-h * dz)) / (2 * h)
+            # third derivatives of the activations are below 2 (times the other factor for swiglu)
+            tol = h * h * (dz.abs() ** 3).sum() * 4 + 1e-4 * (grad.double() * d).abs().sum() + 1e-9
+            assert abs(float((grad.double() * d).sum() - diff)) <= float(tol), (act, name)
+
+
+def test_backward_refusals_and_empty(pkg):
+    x, w = randn(4, 64), randn(32, 64)
+    y, ck = pkg.linear_checkpointed(x, w, activation="silu")
+    dy = torch.ones_like(y)
+    for dt in (BF, F32):
+        e = pkg.LinearCheckpoint(ck.x[:0], ck.x_scale[:, :0], ck.z[:0], ck.z_scale[:, :0], "silu")
+        g = pkg.linear_backward(dy[:0], e, w, need_bias=True, grad_dtype=dt)
+        assert g.x.shape == (0, 64) and not g.weight.any() and not g.bias.any() and g.weight.shape == (32, 64)
+    for args in ((dy[:3], ck, w), (dy.half(), ck, w), (dy, ck, w[:, :32]), (dy, ck, w.float()), (dy.cpu(), ck, w),
+                 (dy, ck._replace(z=None), w), (dy, ck._replace(z_scale=ck.x_scale[:, :2]), w), (dy, ck._replace(x=ck.z), w),
+                 (dy, ck._replace(activation="swiglu"), w), (dy, ck._replace(activation="x"), w)):
+        with pytest.raises(ValueError):
+            pkg.linear_backward(*args)
+    with pytest.raises(ValueError):
+        pkg.linear_backward(dy, ck, w, grad_dtype=torch.float16)
+
+
+# --------------------------------------------------------------------------------- streams, graphs, devices
+@pytest.mark.parametrize("m", [3, 300])
+def test_streams_and_graphs(pkg, m):
+    """Calls on two side streams at once, and two captured graphs replayed together, give the eager results."""
+    xs = [randn(m, 1024, seed=s) for s in (1, 2)]
+    w = randn(512, 1024, seed=3, scale=0.03)
+    dys = [randn(m, 256, seed=s) for s in (4, 5)]
+
+    def step(i):
+        y, ck = pkg.linear_checkpointed(xs[i], w, activation="swiglu")
+        return (y, *pkg.linear_backward(dys[i], ck, w, need_bias=True))
+
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = step(i)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
+    graphs, outs = [], []
+    for i, st in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            outs.append(step(i))
+        graphs.append(g)
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+    xs[0].copy_(xs[1])
+    dys[0].copy_(dys[1])
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs[0], want[1]))
