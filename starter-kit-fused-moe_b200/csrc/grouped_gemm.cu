@@ -36,6 +36,7 @@
 //          reductions (cp.reduce.async.bulk .add.f32), so the top-k combine
 //          happens here, with no separate reduce pass, and overlaps the next
 //          tile's main loop.
+#include "cta_pair.cuh"
 #include "moe_common.cuh"
 #include "moe_kernels.h"
 #include "moe_workspace.h"
@@ -159,35 +160,6 @@ static_assert(num_stages<1, true>() <= MAX_STAGES && num_stages<2, true>() <= MA
 static_assert(GemmCfg<1>::STAGES <= MAX_STAGES && GemmCfg<2>::STAGES <= MAX_STAGES, "barrier arrays");
 static_assert(GemmCfg<1>::SK == 128 && GemmCfg<2>::SK == 128, "the CTA-pair tiles assume 128-wide stages");
 
-// ---- cluster / CTA-pair primitives
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_id() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-  return r;
-}
-// Address of the same shared variable in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// TMA load into this CTA's shared memory whose completion is counted on an
-// mbarrier of either CTA of the pair (cluster address). No multicast.
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar_cluster, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster), "r"(x), "r"(y)
-      : "memory");
-}
 __device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                               uint32_t accumulate) {
   asm volatile(
@@ -195,21 +167,6 @@ __device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, u
       "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-// Arrives once on the mbarrier at this offset in both CTAs of the pair when the
-// leader's issued tcgen05 operations are done.
-__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                   bar), "h"((uint16_t)3)
-               : "memory");
-}
-// Arrive on an mbarrier of the other CTA of the pair (default semantics). The
-// epilogue uses it to hand a TMEM buffer back to the leader's MMA after
-// tcgen05.wait::ld and tcgen05.fence::before_thread_sync; a cluster-scope
-// release here cost ~900 cycles per K-block (measured) and orders nothing the
-// tcgen05 fences do not already order.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 static_assert((GemmCfg<1>::SK == 128 || GemmCfg<1>::SK == 64) && (GemmCfg<2>::SK == 128 || GemmCfg<2>::SK == 64),
               "stage K width");

@@ -1,0 +1,573 @@
+// Dense bf16 products on tcgen05: D[m, n] = sum_k A(m, k) B(n, k), fp32
+// accumulation, with the epilogues of a layer.
+//
+//   forward      A = x   (K-major)     B = W   (K-major)    y = act(D + b) + r, z kept in 8 bits
+//   grad_x       A = dz  (K-major)     B = W   (N-major: contraction over W's rows)
+//   grad_weight  A = dz  (M-major)     B = x^  (N-major: contraction over the tokens)
+//
+// A pair of CTAs (a two-CTA cluster, tcgen05 cta_group::2) computes a 256-row
+// tile of NT columns: each CTA loads its own 128 rows of A and NT / 2 of B's
+// rows, 64 of K per stage, so a stage is at most 32 KB per SM and the operand
+// stream (a single CTA with the same tile needs 48 KB per stage) stays below
+// what an SM takes in from L2 (68 bytes per cycle measured) while the MMA runs
+// at full rate: 512 cycles per 64 of K at NT = 256. Operands arrive by TMA in
+// the 128-byte swizzle, in whichever of the two majors they lie in memory, so
+// nothing is transposed. dz may come as several bf16 terms (see act_grad.cu):
+// the contraction then runs over the terms one after the other with B's
+// coordinates repeating.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (the leader CTA's), 2-9 epilogue. Two
+// accumulators of NT columns in TMEM let a tile's epilogue overlap the next
+// tile's products. Persistent grid, one pair per two SMs; tiles are walked in
+// bands of 8 row tiles so that the tiles in flight share both operands in L2.
+// When there are fewer tiles than pairs, K is split: every slice leaves its
+// fp32 partial tile in the workspace and the slice that arrives last adds them
+// in slice order (so the result does not depend on who was last) and runs the
+// epilogue; no CTA waits for another one's slice.
+//
+// Every wait is bounded (2 s). One that runs out makes the kernel write NaN to
+// the tiles it still owes, so a failed call never returns plausible numbers.
+#include "cta_pair.cuh"
+#include "linear_tile.h"
+#include "train_common.cuh"
+
+namespace moe {
+
+constexpr int kLtStages = 6, kLtStageBytes = 32768, kLtTileA = 16384;
+constexpr int kLtThreads = 320, kLtEpiWarps = 8, kLtTmemCols = 512;
+constexpr int kLtBand = 8;
+
+struct LinearTileSmem {
+  uint64_t full[kLtStages];
+  uint64_t empty[kLtStages];
+  uint64_t tfull[2];
+  uint64_t tempty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  int last;
+  float amax[2][2][2][128];      // [tile parity][column half][gate, up][row]
+};
+constexpr size_t kLtSmem = 1024 + (size_t)kLtStages * kLtStageBytes + sizeof(LinearTileSmem);
+static_assert(kLtSmem <= 232448, "shared memory budget");
+
+// bf16 x bf16 -> f32, M = 256 over the pair; a_mn / b_mn: operand stored with M / N innermost.
+__device__ __forceinline__ uint32_t idesc_bf16(int n, int a_mn, int b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+}
+// Descriptor of an M- or N-major operand in the 128-byte swizzle: 64 values of
+// M (N) by 8 of K make a 1024-byte group; the next 8 of K follow (stride 1024),
+// the next 64 of M are 64 K-rows (8192 bytes) away.
+__device__ __forceinline__ uint64_t sdesc_sw128_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)(8192 >> 4) << 16;    // LBO: next 64 of M / N
+  d |= (uint64_t)(1024 >> 4) << 32;    // SBO: next 8 of K
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+__device__ __forceinline__ void mma_bf16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar_cluster, int x, int y,
+                                                 int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+struct LtUnit {
+  int mt, nt, kb0, kb1, slice;
+  int64_t tile;
+};
+__device__ __forceinline__ LtUnit lt_unit(const LinearTileArgs& a, int64_t u) {
+  LtUnit r;
+  r.tile = u / a.splits;
+  r.slice = (int)(u - r.tile * a.splits);
+  const int64_t per_band = (int64_t)kLtBand * a.n_tiles;
+  const int band = (int)(r.tile / per_band);
+  const int64_t in = r.tile - band * per_band;
+  const int rows = min(kLtBand, a.m_tiles - band * kLtBand);
+  r.nt = (int)(in / rows);
+  r.mt = band * kLtBand + (int)(in - (int64_t)r.nt * rows);
+  r.kb0 = (int)((int64_t)r.slice * a.k_blocks / a.splits);
+  r.kb1 = (int)((int64_t)(r.slice + 1) * a.k_blocks / a.splits);
+  return r;
+}
+
+// ---- epilogue pieces, 16 columns of one row per thread
+__device__ __forceinline__ void lt_bias16(const __nv_bfloat16* bias, int64_t c, int64_t end, float* v) {
+  if (c + 16 <= end && (reinterpret_cast<uintptr_t>(bias + c) & 15) == 0) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(bias + c)), b = __ldg(reinterpret_cast<const uint4*>(bias + c) + 1);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = unpack_bf16(w[i]);
+      v[2 * i] += f.x;
+      v[2 * i + 1] += f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c + i < end) v[i] += __bfloat162float(bias[c + i]);
+  }
+}
+__device__ __forceinline__ void lt_act16(float* v, int act) {
+  if (act == kActNone) return;
+  if (act == kActRelu) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = act_value(v[i], kActRelu);
+  } else if (act == kActGelu) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = act_value(v[i], kActGelu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = act_value(v[i], kActSilu);
+  }
+}
+// y[row, c .. c + 16) = v + residual (columns below `end` only). The residual is
+// read before the same values of y are written by the same thread, so y may be
+// the residual.
+__device__ __forceinline__ void lt_store16(const LinearEpilogue& ep, int vec, int64_t row, int64_t c, int64_t end, float* v) {
+  const bool whole = vec && c + 16 <= end;
+  if (ep.residual != nullptr) {
+    const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr + c;
+    if (whole) {
+      const uint4 a = *reinterpret_cast<const uint4*>(r), b = *(reinterpret_cast<const uint4*>(r) + 1);
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = unpack_bf16(w[i]);
+        v[2 * i] += f.x;
+        v[2 * i + 1] += f.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c + i < end) v[i] += __bfloat162float(r[i]);
+    }
+  }
+  if (ep.y_f32) {
+    float* y = static_cast<float*>(ep.y) + row * ep.ldy + c;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(y)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c + i < end) y[i] = v[i];
+    }
+  } else {
+    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(ep.y) + row * ep.ldy + c;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        reinterpret_cast<uint4*>(y)[i] = make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+                                                    pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c + i < end) y[i] = __float2bfloat16_rn(v[i]);
+    }
+  }
+}
+// Largest magnitude (as bits) of the columns below `end`.
+__device__ __forceinline__ uint32_t lt_amax16(const float* v, int64_t c, int64_t end, uint32_t amax) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (c + i < end) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+  return amax;
+}
+__device__ __forceinline__ void lt_store_z16(uint8_t* z, int64_t c, int64_t end, const float* v, uint32_t code) {
+  const float inv = e8m0_inverse(code);
+  float s[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = code == kTopScaleCode ? hold_finite(v[i] * inv) : v[i] * inv;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = e4m3x4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+  if (c + 16 <= end && (reinterpret_cast<uintptr_t>(z + c) & 15) == 0) {
+    *reinterpret_cast<uint4*>(z + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c + i < end) z[c + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+  }
+}
+
+template <bool A_MN, bool B_MN, bool GATED, bool KEEP>
+__global__ void __launch_bounds__(kLtThreads, 1)
+    linear_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, LinearTileArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  LinearTileSmem& S = *reinterpret_cast<LinearTileSmem*>(smem + kLtStages * kLtStageBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int crank = (int)cluster_rank();
+  const int64_t wid = cluster_id(), G = gridDim.x / 2;
+  const int NT = a.n_tile, H = NT / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kLtStages; ++s) {
+      mbar_init(smem_u32(&S.full[s]), 1);
+      mbar_init(smem_u32(&S.empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&S.tfull[b]), 1);
+      mbar_init(smem_u32(&S.tempty[b]), 2 * kLtEpiWarps);      // both CTAs' epilogues (the leader's copy)
+    }
+    S.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem_base)),
+                 "r"(kLtTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t tmem_base = S.tmem_base;
+  volatile int* abort_flag = &S.abort_flag;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      const uint32_t bytes = 2 * (kLtTileA + H * 128);
+      for (int64_t u = wid; u < a.units && ok && !*abort_flag; u += G) {
+        const LtUnit x = lt_unit(a, u);
+        const int m0 = x.mt * 256 + crank * 128;
+        // B rows of this CTA's half: the next H columns of the tile, or for a gated tile its first-half
+        // (leader) and second-half (peer) rows
+        const int n0 = GATED ? crank * a.gate_rows + x.nt * H : x.nt * NT + crank * H;
+        for (int kb = x.kb0; kb < x.kb1; ++kb, ++it) {
+          const int s = it % kLtStages;
+          if (!mbar_wait(smem_u32(&S.empty[s]), ((it / kLtStages) & 1) ^ 1)) {
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          const uint32_t fb = smem_u32(&S.full[s]);
+          const uint32_t fbl = mapa_shared(fb, 0);
+          const uint32_t sa = smem_u32(smem + s * kLtStageBytes), sb = sa + kLtTileA;
+          const int term = kb / a.term_blocks, kt = (kb - term * a.term_blocks) * 64;
+          if (crank == 0) mbar_arrive_expect_tx(fb, bytes);
+          if constexpr (A_MN) {
+            tma_load_3d_pair(sa, &tmA, fbl, m0, kt, term);
+            tma_load_3d_pair(sa + 8192, &tmA, fbl, m0 + 64, kt, term);
+          } else {
+            tma_load_3d_pair(sa, &tmA, fbl, kt, m0, term);
+          }
+          if constexpr (B_MN) {
+            tma_load_2d_pair(sb, &tmB, fbl, n0, kt);
+            if (H == 128) tma_load_2d_pair(sb + 8192, &tmB, fbl, n0 + 64, kt);
+          } else {
+            tma_load_2d_pair(sb, &tmB, fbl, kt, n0);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader)
+    if (lane == 0 && crank == 0) {
+      const uint32_t idesc = idesc_bf16(NT, A_MN, B_MN);
+      int it = 0, tt = 0;
+      bool ok = true;
+      for (int64_t u = wid; u < a.units && ok && !*abort_flag; u += G, ++tt) {
+        const LtUnit x = lt_unit(a, u);
+        const int b = tt & 1;
+        if (!mbar_wait(smem_u32(&S.tempty[b]), ((tt >> 1) & 1) ^ 1)) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + (uint32_t)(b * 256);
+        for (int kb = x.kb0; kb < x.kb1; ++kb, ++it) {
+          const int s = it % kLtStages;
+          if (!mbar_wait(smem_u32(&S.full[s]), (it / kLtStages) & 1)) {
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * kLtStageBytes), sb = sa + kLtTileA;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint64_t da = A_MN ? sdesc_sw128_mn(sa + kk * 2048) : sdesc_sw128(sa + kk * 32);
+            const uint64_t db = B_MN ? sdesc_sw128_mn(sb + kk * 2048) : sdesc_sw128(sb + kk * 32);
+            mma_bf16_pair(d, da, db, idesc, (kb > x.kb0 || kk) ? 1u : 0u);
+          }
+          mma_commit_pair(smem_u32(&S.empty[s]));
+        }
+        if (ok) mma_commit_pair(smem_u32(&S.tfull[b]));
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3, g = (warp - 2) >> 2;
+    const int r = 32 * q + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
+    const LinearEpilogue& ep = a.ep;
+    const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(ep.bias);
+    const int64_t O = a.out_cols;
+    const int64_t z_blocks = (O + 127) / 128;
+    bool ok = true;
+    int tt = 0;
+    for (int64_t u = wid; u < a.units; u += G, ++tt) {
+      const LtUnit x = lt_unit(a, u);
+      const int b = tt & 1;
+      if (ok && (*abort_flag || !mbar_wait(smem_u32(&S.tfull[b]), (tt >> 1) & 1))) {
+        *abort_flag = 1;
+        ok = false;
+      }
+      tc_fence_after();
+      const uint32_t acc = lane_addr + (uint32_t)(b * 256);
+      const int64_t row = (int64_t)x.mt * 256 + crank * 128 + r;
+      const bool valid = row < a.m;
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&S.tempty[b]), 0));
+      };
+      auto from_tmem = [&](int col, float* v) {
+        if (ok) {
+          tmem_ld16(acc + col, v);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = NAN;
+        }
+      };
+      const bool split = a.splits > 1;
+      // this CTA's half of the tile's slices, [slice][column][row]
+      float* part = split ? a.partial + ((x.tile * a.splits) * 2 + crank) * (int64_t)(NT * 128) + r : nullptr;
+      const int64_t part_step = (int64_t)2 * NT * 128;
+      if (split) {
+        const int w = NT / 2;
+        float* mine = part + x.slice * part_step;
+        for (int c = g * w; c < (g + 1) * w; c += 16) {
+          float v[16];
+          from_tmem(c, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) __stcg(mine + (int64_t)(c + i) * 128, v[i]);
+        }
+        release();
+        __threadfence();
+        named_barrier_sync(1, kLtEpiWarps * 32);
+        if (warp == 2 && lane == 0) S.last = atomicAdd(a.arrivals + x.tile * 2 + crank, 1) == a.splits - 1;
+        named_barrier_sync(1, kLtEpiWarps * 32);
+        const bool last = S.last;
+        named_barrier_sync(1, kLtEpiWarps * 32);       // S.last may be written again
+        if (!last) continue;
+        __threadfence();
+      }
+      auto load = [&](int col, float* v) {
+        if (!split) {
+          from_tmem(col, v);
+          return;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __ldcg(part + (int64_t)(col + i) * 128);
+        for (int s = 1; s < a.splits; ++s)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] += __ldcg(part + s * part_step + (int64_t)(col + i) * 128);
+      };
+
+      if constexpr (!GATED) {
+        const int64_t c_tile = (int64_t)x.nt * NT;
+        uint32_t code = 0;
+        if constexpr (KEEP) {                            // NT = 256: this warp's half is one block of the row
+          uint32_t amax = 0;
+          for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 16) {
+            float v[16];
+            load(c, v);
+            if (bias) lt_bias16(bias, c_tile + c, O, v);
+            amax = lt_amax16(v, c_tile + c, O, amax);
+          }
+          code = e8m0_of_amax(amax);
+          if (valid && c_tile + g * H < O) ep.z_scale[((c_tile >> 7) + g) * a.m + row] = (uint8_t)code;
+        }
+        for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 16) {
+          float v[16];
+          load(c, v);
+          if (bias) lt_bias16(bias, c_tile + c, O, v);
+          if (valid) {
+            if constexpr (KEEP) lt_store_z16(ep.z8 + row * O, c_tile + c, O, v, code);
+            lt_act16(v, ep.act);
+            lt_store16(ep, a.vec, row, c_tile + c, O, v);
+          }
+        }
+      } else {
+        const int w = H / 2;                             // columns of each half per warp
+        const int64_t c_tile = (int64_t)x.nt * H;
+        uint32_t code[2] = {0, 0};
+        if constexpr (KEEP) {                            // NT = 256: a block of each half per tile, shared by two warps
+          uint32_t amax[2] = {0, 0};
+          for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 16)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float v[16];
+              load(h * H + c, v);
+              if (bias) lt_bias16(bias + h * O, c_tile + c, O, v);
+              amax[h] = lt_amax16(v, c_tile + c, O, amax[h]);
+            }
+          S.amax[tt & 1][g][0][r] = __uint_as_float(amax[0]);
+          S.amax[tt & 1][g][1][r] = __uint_as_float(amax[1]);
+          named_barrier_sync(2 + q, 64);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            code[h] = e8m0_of_amax(max(amax[h], __float_as_uint(S.amax[tt & 1][g ^ 1][h][r])));
+            if (valid && g == 0 && c_tile < O) ep.z_scale[(h * z_blocks + (c_tile >> 7)) * a.m + row] = (uint8_t)code[h];
+          }
+        }
+        for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 16) {
+          float v[16], t[16];
+          load(c, v);
+          load(H + c, t);
+          if (bias) {
+            lt_bias16(bias, c_tile + c, O, v);
+            lt_bias16(bias + O, c_tile + c, O, t);
+          }
+          if (valid) {
+            if constexpr (KEEP) {
+              lt_store_z16(ep.z8 + row * O, c_tile + c, O, v, code[0]);
+              lt_store_z16(ep.z8 + (a.m + row) * O, c_tile + c, O, t, code[1]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] *= act_value(t[i], kActSilu);
+            lt_store16(ep, a.vec, row, c_tile + c, O, v);
+          }
+        }
+      }
+      if (!split) release();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();      // neither CTA leaves while the other may still signal its barriers
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kLtTmemCols) : "memory");
+  }
+}
+
+// Row-padded copy of a matrix whose rows TMA cannot read (bases and row strides
+// must be multiples of 16 bytes).
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ src, int64_t lds, int64_t rows,
+                                                       int cols, uint16_t* __restrict__ dst, int64_t ldd) {
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  for (int c = 4 * (blockIdx.y * 256 + threadIdx.x); c < cols; c += 4 * 256 * gridDim.y) {
+    const uint16_t* s = src + row * lds + c;
+    uint16_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i < cols ? s[i] : 0;
+    *reinterpret_cast<uint2*>(dst + row * ldd + c) =
+        make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+  }
+}
+cudaError_t launch_pad_rows(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst, int64_t ldd,
+                            cudaStream_t st) {
+  if (rows == 0) return cudaSuccess;
+  const int gy = ceil_div(cols, 1024) < 8 ? ceil_div(cols, 1024) : 8;
+  pad_rows_kernel<<<dim3((unsigned)rows, gy), 256, 0, st>>>(static_cast<const uint16_t*>(src), lds, rows, (int)cols,
+                                                            static_cast<uint16_t*>(dst), ldd);
+  return cudaGetLastError();
+}
+
+// Tile width and K slices. Cycles per 64 of K and pair, measured on this
+// kernel's main loop: the MMA (2 NT) or the SM's operand intake (16 KB + 64 NT
+// bytes at 68 per cycle); a tile's epilogue hides behind the next tile's
+// products except for the last round. Slices are at least 4 K-blocks deep.
+LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs) {
+  LinearTilePlan best{};
+  double best_cost = 1e300;
+  const int64_t mt = (m + 255) / 256;
+  static const int widths[] = {256, 224, 192, 160, 128};
+  for (int nt : widths) {
+    if (keep && nt != 256) continue;
+    if ((gated && nt % 64) || (b_mn && nt % 128)) continue;
+    const int64_t cols = gated ? nt / 2 : nt;
+    const int64_t tiles = mt * ((n + cols - 1) / cols);
+    const double block = 2.0 * nt + 16 > 241 + 0.94 * nt ? 2.0 * nt + 16 : 241 + 0.94 * nt;
+    for (int s = 1; s <= 16; ++s) {
+      if (s > 1 && (k_blocks < 4 * s || tiles * s > pairs)) break;
+      const int64_t rounds = (tiles * s + pairs - 1) / pairs;
+      const double cost = (double)rounds * ((k_blocks + s - 1) / s) * block + 1500 + 8.0 * nt + (s > 1 ? 1500 + 300.0 * s : 0);
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = {nt, s, tiles};
+      }
+    }
+  }
+  return best;
+}
+
+template <bool A_MN, bool B_MN, bool GATED, bool KEEP>
+static cudaError_t launch_t(const CUtensorMap& tmA, const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms,
+                            cudaStream_t st) {
+  static int clusters_of[64];
+  auto kern = linear_tile_kernel<A_MN, B_MN, GATED, KEEP>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.blockDim = dim3(kLtThreads);
+  cfg.dynamicSmemBytes = kLtSmem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = dev < 64 ? clusters_of[dev] : 0;
+  if (clusters == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLtSmem);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(num_sms & ~1);
+    e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+    if (e != cudaSuccess || clusters < 1) return e != cudaSuccess ? e : cudaErrorInvalidConfiguration;
+    if (clusters > num_sms / 2) clusters = num_sms / 2;
+    if (dev < 64) clusters_of[dev] = clusters;
+  }
+  const int64_t want = a.units < clusters ? a.units : clusters;
+  cfg.gridDim = dim3((unsigned)(2 * want));
+  cfg.stream = st;
+  return cudaLaunchKernelEx(&cfg, kern, tmA, tmB, a);
+}
+
+cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
+                               const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+  if (a_mn && b_mn) return launch_t<true, true, false, false>(tmA, tmB, a, num_sms, st);
+  if (b_mn) return launch_t<false, true, false, false>(tmA, tmB, a, num_sms, st);
+  if (gated) return keep ? launch_t<false, false, true, true>(tmA, tmB, a, num_sms, st)
+                         : launch_t<false, false, true, false>(tmA, tmB, a, num_sms, st);
+  return keep ? launch_t<false, false, false, true>(tmA, tmB, a, num_sms, st)
+              : launch_t<false, false, false, false>(tmA, tmB, a, num_sms, st);
+}
+
+cudaError_t set_debug_waits_linear(unsigned long long limit_ns, int gate_extra) {
+  return set_debug_waits_here(limit_ns, gate_extra);
+}
+
+}  // namespace moe

@@ -94,6 +94,22 @@ int check_workspace(void* ws, size_t bytes, int T, int E) {
 
 void moe::set_last_error(const char* msg) { g_last_error = msg; }
 
+int moe::current_device_sms() { return num_sms_of_current_device(); }
+
+bool moe::encode_bf16(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride,
+                      uint64_t planes, uint64_t plane_stride, uint32_t box_cols, uint32_t box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return false;
+  const int rank = planes ? 3 : 2;
+  cuuint64_t dims[3] = {cols, rows, planes};
+  cuuint64_t strides[2] = {2 * row_stride, 2 * plane_stride};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 extern "C" {
 
 const char* moe_fp8_last_error(void) { return g_last_error.c_str(); }
@@ -483,6 +499,7 @@ int moe_fp8_debug_set_waits(uint64_t wait_limit_ns, int32_t gate_extra) {
   cudaError_t e = moe::set_debug_waits_stream(wait_limit_ns, gate_extra);
   if (e == cudaSuccess) e = moe::set_debug_waits_tile(wait_limit_ns, gate_extra);
   if (e == cudaSuccess) e = moe::set_debug_waits_ep(wait_limit_ns, gate_extra);
+  if (e == cudaSuccess) e = moe::set_debug_waits_linear(wait_limit_ns, gate_extra);
   return e == cudaSuccess ? MOE_OK : cuda_fail(e, "debug_set_waits");
 }
 

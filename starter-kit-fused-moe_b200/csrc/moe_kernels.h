@@ -79,6 +79,13 @@ cudaError_t launch_quantize(const void* x, bool bf16, int T, uint8_t* q, float* 
 cudaError_t set_debug_waits_stream(unsigned long long limit_ns, int gate_extra);
 cudaError_t set_debug_waits_tile(unsigned long long limit_ns, int gate_extra);
 cudaError_t set_debug_waits_ep(unsigned long long limit_ns, int gate_extra);
+cudaError_t set_debug_waits_linear(unsigned long long limit_ns, int gate_extra);
+// SMs of the current device (0 without one).
+int current_device_sms();
+// bf16 tensor map [planes][rows][cols] (rank 2 when planes is 0; strides in
+// elements, multiples of 8), boxes of box_rows x box_cols in the 128-byte swizzle.
+bool encode_bf16(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride, uint64_t planes,
+                 uint64_t plane_stride, uint32_t box_cols, uint32_t box_rows);
 // Text returned by moe_fp8_last_error() on the calling thread.
 void set_last_error(const char* msg);
 cudaError_t set_trace(int on);

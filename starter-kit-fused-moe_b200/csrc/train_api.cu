@@ -4,6 +4,7 @@
 #include <cstdio>
 
 #include "moe_fp8.h"
+#include "linear_tile.h"
 #include "moe_kernels.h"
 #include "train_kernels.h"
 
@@ -40,29 +41,130 @@ int check_sizes(int64_t m, int64_t k, int64_t n, int act) {
   return MOE_OK;
 }
 
-// Workspace of the gradient entry.
+int pairs() {
+  const int n = moe::current_device_sms();
+  return n >= 2 ? n / 2 : 74;
+}
+// TMA reads a matrix in place if its base and row stride are multiples of 16 bytes.
+bool tma_ready(const void* p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0; }
+
+// One tensor-core product: its tile plan and the workspace of its K slices.
+struct Product {
+  moe::LinearTilePlan plan;
+  int64_t term_blocks;
+  int terms;
+  size_t arrivals, partial, bytes;      // arrivals first
+};
+Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gated, bool keep, bool b_mn) {
+  Product p{};
+  p.term_blocks = (k + 63) / 64;
+  p.terms = terms;
+  p.plan = moe::plan_linear_tile(m, out_cols, p.term_blocks * terms, gated, keep, b_mn, pairs());
+  if (p.plan.splits > 1) {
+    p.arrivals = up256((size_t)p.plan.tiles * 2 * sizeof(int));
+    p.partial = (size_t)p.plan.tiles * p.plan.splits * 2 * p.plan.n_tile * 128 * sizeof(float);
+    p.bytes = p.arrivals + p.partial;
+  }
+  return p;
+}
+// A: [terms][rows][..], term stride in elements; the K slices' arrivals must be zero.
+int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, int64_t m, int64_t out_cols, int64_t k,
+                const void* A, int64_t lda, int64_t term_stride, const void* B, int64_t ldb, int64_t b_rows,
+                const moe::LinearEpilogue& ep, uint8_t* arrivals, uint8_t* partial, cudaStream_t st, const char* what) {
+  moe::LinearTileArgs t{};
+  t.m = m;
+  t.out_cols = out_cols;
+  t.gate_rows = gated ? (int)out_cols : 0;
+  t.n_tile = p.plan.n_tile;
+  const int cols = gated ? t.n_tile / 2 : t.n_tile;
+  t.m_tiles = moe::ceil_div(m, 256);
+  t.n_tiles = moe::ceil_div(out_cols, cols);
+  t.term_blocks = (int)p.term_blocks;
+  t.k_blocks = t.term_blocks * p.terms;
+  t.splits = p.plan.splits;
+  t.units = p.plan.tiles * t.splits;
+  t.ep = ep;
+  const int ysize = ep.y_f32 ? 4 : 2;
+  t.vec = aligned(ep.y, 16) && ep.ldy * ysize % 16 == 0 && (!ep.residual || (aligned(ep.residual, 16) && ep.ldr % 8 == 0));
+  t.arrivals = reinterpret_cast<int*>(arrivals);
+  t.partial = reinterpret_cast<float*>(partial);
+  CUtensorMap ma, mb;
+  const uint32_t half = (uint32_t)t.n_tile / 2;
+  const bool ok = (a_mn ? moe::encode_bf16(&ma, A, m, k, lda, p.terms, term_stride, 64, 64)
+                        : moe::encode_bf16(&ma, A, k, m, lda, p.terms, term_stride, 64, 128)) &&
+                  (b_mn ? moe::encode_bf16(&mb, B, out_cols, k, ldb, 0, 0, 64, 64)
+                        : moe::encode_bf16(&mb, B, k, b_rows, ldb, 0, 0, 64, half));
+  if (!ok) {
+    moe::set_last_error("cuTensorMapEncodeTiled failed");
+    return MOE_ERR_CUDA;
+  }
+  return done(moe::launch_linear_tile(a_mn, b_mn, gated, keep, ma, mb, t, 2 * pairs(), st), what);
+}
+
+// Workspace of a forward product.
+struct LinearPlan {
+  Product prod;
+  bool pad_x, pad_w;
+  int64_t ldp;
+  size_t x, w, total;
+};
+LinearPlan linear_plan(const MoeLinearArgs& a) {
+  LinearPlan p{};
+  const bool gated = a.activation == MOE_ACT_SWIGLU;
+  p.prod = plan_product(a.m, gated ? a.n / 2 : a.n, a.k, 1, gated, a.z8 != nullptr, false);
+  p.pad_x = !tma_ready(a.x, a.ldx);
+  p.pad_w = !tma_ready(a.weight, a.ldw);
+  p.ldp = up8(a.k);
+  size_t o = up256(p.prod.bytes);
+  p.x = o;
+  if (p.pad_x) o += up256((size_t)a.m * p.ldp * 2);
+  p.w = o;
+  if (p.pad_w) o += up256((size_t)a.n * p.ldp * 2);
+  p.total = o;
+  return p;
+}
+
+// Workspace of the gradient entry: K-slice arrivals and partials of both
+// products (the partials shared), dz, x^, the padded weights, column sums.
 struct GradPlan {
-  bool need_dz, two_terms;
-  int chunks;
+  bool need_dz, direct, pad_w;
+  int terms, chunks;
   int64_t ldz, ldk;
-  size_t dz, xhat, colsum, tmp, total;
+  Product px, pw;
+  size_t arrivals, partial, dz, xhat, w, colsum, total;
 };
 GradPlan grad_plan(const MoeLinearGradArgs& a) {
   GradPlan p{};
   p.ldz = up8(a.n);
   p.ldk = up8(a.k);
-  p.two_terms = a.grad_f32 && (a.activation != MOE_ACT_NONE || a.grad_y_f32);
-  p.need_dz = a.grad_x || a.grad_weight;
+  p.terms = a.grad_f32 && (a.activation != MOE_ACT_NONE || a.grad_y_f32) ? 2 : 1;
+  // without an activation bf16 gradients are dz themselves
+  p.direct = a.activation == MOE_ACT_NONE && !a.grad_y_f32 && tma_ready(a.grad_y, a.ldg) && a.ldg >= a.n;
+  p.need_dz = (a.grad_x || a.grad_weight) && !p.direct;
   p.chunks = moe::act_grad_chunks(a.m, a.n);
-  size_t o = 0;
+  size_t partial = 0;
+  if (a.grad_x) {
+    p.px = plan_product(a.m, a.k, a.n, p.terms, false, false, true);
+    p.arrivals += p.px.arrivals;
+    partial = p.px.partial;
+    p.pad_w = !tma_ready(a.weight, a.ldw);
+  }
+  if (a.grad_weight) {
+    p.pw = plan_product(a.n, a.k, a.m, p.terms, false, false, true);
+    p.arrivals += p.pw.arrivals;
+    if (p.pw.partial > partial) partial = p.pw.partial;
+  }
+  size_t o = p.arrivals;
+  p.partial = o;
+  o += up256(partial);
   p.dz = o;
-  if (p.need_dz) o += up256((size_t)a.m * p.ldz * 2 * (p.two_terms ? 2 : 1));
+  if (p.need_dz) o += up256((size_t)a.m * p.ldz * 2 * p.terms);
   p.xhat = o;
   if (a.grad_weight) o += up256((size_t)a.m * p.ldk * 2);
+  p.w = o;
+  if (p.pad_w) o += up256((size_t)a.n * p.ldk * 2);
   p.colsum = o;
   if (a.grad_bias) o += up256((size_t)p.chunks * a.n * 4);
-  p.tmp = o;
-  o += up256((size_t)(a.grad_x ? a.m : 0) * a.k * 4) + up256((size_t)(a.grad_weight ? a.n : 0) * a.k * 4);
   p.total = o;
   return p;
 }
@@ -72,8 +174,8 @@ GradPlan grad_plan(const MoeLinearGradArgs& a) {
 extern "C" {
 
 size_t moe_linear_workspace_bytes(const MoeLinearArgs* a) {
-  if (!a || a->m <= 0 || a->n <= 0) return 0;
-  return up256((size_t)a->m * a->n * 4);
+  if (!a || a->m <= 0 || a->n <= 0 || a->k <= 0) return 0;
+  return linear_plan(*a).total;
 }
 
 int moe_linear_run(const MoeLinearArgs* a, void* stream) {
@@ -88,16 +190,23 @@ int moe_linear_run(const MoeLinearArgs* a, void* stream) {
     return bad("linear: a pointer is not aligned to its type");
   if (a->ldx < a->k || a->ldw < a->k || a->ldy < O || (a->residual && a->ldr < 0))
     return bad("linear: a row stride is smaller than the row");
-  const size_t need = moe_linear_workspace_bytes(a);
-  if (need && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need))
-    return workspace_error("linear", need, a->workspace_bytes);
+  const LinearPlan p = linear_plan(*a);
+  if (p.total && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < p.total))
+    return workspace_error("linear", p.total, a->workspace_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* z = static_cast<float*>(a->workspace);
-  cudaError_t e = moe::launch_simple_gemm(a->x, a->ldx, 1, a->weight, a->ldw, 1, a->m, a->n, a->k, false, z, st);
-  if (e != cudaSuccess) return done(e, "linear product");
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  cudaError_t e = cudaSuccess;
+  if (p.prod.plan.splits > 1) e = cudaMemsetAsync(ws, 0, p.prod.arrivals, st);
+  if (e == cudaSuccess && p.pad_x) e = moe::launch_pad_rows(a->x, a->ldx, a->m, a->k, ws + p.x, p.ldp, st);
+  if (e == cudaSuccess && p.pad_w) e = moe::launch_pad_rows(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldp, st);
+  if (e != cudaSuccess) return done(e, "linear: preparing the operands");
   moe::LinearEpilogue ep{a->bias, a->residual, a->y, static_cast<uint8_t*>(a->z8), static_cast<uint8_t*>(a->z_scale),
                          a->ldr, a->ldy, a->activation, a->y_f32};
-  return done(moe::launch_simple_epilogue(z, a->m, a->n, ep, st), "linear epilogue");
+  const void* x = p.pad_x ? ws + p.x : a->x;
+  const void* w = p.pad_w ? ws + p.w : a->weight;
+  const int64_t ldx = p.pad_x ? p.ldp : a->ldx;
+  return run_product(p.prod, false, false, a->activation == MOE_ACT_SWIGLU, a->z8 != nullptr, a->m, O, a->k, x, ldx,
+                     a->m * ldx, w, p.pad_w ? p.ldp : a->ldw, a->n, ep, ws, ws + p.prod.arrivals, st, "linear product");
 }
 
 size_t moe_linear_grad_workspace_bytes(const MoeLinearGradArgs* a) {
@@ -128,47 +237,56 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
     return bad("linear gradient: a pointer is not aligned to its type");
   if (a->ldg < 0 || (a->grad_x && a->ldw < a->k)) return bad("linear gradient: a row stride is smaller than the row");
   const GradPlan p = grad_plan(*a);
-  if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < p.total)
+  if (p.total && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < p.total))
     return workspace_error("linear gradient", p.total, a->workspace_bytes);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  const int terms = p.two_terms ? 2 : 1;
-  moe::ActGradArgs g{};
-  g.dy = a->grad_y;
-  g.z8 = act ? static_cast<const uint8_t*>(a->z8) : nullptr;
-  g.z_scale = static_cast<const uint8_t*>(a->z_scale);
-  g.dz = p.need_dz ? ws + p.dz : nullptr;
-  g.colsum = a->grad_bias ? reinterpret_cast<float*>(ws + p.colsum) : nullptr;
-  g.ldg = a->ldg;
-  g.ldz = p.ldz;
-  g.m = a->m;
-  g.n = a->n;
-  g.act = a->activation;
-  g.dy_f32 = a->grad_y_f32;
-  g.terms = terms;
-  cudaError_t e = moe::launch_act_grad(g, st);
-  if (e != cudaSuccess) return done(e, "activation gradient");
-  if (a->grad_bias) {
-    e = moe::launch_colsum_finish(g.colsum, p.chunks, a->n, a->grad_bias, a->grad_f32 != 0, st);
-    if (e != cudaSuccess) return done(e, "bias gradient");
+  cudaError_t e = cudaSuccess;
+  if (p.arrivals) e = cudaMemsetAsync(ws, 0, p.arrivals, st);
+  if (e != cudaSuccess) return done(e, "linear gradient: clearing the slice counters");
+  if (p.need_dz || a->grad_bias) {
+    moe::ActGradArgs g{};
+    g.dy = a->grad_y;
+    g.z8 = act ? static_cast<const uint8_t*>(a->z8) : nullptr;
+    g.z_scale = static_cast<const uint8_t*>(a->z_scale);
+    g.dz = p.need_dz ? ws + p.dz : nullptr;
+    g.colsum = a->grad_bias ? reinterpret_cast<float*>(ws + p.colsum) : nullptr;
+    g.ldg = a->ldg;
+    g.ldz = p.ldz;
+    g.m = a->m;
+    g.n = a->n;
+    g.act = a->activation;
+    g.dy_f32 = a->grad_y_f32;
+    g.terms = p.terms;
+    e = moe::launch_act_grad(g, st);
+    if (e == cudaSuccess && a->grad_bias)
+      e = moe::launch_colsum_finish(g.colsum, p.chunks, a->n, a->grad_bias, a->grad_f32 != 0, st);
+    if (e != cudaSuccess) return done(e, "activation gradient");
   }
-  float* tmp = reinterpret_cast<float*>(ws + p.tmp);
-  const uint16_t* dz = reinterpret_cast<const uint16_t*>(ws + p.dz);
+  const void* dz = p.direct ? a->grad_y : ws + p.dz;
+  const int64_t ldz = p.direct ? a->ldg : p.ldz, term_stride = a->m * ldz;
+  uint8_t* partial = ws + p.partial;
   if (a->grad_x) {
-    for (int t = 0; t < terms && e == cudaSuccess; ++t)
-      e = moe::launch_simple_gemm(dz + (size_t)t * a->m * p.ldz, p.ldz, 1, a->weight, 1, a->ldw, a->m, a->k, a->n, t > 0,
-                                  tmp, st);
-    if (e == cudaSuccess) e = moe::launch_simple_store(tmp, (int64_t)a->m * a->k, a->grad_x, a->grad_f32 != 0, st);
-    if (e != cudaSuccess) return done(e, "input gradient");
-    tmp += up256((size_t)a->m * a->k * 4) / 4;
+    const void* w = a->weight;
+    int64_t ldw = a->ldw;
+    if (p.pad_w) {
+      e = moe::launch_pad_rows(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldk, st);
+      if (e != cudaSuccess) return done(e, "linear gradient: preparing the weights");
+      w = ws + p.w;
+      ldw = p.ldk;
+    }
+    moe::LinearEpilogue ep{nullptr, nullptr, a->grad_x, nullptr, nullptr, 0, a->k, MOE_ACT_NONE, a->grad_f32};
+    if (int rc = run_product(p.px, false, true, false, false, a->m, a->k, a->n, dz, ldz, term_stride, w, ldw, a->n, ep,
+                             ws, partial, st, "input gradient"))
+      return rc;
   }
   if (a->grad_weight) {
     e = moe::launch_restore(static_cast<const uint8_t*>(a->x8), static_cast<const uint8_t*>(a->x_scale), 1, a->m, a->k,
                             ws + p.xhat, false, p.ldk, st);
-    for (int t = 0; t < terms && e == cudaSuccess; ++t)
-      e = moe::launch_simple_gemm(dz + (size_t)t * a->m * p.ldz, 1, p.ldz, ws + p.xhat, 1, p.ldk, a->n, a->k, a->m, t > 0,
-                                  tmp, st);
-    if (e == cudaSuccess) e = moe::launch_simple_store(tmp, (int64_t)a->n * a->k, a->grad_weight, a->grad_f32 != 0, st);
-    if (e != cudaSuccess) return done(e, "weight gradient");
+    if (e != cudaSuccess) return done(e, "restoring the input checkpoint");
+    moe::LinearEpilogue ep{nullptr, nullptr, a->grad_weight, nullptr, nullptr, 0, a->k, MOE_ACT_NONE, a->grad_f32};
+    if (int rc = run_product(p.pw, true, true, false, false, a->n, a->k, a->m, dz, ldz, term_stride, ws + p.xhat, p.ldk,
+                             a->m, ep, ws + p.px.arrivals, partial, st, "weight gradient"))
+      return rc;
   }
   return MOE_OK;
 }

@@ -31,12 +31,6 @@ cudaError_t launch_checkpoint(const void* x, bool bf16, int64_t rows, int64_t co
 cudaError_t launch_restore(const uint8_t* q, const uint8_t* scale, int64_t batch, int64_t rows, int64_t cols, void* out,
                            bool f32, int64_t ldo, cudaStream_t st);
 
-// z[m, n] = sum_k A(m, k) B(n, k) with arbitrary element strides, f32 out (row stride n).
-cudaError_t launch_simple_gemm(const void* A, int64_t am, int64_t ak, const void* B, int64_t bn, int64_t bk, int m,
-                               int n, int k, bool accumulate, float* out, cudaStream_t st);
-cudaError_t launch_simple_epilogue(const float* z, int m, int n, const LinearEpilogue& ep, cudaStream_t st);
-cudaError_t launch_simple_store(const float* z, int64_t count, void* out, bool f32, cudaStream_t st);
-
 // Gradient of the pre-activation: dz = dy * act'(z), written as bf16 [terms][m][ldz]
 // (terms = 2: the rounding's remainder follows), and per-chunk column sums.
 struct ActGradArgs {
