@@ -20,10 +20,14 @@ namespace moe {
 
 constexpr int kAgRows = 64, kAgCols = 256;
 
-template <int HALVES, bool F32, bool VEC>
+// FAST (dz rounded to bf16 once): hardware exponential and reciprocal, good to
+// 2^-20 of 1 + |z|; the exact ones bound the kernel by arithmetic (121 us instead
+// of 60 at 16384 x 4096) and serve the two-term form.
+template <int HALVES, bool F32, bool VEC, bool FAST>
 __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
   __shared__ float red[8][kAgCols];
   pdl_wait();
+  pdl_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t r0 = (int64_t)blockIdx.y * kAgRows;
   const int64_t rend = min(r0 + kAgRows, (int64_t)a.m);
@@ -96,7 +100,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
       if constexpr (HALVES == 2) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float b = z[1][j], s = sigmoid_f(b), av = z[0][j];
+          const float b = z[1][j], s = FAST ? sigmoid_fast(b) : sigmoid_f(b), av = z[0][j];
           // __fmul_rn: dz is a rounded value, never the inside of an FMA, so the sums do not
           // depend on which outputs are asked for
           z[0][j] = __fmul_rn(dy[j], b * s);
@@ -104,7 +108,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[0][j] = __fmul_rn(dy[j], act_slope(z[0][j], a.act));
+        for (int j = 0; j < 8; ++j) z[0][j] = __fmul_rn(dy[j], act_slope<FAST>(z[0][j], a.act));
       }
     } else {
 #pragma unroll
@@ -117,6 +121,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
       if (dz == nullptr) continue;
       __nv_bfloat16* out = dz + row * a.ldz + (int64_t)h * O;
       float lo[8];
+      if constexpr (!FAST)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float hi = __bfloat162float(__float2bfloat16_rn(z[h][j]));
@@ -126,7 +131,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
         if (col(0) < O) {
           *reinterpret_cast<uint4*>(out + col(0)) = make_uint4(pack_bf16(z[h][0], z[h][1]), pack_bf16(z[h][2], z[h][3]),
                                                                pack_bf16(z[h][4], z[h][5]), pack_bf16(z[h][6], z[h][7]));
-          if (a.terms == 2)
+          if (!FAST && a.terms == 2)
             *reinterpret_cast<uint4*>(out + term + col(0)) =
                 make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
         }
@@ -135,7 +140,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
         for (int j = 0; j < 8; ++j)
           if (col(j) < O) {
             out[col(j)] = __float2bfloat16_rn(z[h][j]);
-            if (a.terms == 2) out[term + col(j)] = __float2bfloat16_rn(lo[j]);
+            if (!FAST && a.terms == 2) out[term + col(j)] = __float2bfloat16_rn(lo[j]);
           }
       }
     }
@@ -160,6 +165,7 @@ __global__ void __launch_bounds__(256) colsum_finish_kernel(const float* __restr
                                                             void* __restrict__ out, int f32) {
   __shared__ double red[8][32];
   pdl_wait();
+  pdl_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + tx;
   double t = 0.0;
@@ -178,14 +184,16 @@ int act_grad_chunks(int m, int) { return ceil_div(m, kAgRows); }
 
 static bool al(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-cudaError_t launch_act_grad(const ActGradArgs& a, cudaStream_t st) {
+cudaError_t launch_act_grad(const ActGradArgs& a, bool pdl, cudaStream_t st) {
   if (a.m == 0 || a.n == 0) return cudaSuccess;
   const bool two = a.act == kActSwiglu;
   const int O = two ? a.n / 2 : a.n;
   const bool vec = al(a.dy, 16) && a.ldg % (a.dy_f32 ? 4 : 8) == 0 && O % 8 == 0 && (!a.z8 || al(a.z8, 8)) &&
                    (!a.dz || (al(a.dz, 16) && a.ldz % 8 == 0));
   const dim3 grid((unsigned)ceil_div(O, kAgCols), (unsigned)act_grad_chunks(a.m, a.n));
-#define MOE_AG(H, F, V) act_grad_kernel<H, F, V><<<grid, 256, 0, st>>>(a, O)
+#define MOE_AG(H, F, V)                                                                                      \
+  return a.terms == 1 ? launch_kernel(act_grad_kernel<H, F, V, true>, grid, dim3(256), 0, st, pdl, a, O) \
+                      : launch_kernel(act_grad_kernel<H, F, V, false>, grid, dim3(256), 0, st, pdl, a, O)
   if (two) {
     if (a.dy_f32) { if (vec) MOE_AG(2, true, true); else MOE_AG(2, true, false); }
     else { if (vec) MOE_AG(2, false, true); else MOE_AG(2, false, false); }
@@ -194,13 +202,11 @@ cudaError_t launch_act_grad(const ActGradArgs& a, cudaStream_t st) {
     else { if (vec) MOE_AG(1, false, true); else MOE_AG(1, false, false); }
   }
 #undef MOE_AG
-  return cudaGetLastError();
 }
 
 cudaError_t launch_colsum_finish(const float* colsum, int chunks, int n, void* out, bool f32, cudaStream_t st) {
   if (n == 0) return cudaSuccess;
-  colsum_finish_kernel<<<ceil_div(n, 32), 256, 0, st>>>(colsum, chunks, n, out, f32);
-  return cudaGetLastError();
+  return launch_kernel(colsum_finish_kernel, dim3(ceil_div(n, 32)), dim3(256), 0, st, true, colsum, chunks, n, out, f32);
 }
 
 }  // namespace moe

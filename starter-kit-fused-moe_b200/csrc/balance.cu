@@ -71,14 +71,15 @@ __device__ __forceinline__ void seq_bounds(const int32_t* cu, int q, int t, int&
   a = min(max(__ldg(cu + q), 0), t);
   b = min(max(__ldg(cu + q + 1), a), t);
 }
-// The last sequence that starts at or before token x (0 if none does).
-__device__ __forceinline__ int seq_of(const int32_t* cu, int s, int x) {
-  if (cu == nullptr) return 0;
-  int lo = 0, hi = s - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(cu + mid) <= x) lo = mid;
-    else hi = mid - 1;
+// The last sequence that starts at or before token x (0 if none does): every
+// round looks at 32 boundaries at once, one per lane.
+__device__ __forceinline__ int seq_of(const int32_t* cu, int s, int x, int lane) {
+  int lo = 0, hi = cu == nullptr ? 1 : s;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+    const uint32_t m = __ballot_sync(0xffffffffu, lane == 0 || (i < hi && __ldg(cu + i) <= x));
+    lo += (31 - __clz(m)) * step;
+    hi = min(hi, lo + step);
   }
   return lo;
 }
@@ -107,7 +108,7 @@ __device__ __forceinline__ float scores(const float* x, int scoring, float* s) {
   if (scoring == 0) {
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
-      s[j] = sigmoid_f(x[j]);
+      s[j] = __fdividef(1.0f, 1.0f + expf(-x[j]));
       sum += s[j];
     }
     return 1.0f / (warp_sum(sum) + kScoreEps);
@@ -140,9 +141,10 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(Balance
   __shared__ int hist[32 * ITEMS];
   __shared__ int tok;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
   if (blockIdx.x == 0 && threadIdx.x == 0) *w.state = 0;
   const int b0 = blockIdx.x * chunk, b1 = min(b0 + chunk, a.t);
-  for (int q = seq_of(a.cu, a.s, b0); q < a.s; ++q) {
+  for (int q = seq_of(a.cu, a.s, b0, lane); q < a.s; ++q) {
     int qa, qb;
     seq_bounds(a.cu, q, a.t, qa, qb);
     if (qa >= b1) break;
@@ -196,6 +198,7 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
   __shared__ int rt[256];
   __shared__ double rl[256];
   __shared__ int last;
+  pdl_wait();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int groups = gridDim.x, g = blockIdx.x;
   const int q = blockIdx.y;
@@ -212,8 +215,9 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
   double p = 0.0;
   int c = 0, n = 0;
   if (!bad) {
-    for (int b = blo + ty; b < bhi; b += 8)
-      if (e < a.e) {
+    if (e < a.e)
+#pragma unroll 4
+      for (int b = blo + ty; b < bhi; b += 8) {
         const int64_t slot = (int64_t)b + q;
         p += (double)w.p[slot * a.e + e];
         c += w.c[slot * a.e + e];
@@ -287,68 +291,114 @@ __global__ void balance_empty_kernel(BalanceArgs a) {
   }
 }
 
+// A block takes `chunk` consecutive tokens, a warp every eighth of them; the
+// coefficients c_e of the sequence at hand are in the warp's registers.
 template <int ITEMS>
-__global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGradArgs a, int per_warp) {
+__global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGradArgs a, int chunk) {
+  __shared__ float scatter[kBalWarps][32 * ITEMS];           // a warp's row of combine-weight gradients, else zero
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t0 = ((int64_t)blockIdx.x * kBalWarps + warp) * per_warp;
-  if (t0 >= a.t) return;
-  const int t1 = (int)min(t0 + per_warp, (int64_t)a.t);
-  const float g = a.grad_loss != nullptr ? __ldg(a.grad_loss) : 0.f;
-  const int live = a.grad_loss != nullptr ? __ldg(a.live) : 0;
-  int q = -1, qa = 0, qb = 0;
-  float coef[ITEMS];
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) coef[j] = 0.f;
-  for (int t = (int)t0; t < t1; ++t) {
-    const int id = lane < a.k ? __ldg(a.idx + (int64_t)t * a.k + lane) : -1;
-    float x[ITEMS], s[ITEMS], dx[ITEMS];
-    load_logits<ITEMS>(a.logits + (int64_t)t * a.e, a.e, lane, x);
-    const bool hit = id >= 0 && id < a.e;
-    const bool token = __any_sync(0xffffffffu, hit);
-    // the token's sequence and its coefficients (t == qa: the first sequence may start after a gap)
-    if (a.grad_loss != nullptr && (q < 0 || t >= qb || t == qa)) {
-      q = seq_of(a.cu, a.s, t);
+  for (int j = 0; j < ITEMS; ++j) scatter[warp][lane + 32 * j] = 0.f;
+  __syncwarp();
+  const int b1 = (int)min((int64_t)(blockIdx.x + 1) * chunk, (int64_t)a.t);
+  const bool with_loss = a.grad_loss != nullptr;
+  const float g = with_loss ? __ldg(a.grad_loss) : 0.f;
+  const int live = with_loss ? __ldg(a.live) : 0;
+  for (int pos = blockIdx.x * chunk; pos < b1;) {
+    int end = b1;
+    float coef[ITEMS];
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) coef[j] = 0.f;
+    if (with_loss) {
+      const int q = seq_of(a.cu, a.s, pos, lane);
+      int qa, qb;
       seq_bounds(a.cu, q, a.t, qa, qb);
-      const int tq = t >= qa && t < qb ? __ldg(a.tokens + q) : 0;   // 0: in no sequence
-      const double f = tq > 0 && live > 0 ? (double)g * a.alpha * a.e / ((double)a.k * live * tq * tq) : 0.0;
+      if (pos < qa) {
+        end = min(qa, b1);                                   // before the first sequence
+      } else if (pos < qb) {
+        end = min(qb, b1);
+        const int tq = __ldg(a.tokens + q);
+        const double f = tq > 0 && live > 0 ? (double)g * a.alpha * a.e / ((double)a.k * live * tq * tq) : 0.0;
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j)
+          if (lane + 32 * j < a.e) coef[j] = (float)(f * __ldg(a.counts + (int64_t)q * a.e + lane + 32 * j));
+      }                                                      // else: behind the last sequence
+    }
+    float next[ITEMS];                                       // the next token's logits are on their way
+    int id_next = -1;
+    if (pos + warp < end) {
+      load_logits<ITEMS>(a.logits + (int64_t)(pos + warp) * a.e, a.e, lane, next);
+      if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(pos + warp) * a.k + lane);
+    }
+    for (int t = pos + warp; t < end; t += kBalWarps) {
+      const int id = id_next;
+      float x[ITEMS], dx[ITEMS];
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j) x[j] = next[j];
+      if (t + kBalWarps < end) {
+        load_logits<ITEMS>(a.logits + (int64_t)(t + kBalWarps) * a.e, a.e, lane, next);
+        if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(t + kBalWarps) * a.k + lane);
+      }
+      const bool hit = id >= 0 && id < a.e;
+      const bool token = __any_sync(0xffffffffu, hit);
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j) dx[j] = 0.f;
+      if (token && with_loss) {
+        // s and its slope (sigmoid: s (1 - s), from one exponential; softmax: s)
+        float s[ITEMS], slope[ITEMS], inv;
+        if (a.scoring == 0) {
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < ITEMS; ++j) {
+            const float e = expf(-fabsf(x[j])), r = __fdividef(1.0f, 1.0f + e);
+            s[j] = x[j] >= 0.f ? r : e * r;                  // NaN: e is NaN
+            slope[j] = e * r * r;
+            sum += s[j];
+          }
+          inv = 1.0f / (warp_sum(sum) + kScoreEps);
+        } else {
+          inv = scores<ITEMS>(x, 1, s);
+#pragma unroll
+          for (int j = 0; j < ITEMS; ++j) slope[j] = s[j];
+        }
+        float inner = 0.f;
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) inner += coef[j] * s[j];
+        inner = warp_sum(inner) * inv;
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) dx[j] = (coef[j] - inner) * inv * slope[j];
+      }
+      if (token && a.grad_weights != nullptr) {
+        const float xs = hit ? __ldg(a.logits + (int64_t)t * a.e + id) : 0.f;
+        const float e = expf(-fabsf(xs)), r = __frcp_rn(1.0f + e);
+        const float top = hit ? (xs >= 0.f ? r : e * r) : 0.f;
+        const float dw = hit ? __ldg(a.grad_weights + (int64_t)t * a.k + lane) * a.route_scale : 0.f;
+        const float total = warp_sum(top) + kScoreEps;
+        const float dot = warp_sum(dw * top);
+        const float d = hit ? (dw - dot / total) / total * (e * r * r) : 0.f;
+        // scattered through shared memory; repeated picks (rare) are added by their first lane in pick order
+        const uint32_t same = __match_any_sync(0xffffffffu, hit ? id : -1 - lane);
+        float sum = d;
+        if (__any_sync(0xffffffffu, same & (same - 1))) {
+          sum = 0.f;
+          for (int i = 0; i < a.k; ++i) {
+            const float v = __shfl_sync(0xffffffffu, d, i);
+            if (same >> i & 1) sum += v;
+          }
+        }
+        const bool first = hit && (same & ((1u << lane) - 1)) == 0;
+        if (first) scatter[warp][id] = sum;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) dx[j] += scatter[warp][lane + 32 * j];
+        __syncwarp();
+        if (first) scatter[warp][id] = 0.f;
+      }
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j)
-        coef[j] = tq > 0 && lane + 32 * j < a.e ? (float)(f * __ldg(a.counts + (int64_t)q * a.e + lane + 32 * j)) : 0.f;
+        if (lane + 32 * j < a.e) a.grad_logits[(int64_t)t * a.e + lane + 32 * j] = dx[j];
     }
-#pragma unroll
-    for (int j = 0; j < ITEMS; ++j) dx[j] = 0.f;
-    if (token && a.grad_loss != nullptr) {
-      const float inv = scores<ITEMS>(x, a.scoring, s);
-      float inner = 0.f;
-#pragma unroll
-      for (int j = 0; j < ITEMS; ++j) inner += coef[j] * s[j];
-      inner = warp_sum(inner) * inv;
-#pragma unroll
-      for (int j = 0; j < ITEMS; ++j) {
-        const float d = (coef[j] - inner) * inv;
-        dx[j] = d * (a.scoring == 0 ? s[j] * sigmoid_f(-x[j]) : s[j]);
-      }
-    }
-    if (token && a.grad_weights != nullptr) {
-      const float xs = hit ? __ldg(a.logits + (int64_t)t * a.e + id) : 0.f;
-      const float top = hit ? sigmoid_f(xs) : 0.f;
-      const float dw = hit ? __ldg(a.grad_weights + (int64_t)t * a.k + lane) * a.route_scale : 0.f;
-      const float total = warp_sum(top) + kScoreEps;
-      const float dot = warp_sum(dw * top);
-      const float d = hit ? (dw - dot / total) / total * (top * sigmoid_f(-xs)) : 0.f;
-      for (int i = 0; i < a.k; ++i) {                        // in pick order; a repeated pick adds up
-        const int ie = __shfl_sync(0xffffffffu, hit ? id : -1, i);
-        const float id_d = __shfl_sync(0xffffffffu, d, i);
-        if (ie >= 0 && (ie & 31) == lane) {
-#pragma unroll
-          for (int j = 0; j < ITEMS; ++j)
-            if (j == ie >> 5) dx[j] += id_d;
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < ITEMS; ++j)
-      if (lane + 32 * j < a.e) a.grad_logits[(int64_t)t * a.e + lane + 32 * j] = dx[j];
+    pos = end;
   }
 }
 
@@ -370,16 +420,16 @@ cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
 #undef MOE_BAL
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  balance_reduce_kernel<<<dim3((unsigned)ceil_div(a.e, 32), (unsigned)a.s), 256, 0, st>>>(a, w, chunk);
-  return cudaGetLastError();
+  return launch_kernel(balance_reduce_kernel, dim3((unsigned)ceil_div(a.e, 32), (unsigned)a.s), dim3(256), 0, st, true, a,
+                       w, chunk);
 }
 
 cudaError_t launch_balance_grad(const BalanceGradArgs& a, cudaStream_t st) {
   if (a.t == 0) return cudaSuccess;
-  int per = ceil_div(a.t, 148 * 8 * kBalWarps);
-  if (per < 1) per = 1;
-  const int grid = ceil_div(a.t, (int64_t)per * kBalWarps);
-#define MOE_BALG(I) balance_grad_kernel<I><<<grid, kBalWarps * 32, 0, st>>>(a, per)
+  int chunk = align_up(ceil_div(a.t, 4 * 148), kBalWarps);     // about four blocks per SM
+  if (chunk < kBalWarps) chunk = kBalWarps;
+  const int grid = ceil_div(a.t, chunk);
+#define MOE_BALG(I) balance_grad_kernel<I><<<grid, kBalWarps * 32, 0, st>>>(a, chunk)
   if (a.e <= 32) MOE_BALG(1);
   else if (a.e <= 64) MOE_BALG(2);
   else if (a.e <= 128) MOE_BALG(4);

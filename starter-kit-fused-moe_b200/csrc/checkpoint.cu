@@ -5,101 +5,111 @@
 // exact in bf16.
 //
 // Both kernels are bound by HBM: 3 bytes per bf16 value to keep, 3 to bring
-// back. 16 lanes take one 128-value block of a row (16-byte loads of bf16), a
-// warp walks R rows of one block column and a CTA holds 8 neighbouring block
-// columns, so each row is read in 2 KB runs and the R scales of a warp leave as
-// one coalesced store ([blocks, rows] keeps the scales of consecutive rows
-// together, the framework's layout).
+// back. A warp walks R rows of one block column and a CTA holds 8 neighbouring
+// block columns, so each row is read in 2 KB runs, and the R scales of a warp
+// leave as one run of bytes ([blocks, rows] keeps the scales of consecutive rows
+// together, the framework's layout). Keeping: 8 lanes take a block of a row (16
+// values each, the maximum found on packed 16-bit magnitudes), so that four
+// rows share each reduction step; 16 lanes per block spent twice the
+// instructions and left the issue slots half busy at 3.7 TB/s.
 #include "train_common.cuh"
 
 namespace moe {
 
 constexpr int kCkWarps = 8;
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// 16 values of a lane as raw words: bf16 columns 8 sub + 64 h (h < 2) or f32
+// columns 4 sub + 32 h (h < 4); element-wise (VEC false) columns sub + 8 j.
+template <typename T_IN>
+constexpr int kCkRaw = sizeof(T_IN) * 4;
 
-// VEC: 16-byte aligned rows and 8 | cols; otherwise element-wise accesses.
 template <typename T_IN, int R, bool VEC>
 __global__ void __launch_bounds__(kCkWarps * 32) checkpoint_kernel(const T_IN* __restrict__ x, int64_t rows,
                                                                    int64_t cols, int64_t ldx, uint8_t* __restrict__ q,
                                                                    uint8_t* __restrict__ scale) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
+  constexpr bool BF = sizeof(T_IN) == 2;
+  constexpr int W = kCkRaw<T_IN>, PER = BF ? 8 : 4, STEP = BF ? 64 : 32, N16 = W / 4;
+  constexpr int ITER = R / 4, U = ITER < (BF ? 4 : 2) ? ITER : (BF ? 4 : 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7, rs = lane >> 3;
   const int64_t kb = (int64_t)blockIdx.y * kCkWarps + warp;
   const int64_t c0 = kb * kBlock;
   if (c0 >= cols) return;
   const int64_t r0 = (int64_t)blockIdx.x * R;
   uint32_t code_mine = 0;
-  constexpr int U = R >= 8 ? 4 : R / 2;          // row pairs in flight
 #pragma unroll 1
-  for (int i0 = 0; i0 < R / 2; i0 += U) {
-    float v[U][8];
+  for (int i0 = 0; i0 < ITER; i0 += U) {
+    uint32_t raw[U][W];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t row = r0 + 2 * (i0 + u) + half;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
-      if (row >= rows) continue;
+      const int64_t row = r0 + 4 * (i0 + u) + rs;
       const T_IN* src = x + row * ldx + c0;
-      if constexpr (VEC) {
-        if (c0 + 8 * sub < cols) {
-          if constexpr (sizeof(T_IN) == 2) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + sub);
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack_bf16(w[j]);
-              v[u][2 * j] = f.x;
-              v[u][2 * j + 1] = f.y;
+      for (int j = 0; j < W; ++j) raw[u][j] = 0;
+      if (row < rows) {
+        if constexpr (VEC) {
+#pragma unroll
+          for (int h = 0; h < N16; ++h)
+            if (c0 + PER * sub + STEP * h < cols)
+              *reinterpret_cast<uint4*>(&raw[u][4 * h]) = __ldg(reinterpret_cast<const uint4*>(src + PER * sub + STEP * h));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + sub + 8 * j < cols) {
+              if constexpr (BF)
+                raw[u][j >> 1] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(src) + sub + 8 * j) << (16 * (j & 1));
+              else
+                raw[u][j] = __ldg(reinterpret_cast<const uint32_t*>(src) + sub + 8 * j);
             }
-          } else {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(src) + 2 * sub);
-            const float4 b = __ldg(reinterpret_cast<const float4*>(src) + 2 * sub + 1);
-            v[u][0] = a.x; v[u][1] = a.y; v[u][2] = a.z; v[u][3] = a.w;
-            v[u][4] = b.x; v[u][5] = b.y; v[u][6] = b.z; v[u][7] = b.w;
-          }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c0 + sub + 16 * j < cols) v[u][j] = (float)src[sub + 16 * j];
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      // largest magnitude as the bits of a float (NaN above infinity above all)
       uint32_t amax = 0;
+      if constexpr (BF) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max(amax, abs_bits(v[u][j]));
-#pragma unroll
-      for (int d = 8; d >= 1; d >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-      const uint32_t code = e8m0_of_amax(amax);
-      // row r0 + l's code moves to lane l
-      const int l0 = 2 * (i0 + u);
-      const uint32_t ca = __shfl_sync(0xffffffffu, code, 0), cb = __shfl_sync(0xffffffffu, code, 16);
-      if (lane == l0) code_mine = ca;
-      if (lane == l0 + 1) code_mine = cb;
-      const int64_t row = r0 + l0 + half;
-      if (row >= rows) continue;
-      const float inv = e8m0_inverse(code);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[u][j] *= inv;
-      if (code == kTopScaleCode) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[u][j] = hold_finite(v[u][j]);
-      }
-      uint8_t* dst = q + row * cols + c0;
-      if constexpr (VEC) {
-        if (c0 + 8 * sub < cols)
-          reinterpret_cast<uint2*>(dst)[sub] =
-              make_uint2(e4m3x4(v[u][0], v[u][1], v[u][2], v[u][3]), e4m3x4(v[u][4], v[u][5], v[u][6], v[u][7]));
+        for (int j = 0; j < W; ++j) amax = __vmaxu2(amax, raw[u][j] & 0x7fff7fffu);
+        amax = max(amax & 0xffff0000u, amax << 16);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c0 + sub + 16 * j < cols)
-            dst[sub + 16 * j] = (uint8_t)__nv_cvt_float_to_fp8(v[u][j], __NV_SATFINITE, __NV_E4M3);
+        for (int j = 0; j < W; ++j) amax = max(amax, raw[u][j] & 0x7fffffffu);
+      }
+#pragma unroll
+      for (int d = 4; d >= 1; d >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+      const uint32_t code = e8m0_of_amax(amax);
+      if (sub == i0 + u) code_mine = code;           // lane (rs, sub) keeps the code of row 4 sub + rs
+      const float inv = e8m0_inverse(code);
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        v[j] = inv * __uint_as_float(!BF ? raw[u][BF ? 0 : j] : j & 1 ? raw[u][j >> 1] & 0xffff0000u : raw[u][j >> 1] << 16);
+      if (code == kTopScaleCode) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = hold_finite(v[j]);
+      }
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = e4m3x4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      const int64_t row = r0 + 4 * (i0 + u) + rs;
+      if (row >= rows) continue;
+      uint8_t* dst = q + row * cols + c0;
+      if constexpr (VEC) {
+#pragma unroll
+        for (int h = 0; h < N16; ++h)
+          if (c0 + PER * sub + STEP * h < cols) {
+            if constexpr (BF) *reinterpret_cast<uint2*>(dst + PER * sub + STEP * h) = make_uint2(o[2 * h], o[2 * h + 1]);
+            else *reinterpret_cast<uint32_t*>(dst + PER * sub + STEP * h) = o[h];
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c0 + sub + 8 * j < cols) dst[sub + 8 * j] = (uint8_t)(o[j >> 2] >> (8 * (j & 3)));
       }
     }
   }
-  if (lane < R && r0 + lane < rows) scale[kb * rows + r0 + lane] = (uint8_t)code_mine;
+  const int64_t row = r0 + 4 * sub + rs;
+  if (sub < ITER && row < rows) scale[kb * rows + row] = (uint8_t)code_mine;
 }
 
 // q, scale -> bf16 / f32 out with row stride ldo; `batch` matrices one after the
@@ -113,6 +123,7 @@ __global__ void __launch_bounds__(kCkWarps * 32) restore_kernel(const uint8_t* _
   const int64_t kb = (int64_t)blockIdx.y * kCkWarps + warp;
   const int64_t c0 = kb * kBlock;
   pdl_wait();
+  pdl_trigger();
   if (c0 >= cols) return;
   q += (int64_t)blockIdx.z * rows * cols;
   scale += (int64_t)blockIdx.z * blocks * rows;
@@ -169,34 +180,34 @@ __global__ void __launch_bounds__(kCkWarps * 32) restore_kernel(const uint8_t* _
 }
 
 // Rows per warp: as many as keep about 16 warps on every SM.
-static int rows_per_warp(int64_t rows, int64_t blocks) {
+static int rows_per_warp(int64_t rows, int64_t blocks, int least) {
   for (int r : {32, 8})
     if ((rows + r - 1) / r * blocks >= 148 * 16) return r;
-  return 2;
+  return least;
 }
 
 template <typename T_IN, bool VEC>
 static cudaError_t checkpoint_r(const T_IN* x, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q, uint8_t* scale,
                                 cudaStream_t st) {
   const int64_t nb = (cols + kBlock - 1) / kBlock;
-  const int r = rows_per_warp(rows, nb);
+  const int r = rows_per_warp(rows, nb, 4);
   const dim3 grid((unsigned)((rows + r - 1) / r), (unsigned)((nb + kCkWarps - 1) / kCkWarps));
   if (r == 32) checkpoint_kernel<T_IN, 32, VEC><<<grid, kCkWarps * 32, 0, st>>>(x, rows, cols, ldx, q, scale);
   else if (r == 8) checkpoint_kernel<T_IN, 8, VEC><<<grid, kCkWarps * 32, 0, st>>>(x, rows, cols, ldx, q, scale);
-  else checkpoint_kernel<T_IN, 2, VEC><<<grid, kCkWarps * 32, 0, st>>>(x, rows, cols, ldx, q, scale);
+  else checkpoint_kernel<T_IN, 4, VEC><<<grid, kCkWarps * 32, 0, st>>>(x, rows, cols, ldx, q, scale);
   return cudaGetLastError();
 }
 
 template <typename T_OUT, bool VEC>
 static cudaError_t restore_r(const uint8_t* q, const uint8_t* scale, int64_t batch, int64_t rows, int64_t cols,
-                             T_OUT* out, int64_t ldo, cudaStream_t st) {
+                             T_OUT* out, int64_t ldo, bool pdl, cudaStream_t st) {
   const int64_t nb = (cols + kBlock - 1) / kBlock;
-  const int r = rows_per_warp(rows, nb * batch);
+  const int r = rows_per_warp(rows, nb * batch, 2);
   const dim3 grid((unsigned)((rows + r - 1) / r), (unsigned)((nb + kCkWarps - 1) / kCkWarps), (unsigned)batch);
-  if (r == 32) restore_kernel<T_OUT, 32, VEC><<<grid, kCkWarps * 32, 0, st>>>(q, scale, rows, cols, nb, out, ldo);
-  else if (r == 8) restore_kernel<T_OUT, 8, VEC><<<grid, kCkWarps * 32, 0, st>>>(q, scale, rows, cols, nb, out, ldo);
-  else restore_kernel<T_OUT, 2, VEC><<<grid, kCkWarps * 32, 0, st>>>(q, scale, rows, cols, nb, out, ldo);
-  return cudaGetLastError();
+  const dim3 block(kCkWarps * 32);
+  if (r == 32) return launch_kernel(restore_kernel<T_OUT, 32, VEC>, grid, block, 0, st, pdl, q, scale, rows, cols, nb, out, ldo);
+  if (r == 8) return launch_kernel(restore_kernel<T_OUT, 8, VEC>, grid, block, 0, st, pdl, q, scale, rows, cols, nb, out, ldo);
+  return launch_kernel(restore_kernel<T_OUT, 2, VEC>, grid, block, 0, st, pdl, q, scale, rows, cols, nb, out, ldo);
 }
 
 static bool al(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -216,17 +227,17 @@ cudaError_t launch_checkpoint(const void* x, bool bf16, int64_t rows, int64_t co
 }
 
 cudaError_t launch_restore(const uint8_t* q, const uint8_t* scale, int64_t batch, int64_t rows, int64_t cols, void* out,
-                           bool f32, int64_t ldo, cudaStream_t st) {
+                           bool f32, int64_t ldo, bool pdl, cudaStream_t st) {
   if (batch == 0 || rows == 0 || cols == 0) return cudaSuccess;
   const bool vec = al(q, 8) && al(out, 16) && cols % 8 == 0 && ldo % (f32 ? 4 : 8) == 0;
   if (f32) {
     auto* p = static_cast<float*>(out);
-    return vec ? restore_r<float, true>(q, scale, batch, rows, cols, p, ldo, st)
-               : restore_r<float, false>(q, scale, batch, rows, cols, p, ldo, st);
+    return vec ? restore_r<float, true>(q, scale, batch, rows, cols, p, ldo, pdl, st)
+               : restore_r<float, false>(q, scale, batch, rows, cols, p, ldo, pdl, st);
   }
   auto* p = static_cast<__nv_bfloat16*>(out);
-  return vec ? restore_r<__nv_bfloat16, true>(q, scale, batch, rows, cols, p, ldo, st)
-             : restore_r<__nv_bfloat16, false>(q, scale, batch, rows, cols, p, ldo, st);
+  return vec ? restore_r<__nv_bfloat16, true>(q, scale, batch, rows, cols, p, ldo, pdl, st)
+             : restore_r<__nv_bfloat16, false>(q, scale, batch, rows, cols, p, ldo, pdl, st);
 }
 
 }  // namespace moe

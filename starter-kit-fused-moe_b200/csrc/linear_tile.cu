@@ -20,10 +20,11 @@
 // accumulators of NT columns in TMEM let a tile's epilogue overlap the next
 // tile's products. Persistent grid, one pair per two SMs; tiles are walked in
 // bands of 8 row tiles so that the tiles in flight share both operands in L2.
-// When there are fewer tiles than pairs, K is split: every slice leaves its
-// fp32 partial tile in the workspace and the slice that arrives last adds them
-// in slice order (so the result does not depend on who was last) and runs the
-// epilogue; no CTA waits for another one's slice.
+// When there are fewer tiles than pairs, K is split: the slices leave fp32
+// partial rows in the workspace and a second kernel, launched to start as this
+// one ends, adds them in slice order and runs the epilogue on all SMs. (Letting
+// the slice that arrives last do it kept the other SMs idle: 36 instead of 20 us
+// at 1037 x 1111 x 515.)
 //
 // Every wait is bounded (2 s). One that runs out makes the kernel write NaN to
 // the tiles it still owes, so a failed call never returns plausible numbers.
@@ -44,8 +45,8 @@ struct LinearTileSmem {
   uint64_t tempty[2];
   uint32_t tmem_base;
   int abort_flag;
-  int last;
   float amax[2][2][2][128];      // [tile parity][column half][gate, up][row]
+  float stage[kLtEpiWarps][32][17];
 };
 constexpr size_t kLtSmem = 1024 + (size_t)kLtStages * kLtStageBytes + sizeof(LinearTileSmem);
 static_assert(kLtSmem <= 232448, "shared memory budget");
@@ -136,8 +137,8 @@ __device__ __forceinline__ void lt_act16(float* v, int act) {
 // y[row, c .. c + 16) = v + residual (columns below `end` only). The residual is
 // read before the same values of y are written by the same thread, so y may be
 // the residual.
-__device__ __forceinline__ void lt_store16(const LinearEpilogue& ep, int vec, int64_t row, int64_t c, int64_t end, float* v) {
-  const bool whole = vec && c + 16 <= end;
+__device__ __forceinline__ void lt_store16(const LinearEpilogue& ep, int64_t row, int64_t c, int64_t end, float* v) {
+  const bool whole = c + 16 <= end;
   if (ep.residual != nullptr) {
     const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr + c;
     if (whole) {
@@ -178,6 +179,28 @@ __device__ __forceinline__ void lt_store16(const LinearEpilogue& ep, int vec, in
         if (c + i < end) y[i] = __float2bfloat16_rn(v[i]);
     }
   }
+}
+// The same for a warp's 32 rows from `row0` when y or the residual cannot be
+// accessed in 16 bytes: through shared memory, so that 16 lanes take neighbouring
+// columns of a row (a lane per row costs a memory transaction per element: the
+// odd-sized 1037 x 1111 x 515 product took 45 us that way).
+__device__ __forceinline__ void lt_store_staged(const LinearEpilogue& ep, float (*stage)[17], int64_t row0, int rows,
+                                                int64_t c, int64_t end, const float* v, int lane) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) stage[lane][i] = v[i];
+  __syncwarp();
+  const int64_t col = c + (lane & 15);
+  if (col < end) {
+#pragma unroll 8
+    for (int r = lane >> 4; r < rows; r += 2) {
+      const int64_t row = row0 + r;
+      float y = stage[r][lane & 15];
+      if (ep.residual != nullptr) y += __bfloat162float(static_cast<const __nv_bfloat16*>(ep.residual)[row * ep.ldr + col]);
+      if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + col] = y;
+      else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + col] = __float2bfloat16_rn(y);
+    }
+  }
+  __syncwarp();
 }
 // Largest magnitude (as bits) of the columns below `end`.
 __device__ __forceinline__ uint32_t lt_amax16(const float* v, int64_t c, int64_t end, uint32_t amax) {
@@ -341,6 +364,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       const uint32_t acc = lane_addr + (uint32_t)(b * 256);
       const int64_t row = (int64_t)x.mt * 256 + crank * 128 + r;
       const bool valid = row < a.m;
+      const int warp_rows = (int)max((int64_t)0, min((int64_t)32, a.m - (row - lane)));
       auto release = [&] {
         tc_fence_before();
         __syncwarp();
@@ -355,40 +379,19 @@ __global__ void __launch_bounds__(kLtThreads, 1)
           for (int i = 0; i < 16; ++i) v[i] = NAN;
         }
       };
-      const bool split = a.splits > 1;
-      // this CTA's half of the tile's slices, [slice][column][row]
-      float* part = split ? a.partial + ((x.tile * a.splits) * 2 + crank) * (int64_t)(NT * 128) + r : nullptr;
-      const int64_t part_step = (int64_t)2 * NT * 128;
-      if (split) {
-        const int w = NT / 2;
-        float* mine = part + x.slice * part_step;
-        for (int c = g * w; c < (g + 1) * w; c += 16) {
+      if (a.splits > 1) {                                // fp32 partial row, in tile order
+        float* p = a.partial + ((int64_t)x.slice * a.m + row) * ((int64_t)a.n_tiles * NT) + (int64_t)x.nt * NT;
+        for (int c = g * H; c < (g + 1) * H; c += 16) {
           float v[16];
           from_tmem(c, v);
+          if (valid)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) __stcg(mine + (int64_t)(c + i) * 128, v[i]);
+            for (int i = 0; i < 4; ++i)
+              __stcg(reinterpret_cast<float4*>(p + c) + i, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
         }
         release();
-        __threadfence();
-        named_barrier_sync(1, kLtEpiWarps * 32);
-        if (warp == 2 && lane == 0) S.last = atomicAdd(a.arrivals + x.tile * 2 + crank, 1) == a.splits - 1;
-        named_barrier_sync(1, kLtEpiWarps * 32);
-        const bool last = S.last;
-        named_barrier_sync(1, kLtEpiWarps * 32);       // S.last may be written again
-        if (!last) continue;
-        __threadfence();
+        continue;
       }
-      auto load = [&](int col, float* v) {
-        if (!split) {
-          from_tmem(col, v);
-          return;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __ldcg(part + (int64_t)(col + i) * 128);
-        for (int s = 1; s < a.splits; ++s)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] += __ldcg(part + s * part_step + (int64_t)(col + i) * 128);
-      };
 
       if constexpr (!GATED) {
         const int64_t c_tile = (int64_t)x.nt * NT;
@@ -397,7 +400,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
           uint32_t amax = 0;
           for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 16) {
             float v[16];
-            load(c, v);
+            from_tmem(c, v);
             if (bias) lt_bias16(bias, c_tile + c, O, v);
             amax = lt_amax16(v, c_tile + c, O, amax);
           }
@@ -406,13 +409,13 @@ __global__ void __launch_bounds__(kLtThreads, 1)
         }
         for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 16) {
           float v[16];
-          load(c, v);
+          from_tmem(c, v);
           if (bias) lt_bias16(bias, c_tile + c, O, v);
-          if (valid) {
-            if constexpr (KEEP) lt_store_z16(ep.z8 + row * O, c_tile + c, O, v, code);
-            lt_act16(v, ep.act);
-            lt_store16(ep, a.vec, row, c_tile + c, O, v);
-          }
+          if constexpr (KEEP)
+            if (valid) lt_store_z16(ep.z8 + row * O, c_tile + c, O, v, code);
+          lt_act16(v, ep.act);
+          if (!a.vec) lt_store_staged(ep, S.stage[warp - 2], row - lane, warp_rows, c_tile + c, O, v, lane);
+          else if (valid) lt_store16(ep, row, c_tile + c, O, v);
         }
       } else {
         const int w = H / 2;                             // columns of each half per warp
@@ -424,7 +427,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float v[16];
-              load(h * H + c, v);
+              from_tmem(h * H + c, v);
               if (bias) lt_bias16(bias + h * O, c_tile + c, O, v);
               amax[h] = lt_amax16(v, c_tile + c, O, amax[h]);
             }
@@ -439,24 +442,24 @@ __global__ void __launch_bounds__(kLtThreads, 1)
         }
         for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 16) {
           float v[16], t[16];
-          load(c, v);
-          load(H + c, t);
+          from_tmem(c, v);
+          from_tmem(H + c, t);
           if (bias) {
             lt_bias16(bias, c_tile + c, O, v);
             lt_bias16(bias + O, c_tile + c, O, t);
           }
-          if (valid) {
-            if constexpr (KEEP) {
+          if constexpr (KEEP)
+            if (valid) {
               lt_store_z16(ep.z8 + row * O, c_tile + c, O, v, code[0]);
               lt_store_z16(ep.z8 + (a.m + row) * O, c_tile + c, O, t, code[1]);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] *= act_value(t[i], kActSilu);
-            lt_store16(ep, a.vec, row, c_tile + c, O, v);
-          }
+          for (int i = 0; i < 16; ++i) v[i] *= act_value(t[i], kActSilu);
+          if (!a.vec) lt_store_staged(ep, S.stage[warp - 2], row - lane, warp_rows, c_tile + c, O, v, lane);
+          else if (valid) lt_store16(ep, row, c_tile + c, O, v);
         }
       }
-      if (!split) release();
+      release();
     }
   }
 
@@ -469,34 +472,129 @@ __global__ void __launch_bounds__(kLtThreads, 1)
   }
 }
 
-// Row-padded copy of a matrix whose rows TMA cannot read (bases and row strides
-// must be multiples of 16 bytes).
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ src, int64_t lds, int64_t rows,
-                                                       int cols, uint16_t* __restrict__ dst, int64_t ldd) {
-  pdl_wait();
-  const int64_t row = blockIdx.x;
-  for (int c = 4 * (blockIdx.y * 256 + threadIdx.x); c < cols; c += 4 * 256 * gridDim.y) {
-    const uint16_t* s = src + row * lds + c;
-    uint16_t v[4];
+__global__ void __launch_bounds__(256) pad_kernel(PadArgs a) {
+  pdl_trigger();
+  // a warp per row, 4 columns per lane
+  const int lane = threadIdx.x & 31;
+  for (int j = 0; j < a.count; ++j)
+    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < a.rows[j]; row += (int64_t)gridDim.x * 8) {
+      const uint16_t* s = static_cast<const uint16_t*>(a.src[j]) + row * a.lds[j];
+      uint16_t* d = static_cast<uint16_t*>(a.dst[j]) + row * a.ldd[j];
+#pragma unroll 4
+      for (int c = 4 * lane; c < a.cols[j]; c += 128) {
+        uint16_t v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c + i < cols ? s[i] : 0;
-    *reinterpret_cast<uint2*>(dst + row * ldd + c) =
-        make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
-  }
+        for (int e = 0; e < 4; ++e) v[e] = c + e < a.cols[j] ? s[c + e] : 0;
+        *reinterpret_cast<uint2*>(d + c) = make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+      }
+    }
 }
-cudaError_t launch_pad_rows(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst, int64_t ldd,
-                            cudaStream_t st) {
-  if (rows == 0) return cudaSuccess;
-  const int gy = ceil_div(cols, 1024) < 8 ? ceil_div(cols, 1024) : 8;
-  pad_rows_kernel<<<dim3((unsigned)rows, gy), 256, 0, st>>>(static_cast<const uint16_t*>(src), lds, rows, (int)cols,
-                                                            static_cast<uint16_t*>(dst), ldd);
+cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
+  if (a.count == 0) return cudaSuccess;
+  int64_t blocks = 1;
+  for (int j = 0; j < a.count; ++j) blocks = blocks > (a.rows[j] + 7) / 8 ? blocks : (a.rows[j] + 7) / 8;
+  pad_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(a);
   return cudaGetLastError();
+}
+
+// Adds the K slices' partial rows in slice order and runs the epilogue. A warp
+// takes one row's block of 128 output columns, 4 per lane, so a block of the
+// 8-bit pre-activation is one warp's; the partial rows come from L2, where the
+// product has just left them.
+template <bool GATED, bool KEEP>
+__global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  const int64_t blocks = (a.out_cols + 127) / 128;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= a.m * blocks) return;
+  const int64_t row = unit / blocks, kb = unit - row * blocks;
+  const int64_t O = a.out_cols, c = kb * 128 + 4 * lane;
+  const int H = GATED ? a.n_tile / 2 : a.n_tile;
+  const int64_t ld = (int64_t)a.n_tiles * a.n_tile, step = a.m * ld;
+  const LinearEpilogue& ep = a.ep;
+  const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(ep.bias);
+  float v[GATED ? 2 : 1][4];
+#pragma unroll
+  for (int h = 0; h < (GATED ? 2 : 1); ++h)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[h][j] = 0.f;
+  if (c < O) {
+    const int64_t nt = c / H;
+    const float* p = a.partial + row * ld + nt * a.n_tile + (c - nt * H);
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+      for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(p + s * step + h * H));
+        v[h][0] += f.x;
+        v[h][1] += f.y;
+        v[h][2] += f.z;
+        v[h][3] += f.w;
+      }
+    if (bias)
+#pragma unroll
+      for (int h = 0; h < (GATED ? 2 : 1); ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < O) v[h][j] += __bfloat162float(bias[h * O + c + j]);
+  }
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < O) amax = max(amax, __float_as_uint(v[h][j]) & 0x7fffffffu);
+      const uint32_t code = e8m0_of_amax(__reduce_max_sync(0xffffffffu, amax));
+      const float inv = e8m0_inverse(code);
+      if (lane == 0) ep.z_scale[(h * blocks + kb) * a.m + row] = (uint8_t)code;
+      float s[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = code == kTopScaleCode ? hold_finite(v[h][j] * inv) : v[h][j] * inv;
+      const uint32_t w = e4m3x4(s[0], s[1], s[2], s[3]);
+      uint8_t* z = ep.z8 + (h * a.m + row) * O + c;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < O) z[j] = (uint8_t)(w >> (8 * j));
+    }
+  }
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    y[j] = GATED ? v[0][j] * act_value(v[GATED ? 1 : 0][j], kActSilu) : act_value(v[0][j], ep.act);
+  const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr + c;
+  if (a.vec && c + 4 <= O) {
+    if (ep.residual) {
+      const uint2 w = *reinterpret_cast<const uint2*>(r);
+      const float2 f0 = unpack_bf16(w.x), f1 = unpack_bf16(w.y);
+      y[0] += f0.x;
+      y[1] += f0.y;
+      y[2] += f1.x;
+      y[3] += f1.y;
+    }
+    if (ep.y_f32)
+      *reinterpret_cast<float4*>(static_cast<float*>(ep.y) + row * ep.ldy + c) = make_float4(y[0], y[1], y[2], y[3]);
+    else
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(ep.y) + row * ep.ldy + c) =
+          make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c + j < O) {
+      if (ep.residual) y[j] += __bfloat162float(r[j]);
+      if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + c + j] = y[j];
+      else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + c + j] = __float2bfloat16_rn(y[j]);
+    }
 }
 
 // Tile width and K slices. Cycles per 64 of K and pair, measured on this
 // kernel's main loop: the MMA (2 NT) or the SM's operand intake (16 KB + 64 NT
 // bytes at 68 per cycle); a tile's epilogue hides behind the next tile's
-// products except for the last round. Slices are at least 4 K-blocks deep.
+// products except for the last round. Slices are at least 4 K-blocks deep; joining
+// them costs a launch and moves 8 bytes per value and slice through L2 (about 3
+// KB per cycle).
 LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs) {
   LinearTilePlan best{};
   double best_cost = 1e300;
@@ -511,7 +609,7 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
     for (int s = 1; s <= 16; ++s) {
       if (s > 1 && (k_blocks < 4 * s || tiles * s > pairs)) break;
       const int64_t rounds = (tiles * s + pairs - 1) / pairs;
-      const double cost = (double)rounds * ((k_blocks + s - 1) / s) * block + 1500 + 8.0 * nt + (s > 1 ? 1500 + 300.0 * s : 0);
+      const double cost = (double)rounds * ((k_blocks + s - 1) / s) * block + 1500 + 8.0 * nt + (s > 1 ? 4000 + 8.0 * s * m * tiles / mt * nt / 3000 : 0);
       if (cost < best_cost) {
         best_cost = cost;
         best = {nt, s, tiles};
@@ -553,17 +651,30 @@ static cudaError_t launch_t(const CUtensorMap& tmA, const CUtensorMap& tmB, cons
   const int64_t want = a.units < clusters ? a.units : clusters;
   cfg.gridDim = dim3((unsigned)(2 * want));
   cfg.stream = st;
+  cfg.numAttrs = a.pdl ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, tmA, tmB, a);
 }
 
-cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
-                               const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
+                                  const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
   if (a_mn && b_mn) return launch_t<true, true, false, false>(tmA, tmB, a, num_sms, st);
   if (b_mn) return launch_t<false, true, false, false>(tmA, tmB, a, num_sms, st);
   if (gated) return keep ? launch_t<false, false, true, true>(tmA, tmB, a, num_sms, st)
                          : launch_t<false, false, true, false>(tmA, tmB, a, num_sms, st);
   return keep ? launch_t<false, false, false, true>(tmA, tmB, a, num_sms, st)
               : launch_t<false, false, false, false>(tmA, tmB, a, num_sms, st);
+}
+
+cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
+                               const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+  cudaError_t e = launch_product(a_mn, b_mn, gated, keep && a.splits == 1, tmA, tmB, a, num_sms, st);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  const dim3 grid((unsigned)ceil_div(a.m * ((a.out_cols + 127) / 128), 8)), block(256);
+  if (gated)
+    return keep ? launch_kernel(linear_join_kernel<true, true>, grid, block, 0, st, true, a)
+                : launch_kernel(linear_join_kernel<true, false>, grid, block, 0, st, true, a);
+  return keep ? launch_kernel(linear_join_kernel<false, true>, grid, block, 0, st, true, a)
+              : launch_kernel(linear_join_kernel<false, false>, grid, block, 0, st, true, a);
 }
 
 cudaError_t set_debug_waits_linear(unsigned long long limit_ns, int gate_extra) {

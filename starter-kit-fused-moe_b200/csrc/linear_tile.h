@@ -16,9 +16,9 @@ struct LinearTileArgs {
   int term_blocks;        // of one term
   int splits;
   int64_t units;          // tiles * splits
+  int pdl;                // launched right behind another kernel of the same call
   int vec;                // y (and the residual) can be accessed in 16 bytes
-  float* partial;         // splits > 1: [units][2][n_tile][128] fp32
-  int* arrivals;          // splits > 1: [tiles][2], zero at launch
+  float* partial;         // splits > 1: fp32 [splits][m][n_tiles * n_tile], 16-byte aligned
   LinearEpilogue ep;
 };
 struct LinearTilePlan {
@@ -28,7 +28,23 @@ struct LinearTilePlan {
 LinearTilePlan plan_linear_tile(int64_t m, int64_t out_cols, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs);
 cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
                                const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st);
-cudaError_t launch_pad_rows(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst, int64_t ldd,
-                            cudaStream_t st);
+// One launch that copies up to two matrices into rows TMA can read (base and row
+// stride multiples of 16 bytes).
+struct PadArgs {
+  const void* src[2];
+  void* dst[2];
+  int64_t lds[2], ldd[2], rows[2];
+  int cols[2];
+  int count;
+  void add(const void* s, int64_t ls, int64_t r, int64_t c, void* d, int64_t ld) {
+    src[count] = s;
+    dst[count] = d;
+    lds[count] = ls;
+    ldd[count] = ld;
+    rows[count] = r;
+    cols[count++] = (int)c;
+  }
+};
+cudaError_t launch_pad(const PadArgs& a, cudaStream_t st);
 
 }  // namespace moe

@@ -53,7 +53,7 @@ struct Product {
   moe::LinearTilePlan plan;
   int64_t term_blocks;
   int terms;
-  size_t arrivals, partial, bytes;      // arrivals first
+  size_t partial;      // bytes
 };
 Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gated, bool keep, bool b_mn) {
   Product p{};
@@ -61,16 +61,15 @@ Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gat
   p.terms = terms;
   p.plan = moe::plan_linear_tile(m, out_cols, p.term_blocks * terms, gated, keep, b_mn, pairs());
   if (p.plan.splits > 1) {
-    p.arrivals = up256((size_t)p.plan.tiles * 2 * sizeof(int));
-    p.partial = (size_t)p.plan.tiles * p.plan.splits * 2 * p.plan.n_tile * 128 * sizeof(float);
-    p.bytes = p.arrivals + p.partial;
+    const int cols = gated ? p.plan.n_tile / 2 : p.plan.n_tile;
+    p.partial = (size_t)p.plan.splits * m * ((out_cols + cols - 1) / cols) * p.plan.n_tile * sizeof(float);
   }
   return p;
 }
-// A: [terms][rows][..], term stride in elements; the K slices' arrivals must be zero.
+// A: [terms][rows][..], term stride in elements.
 int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, int64_t m, int64_t out_cols, int64_t k,
                 const void* A, int64_t lda, int64_t term_stride, const void* B, int64_t ldb, int64_t b_rows,
-                const moe::LinearEpilogue& ep, uint8_t* arrivals, uint8_t* partial, cudaStream_t st, const char* what) {
+                const moe::LinearEpilogue& ep, uint8_t* partial, bool pdl, cudaStream_t st, const char* what) {
   moe::LinearTileArgs t{};
   t.m = m;
   t.out_cols = out_cols;
@@ -84,9 +83,9 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.splits = p.plan.splits;
   t.units = p.plan.tiles * t.splits;
   t.ep = ep;
+  t.pdl = pdl;
   const int ysize = ep.y_f32 ? 4 : 2;
   t.vec = aligned(ep.y, 16) && ep.ldy * ysize % 16 == 0 && (!ep.residual || (aligned(ep.residual, 16) && ep.ldr % 8 == 0));
-  t.arrivals = reinterpret_cast<int*>(arrivals);
   t.partial = reinterpret_cast<float*>(partial);
   CUtensorMap ma, mb;
   const uint32_t half = (uint32_t)t.n_tile / 2;
@@ -104,18 +103,20 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
 // Workspace of a forward product.
 struct LinearPlan {
   Product prod;
-  bool pad_x, pad_w;
+  bool small, pad_x, pad_w;
   int64_t ldp;
   size_t x, w, total;
 };
 LinearPlan linear_plan(const MoeLinearArgs& a) {
   LinearPlan p{};
+  p.small = a.m <= moe::kSmallTokens && a.z8 == nullptr;
+  if (p.small) return p;
   const bool gated = a.activation == MOE_ACT_SWIGLU;
   p.prod = plan_product(a.m, gated ? a.n / 2 : a.n, a.k, 1, gated, a.z8 != nullptr, false);
   p.pad_x = !tma_ready(a.x, a.ldx);
   p.pad_w = !tma_ready(a.weight, a.ldw);
   p.ldp = up8(a.k);
-  size_t o = up256(p.prod.bytes);
+  size_t o = up256(p.prod.partial);
   p.x = o;
   if (p.pad_x) o += up256((size_t)a.m * p.ldp * 2);
   p.w = o;
@@ -124,14 +125,13 @@ LinearPlan linear_plan(const MoeLinearArgs& a) {
   return p;
 }
 
-// Workspace of the gradient entry: K-slice arrivals and partials of both
-// products (the partials shared), dz, x^, the padded weights, column sums.
+// Workspace of the gradient entry: K-slice partials (shared by the products), dz, x^, the padded weights, column sums.
 struct GradPlan {
   bool need_dz, direct, pad_w;
   int terms, chunks;
   int64_t ldz, ldk;
   Product px, pw;
-  size_t arrivals, partial, dz, xhat, w, colsum, total;
+  size_t dz, xhat, w, colsum, total;      // the partials come first
 };
 GradPlan grad_plan(const MoeLinearGradArgs& a) {
   GradPlan p{};
@@ -145,18 +145,14 @@ GradPlan grad_plan(const MoeLinearGradArgs& a) {
   size_t partial = 0;
   if (a.grad_x) {
     p.px = plan_product(a.m, a.k, a.n, p.terms, false, false, true);
-    p.arrivals += p.px.arrivals;
     partial = p.px.partial;
     p.pad_w = !tma_ready(a.weight, a.ldw);
   }
   if (a.grad_weight) {
     p.pw = plan_product(a.n, a.k, a.m, p.terms, false, false, true);
-    p.arrivals += p.pw.arrivals;
     if (p.pw.partial > partial) partial = p.pw.partial;
   }
-  size_t o = p.arrivals;
-  p.partial = o;
-  o += up256(partial);
+  size_t o = up256(partial);
   p.dz = o;
   if (p.need_dz) o += up256((size_t)a.m * p.ldz * 2 * p.terms);
   p.xhat = o;
@@ -195,18 +191,20 @@ int moe_linear_run(const MoeLinearArgs* a, void* stream) {
     return workspace_error("linear", p.total, a->workspace_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  cudaError_t e = cudaSuccess;
-  if (p.prod.plan.splits > 1) e = cudaMemsetAsync(ws, 0, p.prod.arrivals, st);
-  if (e == cudaSuccess && p.pad_x) e = moe::launch_pad_rows(a->x, a->ldx, a->m, a->k, ws + p.x, p.ldp, st);
-  if (e == cudaSuccess && p.pad_w) e = moe::launch_pad_rows(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldp, st);
-  if (e != cudaSuccess) return done(e, "linear: preparing the operands");
   moe::LinearEpilogue ep{a->bias, a->residual, a->y, static_cast<uint8_t*>(a->z8), static_cast<uint8_t*>(a->z_scale),
                          a->ldr, a->ldy, a->activation, a->y_f32};
+  if (p.small) return done(moe::launch_linear_small(a->x, a->ldx, a->weight, a->ldw, a->m, a->k, a->n, ep, st), "linear product");
+  moe::PadArgs pads{};
+  if (p.pad_x) pads.add(a->x, a->ldx, a->m, a->k, ws + p.x, p.ldp);
+  if (p.pad_w) pads.add(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldp);
+  cudaError_t e = moe::launch_pad(pads, st);
+  if (e != cudaSuccess) return done(e, "linear: preparing the operands");
+  const bool launched = pads.count > 0;
   const void* x = p.pad_x ? ws + p.x : a->x;
   const void* w = p.pad_w ? ws + p.w : a->weight;
   const int64_t ldx = p.pad_x ? p.ldp : a->ldx;
   return run_product(p.prod, false, false, a->activation == MOE_ACT_SWIGLU, a->z8 != nullptr, a->m, O, a->k, x, ldx,
-                     a->m * ldx, w, p.pad_w ? p.ldp : a->ldw, a->n, ep, ws, ws + p.prod.arrivals, st, "linear product");
+                     a->m * ldx, w, p.pad_w ? p.ldp : a->ldw, a->n, ep, ws, launched, st, "linear product");
 }
 
 size_t moe_linear_grad_workspace_bytes(const MoeLinearGradArgs* a) {
@@ -241,8 +239,11 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
     return workspace_error("linear gradient", p.total, a->workspace_bytes);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   cudaError_t e = cudaSuccess;
-  if (p.arrivals) e = cudaMemsetAsync(ws, 0, p.arrivals, st);
-  if (e != cudaSuccess) return done(e, "linear gradient: clearing the slice counters");
+  moe::PadArgs pads{};
+  if (p.pad_w) pads.add(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldk);
+  e = moe::launch_pad(pads, st);
+  if (e != cudaSuccess) return done(e, "linear gradient: preparing the operands");
+  bool launched = pads.count > 0;     // later kernels may start behind an earlier one of this call
   if (p.need_dz || a->grad_bias) {
     moe::ActGradArgs g{};
     g.dy = a->grad_y;
@@ -257,35 +258,30 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
     g.act = a->activation;
     g.dy_f32 = a->grad_y_f32;
     g.terms = p.terms;
-    e = moe::launch_act_grad(g, st);
+    e = moe::launch_act_grad(g, launched, st);
+    launched = true;
     if (e == cudaSuccess && a->grad_bias)
       e = moe::launch_colsum_finish(g.colsum, p.chunks, a->n, a->grad_bias, a->grad_f32 != 0, st);
     if (e != cudaSuccess) return done(e, "activation gradient");
   }
   const void* dz = p.direct ? a->grad_y : ws + p.dz;
   const int64_t ldz = p.direct ? a->ldg : p.ldz, term_stride = a->m * ldz;
-  uint8_t* partial = ws + p.partial;
   if (a->grad_x) {
-    const void* w = a->weight;
-    int64_t ldw = a->ldw;
-    if (p.pad_w) {
-      e = moe::launch_pad_rows(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldk, st);
-      if (e != cudaSuccess) return done(e, "linear gradient: preparing the weights");
-      w = ws + p.w;
-      ldw = p.ldk;
-    }
+    const void* w = p.pad_w ? ws + p.w : a->weight;
+    const int64_t ldw = p.pad_w ? p.ldk : a->ldw;
     moe::LinearEpilogue ep{nullptr, nullptr, a->grad_x, nullptr, nullptr, 0, a->k, MOE_ACT_NONE, a->grad_f32};
     if (int rc = run_product(p.px, false, true, false, false, a->m, a->k, a->n, dz, ldz, term_stride, w, ldw, a->n, ep,
-                             ws, partial, st, "input gradient"))
+                             ws, launched, st, "input gradient"))
       return rc;
+    launched = true;
   }
   if (a->grad_weight) {
     e = moe::launch_restore(static_cast<const uint8_t*>(a->x8), static_cast<const uint8_t*>(a->x_scale), 1, a->m, a->k,
-                            ws + p.xhat, false, p.ldk, st);
+                            ws + p.xhat, false, p.ldk, launched, st);
     if (e != cudaSuccess) return done(e, "restoring the input checkpoint");
     moe::LinearEpilogue ep{nullptr, nullptr, a->grad_weight, nullptr, nullptr, 0, a->k, MOE_ACT_NONE, a->grad_f32};
     if (int rc = run_product(p.pw, true, true, false, false, a->n, a->k, a->m, dz, ldz, term_stride, ws + p.xhat, p.ldk,
-                             a->m, ep, ws + p.px.arrivals, partial, st, "weight gradient"))
+                             a->m, ep, ws, true, st, "weight gradient"))
       return rc;
   }
   return MOE_OK;
@@ -310,7 +306,7 @@ int moe_restore_activations(const void* q, const void* scale, int64_t batch, int
   if (batch == 0 || rows == 0 || cols == 0) return MOE_OK;
   if (!q || !scale || !out || !aligned(out, out_f32 ? 4 : 2)) return bad("restore: NULL or misaligned pointer");
   return done(moe::launch_restore(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), batch, rows, cols,
-                                  out, out_f32 != 0, cols, static_cast<cudaStream_t>(stream)),
+                                  out, out_f32 != 0, cols, false, static_cast<cudaStream_t>(stream)),
               "restore");
 }
 

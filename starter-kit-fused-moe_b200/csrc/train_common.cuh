@@ -70,13 +70,16 @@ __device__ __forceinline__ float act_value(float z, int act) {
     default: return z;
   }
 }
+// 1 / (1 + e^-z) with the hardware exponential and reciprocal.
+__device__ __forceinline__ float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+template <bool FAST>
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case kActRelu: return z > 0.f ? 1.f : 0.f;
     case kActGelu:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * (FAST ? __expf(-0.5f * z * z) : expf(-0.5f * z * z));
     case kActSilu: {
-      const float s = sigmoid_f(z);
+      const float s = FAST ? sigmoid_fast(z) : sigmoid_f(z);
       return s * (1.0f + z * (1.0f - s));
     }
     default: return 1.f;
