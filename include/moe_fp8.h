@@ -265,7 +265,7 @@ int moe_fp8_ep_peer_read_error(void* base, void* stream, int32_t* bits);
 /* ---- Dense products around the routed experts (the router's gate, the shared
  * expert), 8-bit activation checkpoints and gradients for training them. No
  * counterpart in the reference, which holds the routed operator alone. Sizes
- * are free (m tokens >= 0, k and n >= 1); matrices are row-major with a row
+ * are free (m tokens in [0, 2^30], k and n in [1, 2^23]); matrices are row-major with a row
  * stride in elements and need the alignment of their type only. Every entry
  * works on the current device, asynchronously on `stream`, and keeps nothing
  * between calls; `workspace` is device scratch, 256-byte aligned, that calls in

@@ -119,6 +119,36 @@ def build_tvm_ffi(force: bool = False) -> pathlib.Path | None:
     return TVM_LIB
 
 
+LAYER_SRC = HERE / "binding" / "layer_binding.cc"
+LAYER_LIB = HERE / "moe_b200_layer.so"
+
+
+def build_layer_binding(force: bool = False) -> pathlib.Path:
+    """Build the Python binding of the layer operators (layer.py) over libmoe_b200.so."""
+    build()
+    if not force and LAYER_LIB.exists() and \
+            LAYER_LIB.stat().st_mtime >= max(LAYER_SRC.stat().st_mtime, (INCLUDE / "moe_fp8.h").stat().st_mtime):
+        return LAYER_LIB
+    import sysconfig
+
+    import torch
+    root = pathlib.Path(torch.__file__).parent
+    cuda = pathlib.Path(nvcc()).parent.parent
+    tmp = LAYER_LIB.with_name(LAYER_LIB.name + ".tmp")
+    cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", str(LAYER_SRC), "-o", str(tmp),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", str(INCLUDE), "-isystem", str(root / "include"), "-isystem", str(root / "include/torch/csrc/api/include"),
+           "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-L", str(HERE), "-lmoe_b200", "-L", str(root / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + str(root / "lib")]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("layer binding build failed")
+    os.replace(tmp, LAYER_LIB)
+    return LAYER_LIB
+
+
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--debug", action="store_true")
@@ -126,4 +156,5 @@ if __name__ == "__main__":
     a = ap.parse_args()
     print(build(debug=a.debug, verbose=a.verbose, force=True))
     if not a.debug:
+        print(build_layer_binding(force=True))
         print(build_tvm_ffi(force=True))

@@ -24,14 +24,15 @@ constexpr int kAgRows = 64, kAgCols = 256;
 // 2^-20 of 1 + |z|; the exact ones bound the kernel by arithmetic (121 us instead
 // of 60 at 16384 x 4096) and serve the two-term form.
 template <int HALVES, bool F32, bool VEC, bool FAST>
-__global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
+__global__ void __launch_bounds__(256, 2) act_grad_kernel(ActGradArgs a, int O) {
   __shared__ float red[8][kAgCols];
+  __shared__ float scales[HALVES][2][kAgRows];
   pdl_wait();
   pdl_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t r0 = (int64_t)blockIdx.y * kAgRows;
+  const int64_t r0 = (int64_t)blockIdx.x * kAgRows;
   const int64_t rend = min(r0 + kAgRows, (int64_t)a.m);
-  const int64_t c0 = (int64_t)blockIdx.x * kAgCols;
+  const int64_t c0 = (int64_t)blockIdx.y * kAgCols;
   auto col = [&](int j) -> int64_t { return VEC ? c0 + 8 * tx + j : c0 + tx + 32 * j; };
   const int64_t nb = (O + 127) / 128;
   __nv_bfloat16* dz = static_cast<__nv_bfloat16*>(a.dz);
@@ -42,106 +43,139 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[h][j] = 0.f;
 
-#pragma unroll 2
-  for (int64_t row = r0 + ty; row < rend; row += 8) {
-    float dy[8], z[HALVES][8];
+  // the chunk's block scales: 2 blocks of 128 columns by 64 rows per half
+  if (a.z8 != nullptr)
+    for (int i = threadIdx.x; i < HALVES * 2 * kAgRows; i += 256) {
+      const int64_t row = r0 + i % kAgRows, kb = 2 * blockIdx.y + (i / kAgRows) % 2;
+      scales[i / (2 * kAgRows)][(i / kAgRows) % 2][i % kAgRows] =
+          row < rend && kb < nb ? e8m0_value(a.z_scale[((int64_t)(i / (2 * kAgRows)) * nb + kb) * a.m + row]) : 0.f;
+    }
+  __syncthreads();
+
+  // VEC: four rows' loads are in flight together
+  constexpr int U = VEC ? 4 : 1;
+  struct Raw {
+    uint32_t dy[F32 ? 8 : 4];
+    uint2 z[HALVES];
+  };
+#pragma unroll 1
+  for (int64_t row0 = r0 + ty; row0 < rend; row0 += 8 * U) {
+    Raw raw[U];
     if constexpr (VEC) {
-      const bool in = col(0) < O;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dy[j] = 0.f;
-      if (in) {
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = row0 + 8 * u;
+#pragma unroll
+        for (int j = 0; j < (F32 ? 8 : 4); ++j) raw[u].dy[j] = 0;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) raw[u].z[h] = make_uint2(0, 0);
+        if (row < rend && col(0) < O) {
+          const uint4* p = F32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(a.dy) + row * a.ldg + col(0))
+                               : reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.dy) + row * a.ldg + col(0));
+#pragma unroll
+          for (int i = 0; i < (F32 ? 2 : 1); ++i) {
+            const uint4 w = __ldg(p + i);
+            raw[u].dy[4 * i] = w.x;
+            raw[u].dy[4 * i + 1] = w.y;
+            raw[u].dy[4 * i + 2] = w.z;
+            raw[u].dy[4 * i + 3] = w.w;
+          }
+          if (a.z8 != nullptr)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+              raw[u].z[h] = __ldg(reinterpret_cast<const uint2*>(a.z8 + ((int64_t)h * a.m + row) * O + col(0)));
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row0 + 8 * u;
+      if (row >= rend) break;
+      float dy[8], z[HALVES][8];
+      if constexpr (VEC) {
         if constexpr (F32) {
-          const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.dy) + row * a.ldg + col(0));
-          const float4 u = __ldg(p), v = __ldg(p + 1);
-          dy[0] = u.x; dy[1] = u.y; dy[2] = u.z; dy[3] = u.w;
-          dy[4] = v.x; dy[5] = v.y; dy[6] = v.z; dy[7] = v.w;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dy[j] = __uint_as_float(raw[u].dy[j]);
         } else {
-          const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.dy) + row * a.ldg + col(0)));
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack_bf16(w[j]);
+            const float2 f = unpack_bf16(raw[u].dy[j]);
             dy[2 * j] = f.x;
             dy[2 * j + 1] = f.y;
           }
         }
-      }
-    } else {
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        dy[j] = 0.f;
-        if (col(j) < O)
-          dy[j] = F32 ? static_cast<const float*>(a.dy)[row * a.ldg + col(j)]
-                      : (float)static_cast<const __nv_bfloat16*>(a.dy)[row * a.ldg + col(j)];
+        for (int j = 0; j < 8; ++j) {
+          dy[j] = 0.f;
+          if (col(j) < O)
+            dy[j] = F32 ? static_cast<const float*>(a.dy)[row * a.ldg + col(j)]
+                        : (float)static_cast<const __nv_bfloat16*>(a.dy)[row * a.ldg + col(j)];
+        }
       }
-    }
-    if (a.z8 != nullptr) {
+      if (a.z8 != nullptr) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          if constexpr (VEC) {
+            const float s = scales[h][tx >> 4][row - r0];        // 8 aligned columns share a block
+            const uint2 w = raw[u].z[h];
+            const float2 p0 = e4m3x2_value(w.x & 0xffffu), p1 = e4m3x2_value(w.x >> 16);
+            const float2 p2 = e4m3x2_value(w.y & 0xffffu), p3 = e4m3x2_value(w.y >> 16);
+            z[h][0] = p0.x * s; z[h][1] = p0.y * s; z[h][2] = p1.x * s; z[h][3] = p1.y * s;
+            z[h][4] = p2.x * s; z[h][5] = p2.y * s; z[h][6] = p3.x * s; z[h][7] = p3.y * s;
+          } else {
+            const uint8_t* zr = a.z8 + ((int64_t)h * a.m + row) * O;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              z[h][j] = col(j) < O ? e4m3_value(zr[col(j)]) * scales[h][j >> 2][row - r0] : 0.f;
+          }
+        }
+        if constexpr (HALVES == 2) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float b = z[1][j], s = FAST ? sigmoid_fast(b) : sigmoid_f(b), av = z[0][j];
+            // __fmul_rn: dz is a rounded value, never the inside of an FMA, so the sums do not
+            // depend on which outputs are asked for
+            z[0][j] = __fmul_rn(dy[j], b * s);
+            z[1][j] = __fmul_rn(dy[j] * av, s * (1.0f + b * (1.0f - s)));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) z[0][j] = __fmul_rn(dy[j], act_slope<FAST>(z[0][j], a.act));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[0][j] = dy[j];
+      }
 #pragma unroll
       for (int h = 0; h < HALVES; ++h) {
-        const uint8_t* zr = a.z8 + ((int64_t)h * a.m + row) * O;
-        const uint8_t* sr = a.z_scale + (int64_t)h * nb * a.m + row;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[h][j] += z[h][j];
+        if (dz == nullptr) continue;
+        __nv_bfloat16* out = dz + row * a.ldz + (int64_t)h * O;
+        float lo[8];
+        if constexpr (!FAST)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float hi = __bfloat162float(__float2bfloat16_rn(z[h][j]));
+          lo[j] = isfinite(hi) ? z[h][j] - hi : 0.f;       // a non-finite value is whole in the first term
+        }
         if constexpr (VEC) {
-          uint2 raw = make_uint2(0, 0);
-          float s = 1.f;
           if (col(0) < O) {
-            raw = __ldg(reinterpret_cast<const uint2*>(zr + col(0)));
-            s = e8m0_value(sr[(col(0) >> 7) * a.m]);       // 8 aligned columns share a block
+            *reinterpret_cast<uint4*>(out + col(0)) = make_uint4(pack_bf16(z[h][0], z[h][1]), pack_bf16(z[h][2], z[h][3]),
+                                                                 pack_bf16(z[h][4], z[h][5]), pack_bf16(z[h][6], z[h][7]));
+            if (!FAST && a.terms == 2)
+              *reinterpret_cast<uint4*>(out + term + col(0)) =
+                  make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
           }
-          const float2 p0 = e4m3x2_value(raw.x & 0xffffu), p1 = e4m3x2_value(raw.x >> 16);
-          const float2 p2 = e4m3x2_value(raw.y & 0xffffu), p3 = e4m3x2_value(raw.y >> 16);
-          z[h][0] = p0.x * s; z[h][1] = p0.y * s; z[h][2] = p1.x * s; z[h][3] = p1.y * s;
-          z[h][4] = p2.x * s; z[h][5] = p2.y * s; z[h][6] = p3.x * s; z[h][7] = p3.y * s;
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            z[h][j] = col(j) < O ? e4m3_value(zr[col(j)]) * e8m0_value(sr[(col(j) >> 7) * a.m]) : 0.f;
+            if (col(j) < O) {
+              out[col(j)] = __float2bfloat16_rn(z[h][j]);
+              if (!FAST && a.terms == 2) out[term + col(j)] = __float2bfloat16_rn(lo[j]);
+            }
         }
-      }
-      if constexpr (HALVES == 2) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float b = z[1][j], s = FAST ? sigmoid_fast(b) : sigmoid_f(b), av = z[0][j];
-          // __fmul_rn: dz is a rounded value, never the inside of an FMA, so the sums do not
-          // depend on which outputs are asked for
-          z[0][j] = __fmul_rn(dy[j], b * s);
-          z[1][j] = __fmul_rn(dy[j] * av, s * (1.0f + b * (1.0f - s)));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[0][j] = __fmul_rn(dy[j], act_slope<FAST>(z[0][j], a.act));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) z[0][j] = dy[j];
-    }
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum[h][j] += z[h][j];
-      if (dz == nullptr) continue;
-      __nv_bfloat16* out = dz + row * a.ldz + (int64_t)h * O;
-      float lo[8];
-      if constexpr (!FAST)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float hi = __bfloat162float(__float2bfloat16_rn(z[h][j]));
-        lo[j] = isfinite(hi) ? z[h][j] - hi : 0.f;       // a non-finite value is whole in the first term
-      }
-      if constexpr (VEC) {
-        if (col(0) < O) {
-          *reinterpret_cast<uint4*>(out + col(0)) = make_uint4(pack_bf16(z[h][0], z[h][1]), pack_bf16(z[h][2], z[h][3]),
-                                                               pack_bf16(z[h][4], z[h][5]), pack_bf16(z[h][6], z[h][7]));
-          if (!FAST && a.terms == 2)
-            *reinterpret_cast<uint4*>(out + term + col(0)) =
-                make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col(j) < O) {
-            out[col(j)] = __float2bfloat16_rn(z[h][j]);
-            if (!FAST && a.terms == 2) out[term + col(j)] = __float2bfloat16_rn(lo[j]);
-          }
       }
     }
   }
@@ -155,7 +189,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a, int O) {
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x];
-    if (c0 + threadIdx.x < O) a.colsum[(int64_t)blockIdx.y * a.n + (int64_t)h * O + c0 + threadIdx.x] = t;
+    if (c0 + threadIdx.x < O) a.colsum[(int64_t)blockIdx.x * a.n + (int64_t)h * O + c0 + threadIdx.x] = t;
   }
 }
 
@@ -190,7 +224,7 @@ cudaError_t launch_act_grad(const ActGradArgs& a, bool pdl, cudaStream_t st) {
   const int O = two ? a.n / 2 : a.n;
   const bool vec = al(a.dy, 16) && a.ldg % (a.dy_f32 ? 4 : 8) == 0 && O % 8 == 0 && (!a.z8 || al(a.z8, 8)) &&
                    (!a.dz || (al(a.dz, 16) && a.ldz % 8 == 0));
-  const dim3 grid((unsigned)ceil_div(O, kAgCols), (unsigned)act_grad_chunks(a.m, a.n));
+  const dim3 grid((unsigned)act_grad_chunks(a.m, a.n), (unsigned)ceil_div(O, kAgCols));
 #define MOE_AG(H, F, V)                                                                                      \
   return a.terms == 1 ? launch_kernel(act_grad_kernel<H, F, V, true>, grid, dim3(256), 0, st, pdl, a, O) \
                       : launch_kernel(act_grad_kernel<H, F, V, false>, grid, dim3(256), 0, st, pdl, a, O)

@@ -20,8 +20,9 @@
 // accumulators of NT columns in TMEM let a tile's epilogue overlap the next
 // tile's products. Persistent grid, one pair per two SMs; tiles are walked in
 // bands of 8 row tiles so that the tiles in flight share both operands in L2.
-// When there are fewer tiles than pairs, K is split: the slices leave fp32
-// partial rows in the workspace and a second kernel, launched to start as this
+// The tiles that do not fill a last round of the pairs (all of them, when there
+// are fewer tiles than pairs) are cut into K slices: the slices leave fp32
+// partial tiles in the workspace and a second kernel, launched to start as this
 // one ends, adds them in slice order and runs the epilogue on all SMs. (Letting
 // the slice that arrives last do it kept the other SMs idle: 36 instead of 20 us
 // at 1037 x 1111 x 515.)
@@ -37,6 +38,7 @@ namespace moe {
 constexpr int kLtStages = 6, kLtStageBytes = 32768, kLtTileA = 16384;
 constexpr int kLtThreads = 320, kLtEpiWarps = 8, kLtTmemCols = 512;
 constexpr int kLtBand = 8;
+constexpr int kLtStagePitch = 80;    // 64-byte row pieces; 80 keeps 16-byte accesses of 8 rows free of bank conflicts
 
 struct LinearTileSmem {
   uint64_t full[kLtStages];
@@ -46,7 +48,7 @@ struct LinearTileSmem {
   uint32_t tmem_base;
   int abort_flag;
   float amax[2][2][2][128];      // [tile parity][column half][gate, up][row]
-  float stage[kLtEpiWarps][32][17];
+  alignas(16) uint8_t stage[kLtEpiWarps][32 * kLtStagePitch];
 };
 constexpr size_t kLtSmem = 1024 + (size_t)kLtStages * kLtStageBytes + sizeof(LinearTileSmem);
 static_assert(kLtSmem <= 232448, "shared memory budget");
@@ -89,22 +91,34 @@ struct LtUnit {
   int mt, nt, kb0, kb1, slice;
   int64_t tile;
 };
+// Row and column tile of a tile index: bands of 8 row tiles, rows fastest.
+__device__ __forceinline__ void lt_place(const LinearTileArgs& a, int64_t tile, int& mt, int& nt) {
+  const int64_t per_band = (int64_t)kLtBand * a.n_tiles;
+  const int band = (int)(tile / per_band);
+  const int in = (int)(tile - band * per_band);
+  const int rows = min(kLtBand, a.m_tiles - band * kLtBand);
+  nt = in / rows;
+  mt = band * kLtBand + in - nt * rows;
+}
 __device__ __forceinline__ LtUnit lt_unit(const LinearTileArgs& a, int64_t u) {
   LtUnit r;
-  r.tile = u / a.splits;
-  r.slice = (int)(u - r.tile * a.splits);
-  const int64_t per_band = (int64_t)kLtBand * a.n_tiles;
-  const int band = (int)(r.tile / per_band);
-  const int64_t in = r.tile - band * per_band;
-  const int rows = min(kLtBand, a.m_tiles - band * kLtBand);
-  r.nt = (int)(in / rows);
-  r.mt = band * kLtBand + (int)(in - (int64_t)r.nt * rows);
-  r.kb0 = (int)((int64_t)r.slice * a.k_blocks / a.splits);
-  r.kb1 = (int)((int64_t)(r.slice + 1) * a.k_blocks / a.splits);
+  if (u < a.full_tiles) {
+    r.tile = u;
+    r.slice = -1;
+    r.kb0 = 0;
+    r.kb1 = a.k_blocks;
+  } else {
+    const int64_t v = u - a.full_tiles, i = v / a.splits;
+    r.tile = a.full_tiles + i;
+    r.slice = (int)(v - i * a.splits);
+    r.kb0 = (int)((int64_t)r.slice * a.k_blocks / a.splits);
+    r.kb1 = (int)((int64_t)(r.slice + 1) * a.k_blocks / a.splits);
+  }
+  lt_place(a, r.tile, r.mt, r.nt);
   return r;
 }
 
-// ---- epilogue pieces, 16 columns of one row per thread
+// ---- epilogue pieces, 16 or 32 columns of one row per thread
 __device__ __forceinline__ void lt_bias16(const __nv_bfloat16* bias, int64_t c, int64_t end, float* v) {
   if (c + 16 <= end && (reinterpret_cast<uintptr_t>(bias + c) & 15) == 0) {
     const uint4 a = __ldg(reinterpret_cast<const uint4*>(bias + c)), b = __ldg(reinterpret_cast<const uint4*>(bias + c) + 1);
@@ -121,71 +135,47 @@ __device__ __forceinline__ void lt_bias16(const __nv_bfloat16* bias, int64_t c, 
       if (c + i < end) v[i] += __bfloat162float(bias[c + i]);
   }
 }
-__device__ __forceinline__ void lt_act16(float* v, int act) {
+__device__ __forceinline__ void lt_bias32(const __nv_bfloat16* bias, int64_t c, int64_t end, float* v) {
+  lt_bias16(bias, c, end, v);
+  lt_bias16(bias, c + 16, end, v + 16);
+}
+__device__ __forceinline__ void lt_act32(float* v, int act) {
   if (act == kActNone) return;
   if (act == kActRelu) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = act_value(v[i], kActRelu);
+    for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActRelu);
   } else if (act == kActGelu) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = act_value(v[i], kActGelu);
+    for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActGelu);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = act_value(v[i], kActSilu);
+    for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActSilu);
   }
 }
-// y[row, c .. c + 16) = v + residual (columns below `end` only). The residual is
-// read before the same values of y are written by the same thread, so y may be
-// the residual.
-__device__ __forceinline__ void lt_store16(const LinearEpilogue& ep, int64_t row, int64_t c, int64_t end, float* v) {
-  const bool whole = c + 16 <= end;
-  if (ep.residual != nullptr) {
-    const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr + c;
-    if (whole) {
-      const uint4 a = *reinterpret_cast<const uint4*>(r), b = *(reinterpret_cast<const uint4*>(r) + 1);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// Stores of a warp's 32 rows go through shared memory: a lane holds a row, so
+// direct stores touch 32 lines with 16 bytes each, and a tile's epilogue took
+// longer than a short contraction (71 us for the gate's input gradient).
+
+// The warp's staged 64-byte row pieces to 64 bytes of `rows` rows each.
+__device__ __forceinline__ void lt_copy_out(const uint8_t* stage, uint8_t* dst, int64_t pitch, int rows, int lane) {
+  __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 f = unpack_bf16(w[i]);
-        v[2 * i] += f.x;
-        v[2 * i + 1] += f.y;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (c + i < end) v[i] += __bfloat162float(r[i]);
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2), o = 16 * (lane & 3);
+    if (r < rows) *reinterpret_cast<uint4*>(dst + r * pitch + o) = *reinterpret_cast<const uint4*>(stage + r * kLtStagePitch + o);
   }
-  if (ep.y_f32) {
-    float* y = static_cast<float*>(ep.y) + row * ep.ldy + c;
-    if (whole) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(y)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (c + i < end) y[i] = v[i];
-    }
-  } else {
-    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(ep.y) + row * ep.ldy + c;
-    if (whole) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        reinterpret_cast<uint4*>(y)[i] = make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
-                                                    pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (c + i < end) y[i] = __float2bfloat16_rn(v[i]);
-    }
-  }
+  __syncwarp();
 }
-// The same for a warp's 32 rows from `row0` when y or the residual cannot be
-// accessed in 16 bytes: through shared memory, so that 16 lanes take neighbouring
-// columns of a row (a lane per row costs a memory transaction per element: the
-// odd-sized 1037 x 1111 x 515 product took 45 us that way).
-__device__ __forceinline__ void lt_store_staged(const LinearEpilogue& ep, float (*stage)[17], int64_t row0, int rows,
-                                                int64_t c, int64_t end, const float* v, int lane) {
+__device__ __forceinline__ void lt_stage_f32(uint8_t* stage, const float* v, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    reinterpret_cast<float4*>(stage + lane * kLtStagePitch)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+// 16 columns element by element (edges, rows that 16-byte accesses cannot
+// reach): 16 lanes take neighbouring columns of a row.
+__device__ __forceinline__ void lt_store16_any(const LinearEpilogue& ep, uint8_t* stage8, int64_t row0, int rows, int64_t c,
+                                               int64_t end, const float* v, int lane) {
+  float(*stage)[17] = reinterpret_cast<float(*)[17]>(stage8);
 #pragma unroll
   for (int i = 0; i < 16; ++i) stage[lane][i] = v[i];
   __syncwarp();
@@ -202,26 +192,78 @@ __device__ __forceinline__ void lt_store_staged(const LinearEpilogue& ep, float 
   }
   __syncwarp();
 }
-// Largest magnitude (as bits) of the columns below `end`.
-__device__ __forceinline__ uint32_t lt_amax16(const float* v, int64_t c, int64_t end, uint32_t amax) {
+// y[row0 .., c .. c + 32) = v + residual for the warp's first `rows` rows,
+// columns below `end`. The warp reads a piece of the residual before it writes
+// the same piece of y, so y may be the residual. All lanes call.
+__device__ __forceinline__ void lt_store32(const LinearEpilogue& ep, int vec, uint8_t* stage, int64_t row0, int rows,
+                                           int64_t c, int64_t end, float* v, int lane) {
+  if (!vec || c + 32 > end) {
+    lt_store16_any(ep, stage, row0, rows, c, end, v, lane);
+    if (c + 16 < end) lt_store16_any(ep, stage, row0, rows, c + 16, end, v + 16, lane);
+    return;
+  }
+  uint8_t* mine = stage + lane * kLtStagePitch;
+  if (ep.residual != nullptr) {
+    const uint8_t* r = reinterpret_cast<const uint8_t*>(static_cast<const __nv_bfloat16*>(ep.residual) + row0 * ep.ldr + c);
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const int rr = 8 * i + (lane >> 2), o = 16 * (lane & 3);
+      if (rr < rows)
+        *reinterpret_cast<uint4*>(stage + rr * kLtStagePitch + o) = *reinterpret_cast<const uint4*>(r + rr * ep.ldr * 2 + o);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 a = reinterpret_cast<const uint4*>(mine)[i];
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack_bf16(w[j]);
+        v[8 * i + 2 * j] += f.x;
+        v[8 * i + 2 * j + 1] += f.y;
+      }
+    }
+    __syncwarp();
+  }
+  if (ep.y_f32) {
+    uint8_t* y = reinterpret_cast<uint8_t*>(static_cast<float*>(ep.y) + row0 * ep.ldy + c);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      lt_stage_f32(stage, v + 16 * h, lane);
+      lt_copy_out(stage, y + 64 * h, ep.ldy * 4, rows, lane);
+    }
+  } else {
+    uint8_t* y = reinterpret_cast<uint8_t*>(static_cast<__nv_bfloat16*>(ep.y) + row0 * ep.ldy + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<uint4*>(mine)[i] = make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+                                                     pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+    lt_copy_out(stage, y, ep.ldy * 2, rows, lane);
+  }
+}
+// Largest magnitude (as bits) of the columns below `end`.
+__device__ __forceinline__ uint32_t lt_amax32(const float* v, int64_t c, int64_t end, uint32_t amax) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
     if (c + i < end) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
   return amax;
 }
-__device__ __forceinline__ void lt_store_z16(uint8_t* z, int64_t c, int64_t end, const float* v, uint32_t code) {
+__device__ __forceinline__ void lt_store_z32(uint8_t* z, int64_t c, int64_t end, const float* v, uint32_t code) {
   const float inv = e8m0_inverse(code);
-  float s[16];
+  uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = code == kTopScaleCode ? hold_finite(v[i] * inv) : v[i] * inv;
-  uint32_t w[4];
+  for (int i = 0; i < 8; ++i) {
+    float s[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = e4m3x4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-  if (c + 16 <= end && (reinterpret_cast<uintptr_t>(z + c) & 15) == 0) {
-    *reinterpret_cast<uint4*>(z + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < 4; ++j) s[j] = code == kTopScaleCode ? hold_finite(v[4 * i + j] * inv) : v[4 * i + j] * inv;
+    w[i] = e4m3x4(s[0], s[1], s[2], s[3]);
+  }
+  if (c + 32 <= end && (reinterpret_cast<uintptr_t>(z + c) & 15) == 0) {
+    reinterpret_cast<uint4*>(z + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(z + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 32; ++i)
       if (c + i < end) z[c + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
   }
 }
@@ -370,24 +412,27 @@ __global__ void __launch_bounds__(kLtThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&S.tempty[b]), 0));
       };
-      auto from_tmem = [&](int col, float* v) {
+      auto from_tmem = [&](int col, float* v) {          // 32 columns
         if (ok) {
           tmem_ld16(acc + col, v);
+          tmem_ld16(acc + col + 16, v + 16);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = NAN;
+          for (int i = 0; i < 32; ++i) v[i] = NAN;
         }
       };
-      if (a.splits > 1) {                                // fp32 partial row, in tile order
-        float* p = a.partial + ((int64_t)x.slice * a.m + row) * ((int64_t)a.n_tiles * NT) + (int64_t)x.nt * NT;
-        for (int c = g * H; c < (g + 1) * H; c += 16) {
-          float v[16];
+      uint8_t* stage = S.stage[warp - 2];
+      if (x.slice >= 0) {                                // fp32 partial tile, [row][column]
+        float* p = a.partial + (((x.tile - a.full_tiles) * a.splits + x.slice) * 256 + crank * 128 + 32 * q) * (int64_t)NT;
+        for (int c = g * H; c < (g + 1) * H; c += 32) {
+          float v[32];
           from_tmem(c, v);
-          if (valid)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              __stcg(reinterpret_cast<float4*>(p + c) + i, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+          for (int h = 0; h < 2; ++h) {
+            lt_stage_f32(stage, v + 16 * h, lane);
+            lt_copy_out(stage, reinterpret_cast<uint8_t*>(p + c + 16 * h), NT * 4, warp_rows, lane);
+          }
         }
         release();
         continue;
@@ -398,24 +443,23 @@ __global__ void __launch_bounds__(kLtThreads, 1)
         uint32_t code = 0;
         if constexpr (KEEP) {                            // NT = 256: this warp's half is one block of the row
           uint32_t amax = 0;
-          for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 16) {
-            float v[16];
+          for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 32) {
+            float v[32];
             from_tmem(c, v);
-            if (bias) lt_bias16(bias, c_tile + c, O, v);
-            amax = lt_amax16(v, c_tile + c, O, amax);
+            if (bias) lt_bias32(bias, c_tile + c, O, v);
+            amax = lt_amax32(v, c_tile + c, O, amax);
           }
           code = e8m0_of_amax(amax);
           if (valid && c_tile + g * H < O) ep.z_scale[((c_tile >> 7) + g) * a.m + row] = (uint8_t)code;
         }
-        for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 16) {
-          float v[16];
+        for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 32) {
+          float v[32];
           from_tmem(c, v);
-          if (bias) lt_bias16(bias, c_tile + c, O, v);
+          if (bias) lt_bias32(bias, c_tile + c, O, v);
           if constexpr (KEEP)
-            if (valid) lt_store_z16(ep.z8 + row * O, c_tile + c, O, v, code);
-          lt_act16(v, ep.act);
-          if (!a.vec) lt_store_staged(ep, S.stage[warp - 2], row - lane, warp_rows, c_tile + c, O, v, lane);
-          else if (valid) lt_store16(ep, row, c_tile + c, O, v);
+            if (valid) lt_store_z32(ep.z8 + row * O, c_tile + c, O, v, code);
+          lt_act32(v, ep.act);
+          lt_store32(ep, a.vec, stage, row - lane, warp_rows, c_tile + c, O, v, lane);
         }
       } else {
         const int w = H / 2;                             // columns of each half per warp
@@ -423,13 +467,13 @@ __global__ void __launch_bounds__(kLtThreads, 1)
         uint32_t code[2] = {0, 0};
         if constexpr (KEEP) {                            // NT = 256: a block of each half per tile, shared by two warps
           uint32_t amax[2] = {0, 0};
-          for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 16)
+          for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 32)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float v[16];
+              float v[32];
               from_tmem(h * H + c, v);
-              if (bias) lt_bias16(bias + h * O, c_tile + c, O, v);
-              amax[h] = lt_amax16(v, c_tile + c, O, amax[h]);
+              if (bias) lt_bias32(bias + h * O, c_tile + c, O, v);
+              amax[h] = lt_amax32(v, c_tile + c, O, amax[h]);
             }
           S.amax[tt & 1][g][0][r] = __uint_as_float(amax[0]);
           S.amax[tt & 1][g][1][r] = __uint_as_float(amax[1]);
@@ -440,23 +484,22 @@ __global__ void __launch_bounds__(kLtThreads, 1)
             if (valid && g == 0 && c_tile < O) ep.z_scale[(h * z_blocks + (c_tile >> 7)) * a.m + row] = (uint8_t)code[h];
           }
         }
-        for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 16) {
-          float v[16], t[16];
+        for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 32) {
+          float v[32], t[32];
           from_tmem(c, v);
           from_tmem(H + c, t);
           if (bias) {
-            lt_bias16(bias, c_tile + c, O, v);
-            lt_bias16(bias + O, c_tile + c, O, t);
+            lt_bias32(bias, c_tile + c, O, v);
+            lt_bias32(bias + O, c_tile + c, O, t);
           }
           if constexpr (KEEP)
             if (valid) {
-              lt_store_z16(ep.z8 + row * O, c_tile + c, O, v, code[0]);
-              lt_store_z16(ep.z8 + (a.m + row) * O, c_tile + c, O, t, code[1]);
+              lt_store_z32(ep.z8 + row * O, c_tile + c, O, v, code[0]);
+              lt_store_z32(ep.z8 + (a.m + row) * O, c_tile + c, O, t, code[1]);
             }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] *= act_value(t[i], kActSilu);
-          if (!a.vec) lt_store_staged(ep, S.stage[warp - 2], row - lane, warp_rows, c_tile + c, O, v, lane);
-          else if (valid) lt_store16(ep, row, c_tile + c, O, v);
+          for (int i = 0; i < 32; ++i) v[i] *= act_value(t[i], kActSilu);
+          lt_store32(ep, a.vec, stage, row - lane, warp_rows, c_tile + c, O, v, lane);
         }
       }
       release();
@@ -472,28 +515,29 @@ __global__ void __launch_bounds__(kLtThreads, 1)
   }
 }
 
+// A warp takes 256 columns of a row, 8 per lane.
 __global__ void __launch_bounds__(256) pad_kernel(PadArgs a) {
   pdl_trigger();
-  // a warp per row, 4 columns per lane
-  const int lane = threadIdx.x & 31;
-  for (int j = 0; j < a.count; ++j)
-    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < a.rows[j]; row += (int64_t)gridDim.x * 8) {
-      const uint16_t* s = static_cast<const uint16_t*>(a.src[j]) + row * a.lds[j];
-      uint16_t* d = static_cast<uint16_t*>(a.dst[j]) + row * a.ldd[j];
-#pragma unroll 4
-      for (int c = 4 * lane; c < a.cols[j]; c += 128) {
-        uint16_t v[4];
+  const int j = blockIdx.z, c = 256 * blockIdx.y + 8 * (threadIdx.x & 31);
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= a.rows[j] || c >= a.cols[j]) return;
+  const uint16_t* s = static_cast<const uint16_t*>(a.src[j]) + row * a.lds[j] + c;
+  uint32_t v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = c + e < a.cols[j] ? s[c + e] : 0;
-        *reinterpret_cast<uint2*>(d + c) = make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
-      }
-    }
+  for (int e = 0; e < 8; ++e) v[e] = c + e < a.cols[j] ? __ldg(s + e) : 0;
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dst[j]) + row * a.ldd[j] + c) =
+      make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
   if (a.count == 0) return cudaSuccess;
-  int64_t blocks = 1;
-  for (int j = 0; j < a.count; ++j) blocks = blocks > (a.rows[j] + 7) / 8 ? blocks : (a.rows[j] + 7) / 8;
-  pad_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(a);
+  int64_t rows = 1;
+  int cols = 1;
+  for (int j = 0; j < a.count; ++j) {
+    rows = rows > a.rows[j] ? rows : a.rows[j];
+    cols = cols > a.cols[j] ? cols : a.cols[j];
+  }
+  if ((cols + 255) / 256 > 65535) return cudaErrorInvalidValue;
+  pad_kernel<<<dim3((unsigned)((rows + 7) / 8), (cols + 255) / 256, a.count), 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -505,13 +549,19 @@ template <bool GATED, bool KEEP>
 __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
   const int lane = threadIdx.x & 31;
   pdl_wait();
-  const int64_t blocks = (a.out_cols + 127) / 128;
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit >= a.m * blocks) return;
-  const int64_t row = unit / blocks, kb = unit - row * blocks;
-  const int64_t O = a.out_cols, c = kb * 128 + 4 * lane;
-  const int H = GATED ? a.n_tile / 2 : a.n_tile;
-  const int64_t ld = (int64_t)a.n_tiles * a.n_tile, step = a.m * ld;
+  const int H = GATED ? a.n_tile / 2 : a.n_tile, col_blocks = (H + 127) / 128;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);     // (tile, row, column block)
+  const int64_t i = unit / (256 * col_blocks);
+  const int rr = (int)(unit - i * 256 * col_blocks) / col_blocks, cb = (int)(unit % col_blocks);
+  int mt, nt;
+  lt_place(a, a.full_tiles + i, mt, nt);
+  const int64_t row = (int64_t)mt * 256 + rr;
+  const int lc = 128 * cb + 4 * lane;                                     // column inside the tile
+  const int64_t O = a.out_cols, c = (int64_t)nt * H + lc;
+  if (row >= a.m || (int64_t)nt * H + 128 * cb >= O) return;              // warp-uniform
+  const bool in = lc < H && c < O;
+  const int64_t end = min(O, (int64_t)(nt + 1) * H);                      // this warp's columns end here
+  const int64_t kb = c / 128, blocks = (O + 127) / 128, step = (int64_t)256 * a.n_tile;
   const LinearEpilogue& ep = a.ep;
   const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(ep.bias);
   float v[GATED ? 2 : 1][4];
@@ -519,9 +569,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
   for (int h = 0; h < (GATED ? 2 : 1); ++h)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[h][j] = 0.f;
-  if (c < O) {
-    const int64_t nt = c / H;
-    const float* p = a.partial + row * ld + nt * a.n_tile + (c - nt * H);
+  if (in) {
+    const float* p = a.partial + i * a.splits * step + (int64_t)rr * a.n_tile + lc;
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s)
 #pragma unroll
@@ -537,7 +586,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
       for (int h = 0; h < (GATED ? 2 : 1); ++h)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (c + j < O) v[h][j] += __bfloat162float(bias[h * O + c + j]);
+          if (c + j < end) v[h][j] += __bfloat162float(bias[h * O + c + j]);
   }
   if constexpr (KEEP) {
 #pragma unroll
@@ -545,7 +594,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
       uint32_t amax = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (c + j < O) amax = max(amax, __float_as_uint(v[h][j]) & 0x7fffffffu);
+        if (c + j < end) amax = max(amax, __float_as_uint(v[h][j]) & 0x7fffffffu);
       const uint32_t code = e8m0_of_amax(__reduce_max_sync(0xffffffffu, amax));
       const float inv = e8m0_inverse(code);
       if (lane == 0) ep.z_scale[(h * blocks + kb) * a.m + row] = (uint8_t)code;
@@ -556,7 +605,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
       uint8_t* z = ep.z8 + (h * a.m + row) * O + c;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (c + j < O) z[j] = (uint8_t)(w >> (8 * j));
+        if (c + j < end) z[j] = (uint8_t)(w >> (8 * j));
     }
   }
   float y[4];
@@ -564,7 +613,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
   for (int j = 0; j < 4; ++j)
     y[j] = GATED ? v[0][j] * act_value(v[GATED ? 1 : 0][j], kActSilu) : act_value(v[0][j], ep.act);
   const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr + c;
-  if (a.vec && c + 4 <= O) {
+  if (a.vec && c + 4 <= end) {
     if (ep.residual) {
       const uint2 w = *reinterpret_cast<const uint2*>(r);
       const float2 f0 = unpack_bf16(w.x), f1 = unpack_bf16(w.y);
@@ -582,37 +631,39 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (c + j < O) {
+    if (c + j < end) {
       if (ep.residual) y[j] += __bfloat162float(r[j]);
       if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + c + j] = y[j];
       else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + c + j] = __float2bfloat16_rn(y[j]);
     }
 }
 
-// Tile width and K slices. Cycles per 64 of K and pair, measured on this
-// kernel's main loop: the MMA (2 NT) or the SM's operand intake (16 KB + 64 NT
-// bytes at 68 per cycle); a tile's epilogue hides behind the next tile's
-// products except for the last round. Slices are at least 4 K-blocks deep; joining
-// them costs a launch and moves 8 bytes per value and slice through L2 (about 3
-// KB per cycle).
+// Tile width and K slices of the last, partial round. Cycles per 64 of K and
+// pair with all pairs at work, measured: 340 + 1.45 NT, at least 600 (711 at NT =
+// 256, 618 at 192; a pair alone takes 545 at any width). A tile's epilogue hides
+// behind the next tile's products except for the last one. Slices are at least 4
+// K-blocks deep; joining them costs a launch and moves 8 bytes per value and
+// slice through L2 (about 3 KB per cycle).
 LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs) {
   LinearTilePlan best{};
   double best_cost = 1e300;
   const int64_t mt = (m + 255) / 256;
-  static const int widths[] = {256, 224, 192, 160, 128};
+  static const int widths[] = {256, 192, 128};
   for (int nt : widths) {
     if (keep && nt != 256) continue;
-    if ((gated && nt % 64) || (b_mn && nt % 128)) continue;
+    if ((gated || b_mn) && nt == 192) continue;      // epilogue warps take 32 columns; 64-wide boxes
     const int64_t cols = gated ? nt / 2 : nt;
-    const int64_t tiles = mt * ((n + cols - 1) / cols);
-    const double block = 2.0 * nt + 16 > 241 + 0.94 * nt ? 2.0 * nt + 16 : 241 + 0.94 * nt;
+    const int64_t tiles = mt * ((n + cols - 1) / cols), tail = tiles % pairs, full = tiles - tail;
+    const double block = 340 + 1.45 * nt > 600 ? 340 + 1.45 * nt : 600;
+    const double rows = m < 256 ? m : 256;
     for (int s = 1; s <= 16; ++s) {
-      if (s > 1 && (k_blocks < 4 * s || tiles * s > pairs)) break;
-      const int64_t rounds = (tiles * s + pairs - 1) / pairs;
-      const double cost = (double)rounds * ((k_blocks + s - 1) / s) * block + 1500 + 8.0 * nt + (s > 1 ? 4000 + 8.0 * s * m * tiles / mt * nt / 3000 : 0);
+      if (s > 1 && (tail == 0 || k_blocks < 4 * s)) break;
+      const int64_t rounds = (tail * s + pairs - 1) / pairs;
+      const double cost = (double)(full / pairs) * k_blocks * block + (double)rounds * ((k_blocks + s - 1) / s) * block +
+                          1500 + 8.0 * nt + (s > 1 ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
       if (cost < best_cost) {
         best_cost = cost;
-        best = {nt, s, tiles};
+        best = {nt, s, s > 1 ? full : tiles, s > 1 ? tail : 0};
       }
     }
   }
@@ -667,9 +718,10 @@ static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, c
 
 cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
                                const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
-  cudaError_t e = launch_product(a_mn, b_mn, gated, keep && a.splits == 1, tmA, tmB, a, num_sms, st);
+  cudaError_t e = launch_product(a_mn, b_mn, gated, keep, tmA, tmB, a, num_sms, st);
   if (e != cudaSuccess || a.splits == 1) return e;
-  const dim3 grid((unsigned)ceil_div(a.m * ((a.out_cols + 127) / 128), 8)), block(256);
+  const int64_t tail = (a.units - a.full_tiles) / a.splits, H = gated ? a.n_tile / 2 : a.n_tile;
+  const dim3 grid((unsigned)(tail * 32 * ((H + 127) / 128))), block(256);
   if (gated)
     return keep ? launch_kernel(linear_join_kernel<true, true>, grid, block, 0, st, true, a)
                 : launch_kernel(linear_join_kernel<true, false>, grid, block, 0, st, true, a);

@@ -15,15 +15,16 @@ struct LinearTileArgs {
   int k_blocks;           // 64-wide K-blocks over all terms of A
   int term_blocks;        // of one term
   int splits;
-  int64_t units;          // tiles * splits
+  int64_t full_tiles;     // tiles done whole; the others are cut into `splits` K slices
+  int64_t units;          // full_tiles + splits * (number of the others)
   int pdl;                // launched right behind another kernel of the same call
   int vec;                // y (and the residual) can be accessed in 16 bytes
-  float* partial;         // splits > 1: fp32 [splits][m][n_tiles * n_tile], 16-byte aligned
+  float* partial;         // splits > 1: fp32 [other tiles][splits][256][n_tile], 16-byte aligned
   LinearEpilogue ep;
 };
 struct LinearTilePlan {
   int n_tile, splits;
-  int64_t tiles;
+  int64_t full, tail;     // whole tiles, tiles cut into K slices
 };
 LinearTilePlan plan_linear_tile(int64_t m, int64_t out_cols, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs);
 cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,

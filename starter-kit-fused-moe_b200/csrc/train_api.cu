@@ -31,11 +31,11 @@ bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % 
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 int64_t up8(int64_t x) { return (x + 7) & ~int64_t(7); }
 
-constexpr int64_t kMaxDim = 1 << 30;
+constexpr int64_t kMaxDim = 1 << 30, kMaxWidth = 1 << 23;
 
 int check_sizes(int64_t m, int64_t k, int64_t n, int act) {
-  if (m < 0 || k < 1 || n < 1 || m > kMaxDim || k > kMaxDim || n > kMaxDim)
-    return bad("m must be in [0, 2^30], k and n in [1, 2^30]");
+  if (m < 0 || k < 1 || n < 1 || m > kMaxDim || k > kMaxWidth || n > kMaxWidth)
+    return bad("m must be in [0, 2^30], k and n in [1, 2^23]");
   if (act < MOE_ACT_NONE || act > MOE_ACT_SWIGLU) return bad("unknown activation");
   if (act == MOE_ACT_SWIGLU && n % 2) return bad("SwiGLU needs an even n");
   return MOE_OK;
@@ -60,10 +60,7 @@ Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gat
   p.term_blocks = (k + 63) / 64;
   p.terms = terms;
   p.plan = moe::plan_linear_tile(m, out_cols, p.term_blocks * terms, gated, keep, b_mn, pairs());
-  if (p.plan.splits > 1) {
-    const int cols = gated ? p.plan.n_tile / 2 : p.plan.n_tile;
-    p.partial = (size_t)p.plan.splits * m * ((out_cols + cols - 1) / cols) * p.plan.n_tile * sizeof(float);
-  }
+  p.partial = (size_t)p.plan.tail * p.plan.splits * 256 * p.plan.n_tile * sizeof(float);
   return p;
 }
 // A: [terms][rows][..], term stride in elements.
@@ -81,7 +78,8 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.term_blocks = (int)p.term_blocks;
   t.k_blocks = t.term_blocks * p.terms;
   t.splits = p.plan.splits;
-  t.units = p.plan.tiles * t.splits;
+  t.full_tiles = p.plan.full;
+  t.units = p.plan.full + p.plan.tail * t.splits;
   t.ep = ep;
   t.pdl = pdl;
   const int ysize = ep.y_f32 ? 4 : 2;
