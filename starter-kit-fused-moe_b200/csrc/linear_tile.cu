@@ -38,7 +38,7 @@ namespace moe {
 constexpr int kLtStages = 6, kLtStageBytes = 32768, kLtTileA = 16384;
 constexpr int kLtThreads = 320, kLtEpiWarps = 8, kLtTmemCols = 512;
 constexpr int kLtBand = 8;
-constexpr int kLtStagePitch = 80;    // 64-byte row pieces; 80 keeps 16-byte accesses of 8 rows free of bank conflicts
+constexpr int kLtStaging = 4096;     // per epilogue warp: a 32 x 32 box of fp32, or two of bf16
 
 struct LinearTileSmem {
   uint64_t full[kLtStages];
@@ -47,10 +47,9 @@ struct LinearTileSmem {
   uint64_t tempty[2];
   uint32_t tmem_base;
   int abort_flag;
-  float amax[2][2][2][128];      // [tile parity][column half][gate, up][row]
-  alignas(16) uint8_t stage[kLtEpiWarps][32 * kLtStagePitch];
+  uint64_t res[kLtEpiWarps][2];   // a warp's residual boxes have arrived
 };
-constexpr size_t kLtSmem = 1024 + (size_t)kLtStages * kLtStageBytes + sizeof(LinearTileSmem);
+constexpr size_t kLtSmem = 1024 + (size_t)kLtStages * kLtStageBytes + (size_t)kLtEpiWarps * kLtStaging + sizeof(LinearTileSmem);
 static_assert(kLtSmem <= 232448, "shared memory budget");
 
 // bf16 x bf16 -> f32, M = 256 over the pair; a_mn / b_mn: operand stored with M / N innermost.
@@ -152,94 +151,69 @@ __device__ __forceinline__ void lt_act32(float* v, int act) {
     for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActSilu);
   }
 }
-// Stores of a warp's 32 rows go through shared memory: a lane holds a row, so
-// direct stores touch 32 lines with 16 bytes each, and a tile's epilogue took
-// longer than a short contraction (71 us for the gate's input gradient).
-
-// The warp's staged 64-byte row pieces to 64 bytes of `rows` rows each.
-__device__ __forceinline__ void lt_copy_out(const uint8_t* stage, uint8_t* dst, int64_t pitch, int rows, int lane) {
-  __syncwarp();
+// Stores of a warp's 32 rows go through shared memory and TMA: a lane holds a
+// row, so direct stores touch 32 lines with 16 bytes each, and a tile's epilogue
+// took longer than a short contraction (71 us for the gate's fp32 input
+// gradient; copying out of shared memory in coalesced pieces 48). The boxes of 32
+// rows by 32 columns lie in the swizzle of the output's tensor map, which also
+// cuts off rows and columns past the matrix.
+__device__ __forceinline__ void lt_stage_f32(uint8_t* box, const float* v, int lane) {       // 128-byte swizzle
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (lane >> 2), o = 16 * (lane & 3);
-    if (r < rows) *reinterpret_cast<uint4*>(dst + r * pitch + o) = *reinterpret_cast<const uint4*>(stage + r * kLtStagePitch + o);
-  }
-  __syncwarp();
+  for (int i = 0; i < 8; ++i)
+    *reinterpret_cast<float4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
-__device__ __forceinline__ void lt_stage_f32(uint8_t* stage, const float* v, int lane) {
+__device__ __forceinline__ uint4* lt_bf16_piece(uint8_t* box, int i, int lane) {             // 64-byte swizzle
+  return reinterpret_cast<uint4*>(box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ void lt_stage_bf16(uint8_t* box, const float* v, int lane) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    reinterpret_cast<float4*>(stage + lane * kLtStagePitch)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    *lt_bf16_piece(box, i, lane) = make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+                                              pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+}
+__device__ __forceinline__ void lt_box_out(const CUtensorMap* m, const uint8_t* box, int x, int64_t y, int lane) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(m, smem_u32(box), x, (int)y);
+    bulk_commit();
+  }
+}
+// Waits until at most N of the warp's stores still read their boxes.
+template <int N>
+__device__ __forceinline__ void lt_boxes_free(int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+  __syncwarp();
 }
 // 16 columns element by element (edges, rows that 16-byte accesses cannot
 // reach): 16 lanes take neighbouring columns of a row.
 __device__ __forceinline__ void lt_store16_any(const LinearEpilogue& ep, uint8_t* stage8, int64_t row0, int rows, int64_t c,
                                                int64_t end, const float* v, int lane) {
   float(*stage)[17] = reinterpret_cast<float(*)[17]>(stage8);
+  const int64_t col = c + (lane & 15);
+  const bool in = col < end;
+  float res[16];                                       // all 16 loads are in flight together
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = (lane >> 4) + 2 * i;
+    res[i] = ep.residual != nullptr && in && r < rows
+                 ? __bfloat162float(static_cast<const __nv_bfloat16*>(ep.residual)[(row0 + r) * ep.ldr + col])
+                 : 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) stage[lane][i] = v[i];
   __syncwarp();
-  const int64_t col = c + (lane & 15);
-  if (col < end) {
-#pragma unroll 8
-    for (int r = lane >> 4; r < rows; r += 2) {
-      const int64_t row = row0 + r;
-      float y = stage[r][lane & 15];
-      if (ep.residual != nullptr) y += __bfloat162float(static_cast<const __nv_bfloat16*>(ep.residual)[row * ep.ldr + col]);
-      if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + col] = y;
-      else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + col] = __float2bfloat16_rn(y);
-    }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = (lane >> 4) + 2 * i;
+    const int64_t row = row0 + r;
+    const float y = stage[r][lane & 15] + res[i];
+    if (!in || r >= rows) continue;
+    if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + col] = y;
+    else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + col] = __float2bfloat16_rn(y);
   }
   __syncwarp();
-}
-// y[row0 .., c .. c + 32) = v + residual for the warp's first `rows` rows,
-// columns below `end`. The warp reads a piece of the residual before it writes
-// the same piece of y, so y may be the residual. All lanes call.
-__device__ __forceinline__ void lt_store32(const LinearEpilogue& ep, int vec, uint8_t* stage, int64_t row0, int rows,
-                                           int64_t c, int64_t end, float* v, int lane) {
-  if (!vec || c + 32 > end) {
-    lt_store16_any(ep, stage, row0, rows, c, end, v, lane);
-    if (c + 16 < end) lt_store16_any(ep, stage, row0, rows, c + 16, end, v + 16, lane);
-    return;
-  }
-  uint8_t* mine = stage + lane * kLtStagePitch;
-  if (ep.residual != nullptr) {
-    const uint8_t* r = reinterpret_cast<const uint8_t*>(static_cast<const __nv_bfloat16*>(ep.residual) + row0 * ep.ldr + c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int rr = 8 * i + (lane >> 2), o = 16 * (lane & 3);
-      if (rr < rows)
-        *reinterpret_cast<uint4*>(stage + rr * kLtStagePitch + o) = *reinterpret_cast<const uint4*>(r + rr * ep.ldr * 2 + o);
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 a = reinterpret_cast<const uint4*>(mine)[i];
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = unpack_bf16(w[j]);
-        v[8 * i + 2 * j] += f.x;
-        v[8 * i + 2 * j + 1] += f.y;
-      }
-    }
-    __syncwarp();
-  }
-  if (ep.y_f32) {
-    uint8_t* y = reinterpret_cast<uint8_t*>(static_cast<float*>(ep.y) + row0 * ep.ldy + c);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      lt_stage_f32(stage, v + 16 * h, lane);
-      lt_copy_out(stage, y + 64 * h, ep.ldy * 4, rows, lane);
-    }
-  } else {
-    uint8_t* y = reinterpret_cast<uint8_t*>(static_cast<__nv_bfloat16*>(ep.y) + row0 * ep.ldy + c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      reinterpret_cast<uint4*>(mine)[i] = make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
-                                                     pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
-    lt_copy_out(stage, y, ep.ldy * 2, rows, lane);
-  }
 }
 // Largest magnitude (as bits) of the columns below `end`.
 __device__ __forceinline__ uint32_t lt_amax32(const float* v, int64_t c, int64_t end, uint32_t amax) {
@@ -270,10 +244,11 @@ __device__ __forceinline__ void lt_store_z32(uint8_t* z, int64_t c, int64_t end,
 
 template <bool A_MN, bool B_MN, bool GATED, bool KEEP>
 __global__ void __launch_bounds__(kLtThreads, 1)
-    linear_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, LinearTileArgs a) {
+    linear_tile_kernel(const __grid_constant__ LinearTileMaps maps, const LinearTileArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  LinearTileSmem& S = *reinterpret_cast<LinearTileSmem*>(smem + kLtStages * kLtStageBytes);
+  uint8_t* staging = smem + kLtStages * kLtStageBytes;
+  LinearTileSmem& S = *reinterpret_cast<LinearTileSmem*>(staging + kLtEpiWarps * kLtStaging);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int crank = (int)cluster_rank();
   const int64_t wid = cluster_id(), G = gridDim.x / 2;
@@ -288,12 +263,14 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       mbar_init(smem_u32(&S.tfull[b]), 1);
       mbar_init(smem_u32(&S.tempty[b]), 2 * kLtEpiWarps);      // both CTAs' epilogues (the leader's copy)
     }
+    for (int w = 0; w < kLtEpiWarps; ++w)
+      for (int b = 0; b < 2; ++b) mbar_init(smem_u32(&S.res[w][b]), 1);
     S.abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&maps.a);
+    tma_prefetch_desc(&maps.b);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem_base)),
@@ -335,16 +312,16 @@ __global__ void __launch_bounds__(kLtThreads, 1)
           const int term = kb / a.term_blocks, kt = (kb - term * a.term_blocks) * 64;
           if (crank == 0) mbar_arrive_expect_tx(fb, bytes);
           if constexpr (A_MN) {
-            tma_load_3d_pair(sa, &tmA, fbl, m0, kt, term);
-            tma_load_3d_pair(sa + 8192, &tmA, fbl, m0 + 64, kt, term);
+            tma_load_3d_pair(sa, &maps.a, fbl, m0, kt, term);
+            tma_load_3d_pair(sa + 8192, &maps.a, fbl, m0 + 64, kt, term);
           } else {
-            tma_load_3d_pair(sa, &tmA, fbl, kt, m0, term);
+            tma_load_3d_pair(sa, &maps.a, fbl, kt, m0, term);
           }
           if constexpr (B_MN) {
-            tma_load_2d_pair(sb, &tmB, fbl, n0, kt);
-            if (H == 128) tma_load_2d_pair(sb + 8192, &tmB, fbl, n0 + 64, kt);
+            tma_load_2d_pair(sb, &maps.b, fbl, n0, kt);
+            if (H == 128) tma_load_2d_pair(sb + 8192, &maps.b, fbl, n0 + 64, kt);
           } else {
-            tma_load_2d_pair(sb, &tmB, fbl, kt, n0);
+            tma_load_2d_pair(sb, &maps.b, fbl, kt, n0);
           }
         }
       }
@@ -393,20 +370,45 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(ep.bias);
     const int64_t O = a.out_cols;
     const int64_t z_blocks = (O + 127) / 128;
+    uint8_t* stage = staging + (warp - 2) * kLtStaging;
+    const uint32_t stage_addr = smem_u32(stage);
+    // y as bf16 in whole boxes with a residual: the residual's boxes are fetched into the boxes y leaves from
+    const bool res_boxes = a.vec && ep.residual != nullptr && !ep.y_f32;
+    constexpr int CHUNKS_H = GATED ? 4 : 2;              // this warp's columns: NT / CHUNKS_H
     bool ok = true;
     int tt = 0;
+    uint32_t res_count = 0;                              // residual boxes waited for
     for (int64_t u = wid; u < a.units; u += G, ++tt) {
       const LtUnit x = lt_unit(a, u);
       const int b = tt & 1;
+      const int64_t row0 = (int64_t)x.mt * 256 + crank * 128 + 32 * q, row = row0 + lane;
+      const bool valid = row < a.m;
+      const int warp_rows = (int)max((int64_t)0, min((int64_t)32, a.m - row0));
+      const int w = NT / CHUNKS_H;                       // columns of y per warp
+      const int64_t c0 = (int64_t)x.nt * (GATED ? H : NT) + g * w;     // the first of them
+      const int chunks = (int)min((int64_t)(w / 32), (O - c0 + 31) / 32);
+      const bool live = warp_rows > 0 && chunks > 0;
+      auto fetch_residual = [&](int j) {                 // chunk j into box j & 1, whose last store has been read
+        if (lane == 0) {
+          const uint32_t bar = smem_u32(&S.res[warp - 2][j & 1]);
+          mbar_arrive_expect_tx(bar, 2048);
+          tma_load_2d(stage_addr + (j & 1) * 2048, &maps.res, bar, (int)c0 + 32 * j, (int)row0);
+        }
+      };
+      auto fetch_first = [&] {
+        if (res_boxes && live && x.slice < 0) {
+          lt_boxes_free<0>(lane);
+          fetch_residual(0);
+          if (chunks > 1) fetch_residual(1);
+        }
+      };
+      if constexpr (!(GATED && KEEP)) fetch_first();     // ahead of the product
       if (ok && (*abort_flag || !mbar_wait(smem_u32(&S.tfull[b]), (tt >> 1) & 1))) {
         *abort_flag = 1;
         ok = false;
       }
       tc_fence_after();
       const uint32_t acc = lane_addr + (uint32_t)(b * 256);
-      const int64_t row = (int64_t)x.mt * 256 + crank * 128 + r;
-      const bool valid = row < a.m;
-      const int warp_rows = (int)max((int64_t)0, min((int64_t)32, a.m - (row - lane)));
       auto release = [&] {
         tc_fence_before();
         __syncwarp();
@@ -422,88 +424,139 @@ __global__ void __launch_bounds__(kLtThreads, 1)
           for (int i = 0; i < 32; ++i) v[i] = NAN;
         }
       };
-      uint8_t* stage = S.stage[warp - 2];
       if (x.slice >= 0) {                                // fp32 partial tile, [row][column]
-        float* p = a.partial + (((x.tile - a.full_tiles) * a.splits + x.slice) * 256 + crank * 128 + 32 * q) * (int64_t)NT;
-        for (int c = g * H; c < (g + 1) * H; c += 32) {
-          float v[32];
-          from_tmem(c, v);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            lt_stage_f32(stage, v + 16 * h, lane);
-            lt_copy_out(stage, reinterpret_cast<uint8_t*>(p + c + 16 * h), NT * 4, warp_rows, lane);
+        if (warp_rows > 0) {
+          const int64_t y0 = ((x.tile - a.full_tiles) * a.splits + x.slice) * 256 + crank * 128 + 32 * q;
+          for (int c = g * H; c < (g + 1) * H; c += 32) {
+            float v[32];
+            from_tmem(c, v);
+            lt_boxes_free<0>(lane);
+            lt_stage_f32(stage, v, lane);
+            lt_box_out(&maps.partial, stage, c, y0, lane);
           }
         }
         release();
         continue;
       }
+      // y's columns [c0 + 32 j, + 32)
+      auto store = [&](int j, float* v) {
+        const int64_t c = c0 + 32 * j;
+        if (!a.vec) {
+          lt_store16_any(ep, stage, row0, warp_rows, c, O, v, lane);
+          if (c + 16 < O) lt_store16_any(ep, stage, row0, warp_rows, c + 16, O, v + 16, lane);
+        } else if (ep.y_f32) {
+          if (ep.residual != nullptr && valid) {
+            const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr;
+            lt_bias32(r, c, O, v);
+          }
+          lt_boxes_free<0>(lane);
+          lt_stage_f32(stage, v, lane);
+          lt_box_out(&maps.out, stage, (int)c, row0, lane);
+        } else {
+          uint8_t* box = stage + (j & 1) * 2048;
+          if (res_boxes) {
+            if (ok && !mbar_wait(smem_u32(&S.res[warp - 2][j & 1]), (res_count >> (j & 1)) & 1)) {
+              *abort_flag = 1;
+              ok = false;
+            }
+            res_count ^= 1u << (j & 1);                  // each box's phase flips with every use
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 p = *lt_bf16_piece(box, i, lane);
+              const uint32_t pw[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack_bf16(pw[e]);
+                v[8 * i + 2 * e] += f.x;
+                v[8 * i + 2 * e + 1] += f.y;
+              }
+            }
+          } else {
+            lt_boxes_free<1>(lane);
+          }
+          lt_stage_bf16(box, v, lane);
+          lt_box_out(&maps.out, box, (int)c, row0, lane);
+          if (res_boxes && j + 2 < chunks) {
+            lt_boxes_free<0>(lane);
+            fetch_residual(j + 2);
+          }
+        }
+      };
 
       if constexpr (!GATED) {
-        const int64_t c_tile = (int64_t)x.nt * NT;
         uint32_t code = 0;
         if constexpr (KEEP) {                            // NT = 256: this warp's half is one block of the row
           uint32_t amax = 0;
-          for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 32) {
+          for (int j = 0; j < chunks; ++j) {
             float v[32];
-            from_tmem(c, v);
-            if (bias) lt_bias32(bias, c_tile + c, O, v);
-            amax = lt_amax32(v, c_tile + c, O, amax);
+            from_tmem(g * H + 32 * j, v);
+            if (bias) lt_bias32(bias, c0 + 32 * j, O, v);
+            amax = lt_amax32(v, c0 + 32 * j, O, amax);
           }
           code = e8m0_of_amax(amax);
-          if (valid && c_tile + g * H < O) ep.z_scale[((c_tile >> 7) + g) * a.m + row] = (uint8_t)code;
+          if (valid && chunks > 0) ep.z_scale[(c0 >> 7) * a.m + row] = (uint8_t)code;
         }
-        for (int c = g * H; c < (g + 1) * H && c_tile + c < O; c += 32) {
-          float v[32];
-          from_tmem(c, v);
-          if (bias) lt_bias32(bias, c_tile + c, O, v);
-          if constexpr (KEEP)
-            if (valid) lt_store_z32(ep.z8 + row * O, c_tile + c, O, v, code);
-          lt_act32(v, ep.act);
-          lt_store32(ep, a.vec, stage, row - lane, warp_rows, c_tile + c, O, v, lane);
-        }
+        if (live)
+          for (int j = 0; j < chunks; ++j) {
+            float v[32];
+            from_tmem(g * H + 32 * j, v);
+            if (bias) lt_bias32(bias, c0 + 32 * j, O, v);
+            if constexpr (KEEP)
+              if (valid) lt_store_z32(ep.z8 + row * O, c0 + 32 * j, O, v, code);
+            lt_act32(v, ep.act);
+            store(j, v);
+          }
       } else {
-        const int w = H / 2;                             // columns of each half per warp
-        const int64_t c_tile = (int64_t)x.nt * H;
         uint32_t code[2] = {0, 0};
         if constexpr (KEEP) {                            // NT = 256: a block of each half per tile, shared by two warps
           uint32_t amax[2] = {0, 0};
-          for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 32)
+          for (int j = 0; j < chunks; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float v[32];
-              from_tmem(h * H + c, v);
-              if (bias) lt_bias32(bias + h * O, c_tile + c, O, v);
-              amax[h] = lt_amax32(v, c_tile + c, O, amax[h]);
+              from_tmem(h * H + g * w + 32 * j, v);
+              if (bias) lt_bias32(bias + h * O, c0 + 32 * j, O, v);
+              amax[h] = lt_amax32(v, c0 + 32 * j, O, amax[h]);
             }
-          S.amax[tt & 1][g][0][r] = __uint_as_float(amax[0]);
-          S.amax[tt & 1][g][1][r] = __uint_as_float(amax[1]);
+          // the maxima pass through the warps' staging boxes
+          lt_boxes_free<0>(lane);
+          uint32_t* mine = reinterpret_cast<uint32_t*>(stage) + lane;
+          const uint32_t* other = reinterpret_cast<const uint32_t*>(stage + (g ? -4 : 4) * kLtStaging) + lane;
+          mine[0] = amax[0];
+          mine[32] = amax[1];
+          fence_proxy_async_smem();                      // the residual's boxes come after these words
           named_barrier_sync(2 + q, 64);
+          code[0] = e8m0_of_amax(max(amax[0], other[0]));
+          code[1] = e8m0_of_amax(max(amax[1], other[32]));
+          named_barrier_sync(2 + q, 64);
+          fetch_first();
+          if (valid && g == 0 && c0 < O)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            code[h] = e8m0_of_amax(max(amax[h], __float_as_uint(S.amax[tt & 1][g ^ 1][h][r])));
-            if (valid && g == 0 && c_tile < O) ep.z_scale[(h * z_blocks + (c_tile >> 7)) * a.m + row] = (uint8_t)code[h];
-          }
+            for (int h = 0; h < 2; ++h) ep.z_scale[(h * z_blocks + (c0 >> 7)) * a.m + row] = (uint8_t)code[h];
         }
-        for (int c = g * w; c < (g + 1) * w && c_tile + c < O; c += 32) {
-          float v[32], t[32];
-          from_tmem(c, v);
-          from_tmem(H + c, t);
-          if (bias) {
-            lt_bias32(bias, c_tile + c, O, v);
-            lt_bias32(bias + O, c_tile + c, O, t);
-          }
-          if constexpr (KEEP)
-            if (valid) {
-              lt_store_z32(ep.z8 + row * O, c_tile + c, O, v, code[0]);
-              lt_store_z32(ep.z8 + (a.m + row) * O, c_tile + c, O, t, code[1]);
+        if (live)
+          for (int j = 0; j < chunks; ++j) {
+            const int64_t c = c0 + 32 * j;
+            float v[32], t[32];
+            from_tmem(g * w + 32 * j, v);
+            from_tmem(H + g * w + 32 * j, t);
+            if (bias) {
+              lt_bias32(bias, c, O, v);
+              lt_bias32(bias + O, c, O, t);
             }
+            if constexpr (KEEP)
+              if (valid) {
+                lt_store_z32(ep.z8 + row * O, c, O, v, code[0]);
+                lt_store_z32(ep.z8 + (a.m + row) * O, c, O, t, code[1]);
+              }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= act_value(t[i], kActSilu);
-          lt_store32(ep, a.vec, stage, row - lane, warp_rows, c_tile + c, O, v, lane);
-        }
+            for (int i = 0; i < 32; ++i) v[i] *= act_value(t[i], kActSilu);
+            store(j, v);
+          }
       }
       release();
     }
+    if (lane == 0) bulk_wait_all();                      // stores complete before the CTA exits
   }
 
   tc_fence_before();
@@ -648,10 +701,10 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
   LinearTilePlan best{};
   double best_cost = 1e300;
   const int64_t mt = (m + 255) / 256;
-  static const int widths[] = {256, 192, 128};
+  static const int widths[] = {256, 192, 128, 64};
   for (int nt : widths) {
     if (keep && nt != 256) continue;
-    if ((gated || b_mn) && nt == 192) continue;      // epilogue warps take 32 columns; 64-wide boxes
+    if ((gated || b_mn) && nt % 128) continue;       // epilogue warps take 32 columns; boxes of 64
     const int64_t cols = gated ? nt / 2 : nt;
     const int64_t tiles = mt * ((n + cols - 1) / cols), tail = tiles % pairs, full = tiles - tail;
     const double block = 340 + 1.45 * nt > 600 ? 340 + 1.45 * nt : 600;
@@ -660,7 +713,7 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
       if (s > 1 && (tail == 0 || k_blocks < 4 * s)) break;
       const int64_t rounds = (tail * s + pairs - 1) / pairs;
       const double cost = (double)(full / pairs) * k_blocks * block + (double)rounds * ((k_blocks + s - 1) / s) * block +
-                          1500 + 8.0 * nt + (s > 1 ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
+                          1500 + 25.0 * nt + (s > 1 ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
       if (cost < best_cost) {
         best_cost = cost;
         best = {nt, s, s > 1 ? full : tiles, s > 1 ? tail : 0};
@@ -671,8 +724,7 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
 }
 
 template <bool A_MN, bool B_MN, bool GATED, bool KEEP>
-static cudaError_t launch_t(const CUtensorMap& tmA, const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms,
-                            cudaStream_t st) {
+static cudaError_t launch_t(const LinearTileMaps& maps, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
   static int clusters_of[64];
   auto kern = linear_tile_kernel<A_MN, B_MN, GATED, KEEP>;
   int dev = 0;
@@ -703,22 +755,22 @@ static cudaError_t launch_t(const CUtensorMap& tmA, const CUtensorMap& tmB, cons
   cfg.gridDim = dim3((unsigned)(2 * want));
   cfg.stream = st;
   cfg.numAttrs = a.pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, tmA, tmB, a);
+  return cudaLaunchKernelEx(&cfg, kern, maps, a);
 }
 
-static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
-                                  const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
-  if (a_mn && b_mn) return launch_t<true, true, false, false>(tmA, tmB, a, num_sms, st);
-  if (b_mn) return launch_t<false, true, false, false>(tmA, tmB, a, num_sms, st);
-  if (gated) return keep ? launch_t<false, false, true, true>(tmA, tmB, a, num_sms, st)
-                         : launch_t<false, false, true, false>(tmA, tmB, a, num_sms, st);
-  return keep ? launch_t<false, false, false, true>(tmA, tmB, a, num_sms, st)
-              : launch_t<false, false, false, false>(tmA, tmB, a, num_sms, st);
+static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
+                                  const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+  if (a_mn && b_mn) return launch_t<true, true, false, false>(maps, a, num_sms, st);
+  if (b_mn) return launch_t<false, true, false, false>(maps, a, num_sms, st);
+  if (gated) return keep ? launch_t<false, false, true, true>(maps, a, num_sms, st)
+                         : launch_t<false, false, true, false>(maps, a, num_sms, st);
+  return keep ? launch_t<false, false, false, true>(maps, a, num_sms, st)
+              : launch_t<false, false, false, false>(maps, a, num_sms, st);
 }
 
-cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
-                               const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
-  cudaError_t e = launch_product(a_mn, b_mn, gated, keep, tmA, tmB, a, num_sms, st);
+cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
+                               const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+  cudaError_t e = launch_product(a_mn, b_mn, gated, keep, maps, a, num_sms, st);
   if (e != cudaSuccess || a.splits == 1) return e;
   const int64_t tail = (a.units - a.full_tiles) / a.splits, H = gated ? a.n_tile / 2 : a.n_tile;
   const dim3 grid((unsigned)(tail * 32 * ((H + 127) / 128))), block(256);

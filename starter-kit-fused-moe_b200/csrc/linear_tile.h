@@ -22,13 +22,18 @@ struct LinearTileArgs {
   float* partial;         // splits > 1: fp32 [other tiles][splits][256][n_tile], 16-byte aligned
   LinearEpilogue ep;
 };
+struct LinearTileMaps {
+  CUtensorMap a, b;       // operands
+  CUtensorMap out, res;   // y and the residual in 32 x 32 boxes (vec)
+  CUtensorMap partial;    // the K slices' tiles in 32 x 32 boxes (splits > 1)
+};
 struct LinearTilePlan {
   int n_tile, splits;
   int64_t full, tail;     // whole tiles, tiles cut into K slices
 };
 LinearTilePlan plan_linear_tile(int64_t m, int64_t out_cols, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs);
-cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const CUtensorMap& tmA,
-                               const CUtensorMap& tmB, const LinearTileArgs& a, int num_sms, cudaStream_t st);
+cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
+                               const LinearTileArgs& a, int num_sms, cudaStream_t st);
 // One launch that copies up to two matrices into rows TMA can read (base and row
 // stride multiples of 16 bytes).
 struct PadArgs {

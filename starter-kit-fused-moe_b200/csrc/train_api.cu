@@ -83,19 +83,27 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.ep = ep;
   t.pdl = pdl;
   const int ysize = ep.y_f32 ? 4 : 2;
-  t.vec = aligned(ep.y, 16) && ep.ldy * ysize % 16 == 0 && (!ep.residual || (aligned(ep.residual, 16) && ep.ldr % 8 == 0));
+  t.vec = aligned(ep.y, 16) && ep.ldy * ysize % 16 == 0 &&
+          (!ep.residual || (aligned(ep.residual, 16) && ep.ldr % 8 == 0 && ep.ldr > 0));
   t.partial = reinterpret_cast<float*>(partial);
-  CUtensorMap ma, mb;
+  moe::LinearTileMaps maps{};
   const uint32_t half = (uint32_t)t.n_tile / 2;
-  const bool ok = (a_mn ? moe::encode_bf16(&ma, A, m, k, lda, p.terms, term_stride, 64, 64)
-                        : moe::encode_bf16(&ma, A, k, m, lda, p.terms, term_stride, 64, 128)) &&
-                  (b_mn ? moe::encode_bf16(&mb, B, out_cols, k, ldb, 0, 0, 64, 64)
-                        : moe::encode_bf16(&mb, B, k, b_rows, ldb, 0, 0, 64, half));
+  bool ok = (a_mn ? moe::encode_matrix(&maps.a, false, A, m, k, lda, p.terms, term_stride, 64, 64)
+                  : moe::encode_matrix(&maps.a, false, A, k, m, lda, p.terms, term_stride, 64, 128)) &&
+            (b_mn ? moe::encode_matrix(&maps.b, false, B, out_cols, k, ldb, 0, 0, 64, 64)
+                  : moe::encode_matrix(&maps.b, false, B, k, b_rows, ldb, 0, 0, 64, half));
+  if (t.vec && t.full_tiles > 0) {
+    ok = ok && moe::encode_matrix(&maps.out, ep.y_f32, ep.y, out_cols, m, ep.ldy, 0, 0, 32, 32);
+    if (ep.residual) ok = ok && moe::encode_matrix(&maps.res, false, ep.residual, out_cols, m, ep.ldr, 0, 0, 32, 32);
+  }
+  if (t.splits > 1)
+    ok = ok && moe::encode_matrix(&maps.partial, true, partial, t.n_tile, (uint64_t)p.plan.tail * t.splits * 256,
+                                  t.n_tile, 0, 0, 32, 32);
   if (!ok) {
     moe::set_last_error("cuTensorMapEncodeTiled failed");
     return MOE_ERR_CUDA;
   }
-  return done(moe::launch_linear_tile(a_mn, b_mn, gated, keep, ma, mb, t, 2 * pairs(), st), what);
+  return done(moe::launch_linear_tile(a_mn, b_mn, gated, keep, maps, t, 2 * pairs(), st), what);
 }
 
 // Workspace of a forward product.

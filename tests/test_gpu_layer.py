@@ -314,6 +314,27 @@ def test_linear_checkpointed(pkg, m, k, n, act):
         assert (amax - slack <= 448 * sc).all() and ((amax + slack > 224 * sc) | (codes[h] == 10)).all()
 
 
+@pytest.mark.parametrize("m, k, n", [(20, 64, 64), (300, 192, 512), (700, 264, 1040), (2600, 128, 2048)])
+@pytest.mark.parametrize("act", ["none", "gelu", "swiglu"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_linear_checkpointed_with_residual(pkg, m, k, n, act, dtype):
+    """The kept blocks do not change with a residual or the output's type, and y is linear()'s up to its rounding."""
+    x, w, b = randn(m, k, seed=1), randn(n, k, seed=2, scale=k ** -0.5), randn(n, seed=3)
+    r = randn(m, n // 2 if act == "swiglu" else n, seed=4)
+    y, ck = pkg.linear_checkpointed(x, w, bias=b, residual=r, activation=act, out_dtype=dtype)
+    z, tz = dense64(x, w, b)
+    ref = act64(z, act) + r.double()
+    check(y, ref, rounded(ref, tol_act(z, tz, act) + ref.abs() * 2.0 ** -23, dtype), "y")
+    plain = pkg.linear_checkpointed(x, w, bias=b, activation=act)[1]
+    if act != "none":
+        assert torch.equal(ck.z.view(torch.uint8), plain.z.view(torch.uint8))
+        assert torch.equal(ck.z_scale.view(torch.uint8), plain.z_scale.view(torch.uint8))
+    own = r.clone() if dtype == BF else None
+    if own is not None:
+        got = pkg.linear_checkpointed(x, w, bias=b, residual=own, activation=act, output=own)[0]
+        assert got is own and torch.equal(own, y)
+
+
 @pytest.mark.parametrize("m, k, n", TRAIN)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("gin, gout", [(BF, BF), (F32, F32), (F32, BF), (BF, F32)])
