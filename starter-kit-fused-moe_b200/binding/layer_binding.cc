@@ -9,6 +9,7 @@
 // between calls.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -105,7 +106,7 @@ int scoring_code(const std::string& s) {
 }
 
 Tensor make(at::IntArrayRef sizes, at::ScalarType t, at::Device dev) {
-  return at::empty(sizes, at::TensorOptions().dtype(t).device(dev));
+  return at::detail::empty_cuda(sizes, t, dev, std::nullopt);   // torch's caching allocator, without the dispatcher
 }
 void* stream_of(at::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }

@@ -218,7 +218,7 @@ int act_grad_chunks(int m, int) { return ceil_div(m, kAgRows); }
 
 static bool al(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-cudaError_t launch_act_grad(const ActGradArgs& a, bool pdl, cudaStream_t st) {
+cudaError_t launch_act_grad(const ActGradArgs& a, cudaStream_t st) {
   if (a.m == 0 || a.n == 0) return cudaSuccess;
   const bool two = a.act == kActSwiglu;
   const int O = two ? a.n / 2 : a.n;
@@ -226,8 +226,8 @@ cudaError_t launch_act_grad(const ActGradArgs& a, bool pdl, cudaStream_t st) {
                    (!a.dz || (al(a.dz, 16) && a.ldz % 8 == 0));
   const dim3 grid((unsigned)act_grad_chunks(a.m, a.n), (unsigned)ceil_div(O, kAgCols));
 #define MOE_AG(H, F, V)                                                                                      \
-  return a.terms == 1 ? launch_kernel(act_grad_kernel<H, F, V, true>, grid, dim3(256), 0, st, pdl, a, O) \
-                      : launch_kernel(act_grad_kernel<H, F, V, false>, grid, dim3(256), 0, st, pdl, a, O)
+  return a.terms == 1 ? launch_kernel(act_grad_kernel<H, F, V, true>, grid, dim3(256), 0, st, true, a, O) \
+                      : launch_kernel(act_grad_kernel<H, F, V, false>, grid, dim3(256), 0, st, true, a, O)
   if (two) {
     if (a.dy_f32) { if (vec) MOE_AG(2, true, true); else MOE_AG(2, true, false); }
     else { if (vec) MOE_AG(2, false, true); else MOE_AG(2, false, false); }

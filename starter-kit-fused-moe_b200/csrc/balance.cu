@@ -33,8 +33,8 @@ namespace moe {
 constexpr int kBalWarps = 8;
 constexpr float kScoreEps = 1e-20f;
 
-static int balance_chunk(int t) {   // tokens per block: about two blocks per SM, a multiple of the warps
-  const int c = align_up(ceil_div(t, 2 * 148), kBalWarps);
+static int balance_chunk(int t) {   // tokens per block: about three blocks per SM, a multiple of the warps
+  const int c = align_up(ceil_div(t, 3 * 148), kBalWarps);
   return c < kBalWarps ? kBalWarps : c;
 }
 
@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(Balance
   __shared__ int hist[32 * ITEMS];
   __shared__ int tok;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
   pdl_trigger();
   if (blockIdx.x == 0 && threadIdx.x == 0) *w.state = 0;
   const int b0 = blockIdx.x * chunk, b1 = min(b0 + chunk, a.t);
@@ -157,10 +158,21 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(Balance
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) acc[j] = 0.f;
     int mine = 0;
+    float next[ITEMS];                                       // the next token's logits are on their way
+    int id_next = -1;
+    if (s0 + warp < s1) {
+      load_logits<ITEMS>(a.logits + (int64_t)(s0 + warp) * a.e, a.e, lane, next);
+      if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(s0 + warp) * a.k + lane);
+    }
     for (int t = s0 + warp; t < s1; t += kBalWarps) {
-      const int id = lane < a.k ? __ldg(a.idx + (int64_t)t * a.k + lane) : -1;
+      const int id = id_next;
       float x[ITEMS], s[ITEMS];
-      load_logits<ITEMS>(a.logits + (int64_t)t * a.e, a.e, lane, x);
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j) x[j] = next[j];
+      if (t + kBalWarps < s1) {
+        load_logits<ITEMS>(a.logits + (int64_t)(t + kBalWarps) * a.e, a.e, lane, next);
+        if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(t + kBalWarps) * a.k + lane);
+      }
       const bool hit = id >= 0 && id < a.e;
       if (!__any_sync(0xffffffffu, hit)) continue;           // padding
       if (hit) atomicAdd(&hist[id], 1);
@@ -199,6 +211,7 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
   __shared__ double rl[256];
   __shared__ int last;
   pdl_wait();
+  pdl_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int groups = gridDim.x, g = blockIdx.x;
   const int q = blockIdx.y;
@@ -300,6 +313,8 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGra
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j) scatter[warp][lane + 32 * j] = 0.f;
   __syncwarp();
+  pdl_wait();
+  pdl_trigger();
   const int b1 = (int)min((int64_t)(blockIdx.x + 1) * chunk, (int64_t)a.t);
   const bool with_loss = a.grad_loss != nullptr;
   const float g = with_loss ? __ldg(a.grad_loss) : 0.f;
@@ -410,7 +425,8 @@ cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
   BalanceWs w;
   balance_ws(a.t, a.e, a.s, static_cast<uint8_t*>(a.workspace), &w);
   const int chunk = balance_chunk(a.t), grid = ceil_div(a.t, chunk);
-#define MOE_BAL(I) balance_partial_kernel<I><<<grid, kBalWarps * 32, 0, st>>>(a, w, chunk)
+  cudaError_t e;
+#define MOE_BAL(I) e = launch_kernel(balance_partial_kernel<I>, dim3(grid), dim3(kBalWarps * 32), 0, st, true, a, w, chunk)
   if (a.e <= 32) MOE_BAL(1);
   else if (a.e <= 64) MOE_BAL(2);
   else if (a.e <= 128) MOE_BAL(4);
@@ -418,7 +434,6 @@ cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
   else if (a.e <= 512) MOE_BAL(16);
   else MOE_BAL(32);
 #undef MOE_BAL
-  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_kernel(balance_reduce_kernel, dim3((unsigned)ceil_div(a.e, 32), (unsigned)a.s), dim3(256), 0, st, true, a,
                        w, chunk);
@@ -429,7 +444,7 @@ cudaError_t launch_balance_grad(const BalanceGradArgs& a, cudaStream_t st) {
   int chunk = align_up(ceil_div(a.t, 4 * 148), kBalWarps);     // about four blocks per SM
   if (chunk < kBalWarps) chunk = kBalWarps;
   const int grid = ceil_div(a.t, chunk);
-#define MOE_BALG(I) balance_grad_kernel<I><<<grid, kBalWarps * 32, 0, st>>>(a, chunk)
+#define MOE_BALG(I) return launch_kernel(balance_grad_kernel<I>, dim3(grid), dim3(kBalWarps * 32), 0, st, true, a, chunk)
   if (a.e <= 32) MOE_BALG(1);
   else if (a.e <= 64) MOE_BALG(2);
   else if (a.e <= 128) MOE_BALG(4);
@@ -437,7 +452,6 @@ cudaError_t launch_balance_grad(const BalanceGradArgs& a, cudaStream_t st) {
   else if (a.e <= 512) MOE_BALG(16);
   else MOE_BALG(32);
 #undef MOE_BALG
-  return cudaGetLastError();
 }
 
 }  // namespace moe

@@ -33,6 +33,8 @@ __global__ void __launch_bounds__(kCkWarps * 32) checkpoint_kernel(const T_IN* _
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7, rs = lane >> 3;
   const int64_t kb = (int64_t)blockIdx.y * kCkWarps + warp;
   const int64_t c0 = kb * kBlock;
+  pdl_wait();
+  pdl_trigger();
   if (c0 >= cols) return;
   const int64_t r0 = (int64_t)blockIdx.x * R;
   uint32_t code_mine = 0;
@@ -192,22 +194,22 @@ static cudaError_t checkpoint_r(const T_IN* x, int64_t rows, int64_t cols, int64
   const int64_t nb = (cols + kBlock - 1) / kBlock;
   const int r = rows_per_warp(rows, nb, 4);
   const dim3 grid((unsigned)((rows + r - 1) / r), (unsigned)((nb + kCkWarps - 1) / kCkWarps));
-  if (r == 32) checkpoint_kernel<T_IN, 32, VEC><<<grid, kCkWarps * 32, 0, st>>>(x, rows, cols, ldx, q, scale);
-  else if (r == 8) checkpoint_kernel<T_IN, 8, VEC><<<grid, kCkWarps * 32, 0, st>>>(x, rows, cols, ldx, q, scale);
-  else checkpoint_kernel<T_IN, 4, VEC><<<grid, kCkWarps * 32, 0, st>>>(x, rows, cols, ldx, q, scale);
-  return cudaGetLastError();
+  const dim3 block(kCkWarps * 32);
+  if (r == 32) return launch_kernel(checkpoint_kernel<T_IN, 32, VEC>, grid, block, 0, st, true, x, rows, cols, ldx, q, scale);
+  if (r == 8) return launch_kernel(checkpoint_kernel<T_IN, 8, VEC>, grid, block, 0, st, true, x, rows, cols, ldx, q, scale);
+  return launch_kernel(checkpoint_kernel<T_IN, 4, VEC>, grid, block, 0, st, true, x, rows, cols, ldx, q, scale);
 }
 
 template <typename T_OUT, bool VEC>
 static cudaError_t restore_r(const uint8_t* q, const uint8_t* scale, int64_t batch, int64_t rows, int64_t cols,
-                             T_OUT* out, int64_t ldo, bool pdl, cudaStream_t st) {
+                             T_OUT* out, int64_t ldo, cudaStream_t st) {
   const int64_t nb = (cols + kBlock - 1) / kBlock;
   const int r = rows_per_warp(rows, nb * batch, 2);
   const dim3 grid((unsigned)((rows + r - 1) / r), (unsigned)((nb + kCkWarps - 1) / kCkWarps), (unsigned)batch);
   const dim3 block(kCkWarps * 32);
-  if (r == 32) return launch_kernel(restore_kernel<T_OUT, 32, VEC>, grid, block, 0, st, pdl, q, scale, rows, cols, nb, out, ldo);
-  if (r == 8) return launch_kernel(restore_kernel<T_OUT, 8, VEC>, grid, block, 0, st, pdl, q, scale, rows, cols, nb, out, ldo);
-  return launch_kernel(restore_kernel<T_OUT, 2, VEC>, grid, block, 0, st, pdl, q, scale, rows, cols, nb, out, ldo);
+  if (r == 32) return launch_kernel(restore_kernel<T_OUT, 32, VEC>, grid, block, 0, st, true, q, scale, rows, cols, nb, out, ldo);
+  if (r == 8) return launch_kernel(restore_kernel<T_OUT, 8, VEC>, grid, block, 0, st, true, q, scale, rows, cols, nb, out, ldo);
+  return launch_kernel(restore_kernel<T_OUT, 2, VEC>, grid, block, 0, st, true, q, scale, rows, cols, nb, out, ldo);
 }
 
 static bool al(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -227,17 +229,17 @@ cudaError_t launch_checkpoint(const void* x, bool bf16, int64_t rows, int64_t co
 }
 
 cudaError_t launch_restore(const uint8_t* q, const uint8_t* scale, int64_t batch, int64_t rows, int64_t cols, void* out,
-                           bool f32, int64_t ldo, bool pdl, cudaStream_t st) {
+                           bool f32, int64_t ldo, cudaStream_t st) {
   if (batch == 0 || rows == 0 || cols == 0) return cudaSuccess;
   const bool vec = al(q, 8) && al(out, 16) && cols % 8 == 0 && ldo % (f32 ? 4 : 8) == 0;
   if (f32) {
     auto* p = static_cast<float*>(out);
-    return vec ? restore_r<float, true>(q, scale, batch, rows, cols, p, ldo, pdl, st)
-               : restore_r<float, false>(q, scale, batch, rows, cols, p, ldo, pdl, st);
+    return vec ? restore_r<float, true>(q, scale, batch, rows, cols, p, ldo, st)
+               : restore_r<float, false>(q, scale, batch, rows, cols, p, ldo, st);
   }
   auto* p = static_cast<__nv_bfloat16*>(out);
-  return vec ? restore_r<__nv_bfloat16, true>(q, scale, batch, rows, cols, p, ldo, pdl, st)
-             : restore_r<__nv_bfloat16, false>(q, scale, batch, rows, cols, p, ldo, pdl, st);
+  return vec ? restore_r<__nv_bfloat16, true>(q, scale, batch, rows, cols, p, ldo, st)
+             : restore_r<__nv_bfloat16, false>(q, scale, batch, rows, cols, p, ldo, st);
 }
 
 }  // namespace moe

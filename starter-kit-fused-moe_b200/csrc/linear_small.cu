@@ -154,16 +154,18 @@ static cudaError_t launch_ls(const LinearSmallArgs& a, bool vec, cudaStream_t st
   int cl = 1;
   while (cl < 8 && groups * cl < 3 * 148 && chunks > kLsWarps * cl) cl *= 2;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = cl;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)groups, cl);
   cfg.blockDim = dim3(kLsWarps * 32);
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return vec ? cudaLaunchKernelEx(&cfg, linear_small_kernel<NT8, GATED, true>, a)
              : cudaLaunchKernelEx(&cfg, linear_small_kernel<NT8, GATED, false>, a);
 }

@@ -568,18 +568,22 @@ __global__ void __launch_bounds__(kLtThreads, 1)
   }
 }
 
-// A warp takes 256 columns of a row, 8 per lane.
+// A warp takes 256 columns of a row, neighbouring lanes neighbouring columns.
 __global__ void __launch_bounds__(256) pad_kernel(PadArgs a) {
+  pdl_wait();
   pdl_trigger();
-  const int j = blockIdx.z, c = 256 * blockIdx.y + 8 * (threadIdx.x & 31);
+  const int j = blockIdx.z, c = 256 * blockIdx.y + (threadIdx.x & 31);
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= a.rows[j] || c >= a.cols[j]) return;
-  const uint16_t* s = static_cast<const uint16_t*>(a.src[j]) + row * a.lds[j] + c;
-  uint32_t v[8];
+  if (row >= a.rows[j]) return;
+  const uint16_t* s = static_cast<const uint16_t*>(a.src[j]) + row * a.lds[j];
+  uint16_t* d = static_cast<uint16_t*>(a.dst[j]) + row * a.ldd[j];
+  uint16_t v[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = c + e < a.cols[j] ? __ldg(s + e) : 0;
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dst[j]) + row * a.ldd[j] + c) =
-      make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  for (int e = 0; e < 8; ++e)
+    if (c + 32 * e < a.cols[j]) v[e] = __ldg(s + c + 32 * e);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (c + 32 * e < a.cols[j]) d[c + 32 * e] = v[e];
 }
 cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
   if (a.count == 0) return cudaSuccess;
@@ -590,8 +594,7 @@ cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
     cols = cols > a.cols[j] ? cols : a.cols[j];
   }
   if ((cols + 255) / 256 > 65535) return cudaErrorInvalidValue;
-  pad_kernel<<<dim3((unsigned)((rows + 7) / 8), (cols + 255) / 256, a.count), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_kernel(pad_kernel, dim3((unsigned)((rows + 7) / 8), (cols + 255) / 256, a.count), dim3(256), 0, st, true, a);
 }
 
 // Adds the K slices' partial rows in slice order and runs the epilogue. A warp
@@ -602,6 +605,7 @@ template <bool GATED, bool KEEP>
 __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
   const int lane = threadIdx.x & 31;
   pdl_wait();
+  pdl_trigger();
   const int H = GATED ? a.n_tile / 2 : a.n_tile, col_blocks = (H + 127) / 128;
   const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);     // (tile, row, column block)
   const int64_t i = unit / (256 * col_blocks);
@@ -754,7 +758,7 @@ static cudaError_t launch_t(const LinearTileMaps& maps, const LinearTileArgs& a,
   const int64_t want = a.units < clusters ? a.units : clusters;
   cfg.gridDim = dim3((unsigned)(2 * want));
   cfg.stream = st;
-  cfg.numAttrs = a.pdl ? 2 : 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, maps, a);
 }
 

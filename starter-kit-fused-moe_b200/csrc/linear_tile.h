@@ -17,7 +17,6 @@ struct LinearTileArgs {
   int splits;
   int64_t full_tiles;     // tiles done whole; the others are cut into `splits` K slices
   int64_t units;          // full_tiles + splits * (number of the others)
-  int pdl;                // launched right behind another kernel of the same call
   int vec;                // y (and the residual) can be accessed in 16 bytes
   float* partial;         // splits > 1: fp32 [other tiles][splits][256][n_tile], 16-byte aligned
   LinearEpilogue ep;

@@ -66,7 +66,7 @@ Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gat
 // A: [terms][rows][..], term stride in elements.
 int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, int64_t m, int64_t out_cols, int64_t k,
                 const void* A, int64_t lda, int64_t term_stride, const void* B, int64_t ldb, int64_t b_rows,
-                const moe::LinearEpilogue& ep, uint8_t* partial, bool pdl, cudaStream_t st, const char* what) {
+                const moe::LinearEpilogue& ep, uint8_t* partial, cudaStream_t st, const char* what) {
   moe::LinearTileArgs t{};
   t.m = m;
   t.out_cols = out_cols;
@@ -81,7 +81,6 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.full_tiles = p.plan.full;
   t.units = p.plan.full + p.plan.tail * t.splits;
   t.ep = ep;
-  t.pdl = pdl;
   const int ysize = ep.y_f32 ? 4 : 2;
   t.vec = aligned(ep.y, 16) && ep.ldy * ysize % 16 == 0 &&
           (!ep.residual || (aligned(ep.residual, 16) && ep.ldr % 8 == 0 && ep.ldr > 0));
@@ -205,12 +204,11 @@ int moe_linear_run(const MoeLinearArgs* a, void* stream) {
   if (p.pad_w) pads.add(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldp);
   cudaError_t e = moe::launch_pad(pads, st);
   if (e != cudaSuccess) return done(e, "linear: preparing the operands");
-  const bool launched = pads.count > 0;
   const void* x = p.pad_x ? ws + p.x : a->x;
   const void* w = p.pad_w ? ws + p.w : a->weight;
   const int64_t ldx = p.pad_x ? p.ldp : a->ldx;
   return run_product(p.prod, false, false, a->activation == MOE_ACT_SWIGLU, a->z8 != nullptr, a->m, O, a->k, x, ldx,
-                     a->m * ldx, w, p.pad_w ? p.ldp : a->ldw, a->n, ep, ws, launched, st, "linear product");
+                     a->m * ldx, w, p.pad_w ? p.ldp : a->ldw, a->n, ep, ws, st, "linear product");
 }
 
 size_t moe_linear_grad_workspace_bytes(const MoeLinearGradArgs* a) {
@@ -249,7 +247,6 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
   if (p.pad_w) pads.add(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldk);
   e = moe::launch_pad(pads, st);
   if (e != cudaSuccess) return done(e, "linear gradient: preparing the operands");
-  bool launched = pads.count > 0;     // later kernels may start behind an earlier one of this call
   if (p.need_dz || a->grad_bias) {
     moe::ActGradArgs g{};
     g.dy = a->grad_y;
@@ -264,8 +261,7 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
     g.act = a->activation;
     g.dy_f32 = a->grad_y_f32;
     g.terms = p.terms;
-    e = moe::launch_act_grad(g, launched, st);
-    launched = true;
+    e = moe::launch_act_grad(g, st);
     if (e == cudaSuccess && a->grad_bias)
       e = moe::launch_colsum_finish(g.colsum, p.chunks, a->n, a->grad_bias, a->grad_f32 != 0, st);
     if (e != cudaSuccess) return done(e, "activation gradient");
@@ -277,17 +273,16 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
     const int64_t ldw = p.pad_w ? p.ldk : a->ldw;
     moe::LinearEpilogue ep{nullptr, nullptr, a->grad_x, nullptr, nullptr, 0, a->k, MOE_ACT_NONE, a->grad_f32};
     if (int rc = run_product(p.px, false, true, false, false, a->m, a->k, a->n, dz, ldz, term_stride, w, ldw, a->n, ep,
-                             ws, launched, st, "input gradient"))
+                             ws, st, "input gradient"))
       return rc;
-    launched = true;
   }
   if (a->grad_weight) {
     e = moe::launch_restore(static_cast<const uint8_t*>(a->x8), static_cast<const uint8_t*>(a->x_scale), 1, a->m, a->k,
-                            ws + p.xhat, false, p.ldk, launched, st);
+                            ws + p.xhat, false, p.ldk, st);
     if (e != cudaSuccess) return done(e, "restoring the input checkpoint");
     moe::LinearEpilogue ep{nullptr, nullptr, a->grad_weight, nullptr, nullptr, 0, a->k, MOE_ACT_NONE, a->grad_f32};
     if (int rc = run_product(p.pw, true, true, false, false, a->n, a->k, a->m, dz, ldz, term_stride, ws + p.xhat, p.ldk,
-                             a->m, ep, ws, true, st, "weight gradient"))
+                             a->m, ep, ws, st, "weight gradient"))
       return rc;
   }
   return MOE_OK;
@@ -312,7 +307,7 @@ int moe_restore_activations(const void* q, const void* scale, int64_t batch, int
   if (batch == 0 || rows == 0 || cols == 0) return MOE_OK;
   if (!q || !scale || !out || !aligned(out, out_f32 ? 4 : 2)) return bad("restore: NULL or misaligned pointer");
   return done(moe::launch_restore(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), batch, rows, cols,
-                                  out, out_f32 != 0, cols, false, static_cast<cudaStream_t>(stream)),
+                                  out, out_f32 != 0, cols, static_cast<cudaStream_t>(stream)),
               "restore");
 }
 

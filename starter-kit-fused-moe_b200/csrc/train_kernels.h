@@ -26,12 +26,13 @@ struct LinearEpilogue {
   int y_f32;
 };
 
-// `pdl`: launched right behind another kernel of the same call (programmatic
-// dependent launch; every kernel here waits for its predecessor before it reads).
+// Every kernel here is launched with programmatic stream serialization: its
+// blocks may become resident while the preceding kernel of the stream ends, and
+// wait for that kernel's completion before they touch global memory.
 cudaError_t launch_checkpoint(const void* x, bool bf16, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q,
                               uint8_t* scale, cudaStream_t st);
 cudaError_t launch_restore(const uint8_t* q, const uint8_t* scale, int64_t batch, int64_t rows, int64_t cols, void* out,
-                           bool f32, int64_t ldo, bool pdl, cudaStream_t st);
+                           bool f32, int64_t ldo, cudaStream_t st);
 
 // Products of at most kSmallTokens tokens without a kept pre-activation
 // (linear_small.cu); larger ones run on linear_tile.cu.
@@ -51,7 +52,7 @@ struct ActGradArgs {
   int m, n, act, dy_f32, terms;
 };
 int act_grad_chunks(int m, int n);
-cudaError_t launch_act_grad(const ActGradArgs& a, bool pdl, cudaStream_t st);
+cudaError_t launch_act_grad(const ActGradArgs& a, cudaStream_t st);
 cudaError_t launch_colsum_finish(const float* colsum, int chunks, int n, void* out, bool f32, cudaStream_t st);
 
 struct BalanceArgs {

@@ -471,3 +471,35 @@ def test_streams_and_graphs(pkg, m):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs[0], want[1]))
+
+
+def test_graph_between_copies(pkg):
+    """Captured calls whose inputs come from copies and other kernels right before them, and whose outputs are
+    copied right after, replay to the eager results (the kernels start while their predecessors end)."""
+    x, w = randn(200, 512, seed=1), randn(256, 512, seed=2, scale=0.05)
+    xs = torch.empty_like(x)
+    outs = [torch.empty(200, 256, dtype=BF, device="cuda") for _ in range(2)]
+
+    def step():
+        xs.copy_(x)
+        a = pkg.linear(xs, w)
+        outs[0].copy_(a)
+        xs.mul_(2)
+        q, s = pkg.checkpoint_activations(xs)
+        b = pkg.linear(pkg.restore_activations(q, s), w)
+        outs[1].copy_(b)
+
+    step()
+    torch.cuda.synchronize()
+    want = [o.clone() for o in outs]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        g.replay()
+        assert all(torch.equal(o, v) for o, v in zip(outs, want))
+    for _ in range(50):
+        step()
+    assert all(torch.equal(o, v) for o, v in zip(outs, want))
