@@ -306,8 +306,7 @@ int moe_linear_run(const MoeLinearArgs* args, void* stream);
  *   dz = dy * act'(z^),  grad_x = dz W,  grad_weight = dz^T x^,  grad_bias = sum over tokens of dz
  * with x^, z^ the values the checkpoints stand for (the residual's gradient is
  * dy). dz is rounded to bf16 for the two products; with grad_f32 it is kept as
- * the sum of two bf16 terms, so that fp32 gradients are not limited by that
- * rounding. NULL outputs are not computed. grad_x, grad_weight and grad_bias are
+ * the sum of three bf16 terms, which hold all its bits. NULL outputs are not computed. grad_x, grad_weight and grad_bias are
  * contiguous, bf16 (f32 if grad_f32), and overwritten. Sums run in a fixed
  * order: repeated calls give the same bits. */
 typedef struct MoeLinearGradArgs {

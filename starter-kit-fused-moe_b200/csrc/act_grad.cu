@@ -6,8 +6,9 @@
 //
 // dz is computed in fp32 and written in bf16, the operand type of the two
 // gradient products (half a step, at most 2^-8 relative, per value; the products sum
-// many of them in fp32). With `terms` = 2 the remainder dz - bf16(dz) follows as
-// a second bf16 matrix, so fp32 gradients keep about 17 bits of dz.
+// many of them in fp32). With `terms` = 3 the remainder follows as two more bf16
+// matrices, which together hold dz's 24 bits, so that fp32 gradients are as
+// exact as an fp32 product (two terms left 2.5e-6 of the result's norm).
 //
 // Bound by HBM: dy, one byte per z value, two (or four) written per dz value.
 // 32 threads take 256 columns (8 neighbouring ones each, 16-byte accesses) and
@@ -22,7 +23,7 @@ constexpr int kAgRows = 64, kAgCols = 256;
 
 // FAST (dz rounded to bf16 once): hardware exponential and reciprocal, good to
 // 2^-20 of 1 + |z|; the exact ones bound the kernel by arithmetic (121 us instead
-// of 60 at 16384 x 4096) and serve the two-term form.
+// of 60 at 16384 x 4096) and serve the three-term form.
 template <int HALVES, bool F32, bool VEC, bool FAST>
 __global__ void __launch_bounds__(256, 2) act_grad_kernel(ActGradArgs a, int O) {
   __shared__ float red[8][kAgCols];
@@ -153,27 +154,25 @@ __global__ void __launch_bounds__(256, 2) act_grad_kernel(ActGradArgs a, int O) 
         for (int j = 0; j < 8; ++j) sum[h][j] += z[h][j];
         if (dz == nullptr) continue;
         __nv_bfloat16* out = dz + row * a.ldz + (int64_t)h * O;
-        float lo[8];
-        if constexpr (!FAST)
+        // FAST: one term; else three, each the rounded remainder of those before it (the
+        // differences are exact); a non-finite value is whole in the first
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float hi = __bfloat162float(__float2bfloat16_rn(z[h][j]));
-          lo[j] = isfinite(hi) ? z[h][j] - hi : 0.f;       // a non-finite value is whole in the first term
-        }
-        if constexpr (VEC) {
-          if (col(0) < O) {
-            *reinterpret_cast<uint4*>(out + col(0)) = make_uint4(pack_bf16(z[h][0], z[h][1]), pack_bf16(z[h][2], z[h][3]),
-                                                                 pack_bf16(z[h][4], z[h][5]), pack_bf16(z[h][6], z[h][7]));
-            if (!FAST && a.terms == 2)
-              *reinterpret_cast<uint4*>(out + term + col(0)) =
-                  make_uint4(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7]));
+        for (int t = 0; t < (FAST ? 1 : 3); ++t) {
+          if constexpr (VEC) {
+            if (col(0) < O)
+              *reinterpret_cast<uint4*>(out + t * term + col(0)) =
+                  make_uint4(pack_bf16(z[h][0], z[h][1]), pack_bf16(z[h][2], z[h][3]), pack_bf16(z[h][4], z[h][5]),
+                             pack_bf16(z[h][6], z[h][7]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col(j) < O) out[t * term + col(j)] = __float2bfloat16_rn(z[h][j]);
           }
-        } else {
+          if constexpr (!FAST)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (col(j) < O) {
-              out[col(j)] = __float2bfloat16_rn(z[h][j]);
-              if (!FAST && a.terms == 2) out[term + col(j)] = __float2bfloat16_rn(lo[j]);
+            for (int j = 0; j < 8; ++j) {
+              const float part = __bfloat162float(__float2bfloat16_rn(z[h][j]));
+              z[h][j] = isfinite(part) ? z[h][j] - part : 0.f;
             }
         }
       }

@@ -16,10 +16,20 @@
 // the contraction then runs over the terms one after the other with B's
 // coordinates repeating.
 //
-// Warps: 0 TMA producer, 1 MMA issuer (the leader CTA's), 2-9 epilogue. Two
-// accumulators of NT columns in TMEM let a tile's epilogue overlap the next
+// Sums. The tensor core adds to its fp32 accumulator by truncation, so a long
+// chain drifts: 8e-6 of the result's norm at K = 7168, 2e-6 at 2048, 5e-7 at
+// 512, where an fp32 product has 9e-7. A bf16 result (2^-8) does not show that,
+// an fp32 one does, and so does a kept pre-activation (one value in 10^4 moves to
+// the next e4m3 step). For those (CHAIN) the chain is cut every 12 (fp32) or 24
+// (kept) K-blocks of 64: the epilogue warps add each partial accumulator to fp32
+// registers, rounding to nearest, while the tensor core fills the other one. The
+// reads of TMEM cost the tensor core about a K-block each, 10 % and 4 %.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (the leader CTA's), 4-11 epilogue. The two
+// accumulators of NT columns in TMEM also let a tile's epilogue overlap the next
 // tile's products. Persistent grid, one pair per two SMs; tiles are walked in
 // bands of 8 row tiles so that the tiles in flight share both operands in L2.
+//
 // The tiles that do not fill a last round of the pairs (all of them, when there
 // are fewer tiles than pairs) are cut into K slices: the slices leave fp32
 // partial tiles in the workspace and a second kernel, launched to start as this
@@ -36,7 +46,12 @@
 namespace moe {
 
 constexpr int kLtStages = 6, kLtStageBytes = 32768, kLtTileA = 16384;
-constexpr int kLtThreads = 320, kLtEpiWarps = 8, kLtTmemCols = 512;
+constexpr int kLtThreads = 384, kLtEpiWarps = 8, kLtTmemCols = 512;
+// CHAIN keeps 128 sums per epilogue thread in registers: the warpgroup of the producer
+// and the MMA issuer hands registers to the two epilogue warpgroups. The split
+// has to add up to what the block is launched with.
+constexpr int kLtRegsLaunch = 168, kLtRegsIssue = 40, kLtRegsEpi = 232;
+static_assert(kLtRegsIssue * 128 + kLtRegsEpi * 256 <= kLtRegsLaunch * kLtThreads, "register split");
 constexpr int kLtBand = 8;
 constexpr int kLtStaging = 4096;     // per epilogue warp: a 32 x 32 box of fp32, or two of bf16
 
@@ -84,6 +99,40 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
       : "memory");
+}
+
+// 32 lanes x 32-bit, 32 or 64 consecutive columns per thread. A load of TMEM
+// queues behind the MMAs issued so far, so partial sums are taken in few
+// instructions: 32 columns at a time held the tensor core up for 1.6 us per
+// accumulator, 64 for 0.8.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%2"
+      "7,%28,%29,%30,%31"
+      "}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%2"
+      "7,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%5"
+      "2,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+        "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+        "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+        "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+        "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+      : "r"(taddr));
 }
 
 struct LtUnit {
@@ -138,7 +187,13 @@ __device__ __forceinline__ void lt_bias32(const __nv_bfloat16* bias, int64_t c, 
   lt_bias16(bias, c, end, v);
   lt_bias16(bias, c + 16, end, v + 16);
 }
-__device__ __forceinline__ void lt_act32(float* v, int act) {
+// bf16 results take silu from the hardware exponential and reciprocal (2^-20 of
+// 1 + |z|), fp32 ones from the exact ones: the epilogue is bound by its
+// instructions, and the exact quotient is half of them.
+__device__ __forceinline__ float lt_silu(float z, bool exact) {
+  return exact ? act_value(z, kActSilu) : z * sigmoid_fast(z);
+}
+__device__ __forceinline__ void lt_act32(float* v, int act, bool exact) {
   if (act == kActNone) return;
   if (act == kActRelu) {
 #pragma unroll
@@ -146,22 +201,47 @@ __device__ __forceinline__ void lt_act32(float* v, int act) {
   } else if (act == kActGelu) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActGelu);
+  } else if (exact) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = lt_silu(v[i], true);
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActSilu);
+    for (int i = 0; i < 32; ++i) v[i] = lt_silu(v[i], false);
   }
 }
-// Stores of a warp's 32 rows go through shared memory and TMA: a lane holds a
-// row, so direct stores touch 32 lines with 16 bytes each, and a tile's epilogue
-// took longer than a short contraction (71 us for the gate's fp32 input
-// gradient; copying out of shared memory in coalesced pieces 48). The boxes of 32
-// rows by 32 columns lie in the swizzle of the output's tensor map, which also
-// cuts off rows and columns past the matrix.
+__device__ __forceinline__ void lt_gate32(float* v, const float* z, bool exact) {
+  if (exact) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= lt_silu(z[i], true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= lt_silu(z[i], false);
+  }
+}
+// Stores of a warp's 32 rows go through shared memory: a lane holds a row, so
+// direct stores touch 32 lines with 16 bytes each, and a tile's epilogue took
+// longer than a short contraction (71 us for the gate's fp32 input gradient).
+// Boxes of 32 rows by 32 columns: bf16 ones leave by TMA, which fetches the
+// residual's boxes too and cuts off what lies past the matrix; fp32 ones are
+// copied out in whole 128-byte lines, because a TMA store queues behind the
+// producer's loads and a warp has room for one fp32 box only (42 us against 33).
 __device__ __forceinline__ void lt_stage_f32(uint8_t* box, const float* v, int lane) {       // 128-byte swizzle
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     *reinterpret_cast<float4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) =
         make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+// `rows` rows of the staged box to dst (16-byte aligned rows `ld` floats apart).
+__device__ __forceinline__ void lt_copy_f32(const uint8_t* box, float* dst, int64_t ld, int rows, int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3), p = lane & 7;
+    if (r < rows)
+      *reinterpret_cast<float4*>(dst + r * ld + 4 * p) =
+          *reinterpret_cast<const float4*>(box + r * 128 + ((p ^ (r & 7)) << 4));
+  }
+  __syncwarp();
 }
 __device__ __forceinline__ uint4* lt_bf16_piece(uint8_t* box, int i, int lane) {             // 64-byte swizzle
   return reinterpret_cast<uint4*>(box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4));
@@ -193,25 +273,28 @@ __device__ __forceinline__ void lt_store16_any(const LinearEpilogue& ep, uint8_t
   float(*stage)[17] = reinterpret_cast<float(*)[17]>(stage8);
   const int64_t col = c + (lane & 15);
   const bool in = col < end;
-  float res[16];                                       // all 16 loads are in flight together
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = (lane >> 4) + 2 * i;
-    res[i] = ep.residual != nullptr && in && r < rows
-                 ? __bfloat162float(static_cast<const __nv_bfloat16*>(ep.residual)[(row0 + r) * ep.ldr + col])
-                 : 0.f;
-  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) stage[lane][i] = v[i];
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = (lane >> 4) + 2 * i;
-    const int64_t row = row0 + r;
-    const float y = stage[r][lane & 15] + res[i];
-    if (!in || r >= rows) continue;
-    if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + col] = y;
-    else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + col] = __float2bfloat16_rn(y);
+  for (int h = 0; h < 16; h += 8) {
+    float res[8];                                      // eight loads in flight
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = (lane >> 4) + 2 * (h + i);
+      res[i] = ep.residual != nullptr && in && r < rows
+                   ? __bfloat162float(static_cast<const __nv_bfloat16*>(ep.residual)[(row0 + r) * ep.ldr + col])
+                   : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = (lane >> 4) + 2 * (h + i);
+      const int64_t row = row0 + r;
+      const float y = stage[r][lane & 15] + res[i];
+      if (!in || r >= rows) continue;
+      if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + col] = y;
+      else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + col] = __float2bfloat16_rn(y);
+    }
   }
   __syncwarp();
 }
@@ -224,12 +307,17 @@ __device__ __forceinline__ uint32_t lt_amax32(const float* v, int64_t c, int64_t
 }
 __device__ __forceinline__ void lt_store_z32(uint8_t* z, int64_t c, int64_t end, const float* v, uint32_t code) {
   const float inv = e8m0_inverse(code);
+  const bool hold = code == kTopScaleCode;
   uint32_t w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float s[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = code == kTopScaleCode ? hold_finite(v[4 * i + j] * inv) : v[4 * i + j] * inv;
+    for (int j = 0; j < 4; ++j) s[j] = v[4 * i + j] * inv;
+    if (hold) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = hold_finite(s[j]);
+    }
     w[i] = e4m3x4(s[0], s[1], s[2], s[3]);
   }
   if (c + 32 <= end && (reinterpret_cast<uintptr_t>(z + c) & 15) == 0) {
@@ -242,7 +330,7 @@ __device__ __forceinline__ void lt_store_z32(uint8_t* z, int64_t c, int64_t end,
   }
 }
 
-template <bool A_MN, bool B_MN, bool GATED, bool KEEP>
+template <bool A_MN, bool B_MN, bool GATED, bool KEEP, bool CHAIN>
 __global__ void __launch_bounds__(kLtThreads, 1)
     linear_tile_kernel(const __grid_constant__ LinearTileMaps maps, const LinearTileArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -287,90 +375,98 @@ __global__ void __launch_bounds__(kLtThreads, 1)
   const uint32_t tmem_base = S.tmem_base;
   volatile int* abort_flag = &S.abort_flag;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      const uint32_t bytes = 2 * (kLtTileA + H * 128);
-      for (int64_t u = wid; u < a.units && ok && !*abort_flag; u += G) {
-        const LtUnit x = lt_unit(a, u);
-        const int m0 = x.mt * 256 + crank * 128;
-        // B rows of this CTA's half: the next H columns of the tile, or for a gated tile its first-half
-        // (leader) and second-half (peer) rows
-        const int n0 = GATED ? crank * a.gate_rows + x.nt * H : x.nt * NT + crank * H;
-        for (int kb = x.kb0; kb < x.kb1; ++kb, ++it) {
-          const int s = it % kLtStages;
-          if (!mbar_wait(smem_u32(&S.empty[s]), ((it / kLtStages) & 1) ^ 1)) {
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          const uint32_t fb = smem_u32(&S.full[s]);
-          const uint32_t fbl = mapa_shared(fb, 0);
-          const uint32_t sa = smem_u32(smem + s * kLtStageBytes), sb = sa + kLtTileA;
-          const int term = kb / a.term_blocks, kt = (kb - term * a.term_blocks) * 64;
-          if (crank == 0) mbar_arrive_expect_tx(fb, bytes);
-          if constexpr (A_MN) {
-            tma_load_3d_pair(sa, &maps.a, fbl, m0, kt, term);
-            tma_load_3d_pair(sa + 8192, &maps.a, fbl, m0 + 64, kt, term);
-          } else {
-            tma_load_3d_pair(sa, &maps.a, fbl, kt, m0, term);
-          }
-          if constexpr (B_MN) {
-            tma_load_2d_pair(sb, &maps.b, fbl, n0, kt);
-            if (H == 128) tma_load_2d_pair(sb + 8192, &maps.b, fbl, n0 + 64, kt);
-          } else {
-            tma_load_2d_pair(sb, &maps.b, fbl, kt, n0);
+  if (warp < 4) {
+    if constexpr (CHAIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLtRegsIssue));
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer
+      if (lane == 0) {
+        int it = 0;
+        bool ok = true;
+        const uint32_t bytes = 2 * (kLtTileA + H * 128);
+        for (int64_t u = wid; u < a.units && ok && !*abort_flag; u += G) {
+          const LtUnit x = lt_unit(a, u);
+          const int m0 = x.mt * 256 + crank * 128;
+          // B rows of this CTA's half: the next H columns of the tile, or for a gated tile its first-half
+          // (leader) and second-half (peer) rows
+          const int n0 = GATED ? crank * a.gate_rows + x.nt * H : x.nt * NT + crank * H;
+          for (int kb = x.kb0; kb < x.kb1; ++kb, ++it) {
+            const int s = it % kLtStages;
+            if (!mbar_wait(smem_u32(&S.empty[s]), ((it / kLtStages) & 1) ^ 1)) {
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            const uint32_t fb = smem_u32(&S.full[s]);
+            const uint32_t fbl = mapa_shared(fb, 0);
+            const uint32_t sa = smem_u32(smem + s * kLtStageBytes), sb = sa + kLtTileA;
+            // the small terms first: the chain's truncation is relative to the running sum
+            const int part = kb / a.term_blocks, kt = (kb - part * a.term_blocks) * 64, term = a.terms - 1 - part;
+            if (crank == 0) mbar_arrive_expect_tx(fb, bytes);
+            if constexpr (A_MN) {
+              tma_load_3d_pair(sa, &maps.a, fbl, m0, kt, term);
+              tma_load_3d_pair(sa + 8192, &maps.a, fbl, m0 + 64, kt, term);
+            } else {
+              tma_load_3d_pair(sa, &maps.a, fbl, kt, m0, term);
+            }
+            if constexpr (B_MN) {
+              tma_load_2d_pair(sb, &maps.b, fbl, n0, kt);
+              if (H == 128) tma_load_2d_pair(sb + 8192, &maps.b, fbl, n0 + 64, kt);
+            } else {
+              tma_load_2d_pair(sb, &maps.b, fbl, kt, n0);
+            }
           }
         }
       }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (leader)
-    if (lane == 0 && crank == 0) {
-      const uint32_t idesc = idesc_bf16(NT, A_MN, B_MN);
-      int it = 0, tt = 0;
-      bool ok = true;
-      for (int64_t u = wid; u < a.units && ok && !*abort_flag; u += G, ++tt) {
-        const LtUnit x = lt_unit(a, u);
-        const int b = tt & 1;
-        if (!mbar_wait(smem_u32(&S.tempty[b]), ((tt >> 1) & 1) ^ 1)) {
-          *abort_flag = 1;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem_base + (uint32_t)(b * 256);
-        for (int kb = x.kb0; kb < x.kb1; ++kb, ++it) {
-          const int s = it % kLtStages;
-          if (!mbar_wait(smem_u32(&S.full[s]), (it / kLtStages) & 1)) {
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * kLtStageBytes), sb = sa + kLtTileA;
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer (leader)
+      if (lane == 0 && crank == 0) {
+        const uint32_t idesc = idesc_bf16(NT, A_MN, B_MN);
+        int it = 0, tt = 0;                                // stages, accumulators
+        bool ok = true;
+        for (int64_t u = wid; u < a.units && ok && !*abort_flag; u += G) {
+          const LtUnit x = lt_unit(a, u);
+          for (int kb = x.kb0; kb < x.kb1 && ok; ++tt) {
+            const int b = tt & 1, end = CHAIN ? min(kb + a.chain, x.kb1) : x.kb1;
+            if (!mbar_wait(smem_u32(&S.tempty[b]), ((tt >> 1) & 1) ^ 1)) {
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t d = tmem_base + (uint32_t)(b * 256);
+            for (bool more = false; kb < end; ++kb, ++it, more = true) {
+              const int s = it % kLtStages;
+              if (!mbar_wait(smem_u32(&S.full[s]), (it / kLtStages) & 1)) {
+                *abort_flag = 1;
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t sa = smem_u32(smem + s * kLtStageBytes), sb = sa + kLtTileA;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint64_t da = A_MN ? sdesc_sw128_mn(sa + kk * 2048) : sdesc_sw128(sa + kk * 32);
-            const uint64_t db = B_MN ? sdesc_sw128_mn(sb + kk * 2048) : sdesc_sw128(sb + kk * 32);
-            mma_bf16_pair(d, da, db, idesc, (kb > x.kb0 || kk) ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk) {
+                const uint64_t da = A_MN ? sdesc_sw128_mn(sa + kk * 2048) : sdesc_sw128(sa + kk * 32);
+                const uint64_t db = B_MN ? sdesc_sw128_mn(sb + kk * 2048) : sdesc_sw128(sb + kk * 32);
+                mma_bf16_pair(d, da, db, idesc, (more || kk) ? 1u : 0u);
+              }
+              mma_commit_pair(smem_u32(&S.empty[s]));
+            }
+            if (ok) mma_commit_pair(smem_u32(&S.tfull[b]));
           }
-          mma_commit_pair(smem_u32(&S.empty[s]));
         }
-        if (ok) mma_commit_pair(smem_u32(&S.tfull[b]));
       }
     }
   } else {
+    if constexpr (CHAIN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLtRegsEpi));
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3, g = (warp - 2) >> 2;
+    const int q = warp & 3, g = (warp - 4) >> 2, ew = warp - 4;
     const int r = 32 * q + lane;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
     const LinearEpilogue& ep = a.ep;
     const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(ep.bias);
     const int64_t O = a.out_cols;
     const int64_t z_blocks = (O + 127) / 128;
-    uint8_t* stage = staging + (warp - 2) * kLtStaging;
+    uint8_t* stage = staging + ew * kLtStaging;
     const uint32_t stage_addr = smem_u32(stage);
     // y as bf16 in whole boxes with a residual: the residual's boxes are fetched into the boxes y leaves from
     const bool res_boxes = a.vec && ep.residual != nullptr && !ep.y_f32;
@@ -378,9 +474,8 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     bool ok = true;
     int tt = 0;
     uint32_t res_count = 0;                              // residual boxes waited for
-    for (int64_t u = wid; u < a.units; u += G, ++tt) {
+    for (int64_t u = wid; u < a.units; u += G) {
       const LtUnit x = lt_unit(a, u);
-      const int b = tt & 1;
       const int64_t row0 = (int64_t)x.mt * 256 + crank * 128 + 32 * q, row = row0 + lane;
       const bool valid = row < a.m;
       const int warp_rows = (int)max((int64_t)0, min((int64_t)32, a.m - row0));
@@ -390,7 +485,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       const bool live = warp_rows > 0 && chunks > 0;
       auto fetch_residual = [&](int j) {                 // chunk j into box j & 1, whose last store has been read
         if (lane == 0) {
-          const uint32_t bar = smem_u32(&S.res[warp - 2][j & 1]);
+          const uint32_t bar = smem_u32(&S.res[ew][j & 1]);
           mbar_arrive_expect_tx(bar, 2048);
           tma_load_2d(stage_addr + (j & 1) * 2048, &maps.res, bar, (int)c0 + 32 * j, (int)row0);
         }
@@ -403,45 +498,91 @@ __global__ void __launch_bounds__(kLtThreads, 1)
         }
       };
       if constexpr (!(GATED && KEEP)) fetch_first();     // ahead of the product
-      if (ok && (*abort_flag || !mbar_wait(smem_u32(&S.tfull[b]), (tt >> 1) & 1))) {
-        *abort_flag = 1;
-        ok = false;
-      }
-      tc_fence_after();
-      const uint32_t acc = lane_addr + (uint32_t)(b * 256);
-      auto release = [&] {
+      // the accumulator at hand (CHAIN: the one whose partial sums are taken)
+      auto wait_acc = [&] {
+        const int b = tt & 1;
+        if (ok && (*abort_flag || !mbar_wait(smem_u32(&S.tfull[b]), (tt >> 1) & 1))) {
+          *abort_flag = 1;
+          ok = false;
+        }
+        tc_fence_after();
+      };
+      auto release = [&] {                               // back to the leader's MMA
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&S.tempty[b]), 0));
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&S.tempty[tt & 1]), 0));
+        ++tt;
       };
+      auto acc_at = [&](int col) { return lane_addr + (uint32_t)((tt & 1) * 256 + col); };
       auto from_tmem = [&](int col, float* v) {          // 32 columns
-        if (ok) {
-          tmem_ld16(acc + col, v);
-          tmem_ld16(acc + col + 16, v + 16);
-          tmem_ld_wait();
-        } else {
+        tmem_ld32(acc_at(col), v);
+        tmem_ld_wait();
+        if (!ok) {                                       // a wait ran out: NaN instead of sums
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = NAN;
         }
       };
+      // CHAIN: the thread's sums, columns g H + i of the tile (gated: g w + i of the first half, and from sum[64]
+      // on those of the second half)
+      float sum[CHAIN ? 128 : 1];
+      if constexpr (CHAIN) {
+        for (int kb = x.kb0; kb < x.kb1; kb += a.chain) {
+          wait_acc();
+          // two loads of up to 64 columns (gated: a half each); columns past w are not used
+          const int col1 = GATED ? H + g * w : g * w + 64;
+          const bool two = GATED || w > 64;
+          if (kb == x.kb0) {
+            tmem_ld64(acc_at(g * w), sum);
+            if (two) tmem_ld64(acc_at(col1), sum + 64);
+            tmem_ld_wait();
+          } else {
+            float v[64];
+            tmem_ld64(acc_at(g * w), v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 64; ++e) sum[e] += v[e];
+            if (two) {
+              tmem_ld64(acc_at(col1), v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 64; ++e) sum[64 + e] += v[e];
+            }
+          }
+          release();
+        }
+        if (!ok) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e) sum[e] = NAN;
+        }
+      } else {
+        wait_acc();
+      }
       if (x.slice >= 0) {                                // fp32 partial tile, [row][column]
         if (warp_rows > 0) {
           const int64_t y0 = ((x.tile - a.full_tiles) * a.splits + x.slice) * 256 + crank * 128 + 32 * q;
-          for (int c = g * H; c < (g + 1) * H; c += 32) {
-            float v[32];
-            from_tmem(c, v);
-            lt_boxes_free<0>(lane);
-            lt_stage_f32(stage, v, lane);
-            lt_box_out(&maps.partial, stage, c, y0, lane);
+          lt_boxes_free<0>(lane);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int lc = GATED && i >= 2 ? 32 * (i - 2) : 32 * i;
+            if (lc >= w) continue;
+            const int col = g * w + lc + (GATED && i >= 2 ? H : 0);
+            if constexpr (CHAIN) {
+              lt_stage_f32(stage, sum + 32 * i, lane);
+            } else {
+              float v[32];
+              from_tmem(col, v);
+              lt_stage_f32(stage, v, lane);
+            }
+            lt_copy_f32(stage, a.partial + y0 * NT + col, NT, warp_rows, lane);
           }
         }
-        release();
+        if constexpr (!CHAIN) release();
         continue;
       }
       // y's columns [c0 + 32 j, + 32)
       auto store = [&](int j, float* v) {
         const int64_t c = c0 + 32 * j;
-        if (!a.vec) {
+        if (!a.vec || (ep.y_f32 && c + 32 > O)) {
           lt_store16_any(ep, stage, row0, warp_rows, c, O, v, lane);
           if (c + 16 < O) lt_store16_any(ep, stage, row0, warp_rows, c + 16, O, v + 16, lane);
         } else if (ep.y_f32) {
@@ -449,13 +590,12 @@ __global__ void __launch_bounds__(kLtThreads, 1)
             const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr;
             lt_bias32(r, c, O, v);
           }
-          lt_boxes_free<0>(lane);
           lt_stage_f32(stage, v, lane);
-          lt_box_out(&maps.out, stage, (int)c, row0, lane);
+          lt_copy_f32(stage, static_cast<float*>(ep.y) + row0 * ep.ldy + c, ep.ldy, warp_rows, lane);
         } else {
           uint8_t* box = stage + (j & 1) * 2048;
           if (res_boxes) {
-            if (ok && !mbar_wait(smem_u32(&S.res[warp - 2][j & 1]), (res_count >> (j & 1)) & 1)) {
+            if (ok && !mbar_wait(smem_u32(&S.res[ew][j & 1]), (res_count >> (j & 1)) & 1)) {
               *abort_flag = 1;
               ok = false;
             }
@@ -483,78 +623,115 @@ __global__ void __launch_bounds__(kLtThreads, 1)
         }
       };
 
-      if constexpr (!GATED) {
-        uint32_t code = 0;
-        if constexpr (KEEP) {                            // NT = 256: this warp's half is one block of the row
-          uint32_t amax = 0;
-          for (int j = 0; j < chunks; ++j) {
-            float v[32];
-            from_tmem(g * H + 32 * j, v);
-            if (bias) lt_bias32(bias, c0 + 32 * j, O, v);
-            amax = lt_amax32(v, c0 + 32 * j, O, amax);
+      if constexpr (CHAIN) {
+        if (bias)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int jj = GATED ? j & 1 : j, h = GATED ? j >> 1 : 0;
+            if (jj < chunks) lt_bias32(bias + h * O, c0 + 32 * jj, O, sum + 32 * j);
           }
-          code = e8m0_of_amax(amax);
-          if (valid && chunks > 0) ep.z_scale[(c0 >> 7) * a.m + row] = (uint8_t)code;
-        }
-        if (live)
-          for (int j = 0; j < chunks; ++j) {
-            float v[32];
-            from_tmem(g * H + 32 * j, v);
-            if (bias) lt_bias32(bias, c0 + 32 * j, O, v);
-            if constexpr (KEEP)
-              if (valid) lt_store_z32(ep.z8 + row * O, c0 + 32 * j, O, v, code);
-            lt_act32(v, ep.act);
-            store(j, v);
+      }
+      uint32_t code[2] = {0, 0};
+      if constexpr (KEEP) {                              // NT = 256: not gated, a warp's half is one block of the row
+        uint32_t amax[2] = {0, 0};
+        if constexpr (CHAIN) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int jj = GATED ? j & 1 : j, h = GATED ? j >> 1 : 0;
+            if (jj < chunks) amax[h] = lt_amax32(sum + 32 * j, c0 + 32 * jj, O, amax[h]);
           }
-      } else {
-        uint32_t code[2] = {0, 0};
-        if constexpr (KEEP) {                            // NT = 256: a block of each half per tile, shared by two warps
-          uint32_t amax[2] = {0, 0};
+        } else {
+#pragma unroll 1
           for (int j = 0; j < chunks; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < (GATED ? 2 : 1); ++h) {
               float v[32];
-              from_tmem(h * H + g * w + 32 * j, v);
+              from_tmem(g * w + 32 * j + h * H, v);
               if (bias) lt_bias32(bias + h * O, c0 + 32 * j, O, v);
               amax[h] = lt_amax32(v, c0 + 32 * j, O, amax[h]);
             }
-          // the maxima pass through the warps' staging boxes
-          lt_boxes_free<0>(lane);
+        }
+        if constexpr (GATED) {                           // a block of each half per tile, shared by two warps:
+          lt_boxes_free<0>(lane);                        // the maxima pass through the warps' staging boxes
           uint32_t* mine = reinterpret_cast<uint32_t*>(stage) + lane;
           const uint32_t* other = reinterpret_cast<const uint32_t*>(stage + (g ? -4 : 4) * kLtStaging) + lane;
           mine[0] = amax[0];
           mine[32] = amax[1];
           fence_proxy_async_smem();                      // the residual's boxes come after these words
           named_barrier_sync(2 + q, 64);
-          code[0] = e8m0_of_amax(max(amax[0], other[0]));
-          code[1] = e8m0_of_amax(max(amax[1], other[32]));
+          amax[0] = max(amax[0], other[0]);
+          amax[1] = max(amax[1], other[32]);
           named_barrier_sync(2 + q, 64);
           fetch_first();
-          if (valid && g == 0 && c0 < O)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) ep.z_scale[(h * z_blocks + (c0 >> 7)) * a.m + row] = (uint8_t)code[h];
         }
-        if (live)
+#pragma unroll
+        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+          code[h] = e8m0_of_amax(amax[h]);
+          if (valid && chunks > 0 && (!GATED || g == 0)) ep.z_scale[(h * z_blocks + (c0 >> 7)) * a.m + row] = (uint8_t)code[h];
+        }
+      }
+      if constexpr (CHAIN) {
+        if (live) {
+          if constexpr (GATED) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (j < chunks) {
+                if constexpr (KEEP)
+                  if (valid) {
+                    lt_store_z32(ep.z8 + row * O, c0 + 32 * j, O, sum + 32 * j, code[0]);
+                    lt_store_z32(ep.z8 + (a.m + row) * O, c0 + 32 * j, O, sum + 64 + 32 * j, code[1]);
+                  }
+                lt_gate32(sum + 32 * j, sum + 64 + 32 * j, ep.y_f32);
+                store(j, sum + 32 * j);
+              }
+          } else {
+#pragma unroll 1
+            for (int j = 0; j < chunks; ++j) {           // one body for the chunks: the sums move down
+              if constexpr (KEEP)
+                if (valid) lt_store_z32(ep.z8 + row * O, c0 + 32 * j, O, sum, code[0]);
+              lt_act32(sum, ep.act, ep.y_f32);
+              store(j, sum);
+#pragma unroll
+              for (int e = 0; e < 96; ++e) sum[e] = sum[e + 32];
+            }
+          }
+        }
+      } else {
+        if (live) {
+          float v[GATED ? 64 : 32];                      // gated: 32 of each half
+#pragma unroll 1
           for (int j = 0; j < chunks; ++j) {
             const int64_t c = c0 + 32 * j;
-            float v[32], t[32];
-            from_tmem(g * w + 32 * j, v);
-            from_tmem(H + g * w + 32 * j, t);
+            if constexpr (GATED) {
+              tmem_ld32(acc_at(g * w + 32 * j), v);
+              tmem_ld32(acc_at(g * w + 32 * j + H), v + 32);
+              tmem_ld_wait();
+              if (!ok) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e) v[e] = NAN;
+              }
+            } else {
+              from_tmem(g * w + 32 * j, v);
+            }
             if (bias) {
               lt_bias32(bias, c, O, v);
-              lt_bias32(bias + O, c, O, t);
+              if constexpr (GATED) lt_bias32(bias + O, c, O, v + 32);
             }
             if constexpr (KEEP)
               if (valid) {
                 lt_store_z32(ep.z8 + row * O, c, O, v, code[0]);
-                lt_store_z32(ep.z8 + (a.m + row) * O, c, O, t, code[1]);
+                if constexpr (GATED) lt_store_z32(ep.z8 + (a.m + row) * O, c, O, v + 32, code[1]);
               }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= act_value(t[i], kActSilu);
+            if constexpr (GATED) {
+              lt_gate32(v, v + 32, ep.y_f32);
+            } else {
+              lt_act32(v, ep.act, ep.y_f32);
+            }
             store(j, v);
           }
+        }
+        release();
       }
-      release();
     }
     if (lane == 0) bulk_wait_all();                      // stores complete before the CTA exits
   }
@@ -727,10 +904,10 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
   return best;
 }
 
-template <bool A_MN, bool B_MN, bool GATED, bool KEEP>
-static cudaError_t launch_t(const LinearTileMaps& maps, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+template <bool A_MN, bool B_MN, bool GATED, bool KEEP, bool CHAIN>
+static cudaError_t launch_c(const LinearTileMaps& maps, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
   static int clusters_of[64];
-  auto kern = linear_tile_kernel<A_MN, B_MN, GATED, KEEP>;
+  auto kern = linear_tile_kernel<A_MN, B_MN, GATED, KEEP, CHAIN>;
   int dev = 0;
   cudaGetDevice(&dev);
   cudaLaunchConfig_t cfg = {};
@@ -760,6 +937,14 @@ static cudaError_t launch_t(const LinearTileMaps& maps, const LinearTileArgs& a,
   cfg.stream = st;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, maps, a);
+}
+
+template <bool A_MN, bool B_MN, bool GATED, bool KEEP>
+static cudaError_t launch_t(const LinearTileMaps& maps, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+  // cut the chain where the result shows its drift and a unit is longer than one piece
+  const int unit = a.full_tiles > 0 ? a.k_blocks : (a.k_blocks + a.splits - 1) / a.splits;
+  if ((KEEP || a.ep.y_f32) && unit > a.chain) return launch_c<A_MN, B_MN, GATED, KEEP, true>(maps, a, num_sms, st);
+  return launch_c<A_MN, B_MN, GATED, KEEP, false>(maps, a, num_sms, st);
 }
 
 static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,

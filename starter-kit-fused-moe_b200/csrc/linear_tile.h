@@ -14,7 +14,9 @@ struct LinearTileArgs {
   int m_tiles, n_tiles, n_tile;
   int k_blocks;           // 64-wide K-blocks over all terms of A
   int term_blocks;        // of one term
+  int terms;
   int splits;
+  int chain;              // K-blocks per accumulator where long sums are cut (fp32 y, kept pre-activations)
   int64_t full_tiles;     // tiles done whole; the others are cut into `splits` K slices
   int64_t units;          // full_tiles + splits * (number of the others)
   int vec;                // y (and the residual) can be accessed in 16 bytes
@@ -23,8 +25,7 @@ struct LinearTileArgs {
 };
 struct LinearTileMaps {
   CUtensorMap a, b;       // operands
-  CUtensorMap out, res;   // y and the residual in 32 x 32 boxes (vec)
-  CUtensorMap partial;    // the K slices' tiles in 32 x 32 boxes (splits > 1)
+  CUtensorMap out, res;   // bf16 y and its residual in 32 x 32 boxes (vec)
 };
 struct LinearTilePlan {
   int n_tile, splits;

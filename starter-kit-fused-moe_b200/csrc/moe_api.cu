@@ -96,19 +96,16 @@ void moe::set_last_error(const char* msg) { g_last_error = msg; }
 
 int moe::current_device_sms() { return num_sms_of_current_device(); }
 
-bool moe::encode_matrix(CUtensorMap* m, bool f32, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride,
-                        uint64_t planes, uint64_t plane_stride, uint32_t box_cols, uint32_t box_rows) {
+bool moe::encode_bf16(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride,
+                      uint64_t planes, uint64_t plane_stride, uint32_t box_cols, uint32_t box_rows) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return false;
-  const int rank = planes ? 3 : 2;
-  const uint64_t size = f32 ? 4 : 2;
   cuuint64_t dims[3] = {cols, rows, planes};
-  cuuint64_t strides[2] = {size * row_stride, size * plane_stride};
+  cuuint64_t strides[2] = {2 * row_stride, 2 * plane_stride};
   cuuint32_t box[3] = {box_cols, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  return fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base),
-            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            size * box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -82,11 +82,11 @@ cudaError_t set_debug_waits_ep(unsigned long long limit_ns, int gate_extra);
 cudaError_t set_debug_waits_linear(unsigned long long limit_ns, int gate_extra);
 // SMs of the current device (0 without one).
 int current_device_sms();
-// Tensor map of a bf16 / fp32 matrix [planes][rows][cols] (rank 2 when planes is
-// 0; strides in elements, multiples of 16 bytes), in boxes of box_rows by
-// box_cols whose rows are 128 or 64 bytes, in the swizzle of that width.
-bool encode_matrix(CUtensorMap* m, bool f32, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride,
-                   uint64_t planes, uint64_t plane_stride, uint32_t box_cols, uint32_t box_rows);
+// Tensor map of a bf16 matrix [planes][rows][cols] (rank 2 when planes is 0;
+// strides in elements, multiples of 8), in boxes of box_rows by box_cols, 64 or 32
+// columns wide, in the swizzle of that width (128 or 64 bytes).
+bool encode_bf16(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride, uint64_t planes,
+                 uint64_t plane_stride, uint32_t box_cols, uint32_t box_rows);
 // Text returned by moe_fp8_last_error() on the calling thread.
 void set_last_error(const char* msg);
 cudaError_t set_trace(int on);

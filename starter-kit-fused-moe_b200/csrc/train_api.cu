@@ -76,8 +76,10 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.m_tiles = moe::ceil_div(m, 256);
   t.n_tiles = moe::ceil_div(out_cols, cols);
   t.term_blocks = (int)p.term_blocks;
+  t.terms = p.terms;
   t.k_blocks = t.term_blocks * p.terms;
   t.splits = p.plan.splits;
+  t.chain = ep.y_f32 ? 12 : 24;
   t.full_tiles = p.plan.full;
   t.units = p.plan.full + p.plan.tail * t.splits;
   t.ep = ep;
@@ -87,17 +89,14 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.partial = reinterpret_cast<float*>(partial);
   moe::LinearTileMaps maps{};
   const uint32_t half = (uint32_t)t.n_tile / 2;
-  bool ok = (a_mn ? moe::encode_matrix(&maps.a, false, A, m, k, lda, p.terms, term_stride, 64, 64)
-                  : moe::encode_matrix(&maps.a, false, A, k, m, lda, p.terms, term_stride, 64, 128)) &&
-            (b_mn ? moe::encode_matrix(&maps.b, false, B, out_cols, k, ldb, 0, 0, 64, 64)
-                  : moe::encode_matrix(&maps.b, false, B, k, b_rows, ldb, 0, 0, 64, half));
-  if (t.vec && t.full_tiles > 0) {
-    ok = ok && moe::encode_matrix(&maps.out, ep.y_f32, ep.y, out_cols, m, ep.ldy, 0, 0, 32, 32);
-    if (ep.residual) ok = ok && moe::encode_matrix(&maps.res, false, ep.residual, out_cols, m, ep.ldr, 0, 0, 32, 32);
+  bool ok = (a_mn ? moe::encode_bf16(&maps.a, A, m, k, lda, p.terms, term_stride, 64, 64)
+                  : moe::encode_bf16(&maps.a, A, k, m, lda, p.terms, term_stride, 64, 128)) &&
+            (b_mn ? moe::encode_bf16(&maps.b, B, out_cols, k, ldb, 0, 0, 64, 64)
+                  : moe::encode_bf16(&maps.b, B, k, b_rows, ldb, 0, 0, 64, half));
+  if (t.vec && !ep.y_f32 && t.full_tiles > 0) {
+    ok = ok && moe::encode_bf16(&maps.out, ep.y, out_cols, m, ep.ldy, 0, 0, 32, 32);
+    if (ep.residual) ok = ok && moe::encode_bf16(&maps.res, ep.residual, out_cols, m, ep.ldr, 0, 0, 32, 32);
   }
-  if (t.splits > 1)
-    ok = ok && moe::encode_matrix(&maps.partial, true, partial, t.n_tile, (uint64_t)p.plan.tail * t.splits * 256,
-                                  t.n_tile, 0, 0, 32, 32);
   if (!ok) {
     moe::set_last_error("cuTensorMapEncodeTiled failed");
     return MOE_ERR_CUDA;
@@ -142,7 +141,7 @@ GradPlan grad_plan(const MoeLinearGradArgs& a) {
   GradPlan p{};
   p.ldz = up8(a.n);
   p.ldk = up8(a.k);
-  p.terms = a.grad_f32 && (a.activation != MOE_ACT_NONE || a.grad_y_f32) ? 2 : 1;
+  p.terms = a.grad_f32 && (a.activation != MOE_ACT_NONE || a.grad_y_f32) ? 3 : 1;
   // without an activation bf16 gradients are dz themselves
   p.direct = a.activation == MOE_ACT_NONE && !a.grad_y_f32 && tma_ready(a.grad_y, a.ldg) && a.ldg >= a.n;
   p.need_dz = (a.grad_x || a.grad_weight) && !p.direct;

@@ -41,7 +41,7 @@ cudaError_t launch_linear_small(const void* x, int64_t ldx, const void* w, int64
                                 const LinearEpilogue& ep, cudaStream_t st);
 
 // Gradient of the pre-activation: dz = dy * act'(z), written as bf16 [terms][m][ldz]
-// (terms = 2: the rounding's remainder follows), and per-chunk column sums.
+// (terms = 3: the roundings' remainders follow), and per-chunk column sums.
 struct ActGradArgs {
   const void* dy;          // bf16 / f32 [m, O], row stride ldg
   const uint8_t* z8;       // as LinearEpilogue; NULL when act is none

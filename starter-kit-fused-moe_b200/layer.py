@@ -150,7 +150,7 @@ def linear_backward(grad_output, checkpoint, weight, need_x=True, need_weight=Tr
     over the tokens, with x^ and z^ the checkpoint's values; a gradient that is
     not asked for is None. (The residual's gradient is grad_output.)
     grad_output is bf16 or f32 [M, O]. With grad_dtype bf16, dz is rounded to
-    bf16 for the products; with f32 it enters them as the sum of two bf16 terms.
+    bf16 for the products; with f32 it enters them as the sum of three bf16 terms.
     Repeated calls give the same bits.
     """
     c = checkpoint
