@@ -20,7 +20,7 @@
 // chain drifts: 8e-6 of the result's norm at K = 7168, 2e-6 at 2048, 5e-7 at
 // 512, where an fp32 product has 9e-7. A bf16 result (2^-8) does not show that,
 // an fp32 one does, and so does a kept pre-activation (one value in 10^4 moves to
-// the next e4m3 step). For those (CHAIN) the chain is cut every 12 (fp32) or 24
+// the next e4m3 step). For those (CHAIN) the chain is cut every 16 (fp32) or 24
 // (kept) K-blocks of 64: the epilogue warps add each partial accumulator to fp32
 // registers, rounding to nearest, while the tensor core fills the other one. The
 // reads of TMEM cost the tensor core about a K-block each, 10 % and 4 %.
@@ -133,6 +133,20 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
         "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
         "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
       : "r"(taddr));
+}
+
+// The producer's and the issuer's loops run with their whole warp converged and
+// elect one lane around the instructions themselves: the operands then stay in
+// uniform registers. Under a lane == 0 branch every tcgen05.mma cost 62 cycles of
+// issue and the loop 545 a stage, as long as the MMAs themselves at NT = 256.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 
 struct LtUnit {
@@ -379,80 +393,98 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     if constexpr (CHAIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLtRegsIssue));
     if (warp == 0) {
       // ------------------------------------------------------------ TMA producer
-      if (lane == 0) {
-        int it = 0;
-        bool ok = true;
-        const uint32_t bytes = 2 * (kLtTileA + H * 128);
-        for (int64_t u = wid; u < a.units && ok && !*abort_flag; u += G) {
-          const LtUnit x = lt_unit(a, u);
-          const int m0 = x.mt * 256 + crank * 128;
-          // B rows of this CTA's half: the next H columns of the tile, or for a gated tile its first-half
-          // (leader) and second-half (peer) rows
-          const int n0 = GATED ? crank * a.gate_rows + x.nt * H : x.nt * NT + crank * H;
-          for (int kb = x.kb0; kb < x.kb1; ++kb, ++it) {
-            const int s = it % kLtStages;
-            if (!mbar_wait(smem_u32(&S.empty[s]), ((it / kLtStages) & 1) ^ 1)) {
-              *abort_flag = 1;
-              ok = false;
-              break;
-            }
-            const uint32_t fb = smem_u32(&S.full[s]);
-            const uint32_t fbl = mapa_shared(fb, 0);
-            const uint32_t sa = smem_u32(smem + s * kLtStageBytes), sb = sa + kLtTileA;
-            // the small terms first: the chain's truncation is relative to the running sum
-            const int part = kb / a.term_blocks, kt = (kb - part * a.term_blocks) * 64, term = a.terms - 1 - part;
-            if (crank == 0) mbar_arrive_expect_tx(fb, bytes);
+      int s = 0;
+      uint32_t parity = 1;
+      bool ok = true;
+      const uint32_t bytes = 2 * (kLtTileA + H * 128);
+      const uint32_t full0 = smem_u32(&S.full[0]), empty0 = smem_u32(&S.empty[0]), stage0 = smem_u32(smem);
+      const uint32_t leader0 = mapa_shared(full0, 0);      // both CTAs' loads complete on the leader's barriers
+      const int k_end = a.term_blocks * 64;
+      for (int64_t u = wid; u < a.units && ok && !__shfl_sync(0xffffffffu, *abort_flag, 0); u += G) {
+        const LtUnit x = lt_unit(a, u);
+        const int m0 = x.mt * 256 + crank * 128;
+        // B rows of this CTA's half: the next H columns of the tile, or for a gated tile its first-half
+        // (leader) and second-half (peer) rows
+        const int n0 = GATED ? crank * a.gate_rows + x.nt * H : x.nt * NT + crank * H;
+        // the small terms first: the chain's truncation is relative to the running sum
+        int term = a.terms - 1 - x.kb0 / a.term_blocks;
+        int kt = (x.kb0 % a.term_blocks) * 64;
+        for (int kb = x.kb0; kb < x.kb1; ++kb) {
+          if (!warp_wait(empty0 + 8 * s, parity)) {
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          const uint32_t sa = stage0 + s * kLtStageBytes, sb = sa + kLtTileA, bar = leader0 + 8 * s;
+          if (elect_one()) {
+            if (crank == 0) mbar_arrive_expect_tx(full0 + 8 * s, bytes);
             if constexpr (A_MN) {
-              tma_load_3d_pair(sa, &maps.a, fbl, m0, kt, term);
-              tma_load_3d_pair(sa + 8192, &maps.a, fbl, m0 + 64, kt, term);
+              tma_load_3d_pair(sa, &maps.a, bar, m0, kt, term);
+              tma_load_3d_pair(sa + 8192, &maps.a, bar, m0 + 64, kt, term);
             } else {
-              tma_load_3d_pair(sa, &maps.a, fbl, kt, m0, term);
+              tma_load_3d_pair(sa, &maps.a, bar, kt, m0, term);
             }
             if constexpr (B_MN) {
-              tma_load_2d_pair(sb, &maps.b, fbl, n0, kt);
-              if (H == 128) tma_load_2d_pair(sb + 8192, &maps.b, fbl, n0 + 64, kt);
+              tma_load_2d_pair(sb, &maps.b, bar, n0, kt);
+              if (H == 128) tma_load_2d_pair(sb + 8192, &maps.b, bar, n0 + 64, kt);
             } else {
-              tma_load_2d_pair(sb, &maps.b, fbl, kt, n0);
+              tma_load_2d_pair(sb, &maps.b, bar, kt, n0);
             }
+          }
+          kt += 64;
+          if (kt == k_end) {
+            kt = 0;
+            --term;
+          }
+          if (++s == kLtStages) {
+            s = 0;
+            parity ^= 1;
           }
         }
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 && crank == 0) {
       // ------------------------------------------------------------ MMA issuer (leader)
-      if (lane == 0 && crank == 0) {
-        const uint32_t idesc = idesc_bf16(NT, A_MN, B_MN);
-        int it = 0, tt = 0;                                // stages, accumulators
-        bool ok = true;
-        for (int64_t u = wid; u < a.units && ok && !*abort_flag; u += G) {
-          const LtUnit x = lt_unit(a, u);
-          for (int kb = x.kb0; kb < x.kb1 && ok; ++tt) {
-            const int b = tt & 1, end = CHAIN ? min(kb + a.chain, x.kb1) : x.kb1;
-            if (!mbar_wait(smem_u32(&S.tempty[b]), ((tt >> 1) & 1) ^ 1)) {
+      const uint32_t idesc = idesc_bf16(NT, A_MN, B_MN);
+      int s = 0, tt = 0;                                   // stage, accumulator
+      uint32_t parity = 0;
+      bool ok = true;
+      const uint32_t full0 = smem_u32(&S.full[0]), empty0 = smem_u32(&S.empty[0]);
+      // descriptors of stage 0; an address step of n bytes is n / 16 in their low word
+      const uint64_t a0 = A_MN ? sdesc_sw128_mn(smem_u32(smem)) : sdesc_sw128(smem_u32(smem));
+      const uint64_t b0 = B_MN ? sdesc_sw128_mn(smem_u32(smem) + kLtTileA) : sdesc_sw128(smem_u32(smem) + kLtTileA);
+      for (int64_t u = wid; u < a.units && ok && !__shfl_sync(0xffffffffu, *abort_flag, 0); u += G) {
+        const LtUnit x = lt_unit(a, u);
+        for (int kb = x.kb0; kb < x.kb1 && ok; ++tt) {
+          const int b = tt & 1, end = CHAIN ? min(kb + a.chain, x.kb1) : x.kb1;
+          if (!warp_wait(smem_u32(&S.tempty[b]), ((tt >> 1) & 1) ^ 1)) {
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem_base + (uint32_t)(b * 256);
+          uint32_t more = 0;
+          for (; kb < end; ++kb, more = 1) {
+            if (!warp_wait(full0 + 8 * s, parity)) {
               *abort_flag = 1;
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint32_t d = tmem_base + (uint32_t)(b * 256);
-            for (bool more = false; kb < end; ++kb, ++it, more = true) {
-              const int s = it % kLtStages;
-              if (!mbar_wait(smem_u32(&S.full[s]), (it / kLtStages) & 1)) {
-                *abort_flag = 1;
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              const uint32_t sa = smem_u32(smem + s * kLtStageBytes), sb = sa + kLtTileA;
+            const uint64_t da = a0 + (uint32_t)(s * (kLtStageBytes / 16)), db = b0 + (uint32_t)(s * (kLtStageBytes / 16));
+            if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) {
-                const uint64_t da = A_MN ? sdesc_sw128_mn(sa + kk * 2048) : sdesc_sw128(sa + kk * 32);
-                const uint64_t db = B_MN ? sdesc_sw128_mn(sb + kk * 2048) : sdesc_sw128(sb + kk * 32);
-                mma_bf16_pair(d, da, db, idesc, (more || kk) ? 1u : 0u);
-              }
-              mma_commit_pair(smem_u32(&S.empty[s]));
+              for (int kk = 0; kk < 4; ++kk)
+                mma_bf16_pair(d, da + kk * (A_MN ? 128 : 2), db + kk * (B_MN ? 128 : 2), idesc, kk ? 1u : more);
+              mma_commit_pair(empty0 + 8 * s);
             }
-            if (ok) mma_commit_pair(smem_u32(&S.tfull[b]));
+            if (++s == kLtStages) {
+              s = 0;
+              parity ^= 1;
+            }
           }
+          if (ok && elect_one()) mma_commit_pair(smem_u32(&S.tfull[b]));
+          __syncwarp();
         }
       }
     }
@@ -873,28 +905,32 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
 }
 
 // Tile width and K slices of the last, partial round. Cycles per 64 of K and
-// pair with all pairs at work, measured: 340 + 1.45 NT, at least 600 (711 at NT =
-// 256, 618 at 192; a pair alone takes 545 at any width). A tile's epilogue hides
-// behind the next tile's products except for the last one. Slices are at least 4
-// K-blocks deep; joining them costs a launch and moves 8 bytes per value and
-// slice through L2 (about 3 KB per cycle).
+// pair, measured: 2.1 NT for a pair alone (the MMA), 174 + 2.3 NT with all pairs
+// at work (758 at NT = 256, 590 at 192, 466 at 128), and no less than the
+// operands' way from HBM (3.4 KB per cycle). A tile's epilogue hides behind the
+// next tile's products except for the last one. Slices are at least 4 K-blocks
+// deep; joining them costs a launch and moves 8 bytes per value and slice
+// through L2 (about 3 KB per cycle).
 LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs) {
   LinearTilePlan best{};
   double best_cost = 1e300;
   const int64_t mt = (m + 255) / 256;
+  const double hbm = 128.0 * k_blocks * (m + (gated ? 2 : 1) * n) / 3400;
   static const int widths[] = {256, 192, 128, 64};
   for (int nt : widths) {
     if (keep && nt != 256) continue;
     if ((gated || b_mn) && nt % 128) continue;       // epilogue warps take 32 columns; boxes of 64
     const int64_t cols = gated ? nt / 2 : nt;
     const int64_t tiles = mt * ((n + cols - 1) / cols), tail = tiles % pairs, full = tiles - tail;
-    const double block = 340 + 1.45 * nt > 600 ? 340 + 1.45 * nt : 600;
+    const double alone = 2.1 * nt, crowded = 174 + 2.3 * nt;
     const double rows = m < 256 ? m : 256;
     for (int s = 1; s <= 16; ++s) {
       if (s > 1 && (tail == 0 || k_blocks < 4 * s)) break;
-      const int64_t rounds = (tail * s + pairs - 1) / pairs;
-      const double cost = (double)(full / pairs) * k_blocks * block + (double)rounds * ((k_blocks + s - 1) / s) * block +
-                          1500 + 25.0 * nt + (s > 1 ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
+      const int64_t units = tail * s, rounds = (units + pairs - 1) / pairs;
+      const double busy = units < pairs ? (double)units / pairs : 1.0;
+      double cost = (double)(full / pairs) * k_blocks * crowded +
+                    (double)rounds * ((k_blocks + s - 1) / s) * (alone + busy * (crowded - alone));
+      cost = (cost > hbm ? cost : hbm) + 1500 + 25.0 * nt + (s > 1 ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
       if (cost < best_cost) {
         best_cost = cost;
         best = {nt, s, s > 1 ? full : tiles, s > 1 ? tail : 0};

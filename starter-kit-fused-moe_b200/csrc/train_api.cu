@@ -79,7 +79,7 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.terms = p.terms;
   t.k_blocks = t.term_blocks * p.terms;
   t.splits = p.plan.splits;
-  t.chain = ep.y_f32 ? 12 : 24;
+  t.chain = ep.y_f32 ? 16 : 24;
   t.full_tiles = p.plan.full;
   t.units = p.plan.full + p.plan.tail * t.splits;
   t.ep = ep;
