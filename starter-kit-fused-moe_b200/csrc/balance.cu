@@ -84,10 +84,27 @@ __device__ __forceinline__ int seq_of(const int32_t* cu, int s, int x, int lane)
   return lo;
 }
 
-template <int ITEMS>
+// The experts of a lane: lane + 32 j, or (VEC: E = 32 ITEMS, a multiple of 128,
+// 16-byte aligned rows) groups of four, 128 apart.
+template <bool VEC>
+__device__ __forceinline__ int expert_of(int lane, int j) {
+  return VEC ? 4 * lane + (j & 3) + 128 * (j >> 2) : lane + 32 * j;
+}
+template <int ITEMS, bool VEC>
 __device__ __forceinline__ void load_logits(const float* row, int e, int lane, float* x) {
+  if constexpr (VEC) {
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) x[j] = lane + 32 * j < e ? __ldg(row + lane + 32 * j) : -INFINITY;
+    for (int j = 0; j < ITEMS; j += 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(row + 32 * j) + lane);
+      x[j] = v.x;
+      x[j + 1] = v.y;
+      x[j + 2] = v.z;
+      x[j + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) x[j] = lane + 32 * j < e ? __ldg(row + lane + 32 * j) : -INFINITY;
+  }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -101,14 +118,16 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Unnormalised scores of a token (experts past E: 0) and the inverse of their sum.
+// Unnormalised scores of a token (experts past E: 0) and the inverse of their
+// sum. The hardware exponential and reciprocal are good to 2^-21 of a score at
+// |logit| = 8, and the kernels are bound by their instructions with the exact ones.
 template <int ITEMS>
 __device__ __forceinline__ float scores(const float* x, int scoring, float* s) {
   float sum = 0.f;
   if (scoring == 0) {
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
-      s[j] = __fdividef(1.0f, 1.0f + expf(-x[j]));
+      s[j] = sigmoid_fast(x[j]);
       sum += s[j];
     }
     return 1.0f / (warp_sum(sum) + kScoreEps);
@@ -129,14 +148,14 @@ __device__ __forceinline__ float scores(const float* x, int scoring, float* s) {
   }
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j) {
-    s[j] = expf(x[j] - m);
+    s[j] = __expf(x[j] - m);
     sum += s[j];
   }
   return 1.0f / warp_sum(sum);
 }
 
-template <int ITEMS>
-__global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(BalanceArgs a, BalanceWs w, int chunk) {
+template <int ITEMS, bool VEC>
+__global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_partial_kernel(BalanceArgs a, BalanceWs w, int chunk) {
   __shared__ float psum[kBalWarps][32 * ITEMS > 256 ? 256 : 32 * ITEMS];
   __shared__ int hist[32 * ITEMS];
   __shared__ int tok;
@@ -161,7 +180,7 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(Balance
     float next[ITEMS];                                       // the next token's logits are on their way
     int id_next = -1;
     if (s0 + warp < s1) {
-      load_logits<ITEMS>(a.logits + (int64_t)(s0 + warp) * a.e, a.e, lane, next);
+      load_logits<ITEMS, VEC>(a.logits + (int64_t)(s0 + warp) * a.e, a.e, lane, next);
       if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(s0 + warp) * a.k + lane);
     }
     for (int t = s0 + warp; t < s1; t += kBalWarps) {
@@ -170,7 +189,7 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(Balance
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j) x[j] = next[j];
       if (t + kBalWarps < s1) {
-        load_logits<ITEMS>(a.logits + (int64_t)(t + kBalWarps) * a.e, a.e, lane, next);
+        load_logits<ITEMS, VEC>(a.logits + (int64_t)(t + kBalWarps) * a.e, a.e, lane, next);
         if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(t + kBalWarps) * a.k + lane);
       }
       const bool hit = id >= 0 && id < a.e;
@@ -188,7 +207,7 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(Balance
     for (int j0 = 0; j0 < ITEMS; j0 += 8) {
       __syncthreads();
 #pragma unroll
-      for (int j = j0; j < j0 + 8 && j < ITEMS; ++j) psum[warp][lane + 32 * (j - j0)] = acc[j];
+      for (int j = j0; j < j0 + 8 && j < ITEMS; ++j) psum[warp][expert_of<VEC>(lane, j - j0)] = acc[j];
       __syncthreads();
       const int i = threadIdx.x, e = 32 * j0 + i;
       if (i < 32 * ITEMS && e < a.e) {
@@ -207,8 +226,7 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_partial_kernel(Balance
 __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, BalanceWs w, int chunk) {
   __shared__ double rp[8][32];
   __shared__ int rc[8][32];
-  __shared__ int rt[256];
-  __shared__ double rl[256];
+  __shared__ int rt[8];
   __shared__ int last;
   pdl_wait();
   pdl_trigger();
@@ -239,19 +257,17 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
   }
   rp[ty][tx] = p;
   rc[ty][tx] = c;
-  rt[threadIdx.x] = n;
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (tx == 0) rt[ty] = n;
   __syncthreads();
-  for (int d = 128; d >= 1; d >>= 1) {
-    if (threadIdx.x < d) rt[threadIdx.x] += rt[threadIdx.x + d];
-    __syncthreads();
-  }
-  const int tq = rt[0];
-  double term = 0.0;
   if (ty == 0) {
+    int tq = 0;
+    for (int i = 0; i < 8; ++i) tq += rt[i];
     for (int i = 1; i < 8; ++i) {
       p += rp[i][tx];
       c += rc[i][tx];
     }
+    double term = 0.0;
     if (e < a.e) {
       const double mean = tq > 0 ? p / tq : 0.0;
       a.mean_scores[(int64_t)q * a.e + e] = bad ? NAN : (float)mean;
@@ -270,24 +286,26 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
   __syncthreads();
   if (!last) return;
   __threadfence();
-  double l = 0.0;
+  double l = 0.0;                                            // fixed order: strided sums, then two trees
   int live = 0;
   const int64_t parts = (int64_t)a.s * groups;
   for (int64_t i = threadIdx.x; i < parts; i += 256) l += __ldcg(w.loss + i);
   for (int i = threadIdx.x; i < a.s; i += 256) live += __ldcg(a.tokens + i) > 0;
-  rl[threadIdx.x] = l;
-  rt[threadIdx.x] = live;
-  __syncthreads();
-  for (int d = 128; d >= 1; d >>= 1) {
-    if (threadIdx.x < d) {
-      rl[threadIdx.x] += rl[threadIdx.x + d];
-      rt[threadIdx.x] += rt[threadIdx.x + d];
-    }
-    __syncthreads();
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  live = __reduce_add_sync(0xffffffffu, live);
+  if (tx == 0) {
+    rp[0][ty] = l;
+    rt[ty] = live;
   }
+  __syncthreads();
   if (threadIdx.x == 0) {
-    *a.loss = (float)(rt[0] > 0 ? (double)a.alpha * rl[0] / rt[0] : rl[0]);   // rl is 0 (or NaN) without sequences
-    *a.live = rt[0];
+    for (int i = 1; i < 8; ++i) {
+      l += rp[0][i];
+      live += rt[i];
+    }
+    *a.loss = (float)(live > 0 ? (double)a.alpha * l / live : l);   // l is 0 (or NaN) without sequences
+    *a.live = live;
   }
 }
 
@@ -306,9 +324,9 @@ __global__ void balance_empty_kernel(BalanceArgs a) {
 
 // A block takes `chunk` consecutive tokens, a warp every eighth of them; the
 // coefficients c_e of the sequence at hand are in the warp's registers.
-template <int ITEMS>
-__global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGradArgs a, int chunk) {
-  __shared__ float scatter[kBalWarps][32 * ITEMS];           // a warp's row of combine-weight gradients, else zero
+template <int ITEMS, bool VEC>
+__global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_grad_kernel(BalanceGradArgs a, int chunk) {
+  __shared__ alignas(16) float scatter[kBalWarps][32 * ITEMS];           // a warp's row of combine-weight gradients, else zero
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j) scatter[warp][lane + 32 * j] = 0.f;
@@ -321,6 +339,12 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGra
   const int live = with_loss ? __ldg(a.live) : 0;
   for (int pos = blockIdx.x * chunk; pos < b1;) {
     int end = b1;
+    float next[ITEMS];                                       // the next token's logits are on their way
+    int id_next = -1;
+    if (pos + warp < b1) {
+      load_logits<ITEMS, VEC>(a.logits + (int64_t)(pos + warp) * a.e, a.e, lane, next);
+      if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(pos + warp) * a.k + lane);
+    }
     float coef[ITEMS];
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) coef[j] = 0.f;
@@ -336,14 +360,8 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGra
         const double f = tq > 0 && live > 0 ? (double)g * a.alpha * a.e / ((double)a.k * live * tq * tq) : 0.0;
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j)
-          if (lane + 32 * j < a.e) coef[j] = (float)(f * __ldg(a.counts + (int64_t)q * a.e + lane + 32 * j));
+          if (VEC || lane + 32 * j < a.e) coef[j] = (float)(f * __ldg(a.counts + (int64_t)q * a.e + expert_of<VEC>(lane, j)));
       }                                                      // else: behind the last sequence
-    }
-    float next[ITEMS];                                       // the next token's logits are on their way
-    int id_next = -1;
-    if (pos + warp < end) {
-      load_logits<ITEMS>(a.logits + (int64_t)(pos + warp) * a.e, a.e, lane, next);
-      if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(pos + warp) * a.k + lane);
     }
     for (int t = pos + warp; t < end; t += kBalWarps) {
       const int id = id_next;
@@ -351,7 +369,7 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGra
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j) x[j] = next[j];
       if (t + kBalWarps < end) {
-        load_logits<ITEMS>(a.logits + (int64_t)(t + kBalWarps) * a.e, a.e, lane, next);
+        load_logits<ITEMS, VEC>(a.logits + (int64_t)(t + kBalWarps) * a.e, a.e, lane, next);
         if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(t + kBalWarps) * a.k + lane);
       }
       const bool hit = id >= 0 && id < a.e;
@@ -365,7 +383,7 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGra
           float sum = 0.f;
 #pragma unroll
           for (int j = 0; j < ITEMS; ++j) {
-            const float e = expf(-fabsf(x[j])), r = __fdividef(1.0f, 1.0f + e);
+            const float e = __expf(-fabsf(x[j])), r = __fdividef(1.0f, 1.0f + e);
             s[j] = x[j] >= 0.f ? r : e * r;                  // NaN: e is NaN
             slope[j] = e * r * r;
             sum += s[j];
@@ -385,7 +403,7 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGra
       }
       if (token && a.grad_weights != nullptr) {
         const float xs = hit ? __ldg(a.logits + (int64_t)t * a.e + id) : 0.f;
-        const float e = expf(-fabsf(xs)), r = __frcp_rn(1.0f + e);
+        const float e = __expf(-fabsf(xs)), r = __fdividef(1.0f, 1.0f + e);
         const float top = hit ? (xs >= 0.f ? r : e * r) : 0.f;
         const float dw = hit ? __ldg(a.grad_weights + (int64_t)t * a.k + lane) * a.route_scale : 0.f;
         const float total = warp_sum(top) + kScoreEps;
@@ -405,13 +423,20 @@ __global__ void __launch_bounds__(kBalWarps * 32) balance_grad_kernel(BalanceGra
         if (first) scatter[warp][id] = sum;
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < ITEMS; ++j) dx[j] += scatter[warp][lane + 32 * j];
+        for (int j = 0; j < ITEMS; ++j) dx[j] += scatter[warp][expert_of<VEC>(lane, j)];
         __syncwarp();
         if (first) scatter[warp][id] = 0.f;
       }
+      float* out = a.grad_logits + (int64_t)t * a.e;
+      if constexpr (VEC) {
 #pragma unroll
-      for (int j = 0; j < ITEMS; ++j)
-        if (lane + 32 * j < a.e) a.grad_logits[(int64_t)t * a.e + lane + 32 * j] = dx[j];
+        for (int j = 0; j < ITEMS; j += 4)
+          reinterpret_cast<float4*>(out + 32 * j)[lane] = make_float4(dx[j], dx[j + 1], dx[j + 2], dx[j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j)
+          if (lane + 32 * j < a.e) out[lane + 32 * j] = dx[j];
+      }
     }
     pos = end;
   }
@@ -425,14 +450,16 @@ cudaError_t launch_balance(const BalanceArgs& a, cudaStream_t st) {
   BalanceWs w;
   balance_ws(a.t, a.e, a.s, static_cast<uint8_t*>(a.workspace), &w);
   const int chunk = balance_chunk(a.t), grid = ceil_div(a.t, chunk);
+  const bool vec = a.e % 128 == 0 && (a.e & (a.e - 1)) == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
+  const dim3 block(kBalWarps * 32);
   cudaError_t e;
-#define MOE_BAL(I) e = launch_kernel(balance_partial_kernel<I>, dim3(grid), dim3(kBalWarps * 32), 0, st, true, a, w, chunk)
-  if (a.e <= 32) MOE_BAL(1);
-  else if (a.e <= 64) MOE_BAL(2);
-  else if (a.e <= 128) MOE_BAL(4);
-  else if (a.e <= 256) MOE_BAL(8);
-  else if (a.e <= 512) MOE_BAL(16);
-  else MOE_BAL(32);
+#define MOE_BAL(I, V) e = launch_kernel(balance_partial_kernel<I, V>, dim3(grid), block, 0, st, true, a, w, chunk)
+  if (a.e <= 32) MOE_BAL(1, false);
+  else if (a.e <= 64) MOE_BAL(2, false);
+  else if (a.e <= 128) { if (vec) MOE_BAL(4, true); else MOE_BAL(4, false); }
+  else if (a.e <= 256) { if (vec) MOE_BAL(8, true); else MOE_BAL(8, false); }
+  else if (a.e <= 512) { if (vec) MOE_BAL(16, true); else MOE_BAL(16, false); }
+  else { if (vec) MOE_BAL(32, true); else MOE_BAL(32, false); }
 #undef MOE_BAL
   if (e != cudaSuccess) return e;
   return launch_kernel(balance_reduce_kernel, dim3((unsigned)ceil_div(a.e, 32), (unsigned)a.s), dim3(256), 0, st, true, a,
@@ -444,13 +471,17 @@ cudaError_t launch_balance_grad(const BalanceGradArgs& a, cudaStream_t st) {
   int chunk = align_up(ceil_div(a.t, 4 * 148), kBalWarps);     // about four blocks per SM
   if (chunk < kBalWarps) chunk = kBalWarps;
   const int grid = ceil_div(a.t, chunk);
-#define MOE_BALG(I) return launch_kernel(balance_grad_kernel<I>, dim3(grid), dim3(kBalWarps * 32), 0, st, true, a, chunk)
-  if (a.e <= 32) MOE_BALG(1);
-  else if (a.e <= 64) MOE_BALG(2);
-  else if (a.e <= 128) MOE_BALG(4);
-  else if (a.e <= 256) MOE_BALG(8);
-  else if (a.e <= 512) MOE_BALG(16);
-  else MOE_BALG(32);
+  const bool vec = a.e % 128 == 0 && (a.e & (a.e - 1)) == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(a.grad_logits) % 16 == 0;
+  const dim3 block(kBalWarps * 32);
+#define MOE_BALG(I, V) return launch_kernel(balance_grad_kernel<I, V>, dim3(grid), block, 0, st, true, a, chunk)
+  if (a.e <= 32) MOE_BALG(1, false);
+  if (a.e <= 64) MOE_BALG(2, false);
+  if (a.e <= 128) { if (vec) MOE_BALG(4, true); MOE_BALG(4, false); }
+  if (a.e <= 256) { if (vec) MOE_BALG(8, true); MOE_BALG(8, false); }
+  if (a.e <= 512) { if (vec) MOE_BALG(16, true); MOE_BALG(16, false); }
+  if (vec) MOE_BALG(32, true);
+  MOE_BALG(32, false);
 #undef MOE_BALG
 }
 

@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
 // Tile width and K slices of the last, partial round. Cycles per 64 of K and
 // pair, measured: 2.1 NT for a pair alone (the MMA), 174 + 2.3 NT with all pairs
 // at work (758 at NT = 256, 590 at 192, 466 at 128), and no less than the
-// operands' way from HBM (3.4 KB per cycle). A tile's epilogue hides behind the
+// operands' way from HBM (3.4 KB per cycle); 800 for a change of tile. A tile's epilogue hides behind the
 // next tile's products except for the last one. Slices are at least 4 K-blocks
 // deep; joining them costs a launch and moves 8 bytes per value and slice
 // through L2 (about 3 KB per cycle).
@@ -928,9 +928,9 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
       if (s > 1 && (tail == 0 || k_blocks < 4 * s)) break;
       const int64_t units = tail * s, rounds = (units + pairs - 1) / pairs;
       const double busy = units < pairs ? (double)units / pairs : 1.0;
-      double cost = (double)(full / pairs) * k_blocks * crowded +
-                    (double)rounds * ((k_blocks + s - 1) / s) * (alone + busy * (crowded - alone));
-      cost = (cost > hbm ? cost : hbm) + 1500 + 25.0 * nt + (s > 1 ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
+      double cost = (double)(full / pairs) * (k_blocks * crowded + 800) +
+                    (double)rounds * ((k_blocks + s - 1) / s * (alone + busy * (crowded - alone)) + 800);
+      cost = (cost > hbm ? cost : hbm) + 1500 + 12.0 * nt + (s > 1 ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
       if (cost < best_cost) {
         best_cost = cost;
         best = {nt, s, s > 1 ? full : tiles, s > 1 ? tail : 0};
