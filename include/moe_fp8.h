@@ -299,6 +299,8 @@ typedef struct MoeLinearArgs {
   int32_t activation;
   int32_t y_f32;
 } MoeLinearArgs;
+/* Workspace of a call with these arguments; all but the workspace itself must be
+ * filled in (it depends on sizes, strides and the pointers' alignment). */
 size_t moe_linear_workspace_bytes(const MoeLinearArgs* args);
 int moe_linear_run(const MoeLinearArgs* args, void* stream);
 

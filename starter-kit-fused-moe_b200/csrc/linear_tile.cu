@@ -35,7 +35,10 @@
 // partial tiles in the workspace and a second kernel, launched to start as this
 // one ends, adds them in slice order and runs the epilogue on all SMs. (Letting
 // the slice that arrives last do it kept the other SMs idle: 36 instead of 20 us
-// at 1037 x 1111 x 515.)
+// at 1037 x 1111 x 515.) Outputs whose rows 16-byte accesses cannot reach take
+// that way for every tile: the second kernel reaches any column with whole
+// warps, while a lane holding a row of the tile stores element by element (215
+// instead of 60 us for a kept 1911 x 594 x 5181 product).
 //
 // Every wait is bounded (2 s). One that runs out makes the kernel write NaN to
 // the tiles it still owes, so a failed call never returns plausible numbers.
@@ -245,15 +248,25 @@ __device__ __forceinline__ void lt_stage_f32(uint8_t* box, const float* v, int l
     *reinterpret_cast<float4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) =
         make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
-// `rows` rows of the staged box to dst (16-byte aligned rows `ld` floats apart).
-__device__ __forceinline__ void lt_copy_f32(const uint8_t* box, float* dst, int64_t ld, int rows, int lane) {
+// `rows` rows and `cols` columns of the staged box to dst (16-byte aligned rows `ld` floats apart).
+__device__ __forceinline__ void lt_copy_f32(const uint8_t* box, float* dst, int64_t ld, int rows, int64_t cols, int lane) {
   __syncwarp();
+  const int p = lane & 7;
+  dst += 4 * p;
+  cols -= 4 * p;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = 4 * i + (lane >> 3), p = lane & 7;
-    if (r < rows)
-      *reinterpret_cast<float4*>(dst + r * ld + 4 * p) =
-          *reinterpret_cast<const float4*>(box + r * 128 + ((p ^ (r & 7)) << 4));
+    const int r = 4 * i + (lane >> 3);
+    const float4 v = *reinterpret_cast<const float4*>(box + r * 128 + ((p ^ (r & 7)) << 4));
+    float* d = dst + r * ld;
+    if (r >= rows || cols <= 0) continue;
+    if (cols >= 4) {
+      *reinterpret_cast<float4*>(d) = v;
+    } else {
+      d[0] = v.x;
+      if (cols > 1) d[1] = v.y;
+      if (cols > 2) d[2] = v.z;
+    }
   }
   __syncwarp();
 }
@@ -280,38 +293,6 @@ __device__ __forceinline__ void lt_boxes_free(int lane) {
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
   __syncwarp();
 }
-// 16 columns element by element (edges, rows that 16-byte accesses cannot
-// reach): 16 lanes take neighbouring columns of a row.
-__device__ __forceinline__ void lt_store16_any(const LinearEpilogue& ep, uint8_t* stage8, int64_t row0, int rows, int64_t c,
-                                               int64_t end, const float* v, int lane) {
-  float(*stage)[17] = reinterpret_cast<float(*)[17]>(stage8);
-  const int64_t col = c + (lane & 15);
-  const bool in = col < end;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) stage[lane][i] = v[i];
-  __syncwarp();
-#pragma unroll
-  for (int h = 0; h < 16; h += 8) {
-    float res[8];                                      // eight loads in flight
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = (lane >> 4) + 2 * (h + i);
-      res[i] = ep.residual != nullptr && in && r < rows
-                   ? __bfloat162float(static_cast<const __nv_bfloat16*>(ep.residual)[(row0 + r) * ep.ldr + col])
-                   : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = (lane >> 4) + 2 * (h + i);
-      const int64_t row = row0 + r;
-      const float y = stage[r][lane & 15] + res[i];
-      if (!in || r >= rows) continue;
-      if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + col] = y;
-      else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + col] = __float2bfloat16_rn(y);
-    }
-  }
-  __syncwarp();
-}
 // Largest magnitude (as bits) of the columns below `end`.
 __device__ __forceinline__ uint32_t lt_amax32(const float* v, int64_t c, int64_t end, uint32_t amax) {
 #pragma unroll
@@ -334,14 +315,8 @@ __device__ __forceinline__ void lt_store_z32(uint8_t* z, int64_t c, int64_t end,
     }
     w[i] = e4m3x4(s[0], s[1], s[2], s[3]);
   }
-  if (c + 32 <= end && (reinterpret_cast<uintptr_t>(z + c) & 15) == 0) {
-    reinterpret_cast<uint4*>(z + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    reinterpret_cast<uint4*>(z + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (c + i < end) z[c + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
-  }
+  if (c + 16 <= end) *reinterpret_cast<uint4*>(z + c) = make_uint4(w[0], w[1], w[2], w[3]);     // end: a multiple of 16
+  if (c + 32 <= end) *reinterpret_cast<uint4*>(z + c + 16) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 template <bool A_MN, bool B_MN, bool GATED, bool KEEP, bool CHAIN>
@@ -501,7 +476,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     uint8_t* stage = staging + ew * kLtStaging;
     const uint32_t stage_addr = smem_u32(stage);
     // y as bf16 in whole boxes with a residual: the residual's boxes are fetched into the boxes y leaves from
-    const bool res_boxes = a.vec && ep.residual != nullptr && !ep.y_f32;
+    const bool res_boxes = ep.residual != nullptr && !ep.y_f32;
     constexpr int CHUNKS_H = GATED ? 4 : 2;              // this warp's columns: NT / CHUNKS_H
     bool ok = true;
     int tt = 0;
@@ -605,7 +580,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
               from_tmem(col, v);
               lt_stage_f32(stage, v, lane);
             }
-            lt_copy_f32(stage, a.partial + y0 * NT + col, NT, warp_rows, lane);
+            lt_copy_f32(stage, a.partial + y0 * NT + col, NT, warp_rows, 32, lane);
           }
         }
         if constexpr (!CHAIN) release();
@@ -614,16 +589,13 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       // y's columns [c0 + 32 j, + 32)
       auto store = [&](int j, float* v) {
         const int64_t c = c0 + 32 * j;
-        if (!a.vec || (ep.y_f32 && c + 32 > O)) {
-          lt_store16_any(ep, stage, row0, warp_rows, c, O, v, lane);
-          if (c + 16 < O) lt_store16_any(ep, stage, row0, warp_rows, c + 16, O, v + 16, lane);
-        } else if (ep.y_f32) {
+        if (ep.y_f32) {
           if (ep.residual != nullptr && valid) {
             const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr;
             lt_bias32(r, c, O, v);
           }
           lt_stage_f32(stage, v, lane);
-          lt_copy_f32(stage, static_cast<float*>(ep.y) + row0 * ep.ldy + c, ep.ldy, warp_rows, lane);
+          lt_copy_f32(stage, static_cast<float*>(ep.y) + row0 * ep.ldy + c, ep.ldy, warp_rows, O - c, lane);
         } else {
           uint8_t* box = stage + (j & 1) * 2048;
           if (res_boxes) {
@@ -777,22 +749,37 @@ __global__ void __launch_bounds__(kLtThreads, 1)
   }
 }
 
-// A warp takes 256 columns of a row, neighbouring lanes neighbouring columns.
+// A warp takes 512 columns of a row, as 4-byte words: where the row starts at an
+// odd element, a word's halves come from two neighbouring aligned words (the
+// second one from L1). Words that reach past the row are read in halves.
+__device__ __forceinline__ uint32_t pad_word(const uint16_t* row, int first, int cols) {   // elements first, first + 1
+  if (first >= 0 && first + 1 < cols) return __ldg(reinterpret_cast<const uint32_t*>(row + first));
+  uint32_t v = 0;
+  if (first >= 0 && first < cols) v = __ldg(row + first);
+  if (first + 1 >= 0 && first + 1 < cols) v |= (uint32_t)__ldg(row + first + 1) << 16;
+  return v;
+}
 __global__ void __launch_bounds__(256) pad_kernel(PadArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int j = blockIdx.z, c = 256 * blockIdx.y + (threadIdx.x & 31);
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= a.rows[j]) return;
-  const uint16_t* s = static_cast<const uint16_t*>(a.src[j]) + row * a.lds[j];
-  uint16_t* d = static_cast<uint16_t*>(a.dst[j]) + row * a.ldd[j];
-  uint16_t v[8];
+  const int j = blockIdx.z, lane = threadIdx.x & 31, w0 = 256 * blockIdx.y + lane, cols = a.cols[j];
+  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < a.rows[j]; row += (int64_t)gridDim.x * 8) {
+    const uint16_t* s = static_cast<const uint16_t*>(a.src[j]) + row * a.lds[j];
+    uint32_t* d = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.dst[j]) + row * a.ldd[j]);
+    const bool odd = reinterpret_cast<uintptr_t>(s) & 2;
+    uint32_t v[8], u[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (c + 32 * e < a.cols[j]) v[e] = __ldg(s + c + 32 * e);
+    for (int e = 0; e < 8; ++e) {
+      const int c = 2 * (w0 + 32 * e);
+      v[e] = pad_word(s, odd ? c - 1 : c, cols);
+      if (odd) u[e] = pad_word(s, c + 1, cols);
+    }
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (c + 32 * e < a.cols[j]) d[c + 32 * e] = v[e];
+    for (int e = 0; e < 8; ++e) {
+      const int c = 2 * (w0 + 32 * e);
+      if (c < cols) d[w0 + 32 * e] = odd ? v[e] >> 16 | u[e] << 16 : v[e];
+    }
+  }
 }
 cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
   if (a.count == 0) return cudaSuccess;
@@ -802,106 +789,149 @@ cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
     rows = rows > a.rows[j] ? rows : a.rows[j];
     cols = cols > a.cols[j] ? cols : a.cols[j];
   }
-  if ((cols + 255) / 256 > 65535) return cudaErrorInvalidValue;
-  return launch_kernel(pad_kernel, dim3((unsigned)((rows + 7) / 8), (cols + 255) / 256, a.count), dim3(256), 0, st, true, a);
+  const int segments = (cols + 511) / 512;                 // cols <= 2^23
+  int64_t blocks = (rows + 7) / 8;
+  if (blocks * segments > 148 * 32) blocks = (148 * 32 + segments - 1) / segments;
+  return launch_kernel(pad_kernel, dim3((unsigned)blocks, segments, a.count), dim3(256), 0, st, true, a);
 }
 
 // Adds the K slices' partial rows in slice order and runs the epilogue. A warp
-// takes one row's block of 128 output columns, 4 per lane, so a block of the
-// 8-bit pre-activation is one warp's; the partial rows come from L2, where the
-// product has just left them.
-template <bool GATED, bool KEEP>
+// takes a block of 128 output columns of R rows, so a block of the 8-bit
+// pre-activation is one warp's; the partial rows come from L2, where the product
+// has just left them, those of up to four rows in flight together. VEC: 4 neighbouring
+// columns per lane and 16-byte rows; else columns lane + 32 j, one by one.
+template <bool GATED, bool KEEP, bool VEC, int R>
 __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
   const int lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
   const int H = GATED ? a.n_tile / 2 : a.n_tile, col_blocks = (H + 127) / 128;
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);     // (tile, row, column block)
-  const int64_t i = unit / (256 * col_blocks);
-  const int rr = (int)(unit - i * 256 * col_blocks) / col_blocks, cb = (int)(unit % col_blocks);
+  const uint32_t per_tile = 256 / (8 * R) * col_blocks;                    // blocks of 8 R rows and 128 columns
+  const uint32_t i = blockIdx.x / per_tile, in = blockIdx.x - i * per_tile;
+  const int r0 = (int)(in / col_blocks) * 8 * R + (threadIdx.x >> 5) * R, cb = (int)(in % col_blocks);
   int mt, nt;
   lt_place(a, a.full_tiles + i, mt, nt);
-  const int64_t row = (int64_t)mt * 256 + rr;
-  const int lc = 128 * cb + 4 * lane;                                     // column inside the tile
-  const int64_t O = a.out_cols, c = (int64_t)nt * H + lc;
-  if (row >= a.m || (int64_t)nt * H + 128 * cb >= O) return;              // warp-uniform
-  const bool in = lc < H && c < O;
-  const int64_t end = min(O, (int64_t)(nt + 1) * H);                      // this warp's columns end here
-  const int64_t kb = c / 128, blocks = (O + 127) / 128, step = (int64_t)256 * a.n_tile;
+  const int64_t row0 = (int64_t)mt * 256 + r0;
+  const int64_t O = a.out_cols, c0 = (int64_t)nt * H + 128 * cb;          // the warp's first column
+  if (row0 >= a.m || c0 >= O) return;                                     // warp-uniform
+  const int rows = (int)min((int64_t)R, a.m - row0);
+  const int width = (int)min((int64_t)min(128, H - 128 * cb), O - c0);    // its columns
+  const int64_t kb = c0 / 128, blocks = (O + 127) / 128, step = (int64_t)256 * a.n_tile;
   const LinearEpilogue& ep = a.ep;
   const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(ep.bias);
-  float v[GATED ? 2 : 1][4];
+  auto col = [&](int j) { return VEC ? 4 * lane + j : lane + 32 * j; };
+  constexpr int HALVES = GATED ? 2 : 1, U = R < 4 ? R : 4;
+  float b[HALVES][4];
 #pragma unroll
-  for (int h = 0; h < (GATED ? 2 : 1); ++h)
+  for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[h][j] = 0.f;
-  if (in) {
-    const float* p = a.partial + i * a.splits * step + (int64_t)rr * a.n_tile + lc;
-#pragma unroll 4
+    for (int j = 0; j < 4; ++j) b[h][j] = bias && col(j) < width ? __bfloat162float(bias[h * O + c0 + col(j)]) : 0.f;
+  const float* tile = a.partial + (int64_t)i * a.splits * step + (int64_t)r0 * a.n_tile + 128 * cb;
+#pragma unroll 1
+  for (int rb = 0; rb < rows; rb += U) {
+    float v[U][HALVES][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[u][h][j] = 0.f;
+#pragma unroll 2
     for (int s = 0; s < a.splits; ++s)
 #pragma unroll
-      for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-        const float4 f = __ldcg(reinterpret_cast<const float4*>(p + s * step + h * H));
-        v[h][0] += f.x;
-        v[h][1] += f.y;
-        v[h][2] += f.z;
-        v[h][3] += f.w;
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          if (rb + u >= rows) continue;
+          const float* q = tile + s * step + (int64_t)(rb + u) * a.n_tile + h * H;
+          if constexpr (VEC) {
+            if (col(0) >= width) continue;                                // a tile's width is a multiple of 32
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(q) + lane);
+            v[u][h][0] += f.x;
+            v[u][h][1] += f.y;
+            v[u][h][2] += f.z;
+            v[u][h][3] += f.w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (col(j) < width) v[u][h][j] += __ldcg(q + lane + 32 * j);
+          }
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (rb + u >= rows) continue;
+      const int64_t row = row0 + rb + u;
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[u][h][j] += b[h][j];
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          uint32_t amax = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (col(j) < width) amax = max(amax, __float_as_uint(v[u][h][j]) & 0x7fffffffu);
+          const uint32_t code = e8m0_of_amax(__reduce_max_sync(0xffffffffu, amax));
+          const float inv = e8m0_inverse(code);
+          if (lane == 0) ep.z_scale[(h * blocks + kb) * a.m + row] = (uint8_t)code;
+          float s[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[j] = code == kTopScaleCode ? hold_finite(v[u][h][j] * inv) : v[u][h][j] * inv;
+          const uint32_t w = e4m3x4(s[0], s[1], s[2], s[3]);
+          uint8_t* z = ep.z8 + (h * a.m + row) * O + c0;
+          if constexpr (VEC) {
+            if (col(0) < width) *reinterpret_cast<uint32_t*>(z + col(0)) = w;   // O is a multiple of 16
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (col(j) < width) z[col(j)] = (uint8_t)(w >> (8 * j));
+          }
+        }
       }
-    if (bias)
-#pragma unroll
-      for (int h = 0; h < (GATED ? 2 : 1); ++h)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < end) v[h][j] += __bfloat162float(bias[h * O + c + j]);
-  }
-  if constexpr (KEEP) {
-#pragma unroll
-    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-      uint32_t amax = 0;
+      float y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (c + j < end) amax = max(amax, __float_as_uint(v[h][j]) & 0x7fffffffu);
-      const uint32_t code = e8m0_of_amax(__reduce_max_sync(0xffffffffu, amax));
-      const float inv = e8m0_inverse(code);
-      if (lane == 0) ep.z_scale[(h * blocks + kb) * a.m + row] = (uint8_t)code;
-      float s[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = code == kTopScaleCode ? hold_finite(v[h][j] * inv) : v[h][j] * inv;
-      const uint32_t w = e4m3x4(s[0], s[1], s[2], s[3]);
-      uint8_t* z = ep.z8 + (h * a.m + row) * O + c;
+        y[j] = GATED ? v[u][0][j] * lt_silu(v[u][HALVES - 1][j], ep.y_f32)
+                     : ep.act == kActSilu ? lt_silu(v[u][0][j], ep.y_f32) : act_value(v[u][0][j], ep.act);
+      const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr + c0;
+      float* yf = static_cast<float*>(ep.y) + row * ep.ldy + c0;
+      __nv_bfloat16* yb = static_cast<__nv_bfloat16*>(ep.y) + row * ep.ldy + c0;
+      if (VEC && col(3) < width) {
+        if (ep.residual) {
+          const uint2 w = *reinterpret_cast<const uint2*>(r + col(0));
+          const float2 f0 = unpack_bf16(w.x), f1 = unpack_bf16(w.y);
+          y[0] += f0.x;
+          y[1] += f0.y;
+          y[2] += f1.x;
+          y[3] += f1.y;
+        }
+        if (ep.y_f32) *reinterpret_cast<float4*>(yf + col(0)) = make_float4(y[0], y[1], y[2], y[3]);
+        else *reinterpret_cast<uint2*>(yb + col(0)) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        continue;
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (c + j < end) z[j] = (uint8_t)(w >> (8 * j));
+        if (col(j) < width) {
+          if (ep.residual) y[j] += __bfloat162float(r[col(j)]);
+          if (ep.y_f32) yf[col(j)] = y[j];
+          else yb[col(j)] = __float2bfloat16_rn(y[j]);
+        }
     }
   }
-  float y[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    y[j] = GATED ? v[0][j] * act_value(v[GATED ? 1 : 0][j], kActSilu) : act_value(v[0][j], ep.act);
-  const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr + c;
-  if (a.vec && c + 4 <= end) {
-    if (ep.residual) {
-      const uint2 w = *reinterpret_cast<const uint2*>(r);
-      const float2 f0 = unpack_bf16(w.x), f1 = unpack_bf16(w.y);
-      y[0] += f0.x;
-      y[1] += f0.y;
-      y[2] += f1.x;
-      y[3] += f1.y;
-    }
-    if (ep.y_f32)
-      *reinterpret_cast<float4*>(static_cast<float*>(ep.y) + row * ep.ldy + c) = make_float4(y[0], y[1], y[2], y[3]);
-    else
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(ep.y) + row * ep.ldy + c) =
-          make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (c + j < end) {
-      if (ep.residual) y[j] += __bfloat162float(r[j]);
-      if (ep.y_f32) static_cast<float*>(ep.y)[row * ep.ldy + c + j] = y[j];
-      else static_cast<__nv_bfloat16*>(ep.y)[row * ep.ldy + c + j] = __float2bfloat16_rn(y[j]);
-    }
+}
+
+template <bool GATED, bool KEEP>
+static cudaError_t launch_join(const LinearTileArgs& a, cudaStream_t st) {
+  const int64_t tail = (a.units - a.full_tiles) / a.splits, H = GATED ? a.n_tile / 2 : a.n_tile;
+  const int64_t col_blocks = (H + 127) / 128, rows = a.m < 256 ? a.m : 256;
+  // 8 rows per warp once that leaves 16 warps per SM, else one
+  const bool many = tail * col_blocks * rows / 8 >= 148 * 16;
+  const dim3 grid((unsigned)(tail * col_blocks * (many ? 4 : 32))), block(256);
+#define MOE_JOIN(V, R) launch_kernel(linear_join_kernel<GATED, KEEP, V, R>, grid, block, 0, st, true, a)
+  if (many) return a.vec ? MOE_JOIN(true, 8) : MOE_JOIN(false, 8);
+  return a.vec ? MOE_JOIN(true, 1) : MOE_JOIN(false, 1);
+#undef MOE_JOIN
 }
 
 // Tile width and K slices of the last, partial round. Cycles per 64 of K and
@@ -911,7 +941,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
 // next tile's products except for the last one. Slices are at least 4 K-blocks
 // deep; joining them costs a launch and moves 8 bytes per value and slice
 // through L2 (about 3 KB per cycle).
-LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs) {
+LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gated, bool keep, bool b_mn, bool direct,
+                                int pairs) {
   LinearTilePlan best{};
   double best_cost = 1e300;
   const int64_t mt = (m + 255) / 256;
@@ -921,7 +952,7 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
     if (keep && nt != 256) continue;
     if ((gated || b_mn) && nt % 128) continue;       // epilogue warps take 32 columns; boxes of 64
     const int64_t cols = gated ? nt / 2 : nt;
-    const int64_t tiles = mt * ((n + cols - 1) / cols), tail = tiles % pairs, full = tiles - tail;
+    const int64_t tiles = mt * ((n + cols - 1) / cols), tail = direct ? tiles % pairs : tiles, full = tiles - tail;
     const double alone = 2.1 * nt, crowded = 174 + 2.3 * nt;
     const double rows = m < 256 ? m : 256;
     for (int s = 1; s <= 16; ++s) {
@@ -930,10 +961,11 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
       const double busy = units < pairs ? (double)units / pairs : 1.0;
       double cost = (double)(full / pairs) * (k_blocks * crowded + 800) +
                     (double)rounds * ((k_blocks + s - 1) / s * (alone + busy * (crowded - alone)) + 800);
-      cost = (cost > hbm ? cost : hbm) + 1500 + 12.0 * nt + (s > 1 ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
+      const bool join = s > 1 || !direct;
+      cost = (cost > hbm ? cost : hbm) + 1500 + 12.0 * nt + (join ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
       if (cost < best_cost) {
         best_cost = cost;
-        best = {nt, s, s > 1 ? full : tiles, s > 1 ? tail : 0};
+        best = {nt, s, join ? full : tiles, join ? tail : 0};
       }
     }
   }
@@ -996,14 +1028,9 @@ static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, c
 cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
                                const LinearTileArgs& a, int num_sms, cudaStream_t st) {
   cudaError_t e = launch_product(a_mn, b_mn, gated, keep, maps, a, num_sms, st);
-  if (e != cudaSuccess || a.splits == 1) return e;
-  const int64_t tail = (a.units - a.full_tiles) / a.splits, H = gated ? a.n_tile / 2 : a.n_tile;
-  const dim3 grid((unsigned)(tail * 32 * ((H + 127) / 128))), block(256);
-  if (gated)
-    return keep ? launch_kernel(linear_join_kernel<true, true>, grid, block, 0, st, true, a)
-                : launch_kernel(linear_join_kernel<true, false>, grid, block, 0, st, true, a);
-  return keep ? launch_kernel(linear_join_kernel<false, true>, grid, block, 0, st, true, a)
-              : launch_kernel(linear_join_kernel<false, false>, grid, block, 0, st, true, a);
+  if (e != cudaSuccess || a.units == a.full_tiles) return e;
+  if (gated) return keep ? launch_join<true, true>(a, st) : launch_join<true, false>(a, st);
+  return keep ? launch_join<false, true>(a, st) : launch_join<false, false>(a, st);
 }
 
 cudaError_t set_debug_waits_linear(unsigned long long limit_ns, int gate_extra) {

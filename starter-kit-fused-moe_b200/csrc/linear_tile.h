@@ -17,10 +17,10 @@ struct LinearTileArgs {
   int terms;
   int splits;
   int chain;              // K-blocks per accumulator where long sums are cut (fp32 y, kept pre-activations)
-  int64_t full_tiles;     // tiles done whole; the others are cut into `splits` K slices
+  int64_t full_tiles;     // tiles done whole; the others leave `splits` K slices to the join
   int64_t units;          // full_tiles + splits * (number of the others)
-  int vec;                // y (and the residual) can be accessed in 16 bytes
-  float* partial;         // splits > 1: fp32 [other tiles][splits][256][n_tile], 16-byte aligned
+  int vec;                // rows of y, the residual and the kept z can be accessed in 16 bytes (else full_tiles is 0)
+  float* partial;         // fp32 [tiles not whole][splits][256][n_tile], 16-byte aligned
   LinearEpilogue ep;
 };
 struct LinearTileMaps {
@@ -29,9 +29,10 @@ struct LinearTileMaps {
 };
 struct LinearTilePlan {
   int n_tile, splits;
-  int64_t full, tail;     // whole tiles, tiles cut into K slices
+  int64_t full, tail;     // whole tiles, tiles left to the join
 };
-LinearTilePlan plan_linear_tile(int64_t m, int64_t out_cols, int64_t k_blocks, bool gated, bool keep, bool b_mn, int pairs);
+LinearTilePlan plan_linear_tile(int64_t m, int64_t out_cols, int64_t k_blocks, bool gated, bool keep, bool b_mn, bool direct,
+                                int pairs);
 cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
                                const LinearTileArgs& a, int num_sms, cudaStream_t st);
 // One launch that copies up to two matrices into rows TMA can read (base and row

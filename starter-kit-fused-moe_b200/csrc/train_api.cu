@@ -51,15 +51,23 @@ bool tma_ready(const void* p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0
 // One tensor-core product: its tile plan and the workspace of its K slices.
 struct Product {
   moe::LinearTilePlan plan;
+  bool direct;
   int64_t term_blocks;
   int terms;
   size_t partial;      // bytes
 };
-Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gated, bool keep, bool b_mn) {
+// Whether 16-byte accesses reach every row of y, the residual and the kept z.
+bool direct_rows(const moe::LinearEpilogue& ep, int64_t out_cols) {
+  return aligned(ep.y, 16) && ep.ldy * (ep.y_f32 ? 4 : 2) % 16 == 0 &&
+         (!ep.residual || (aligned(ep.residual, 16) && ep.ldr % 8 == 0 && ep.ldr > 0)) &&
+         (!ep.z8 || (aligned(ep.z8, 16) && out_cols % 16 == 0));
+}
+Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gated, const moe::LinearEpilogue& ep, bool b_mn) {
   Product p{};
+  p.direct = direct_rows(ep, out_cols);
   p.term_blocks = (k + 63) / 64;
   p.terms = terms;
-  p.plan = moe::plan_linear_tile(m, out_cols, p.term_blocks * terms, gated, keep, b_mn, pairs());
+  p.plan = moe::plan_linear_tile(m, out_cols, p.term_blocks * terms, gated, ep.z8 != nullptr, b_mn, p.direct, pairs());
   p.partial = (size_t)p.plan.tail * p.plan.splits * 256 * p.plan.n_tile * sizeof(float);
   return p;
 }
@@ -83,9 +91,7 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.full_tiles = p.plan.full;
   t.units = p.plan.full + p.plan.tail * t.splits;
   t.ep = ep;
-  const int ysize = ep.y_f32 ? 4 : 2;
-  t.vec = aligned(ep.y, 16) && ep.ldy * ysize % 16 == 0 &&
-          (!ep.residual || (aligned(ep.residual, 16) && ep.ldr % 8 == 0 && ep.ldr > 0));
+  t.vec = p.direct;
   t.partial = reinterpret_cast<float*>(partial);
   moe::LinearTileMaps maps{};
   const uint32_t half = (uint32_t)t.n_tile / 2;
@@ -111,12 +117,19 @@ struct LinearPlan {
   int64_t ldp;
   size_t x, w, total;
 };
+moe::LinearEpilogue epilogue_of(const MoeLinearArgs& a) {
+  return {a.bias, a.residual, a.y, static_cast<uint8_t*>(a.z8), static_cast<uint8_t*>(a.z_scale),
+          a.ldr, a.ldy, a.activation, a.y_f32};
+}
+moe::LinearEpilogue plain_epilogue(void* y, int64_t ldy, int f32) {
+  return {nullptr, nullptr, y, nullptr, nullptr, 0, ldy, MOE_ACT_NONE, f32};
+}
 LinearPlan linear_plan(const MoeLinearArgs& a) {
   LinearPlan p{};
   p.small = a.m <= moe::kSmallTokens && a.z8 == nullptr;
   if (p.small) return p;
   const bool gated = a.activation == MOE_ACT_SWIGLU;
-  p.prod = plan_product(a.m, gated ? a.n / 2 : a.n, a.k, 1, gated, a.z8 != nullptr, false);
+  p.prod = plan_product(a.m, gated ? a.n / 2 : a.n, a.k, 1, gated, epilogue_of(a), false);
   p.pad_x = !tma_ready(a.x, a.ldx);
   p.pad_w = !tma_ready(a.weight, a.ldw);
   p.ldp = up8(a.k);
@@ -148,12 +161,12 @@ GradPlan grad_plan(const MoeLinearGradArgs& a) {
   p.chunks = moe::act_grad_chunks(a.m, a.n);
   size_t partial = 0;
   if (a.grad_x) {
-    p.px = plan_product(a.m, a.k, a.n, p.terms, false, false, true);
+    p.px = plan_product(a.m, a.k, a.n, p.terms, false, plain_epilogue(a.grad_x, a.k, a.grad_f32), true);
     partial = p.px.partial;
     p.pad_w = !tma_ready(a.weight, a.ldw);
   }
   if (a.grad_weight) {
-    p.pw = plan_product(a.n, a.k, a.m, p.terms, false, false, true);
+    p.pw = plan_product(a.n, a.k, a.m, p.terms, false, plain_epilogue(a.grad_weight, a.k, a.grad_f32), true);
     if (p.pw.partial > partial) partial = p.pw.partial;
   }
   size_t o = up256(partial);
@@ -195,8 +208,7 @@ int moe_linear_run(const MoeLinearArgs* a, void* stream) {
     return workspace_error("linear", p.total, a->workspace_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  moe::LinearEpilogue ep{a->bias, a->residual, a->y, static_cast<uint8_t*>(a->z8), static_cast<uint8_t*>(a->z_scale),
-                         a->ldr, a->ldy, a->activation, a->y_f32};
+  const moe::LinearEpilogue ep = epilogue_of(*a);
   if (p.small) return done(moe::launch_linear_small(a->x, a->ldx, a->weight, a->ldw, a->m, a->k, a->n, ep, st), "linear product");
   moe::PadArgs pads{};
   if (p.pad_x) pads.add(a->x, a->ldx, a->m, a->k, ws + p.x, p.ldp);
@@ -270,7 +282,7 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
   if (a->grad_x) {
     const void* w = p.pad_w ? ws + p.w : a->weight;
     const int64_t ldw = p.pad_w ? p.ldk : a->ldw;
-    moe::LinearEpilogue ep{nullptr, nullptr, a->grad_x, nullptr, nullptr, 0, a->k, MOE_ACT_NONE, a->grad_f32};
+    const moe::LinearEpilogue ep = plain_epilogue(a->grad_x, a->k, a->grad_f32);
     if (int rc = run_product(p.px, false, true, false, false, a->m, a->k, a->n, dz, ldz, term_stride, w, ldw, a->n, ep,
                              ws, st, "input gradient"))
       return rc;
@@ -279,7 +291,7 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
     e = moe::launch_restore(static_cast<const uint8_t*>(a->x8), static_cast<const uint8_t*>(a->x_scale), 1, a->m, a->k,
                             ws + p.xhat, false, p.ldk, st);
     if (e != cudaSuccess) return done(e, "restoring the input checkpoint");
-    moe::LinearEpilogue ep{nullptr, nullptr, a->grad_weight, nullptr, nullptr, 0, a->k, MOE_ACT_NONE, a->grad_f32};
+    const moe::LinearEpilogue ep = plain_epilogue(a->grad_weight, a->k, a->grad_f32);
     if (int rc = run_product(p.pw, true, true, false, false, a->n, a->k, a->m, dz, ldz, term_stride, ws + p.xhat, p.ldk,
                              a->m, ep, ws, st, "weight gradient"))
       return rc;
