@@ -156,7 +156,8 @@ int moe_fp8_read_device_error(void* workspace, void* stream, int32_t* bits);
  * on the current device): `wait_limit_ns` replaces the 2 s limit of every
  * device-side wait (the expert-parallel flag waits included), and `gate_extra` is added to the target of the streaming
  * kernel's GEMM2 gate (the count of finished GEMM1 tiles it waits for), so a
- * test can make that wait run out without faulting anything. Restore with
+ * test can make that wait run out without faulting anything (non-zero, it also
+ * makes moe_linear_run's tile kernel withhold its accumulators). Restore with
  * (2000000000, 0). Returns MOE_OK or MOE_ERR_INVALID_ARGUMENT / MOE_ERR_CUDA.
  * Replaces nothing in the reference (its kernels have no bounded waits). */
 int moe_fp8_debug_set_waits(uint64_t wait_limit_ns, int32_t gate_extra);
@@ -268,7 +269,8 @@ int moe_fp8_ep_peer_read_error(void* base, void* stream, int32_t* bits);
  * are free (m tokens in [0, 2^30], k and n in [1, 2^23]); matrices are row-major with a row
  * stride in elements and need the alignment of their type only. Every entry
  * works on the current device, asynchronously on `stream`, and keeps nothing
- * between calls; `workspace` is device scratch, 256-byte aligned, that calls in
+ * between calls (a wait inside the tile kernel that runs out makes the call's
+ * output NaN); `workspace` is device scratch, 256-byte aligned, that calls in
  * flight on different streams (and different captured graphs) must not share. */
 #define MOE_ACT_NONE 0
 #define MOE_ACT_RELU 1

@@ -41,7 +41,8 @@
 // instead of 60 us for a kept 1911 x 594 x 5181 product).
 //
 // Every wait is bounded (2 s). One that runs out makes the kernel write NaN to
-// the tiles it still owes, so a failed call never returns plausible numbers.
+// the tiles it still owes, so a failed call never returns plausible numbers; the
+// block then gives its copies in flight a millisecond before it leaves.
 #include "cta_pair.cuh"
 #include "linear_tile.h"
 #include "train_common.cuh"
@@ -420,6 +421,8 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     } else if (warp == 1 && crank == 0) {
       // ------------------------------------------------------------ MMA issuer (leader)
       const uint32_t idesc = idesc_bf16(NT, A_MN, B_MN);
+      // test hook: a non-zero value withholds the accumulators, so that the epilogue's wait runs out
+      const bool withhold = *reinterpret_cast<const volatile int*>(&g_gate_extra) != 0;
       int s = 0, tt = 0;                                   // stage, accumulator
       uint32_t parity = 0;
       bool ok = true;
@@ -458,7 +461,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
               parity ^= 1;
             }
           }
-          if (ok && elect_one()) mma_commit_pair(smem_u32(&S.tfull[b]));
+          if (ok && !withhold && elect_one()) mma_commit_pair(smem_u32(&S.tfull[b]));
           __syncwarp();
         }
       }
@@ -742,6 +745,11 @@ __global__ void __launch_bounds__(kLtThreads, 1)
 
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) {
+    }
+  }
   cluster_sync_all();      // neither CTA leaves while the other may still signal its barriers
   if (warp == 1) {
     tc_fence_after();

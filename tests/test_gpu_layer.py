@@ -503,3 +503,47 @@ def test_graph_between_copies(pkg):
     for _ in range(50):
         step()
     assert all(torch.equal(o, v) for o, v in zip(outs, want))
+
+
+@pytest.mark.parametrize("m, n, act", [(300, 512, "none"), (100, 4096, "swiglu"), (300, 130, "gelu")])
+def test_wait_that_runs_out_gives_nan(pkg, m, n, act):
+    """A product whose accumulators never come (a host-set test hook) returns NaN after the shortened limit, and the
+    next call is right again."""
+    x, w = randn(m, 256, seed=1), randn(n, 256, seed=2, scale=0.06)
+    want = pkg.linear(x, w, activation=act)
+    lib = pkg.load_library()
+    torch.cuda.synchronize()
+    assert lib.moe_fp8_debug_set_waits(20_000_000, 1) == 0
+    try:
+        bad = pkg.linear(x, w, activation=act)
+        bad32 = pkg.linear(x, w, activation=act, out_dtype=F32)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.moe_fp8_debug_set_waits(2_000_000_000, 0) == 0
+    assert torch.isnan(bad).all() and torch.isnan(bad32).all()
+    assert torch.equal(pkg.linear(x, w, activation=act), want)
+
+
+def test_offsets_past_32_bits(pkg):
+    """More than 2^31 elements: the last rows of a product and of a checkpoint are those of the rows alone."""
+    m, k, n = 300_100, 64, 7168
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    x, w = randn(m, k, seed=1), randn(n, k, seed=2, scale=0.1)
+    y = pkg.linear(x, w)
+    z, tz = dense64(x[-40:], w)
+    check(y[-40:], z, rounded(z, tz, BF), "last rows")
+    q, s = pkg.checkpoint_activations(y)
+    q2, s2 = pkg.checkpoint_activations(y[-40:])
+    assert torch.equal(q[-40:].view(torch.uint8), q2.view(torch.uint8))
+    assert torch.equal(s[:, -40:].contiguous().view(torch.uint8), s2.view(torch.uint8))
+    r = pkg.restore_activations(q, s)
+    assert torch.equal(r[-40:], pkg.restore_activations(q2, s2))
+    del r, z, tz
+    dy = y[:, :1].expand(m, 8)                        # a broadcast gradient of a product with 8 outputs
+    ck = pkg.LinearCheckpoint(q, s, None, None, "none")
+    g = pkg.linear_backward(dy, ck, randn(8, n, seed=3), need_x=True, need_bias=True, grad_dtype=F32)
+    ref = dy[-40:].double() @ randn(8, n, seed=3).double()
+    check(g.x[-40:], ref, ref.abs() * 2.0 ** -20 + 1e-4, "grad_x of the last rows")
+    want = dy[:, 0].double().sum()
+    assert abs(float(g.bias[0].double() - want)) <= 2.0 ** -16 * float(dy[:, 0].double().abs().sum())
