@@ -7,11 +7,10 @@
 // loads W straight into mma.sync fragments with 16-byte loads: lane (g, t) of
 // the m16n8k16 layout takes 8 neighbouring values of row g at 8 t, and the
 // token operand is taken at the same positions, so the permutation of K inside
-// a chunk cancels and nothing passes through shared memory. A 16 x 8 tile of
-// tcgen05 would use a sixteenth of its rows here; the tensor work (1 / 8 of
-// peak rate needed at 8 tokens) is not what bounds this. The partial sums meet
-// in shared memory, then across the cluster in distributed shared memory, both
-// in a fixed order.
+// a chunk cancels and nothing passes through shared memory. (A tcgen05 tile would
+// spend its rows on padding; the tensor work is not what bounds this.) The partial
+// sums meet in shared memory, then across the cluster in distributed shared memory,
+// both in a fixed order.
 #include "cta_pair.cuh"
 #include "train_common.cuh"
 
