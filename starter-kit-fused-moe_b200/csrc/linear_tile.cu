@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     // y as bf16 in whole boxes with a residual: the residual's boxes are fetched into the boxes y leaves from
     const bool res_boxes = ep.residual != nullptr && !ep.y_f32;
     constexpr int CHUNKS_H = GATED ? 4 : 2;              // this warp's columns: NT / CHUNKS_H
-    bool ok = true;
+    bool ok = true, res_ok = true;
     int tt = 0;
     uint32_t res_count = 0;                              // residual boxes waited for
     for (int64_t u = wid; u < a.units; u += G) {
@@ -602,9 +602,14 @@ __global__ void __launch_bounds__(kLtThreads, 1)
         } else {
           uint8_t* box = stage + (j & 1) * 2048;
           if (res_boxes) {
-            if (ok && !mbar_wait(smem_u32(&S.res[ew][j & 1]), (res_count >> (j & 1)) & 1)) {
+            // waited for in a failed call too: a box that arrives later would cover the NaN staged here
+            if (res_ok && !mbar_wait(smem_u32(&S.res[ew][j & 1]), (res_count >> (j & 1)) & 1)) {
               *abort_flag = 1;
-              ok = false;
+              ok = res_ok = false;
+            }
+            if (!res_ok) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = NAN;
             }
             res_count ^= 1u << (j & 1);                  // each box's phase flips with every use
 #pragma unroll

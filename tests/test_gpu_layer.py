@@ -524,6 +524,28 @@ def test_wait_that_runs_out_gives_nan(pkg, m, n, act):
     assert torch.equal(pkg.linear(x, w, activation=act), want)
 
 
+@pytest.mark.parametrize("m, k, n, act", [(4096, 256, 7168, "none"), (2048, 2048, 4096, "swiglu")])
+def test_wait_that_runs_out_with_residual_and_checkpoint(pkg, m, k, n, act):
+    """The same over many tiles per SM, where the residual's boxes are fetched ahead of the products."""
+    o = n // 2 if act == "swiglu" else n
+    x, w, r = randn(m, k, seed=1), randn(n, k, seed=2, scale=0.06), randn(m, o, seed=3)
+    want = pkg.linear(x, w, residual=r, activation=act)
+    lib = pkg.load_library()
+    torch.cuda.synchronize()
+    assert lib.moe_fp8_debug_set_waits(20_000_000, 1) == 0
+    try:
+        bad = pkg.linear(x, w, residual=r, activation=act)
+        bad32 = pkg.linear(x, w, residual=r, activation=act, out_dtype=F32)
+        kept, ck = pkg.linear_checkpointed(x, w, residual=r, activation=act)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.moe_fp8_debug_set_waits(2_000_000_000, 0) == 0
+    assert torch.isnan(bad).all() and torch.isnan(bad32).all() and torch.isnan(kept).all()
+    if act != "none":
+        assert torch.isnan(pkg.restore_activations(ck.z, ck.z_scale)).all()
+    assert torch.equal(pkg.linear(x, w, residual=r, activation=act), want)
+
+
 def test_offsets_past_32_bits(pkg):
     """More than 2^31 elements: the last rows of a product and of a checkpoint are those of the rows alone."""
     m, k, n = 300_100, 64, 7168
