@@ -280,7 +280,7 @@ int moe_fp8_ep_peer_read_error(void* base, void* stream, int32_t* bits);
 
 /* y = act(x W^T + bias) + residual; O = n / 2 for MOE_ACT_SWIGLU, n otherwise.
  * bf16 products are summed in fp32, everything after them is computed in fp32
- * and rounded once. y may be the residual itself (same pointer and stride); it
+ * and rounded once. y may be the residual itself (bf16, same pointer and stride); it
  * must not overlap the other inputs. With z8 / z_scale given, the
  * pre-activation z = x W^T + bias is also kept as an 8-bit checkpoint (see
  * moe_checkpoint_activations): [m, n] and [ceil(n / 128), m], or, for

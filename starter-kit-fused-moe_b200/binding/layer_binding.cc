@@ -90,7 +90,17 @@ std::pair<uintptr_t, uintptr_t> span(const Tensor& t) {
 }
 bool overlap(const Tensor& a, const Tensor& b) {
   const auto x = span(a), y = span(b);
-  return x.first < y.second && y.first < x.second;
+  if (x.first >= y.second || y.first >= x.second) return false;
+  // column slices of the same rows lie side by side
+  if (a.dim() == 2 && b.dim() == 2 && a.stride(1) == 1 && b.stride(1) == 1) {
+    const int64_t pitch = a.stride(0) * a.element_size();
+    const int64_t wa = a.size(1) * a.element_size(), wb = b.size(1) * b.element_size();
+    if (pitch > 0 && pitch == b.stride(0) * b.element_size() && wa <= pitch) {
+      const int64_t d = (int64_t)(y.first - x.first) % pitch, at = d < 0 ? d + pitch : d;
+      return !(at >= wa && at + wb <= pitch);
+    }
+  }
+  return true;
 }
 
 int activation_code(const std::string& s) {
@@ -186,7 +196,7 @@ std::tuple<Tensor, OptTensor, OptTensor> linear(const Tensor& x, const Tensor& w
     if (overlap(*output, weight)) refuse("output overlaps weight");
     if (bias && overlap(*output, *bias)) refuse("output overlaps bias");
     if (residual && overlap(*output, *residual) &&
-        !(output->data_ptr() == residual->data_ptr() && output->strides() == residual->strides()))
+        !(out_dtype == at::kBFloat16 && output->data_ptr() == residual->data_ptr() && output->strides() == residual->strides()))
       refuse("output may be the residual itself but not overlap it otherwise");
     if (rows_readable(*output)) y = *output;
   }

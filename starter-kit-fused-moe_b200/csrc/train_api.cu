@@ -203,6 +203,8 @@ int moe_linear_run(const MoeLinearArgs* a, void* stream) {
     return bad("linear: a pointer is not aligned to its type");
   if (a->ldx < a->k || a->ldw < a->k || a->ldy < O || (a->residual && a->ldr < 0))
     return bad("linear: a row stride is smaller than the row");
+  if (a->residual == a->y && (a->y_f32 || a->ldr != a->ldy))
+    return bad("linear: y may be the residual itself only as bf16 and with its row stride");
   const LinearPlan p = linear_plan(*a);
   if (p.total && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < p.total))
     return workspace_error("linear", p.total, a->workspace_bytes);

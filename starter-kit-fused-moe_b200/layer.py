@@ -126,7 +126,8 @@ def linear(x, weight, bias=None, residual=None, activation="none", out_dtype=tor
     of the N columns times silu of the second half, as in the routed experts;
     O = N / 2, otherwise O = N). Products are summed in fp32; the result is
     rounded once to `out_dtype` (bf16 or f32). `output` [M, O] is written in
-    place when given and returned; it may be the residual itself. Any sizes with
+    place when given and returned; it may be the residual itself (bf16) or columns
+    beside x or the residual in the same rows, but not overlap an input. Any sizes with
     K, N >= 1 and any strides (rows that are not contiguous are copied first).
     f32 logits for `route` and `run` come from `out_dtype=torch.float32`.
     """

@@ -177,6 +177,28 @@ def test_linear_empty_and_refusals(pkg):
         pkg.linear(sq[:8], sq, residual=r[:8], output=r[1:])
 
 
+@pytest.mark.parametrize("m, k, n", [(5, 64, 40), (90, 72, 37), (700, 128, 96)])
+def test_linear_columns_of_one_buffer(pkg, m, k, n):
+    """x, y and the residual as columns side by side: the neighbours stay as they are."""
+    buf = randn(m, k + 2 * n + 3, seed=5)
+    before, w = buf.clone(), randn(n, k, seed=6, scale=0.1)
+    x, y, r = buf[:, :k], buf[:, k:k + n], buf[:, k + n:k + 2 * n]
+    want = pkg.linear(x, w, residual=r)
+    pkg.linear(x, w, residual=r, output=y)
+    assert torch.equal(y, want)
+    buf[:, k:k + n] = before[:, k:k + n]
+    assert torch.equal(buf, before)
+    with pytest.raises(ValueError, match="overlaps x"):
+        pkg.linear(x, w, output=buf[:, k - 1:k - 1 + n])
+
+
+def test_linear_residual_of_another_type_in_the_same_place(pkg):
+    x, w, out = randn(8, 64), randn(64, 64), torch.zeros(8, 64, device="cuda")
+    r = out.view(BF).as_strided((8, 64), (64, 1))
+    with pytest.raises(ValueError, match="residual"):
+        pkg.linear(x, w, residual=r, output=out, out_dtype=F32)
+
+
 # --------------------------------------------------------------------------------- checkpoints
 def quantize64(x):
     """(values, codes) of the format, element by element in 64 bits."""

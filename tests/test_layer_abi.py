@@ -47,6 +47,13 @@ def test_linear_refusals(layer, lib, pkg, kw, text):
     assert text in lib.moe_fp8_last_error()
 
 
+@pytest.mark.parametrize("kw", [{"y_f32": 1, "ldr": 32}, {"ldr": 40}])
+def test_linear_residual_that_is_not_y_itself(layer, lib, kw):
+    a = linear_args(layer, residual=FAKE, **kw)
+    assert lib.moe_linear_run(ctypes.byref(a), None) == 1
+    assert b"residual itself" in lib.moe_fp8_last_error()
+
+
 def test_linear_workspace_refusal_and_empty(layer, lib):
     a = linear_args(layer, m=600, k=7168, n=4096, ldx=7168, ldw=7168, ldy=4096)
     need = lib.moe_linear_workspace_bytes(ctypes.byref(a))
