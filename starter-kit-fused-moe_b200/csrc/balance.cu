@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
     for (int d = 16; d >= 1; d >>= 1) term += __shfl_xor_sync(0xffffffffu, term, d);
     if (tx == 0) {
       w.loss[(int64_t)q * groups + g] = bad ? (double)NAN : term;
-      if (g == 0) a.tokens[q] = tq;
+      if (g == 0) a.tokens[q] = bad ? -1 : tq;
       __threadfence();
       last = atomicAdd(w.state, 1) == (int)(gridDim.x * gridDim.y) - 1;
     }
@@ -287,13 +287,18 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
   if (!last) return;
   __threadfence();
   double l = 0.0;                                            // fixed order: strided sums, then two trees
-  int live = 0;
+  int live = 0, wrong = 0;
   const int64_t parts = (int64_t)a.s * groups;
   for (int64_t i = threadIdx.x; i < parts; i += 256) l += __ldcg(w.loss + i);
-  for (int i = threadIdx.x; i < a.s; i += 256) live += __ldcg(a.tokens + i) > 0;
+  for (int i = threadIdx.x; i < a.s; i += 256) {
+    const int n_i = __ldcg(a.tokens + i);
+    live += n_i > 0;
+    wrong |= n_i < 0;
+  }
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
   live = __reduce_add_sync(0xffffffffu, live);
+  const bool any_wrong = __syncthreads_or(wrong);
   if (tx == 0) {
     rp[0][ty] = l;
     rt[ty] = live;
@@ -305,7 +310,7 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
       live += rt[i];
     }
     *a.loss = (float)(live > 0 ? (double)a.alpha * l / live : l);   // l is 0 (or NaN) without sequences
-    *a.live = live;
+    *a.live = any_wrong ? -1 : live;
   }
 }
 
@@ -347,8 +352,8 @@ __global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_gr
     }
     float coef[ITEMS];
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) coef[j] = 0.f;
-    if (with_loss) {
+    for (int j = 0; j < ITEMS; ++j) coef[j] = live < 0 ? NAN : 0.f;        // wrong boundaries: no gradient either
+    if (with_loss && live >= 0) {
       const int q = seq_of(a.cu, a.s, pos, lane);
       int qa, qb;
       seq_bounds(a.cu, q, a.t, qa, qb);

@@ -342,6 +342,9 @@ int moe_balance_loss(const MoeBalanceArgs* a, void* stream) {
   if (!a->loss || !a->counts || !a->tokens || !a->mean_scores || !a->sequences) return bad("balance: an output is NULL");
   if (a->num_tokens > 0 && (!a->routing_logits || !a->topk_idx || !aligned(a->routing_logits, 4) || !aligned(a->topk_idx, 4)))
     return bad("balance: NULL or misaligned input");
+  if (!aligned(a->cu_seqlens, 4) || !aligned(a->loss, 4) || !aligned(a->counts, 4) || !aligned(a->tokens, 4) ||
+      !aligned(a->mean_scores, 4) || !aligned(a->sequences, 4))
+    return bad("balance: a pointer is not aligned to its type");
   if (!a->cu_seqlens && a->num_sequences != 1) return bad("balance: one sequence without cu_seqlens");
   const size_t need = moe_balance_workspace_bytes(a->num_tokens, a->num_experts, a->num_sequences);
   if (need && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need))
@@ -357,7 +360,9 @@ int moe_balance_loss_grad(const MoeBalanceGradArgs* a, void* stream) {
   if (int rc = check_balance(a->num_tokens, a->num_experts, a->top_k, a->num_sequences, a->scoring)) return rc;
   if (a->num_tokens == 0) return MOE_OK;
   if (!a->routing_logits || !a->topk_idx || !a->grad_logits || !aligned(a->routing_logits, 4) ||
-      !aligned(a->topk_idx, 4) || !aligned(a->grad_logits, 4) || !aligned(a->grad_topk_weights, 4))
+      !aligned(a->topk_idx, 4) || !aligned(a->grad_logits, 4) || !aligned(a->grad_topk_weights, 4) ||
+      !aligned(a->cu_seqlens, 4) || !aligned(a->counts, 4) || !aligned(a->tokens, 4) || !aligned(a->sequences, 4) ||
+      !aligned(a->grad_loss, 4))
     return bad("balance gradient: NULL or misaligned pointer");
   if (a->grad_loss && (!a->counts || !a->tokens || !a->sequences))
     return bad("balance gradient: grad_loss needs counts, tokens and sequences");

@@ -161,6 +161,16 @@ def test_balance_empty_and_bad_boundaries(pkg):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_balance_bad_boundaries_leave_no_gradient(pkg, scoring):
+    x, idx, dw = inputs(40, 32, 2)
+    for cuts in ([0, 30, 20, 40], [-5, 10, 40], [0, 10, 41], [10, 5]):
+        cu = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+        b = pkg.balance_loss(x, idx, cu_seqlens=cu, scoring=scoring)
+        assert torch.isnan(b.loss) and int(b.sequences) == -1
+        assert torch.isnan(pkg.balance_loss_backward(x, idx, b, cu_seqlens=cu, scoring=scoring)).all()
+
+
 def test_balance_weights_only_and_refusals(pkg):
     x, idx, dw = inputs(40, 32, 2)
     g = pkg.balance_loss_backward(x, idx, None, grad_topk_weights=dw, routed_scaling_factor=1.5)

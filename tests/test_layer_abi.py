@@ -135,6 +135,13 @@ def test_balance_refusals(layer, lib, kw):
     assert lib.moe_balance_loss_grad(ctypes.byref(balance_args(layer, "MoeBalanceGradArgs", **kw)), None) == 1
 
 
+@pytest.mark.parametrize("name", ["cu_seqlens", "counts", "tokens", "sequences"])
+def test_balance_misaligned_pointers(layer, lib, name):
+    for entry, cls in ((lib.moe_balance_loss, "MoeBalanceArgs"), (lib.moe_balance_loss_grad, "MoeBalanceGradArgs")):
+        assert entry(ctypes.byref(balance_args(layer, cls, **{name: FAKE + 2})), None) == 1
+        assert b"aligned" in lib.moe_fp8_last_error()
+
+
 def test_balance_refusals_of_one_entry(layer, lib):
     for kw in ({"loss": None}, {"counts": None}, {"tokens": None}, {"mean_scores": None}, {"sequences": None}):
         assert lib.moe_balance_loss(ctypes.byref(balance_args(layer, **kw)), None) == 1
