@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       const int chunks = (int)min((int64_t)(w / 32), (O - c0 + 31) / 32);
       const bool live = warp_rows > 0 && chunks > 0;
       auto fetch_residual = [&](int j) {                 // chunk j into box j & 1, whose last store has been read
-        if (lane == 0) {
+        if (lane == 0 && res_ok) {                       // a box that never came may not be armed again
           const uint32_t bar = smem_u32(&S.res[ew][j & 1]);
           mbar_arrive_expect_tx(bar, 2048);
           tma_load_2d(stage_addr + (j & 1) * 2048, &maps.res, bar, (int)c0 + 32 * j, (int)row0);
