@@ -380,10 +380,10 @@ typedef struct MoeBalanceGradArgs {
   const float* routing_logits;
   const int32_t* topk_idx;
   const int32_t* cu_seqlens;
-  const int32_t* counts;            /* as moe_balance_loss wrote them */
+  const int32_t* counts;            /* as moe_balance_loss wrote them; all three NULL: no loss part */
   const int32_t* tokens;
   const int32_t* sequences;
-  const float* grad_loss;           /* device scalar, or NULL: no loss part (counts .. sequences unused) */
+  const float* grad_loss;           /* device scalar, or NULL: 1 (a factor known to the host goes into alpha) */
   const float* grad_topk_weights;   /* f32 [T, k] or NULL */
   float* grad_logits;               /* f32 [T, E], overwritten */
   int32_t num_tokens, num_experts, top_k, num_sequences;

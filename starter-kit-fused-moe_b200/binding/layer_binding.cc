@@ -118,6 +118,27 @@ int scoring_code(const std::string& s) {
 Tensor make(at::IntArrayRef sizes, at::ScalarType t, at::Device dev) {
   return at::detail::empty_cuda(sizes, t, dev, std::nullopt);   // torch's caching allocator, without the dispatcher
 }
+// The tensors of a call that live and die together, from one allocation (an
+// allocation costs 0.7 us, several of them as much as the kernels of a short call).
+struct Together {
+  at::Device dev;
+  int64_t bytes = 0;
+  c10::Storage storage;
+  int64_t add(int64_t n) {
+    const int64_t at = bytes;
+    bytes += (n + 255) & ~int64_t(255);
+    return at;
+  }
+  void allocate() { storage = make({bytes}, at::kByte, dev).storage(); }
+  Tensor view(int64_t at, at::IntArrayRef sizes, at::ScalarType t) const {
+    Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(storage), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                        c10::scalarTypeToTypeMeta(t));
+    r.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    r.unsafeGetTensorImpl()->set_storage_offset(at / c10::elementSize(t));
+    return r;
+  }
+};
+
 void* stream_of(at::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
 
@@ -127,7 +148,10 @@ std::pair<Tensor, Tensor> checkpoint(const Tensor& x) {
   const auto dev = x.device();
   const c10::cuda::CUDAGuard guard(dev);
   const int64_t T = x.size(0), K = x.size(1);
-  Tensor q = make({T, K}, at::kFloat8_e4m3fn, dev), s = make({blocks_of(K), T}, at::kFloat8_e8m0fnu, dev);
+  Together out{dev};
+  const int64_t at_q = out.add(T * K), at_s = out.add(blocks_of(K) * T);
+  out.allocate();
+  Tensor q = out.view(at_q, {T, K}, at::kFloat8_e4m3fn), s = out.view(at_s, {blocks_of(K), T}, at::kFloat8_e8m0fnu);
   if (x.numel()) {
     int64_t ld;
     const Tensor xr = rows(x, ld);
@@ -216,12 +240,16 @@ std::tuple<Tensor, OptTensor, OptTensor> linear(const Tensor& x, const Tensor& w
   a.y_f32 = out_dtype == at::kFloat;
   OptTensor z, zs;
   if (keep && act) {
-    if (act == MOE_ACT_SWIGLU) {
-      z = make({2, M, O}, at::kFloat8_e4m3fn, dev);
-      zs = make({2, blocks_of(O), M}, at::kFloat8_e8m0fnu, dev);
+    const int64_t halves = act == MOE_ACT_SWIGLU ? 2 : 1;
+    Together kept{dev};
+    const int64_t at_z = kept.add(halves * M * O), at_s = kept.add(halves * blocks_of(O) * M);
+    kept.allocate();
+    if (halves == 2) {
+      z = kept.view(at_z, {2, M, O}, at::kFloat8_e4m3fn);
+      zs = kept.view(at_s, {2, blocks_of(O), M}, at::kFloat8_e8m0fnu);
     } else {
-      z = make({M, O}, at::kFloat8_e4m3fn, dev);
-      zs = make({blocks_of(O), M}, at::kFloat8_e8m0fnu, dev);
+      z = kept.view(at_z, {M, O}, at::kFloat8_e4m3fn);
+      zs = kept.view(at_s, {blocks_of(O), M}, at::kFloat8_e8m0fnu);
     }
     a.z8 = z->data_ptr();
     a.z_scale = zs->data_ptr();
@@ -240,6 +268,14 @@ std::tuple<Tensor, OptTensor, OptTensor> linear(const Tensor& x, const Tensor& w
     y = *output;
   }
   return {y, z, zs};
+}
+
+std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor> linear_checkpointed(
+    const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, const std::string& activation,
+    at::ScalarType out_dtype, const OptTensor& output) {
+  auto [y, z, z_scale] = linear(x, weight, bias, residual, activation, out_dtype, output, true);
+  auto [q, scale] = checkpoint(x);
+  return {y, q, scale, z, z_scale};
 }
 
 std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(const Tensor& grad_output, const Tensor& x8,
@@ -351,8 +387,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> balance_loss(const Tensor& lo
   const Router r = router(logits, idx, cu, scoring);
   const auto dev = logits.device();
   const c10::cuda::CUDAGuard guard(dev);
-  Tensor loss = make({}, at::kFloat, dev), counts = make({r.S, r.E}, at::kInt, dev), tokens = make({r.S}, at::kInt, dev);
-  Tensor mean = make({r.S, r.E}, at::kFloat, dev), live = make({}, at::kInt, dev);
+  Together out{dev};
+  const int64_t at_loss = out.add(4), at_counts = out.add(4 * r.S * r.E), at_tokens = out.add(4 * r.S);
+  const int64_t at_mean = out.add(4 * r.S * r.E), at_live = out.add(4);
+  out.allocate();
+  Tensor loss = out.view(at_loss, {}, at::kFloat), counts = out.view(at_counts, {r.S, r.E}, at::kInt);
+  Tensor tokens = out.view(at_tokens, {r.S}, at::kInt), mean = out.view(at_mean, {r.S, r.E}, at::kFloat);
+  Tensor live = out.view(at_live, {}, at::kInt);
   const size_t need = moe_balance_workspace_bytes((int32_t)r.T, (int32_t)r.E, (int32_t)r.S);
   Tensor ws = make({(int64_t)need}, at::kByte, dev);
   MoeBalanceArgs a{};
@@ -388,7 +429,12 @@ Tensor balance_loss_backward(const Tensor& logits, const Tensor& idx, const OptT
   if (grad_loss) {
     if (grad_loss->numel() != 1 || grad_loss->scalar_type() != at::kFloat || grad_loss->device() != dev)
       refuse("grad_loss must be a number or one f32 value on the logits' device");
-    if (!counts || !tokens || !live) refuse("grad_loss needs what balance_loss returned");
+    if (!counts) refuse("grad_loss needs what balance_loss returned");
+    g = grad_loss->contiguous();
+    a.grad_loss = static_cast<const float*>(g.data_ptr());
+  }
+  if (counts) {
+    if (!tokens || !live) refuse("balance must be what balance_loss returned");
     check(*counts, "balance.counts", 2, {at::kInt}, dev);
     shape(*counts, "balance.counts", {r.S, r.E});
     check(*tokens, "balance.tokens", 1, {at::kInt}, dev);
@@ -397,11 +443,9 @@ Tensor balance_loss_backward(const Tensor& logits, const Tensor& idx, const OptT
     c = counts->contiguous();
     t = tokens->contiguous();
     l = live->contiguous();
-    g = grad_loss->contiguous();
     a.counts = static_cast<const int32_t*>(c.data_ptr());
     a.tokens = static_cast<const int32_t*>(t.data_ptr());
     a.sequences = static_cast<const int32_t*>(l.data_ptr());
-    a.grad_loss = static_cast<const float*>(g.data_ptr());
   }
   if (grad_weights) {
     check(*grad_weights, "grad_topk_weights", 2, {at::kFloat}, dev);
@@ -429,6 +473,7 @@ Tensor balance_loss_backward(const Tensor& logits, const Tensor& idx, const OptT
 
 PYBIND11_MODULE(moe_b200_layer, m) {
   m.def("linear", &linear);
+  m.def("linear_checkpointed", &linear_checkpointed);
   m.def("linear_backward", &linear_backward);
   m.def("checkpoint", &checkpoint);
   m.def("restore", &restore);

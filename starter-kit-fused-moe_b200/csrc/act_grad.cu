@@ -195,15 +195,15 @@ __global__ void __launch_bounds__(256, 2) act_grad_kernel(ActGradArgs a, int O) 
 // Sums of the chunks' column sums, 32 columns per block, 8 interleaved chunk
 // groups; fp64 because a long batch adds hundreds of chunks.
 __global__ void __launch_bounds__(256) colsum_finish_kernel(const float* __restrict__ colsum, int chunks, int n,
-                                                            void* __restrict__ out, int f32) {
+                                                            void* __restrict__ out, int f32, int early) {
   __shared__ double red[8][32];
-  pdl_wait();
+  if (!early) pdl_wait();
   pdl_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + tx;
   double t = 0.0;
   if (c < n)
-    for (int i = ty; i < chunks; i += 8) t += (double)colsum[(int64_t)i * n + c];
+    for (int i = ty; i < chunks; i += 8) t += (double)__ldcg(colsum + (int64_t)i * n + c);
   red[ty][tx] = t;
   __syncthreads();
   if (ty == 0 && c < n) {
@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(256) colsum_finish_kernel(const float* __restr
     if (f32) static_cast<float*>(out)[c] = (float)t;
     else static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn((float)t);
   }
+  if (early) pdl_wait();
 }
 
 int act_grad_chunks(int m, int) { return ceil_div(m, kAgRows); }
@@ -237,9 +238,10 @@ cudaError_t launch_act_grad(const ActGradArgs& a, cudaStream_t st) {
 #undef MOE_AG
 }
 
-cudaError_t launch_colsum_finish(const float* colsum, int chunks, int n, void* out, bool f32, cudaStream_t st) {
+cudaError_t launch_colsum_finish(const float* colsum, int chunks, int n, void* out, bool f32, bool early, cudaStream_t st) {
   if (n == 0) return cudaSuccess;
-  return launch_kernel(colsum_finish_kernel, dim3(ceil_div(n, 32)), dim3(256), 0, st, true, colsum, chunks, n, out, f32);
+  return launch_kernel(colsum_finish_kernel, dim3(ceil_div(n, 32)), dim3(256), 0, st, true, colsum, chunks, n, out, (int)f32,
+                       (int)early);
 }
 
 }  // namespace moe

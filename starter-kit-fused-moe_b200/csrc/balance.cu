@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_gr
   pdl_wait();
   pdl_trigger();
   const int b1 = (int)min((int64_t)(blockIdx.x + 1) * chunk, (int64_t)a.t);
-  const bool with_loss = a.grad_loss != nullptr;
-  const float g = with_loss ? __ldg(a.grad_loss) : 0.f;
+  const bool with_loss = a.counts != nullptr;
+  const float g = a.grad_loss != nullptr ? __ldg(a.grad_loss) : 1.f;
   const int live = with_loss ? __ldg(a.live) : 0;
   for (int pos = blockIdx.x * chunk; pos < b1;) {
     int end = b1;

@@ -20,10 +20,12 @@
 // chain drifts: 8e-6 of the result's norm at K = 7168, 2e-6 at 2048, 5e-7 at
 // 512, where an fp32 product has 9e-7. A bf16 result (2^-8) does not show that,
 // an fp32 one does, and so does a kept pre-activation (one value in 10^4 moves to
-// the next e4m3 step). For those (CHAIN) the chain is cut every 16 (fp32) or 24
-// (kept) K-blocks of 64: the epilogue warps add each partial accumulator to fp32
-// registers, rounding to nearest, while the tensor core fills the other one. The
-// reads of TMEM cost the tensor core about a K-block each, 10 % and 4 %.
+// the next e4m3 step). For those (CHAIN) the chain is cut every 16 K-blocks of 64
+// (fp32), 6 (fp32 gated, where both factors drift the same way: 1.7e-6 at K = 768
+// with 16, 9e-7 with 8) or 12 (kept): the epilogue warps add each partial
+// accumulator to fp32 registers, rounding to nearest, while the tensor core fills
+// the other one. The reads of TMEM cost the tensor core about a K-block each: 217
+// instead of 210 us with 24 for the checkpointed product of 4096 x 7168 x 4096.
 //
 // Warps: 0 TMA producer, 1 MMA issuer (the leader CTA's), 4-11 epilogue. The two
 // accumulators of NT columns in TMEM also let a tile's epilogue overlap the next
@@ -35,10 +37,10 @@
 // partial tiles in the workspace and a second kernel, launched to start as this
 // one ends, adds them in slice order and runs the epilogue on all SMs. (Letting
 // the slice that arrives last do it kept the other SMs idle: 36 instead of 20 us
-// at 1037 x 1111 x 515.) Outputs whose rows 16-byte accesses cannot reach take
-// that way for every tile: the second kernel reaches any column with whole
-// warps, while a lane holding a row of the tile stores element by element (215
-// instead of 60 us for a kept 1911 x 594 x 5181 product).
+// at 1037 x 1111 x 515.) With a kept pre-activation, outputs whose rows 16-byte
+// accesses cannot reach take that way for every tile: the second kernel reaches
+// any column with whole warps, while a lane holding a row of the tile stores
+// element by element (215 instead of 60 us for a 1911 x 594 x 5181 product).
 //
 // Every wait is bounded (2 s). One that runs out makes the kernel write NaN to
 // the tiles it still owes, so a failed call never returns plausible numbers; the
@@ -166,6 +168,7 @@ __device__ __forceinline__ void lt_place(const LinearTileArgs& a, int64_t tile, 
   nt = in / rows;
   mt = band * kLtBand + in - nt * rows;
 }
+template <bool FLIP>
 __device__ __forceinline__ LtUnit lt_unit(const LinearTileArgs& a, int64_t u) {
   LtUnit r;
   if (u < a.full_tiles) {
@@ -180,7 +183,12 @@ __device__ __forceinline__ LtUnit lt_unit(const LinearTileArgs& a, int64_t u) {
     r.kb0 = (int)((int64_t)r.slice * a.k_blocks / a.splits);
     r.kb1 = (int)((int64_t)(r.slice + 1) * a.k_blocks / a.splits);
   }
-  lt_place(a, r.tile, r.mt, r.nt);
+  if constexpr (FLIP) {
+    r.mt = (int)r.tile;
+    r.nt = 0;
+  } else {
+    lt_place(a, r.tile, r.mt, r.nt);
+  }
   return r;
 }
 
@@ -271,6 +279,40 @@ __device__ __forceinline__ void lt_copy_f32(const uint8_t* box, float* dst, int6
   }
   __syncwarp();
 }
+// The same for rows that 16-byte accesses cannot reach: a row of the box per
+// store, a column per lane, the residual read the same way. Eight rows at a
+// time: all 32 at once made the loop's code too long for its few passes (a 128 x
+// 480 x 340 product 9.1 instead of 7.3 us).
+__device__ __forceinline__ void lt_copy_rows(const uint8_t* box, const LinearEpilogue& ep, int64_t row0, int64_t c, int rows,
+                                             int64_t cols, int lane) {
+  __syncwarp();
+  const bool in = lane < cols;
+  const __nv_bfloat16* res = static_cast<const __nv_bfloat16*>(ep.residual) + row0 * ep.ldr + c + lane;
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + i;
+      v[i] = *reinterpret_cast<const float*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+    }
+    if (ep.residual != nullptr) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = in && r0 + i < rows ? __bfloat162float(res[(r0 + i) * ep.ldr]) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += f[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!in || r0 + i >= rows) continue;
+      const int64_t at = (row0 + r0 + i) * ep.ldy + c + lane;
+      if (ep.y_f32) static_cast<float*>(ep.y)[at] = v[i];
+      else static_cast<__nv_bfloat16*>(ep.y)[at] = __float2bfloat16_rn(v[i]);
+    }
+  }
+  __syncwarp();
+}
 __device__ __forceinline__ uint4* lt_bf16_piece(uint8_t* box, int i, int lane) {             // 64-byte swizzle
   return reinterpret_cast<uint4*>(box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4));
 }
@@ -320,7 +362,7 @@ __device__ __forceinline__ void lt_store_z32(uint8_t* z, int64_t c, int64_t end,
   if (c + 32 <= end) *reinterpret_cast<uint4*>(z + c + 16) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-template <bool A_MN, bool B_MN, bool GATED, bool KEEP, bool CHAIN>
+template <bool A_MN, bool B_MN, bool GATED, bool KEEP, bool CHAIN, bool FLIP>
 __global__ void __launch_bounds__(kLtThreads, 1)
     linear_tile_kernel(const __grid_constant__ LinearTileMaps maps, const LinearTileArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -360,7 +402,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
   __syncthreads();
   cluster_sync_all();
   tc_fence_after();
-  pdl_wait();
+  if (!a.early) pdl_wait();
   pdl_trigger();
   const uint32_t tmem_base = S.tmem_base;
   volatile int* abort_flag = &S.abort_flag;
@@ -377,11 +419,11 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       const uint32_t leader0 = mapa_shared(full0, 0);      // both CTAs' loads complete on the leader's barriers
       const int k_end = a.term_blocks * 64;
       for (int64_t u = wid; u < a.units && ok && !__shfl_sync(0xffffffffu, *abort_flag, 0); u += G) {
-        const LtUnit x = lt_unit(a, u);
-        const int m0 = x.mt * 256 + crank * 128;
+        const LtUnit x = lt_unit<FLIP>(a, u);
+        const int m0 = FLIP && GATED ? crank * a.gate_rows + x.mt * 128 : x.mt * 256 + crank * 128;
         // B rows of this CTA's half: the next H columns of the tile, or for a gated tile its first-half
         // (leader) and second-half (peer) rows
-        const int n0 = GATED ? crank * a.gate_rows + x.nt * H : x.nt * NT + crank * H;
+        const int n0 = GATED && !FLIP ? crank * a.gate_rows + x.nt * H : x.nt * NT + crank * H;
         // the small terms first: the chain's truncation is relative to the running sum
         int term = a.terms - 1 - x.kb0 / a.term_blocks;
         int kt = (x.kb0 % a.term_blocks) * 64;
@@ -431,7 +473,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       const uint64_t a0 = A_MN ? sdesc_sw128_mn(smem_u32(smem)) : sdesc_sw128(smem_u32(smem));
       const uint64_t b0 = B_MN ? sdesc_sw128_mn(smem_u32(smem) + kLtTileA) : sdesc_sw128(smem_u32(smem) + kLtTileA);
       for (int64_t u = wid; u < a.units && ok && !__shfl_sync(0xffffffffu, *abort_flag, 0); u += G) {
-        const LtUnit x = lt_unit(a, u);
+        const LtUnit x = lt_unit<FLIP>(a, u);
         for (int kb = x.kb0; kb < x.kb1 && ok; ++tt) {
           const int b = tt & 1, end = CHAIN ? min(kb + a.chain, x.kb1) : x.kb1;
           if (!warp_wait(smem_u32(&S.tempty[b]), ((tt >> 1) & 1) ^ 1)) {
@@ -479,13 +521,13 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     uint8_t* stage = staging + ew * kLtStaging;
     const uint32_t stage_addr = smem_u32(stage);
     // y as bf16 in whole boxes with a residual: the residual's boxes are fetched into the boxes y leaves from
-    const bool res_boxes = ep.residual != nullptr && !ep.y_f32;
+    const bool res_boxes = ep.residual != nullptr && !ep.y_f32 && a.vec;
     constexpr int CHUNKS_H = GATED ? 4 : 2;              // this warp's columns: NT / CHUNKS_H
     bool ok = true, res_ok = true;
     int tt = 0;
     uint32_t res_count = 0;                              // residual boxes waited for
     for (int64_t u = wid; u < a.units; u += G) {
-      const LtUnit x = lt_unit(a, u);
+      const LtUnit x = lt_unit<FLIP>(a, u);
       const int64_t row0 = (int64_t)x.mt * 256 + crank * 128 + 32 * q, row = row0 + lane;
       const bool valid = row < a.m;
       const int warp_rows = (int)max((int64_t)0, min((int64_t)32, a.m - row0));
@@ -567,6 +609,21 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       } else {
         wait_acc();
       }
+      if constexpr (FLIP) {                              // always a slice: fp32 [token][column], a lane holds a column
+        const int first = g * H;                         // of this warp's tokens
+        float* dst = a.partial + ((x.tile * a.splits + x.slice) * NT + first) * 256 + crank * 128 + r;
+        const int tokens = (int)min((int64_t)H, a.m - first);
+#pragma unroll 1
+        for (int i = 0; i < tokens; i += 32) {
+          float v[32];
+          from_tmem(first + i, v);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (i + e < tokens) __stcg(dst + (i + e) * 256, v[e]);
+        }
+        release();
+        continue;
+      }
       if (x.slice >= 0) {                                // fp32 partial tile, [row][column]
         if (warp_rows > 0) {
           const int64_t y0 = ((x.tile - a.full_tiles) * a.splits + x.slice) * 256 + crank * 128 + 32 * q;
@@ -592,7 +649,10 @@ __global__ void __launch_bounds__(kLtThreads, 1)
       // y's columns [c0 + 32 j, + 32)
       auto store = [&](int j, float* v) {
         const int64_t c = c0 + 32 * j;
-        if (ep.y_f32) {
+        if (!KEEP && !a.vec) {
+          lt_stage_f32(stage, v, lane);
+          lt_copy_rows(stage, ep, row0, c, warp_rows, O - c, lane);
+        } else if (ep.y_f32) {
           if (ep.residual != nullptr && valid) {
             const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(ep.residual) + row * ep.ldr;
             lt_bias32(r, c, O, v);
@@ -760,20 +820,15 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kLtTmemCols) : "memory");
   }
+  if (a.early) pdl_wait();
 }
 
 // A warp takes 512 columns of a row, as 4-byte words: where the row starts at an
 // odd element, a word's halves come from two neighbouring aligned words (the
-// second one from L1). Words that reach past the row are read in halves.
-__device__ __forceinline__ uint32_t pad_word(const uint16_t* row, int first, int cols) {   // elements first, first + 1
-  if (first >= 0 && first + 1 < cols) return __ldg(reinterpret_cast<const uint32_t*>(row + first));
-  uint32_t v = 0;
-  if (first >= 0 && first < cols) v = __ldg(row + first);
-  if (first + 1 >= 0 && first + 1 < cols) v |= (uint32_t)__ldg(row + first + 1) << 16;
-  return v;
-}
+// second one from L1, or from L2 in an early launch). Words that reach past the row are read in halves.
+template <bool EARLY>
 __global__ void __launch_bounds__(256) pad_kernel(PadArgs a) {
-  pdl_wait();
+  if (!EARLY) pdl_wait();
   pdl_trigger();
   const int j = blockIdx.z, lane = threadIdx.x & 31, w0 = 256 * blockIdx.y + lane, cols = a.cols[j];
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < a.rows[j]; row += (int64_t)gridDim.x * 8) {
@@ -784,8 +839,8 @@ __global__ void __launch_bounds__(256) pad_kernel(PadArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int c = 2 * (w0 + 32 * e);
-      v[e] = pad_word(s, odd ? c - 1 : c, cols);
-      if (odd) u[e] = pad_word(s, c + 1, cols);
+      v[e] = load_pair<EARLY>(s, odd ? c - 1 : c, 0, cols);
+      if (odd) u[e] = load_pair<EARLY>(s, c + 1, 0, cols);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -793,6 +848,7 @@ __global__ void __launch_bounds__(256) pad_kernel(PadArgs a) {
       if (c < cols) d[w0 + 32 * e] = odd ? v[e] >> 16 | u[e] << 16 : v[e];
     }
   }
+  if (EARLY) pdl_wait();
 }
 cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
   if (a.count == 0) return cudaSuccess;
@@ -805,7 +861,9 @@ cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
   const int segments = (cols + 511) / 512;                 // cols <= 2^23
   int64_t blocks = (rows + 7) / 8;
   if (blocks * segments > 148 * 32) blocks = (148 * 32 + segments - 1) / segments;
-  return launch_kernel(pad_kernel, dim3((unsigned)blocks, segments, a.count), dim3(256), 0, st, true, a);
+  const dim3 grid((unsigned)blocks, segments, a.count);
+  return a.early ? launch_kernel(pad_kernel<true>, grid, dim3(256), 0, st, true, a)
+                 : launch_kernel(pad_kernel<false>, grid, dim3(256), 0, st, true, a);
 }
 
 // Adds the K slices' partial rows in slice order and runs the epilogue. A warp
@@ -816,20 +874,23 @@ cudaError_t launch_pad(const PadArgs& a, cudaStream_t st) {
 template <bool GATED, bool KEEP, bool VEC, int R>
 __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
   const int lane = threadIdx.x & 31;
-  pdl_wait();
+  if (!a.join_early) pdl_wait();
   pdl_trigger();
-  const int H = GATED ? a.n_tile / 2 : a.n_tile, col_blocks = (H + 127) / 128;
-  const uint32_t per_tile = 256 / (8 * R) * col_blocks;                    // blocks of 8 R rows and 128 columns
+  const int cols = a.flip ? 256 : a.n_tile, H = GATED ? cols / 2 : cols, col_blocks = (H + 127) / 128;
+  const uint32_t per_tile = a.tile_rows / (8 * R) * col_blocks;                    // blocks of 8 R rows and 128 columns
   const uint32_t i = blockIdx.x / per_tile, in = blockIdx.x - i * per_tile;
   const int r0 = (int)(in / col_blocks) * 8 * R + (threadIdx.x >> 5) * R, cb = (int)(in % col_blocks);
   int mt, nt;
   lt_place(a, a.full_tiles + i, mt, nt);
   const int64_t row0 = (int64_t)mt * 256 + r0;
   const int64_t O = a.out_cols, c0 = (int64_t)nt * H + 128 * cb;          // the warp's first column
-  if (row0 >= a.m || c0 >= O) return;                                     // warp-uniform
+  if (row0 >= a.m || c0 >= O) {                                           // warp-uniform
+    if (a.join_early) pdl_wait();
+    return;
+  }
   const int rows = (int)min((int64_t)R, a.m - row0);
   const int width = (int)min((int64_t)min(128, H - 128 * cb), O - c0);    // its columns
-  const int64_t kb = c0 / 128, blocks = (O + 127) / 128, step = (int64_t)256 * a.n_tile;
+  const int64_t kb = c0 / 128, blocks = (O + 127) / 128, step = (int64_t)a.tile_rows * cols;
   const LinearEpilogue& ep = a.ep;
   const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(ep.bias);
   auto col = [&](int j) { return VEC ? 4 * lane + j : lane + 32 * j; };
@@ -839,7 +900,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
   for (int h = 0; h < HALVES; ++h)
 #pragma unroll
     for (int j = 0; j < 4; ++j) b[h][j] = bias && col(j) < width ? __bfloat162float(bias[h * O + c0 + col(j)]) : 0.f;
-  const float* tile = a.partial + (int64_t)i * a.splits * step + (int64_t)r0 * a.n_tile + 128 * cb;
+  const float* tile = a.partial + (int64_t)i * a.splits * step + (int64_t)r0 * cols + 128 * cb;
 #pragma unroll 1
   for (int rb = 0; rb < rows; rb += U) {
     float v[U][HALVES][4];
@@ -856,7 +917,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
           if (rb + u >= rows) continue;
-          const float* q = tile + s * step + (int64_t)(rb + u) * a.n_tile + h * H;
+          const float* q = tile + s * step + (int64_t)(rb + u) * cols + h * H;
           if constexpr (VEC) {
             if (col(0) >= width) continue;                                // a tile's width is a multiple of 32
             const float4 f = __ldcg(reinterpret_cast<const float4*>(q) + lane);
@@ -932,15 +993,16 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
         }
     }
   }
+  if (a.join_early) pdl_wait();
 }
 
 template <bool GATED, bool KEEP>
 static cudaError_t launch_join(const LinearTileArgs& a, cudaStream_t st) {
-  const int64_t tail = (a.units - a.full_tiles) / a.splits, H = GATED ? a.n_tile / 2 : a.n_tile;
-  const int64_t col_blocks = (H + 127) / 128, rows = a.m < 256 ? a.m : 256;
+  const int64_t tail = (a.units - a.full_tiles) / a.splits, cols = a.flip ? 256 : a.n_tile;
+  const int64_t col_blocks = ((GATED ? cols / 2 : cols) + 127) / 128, rows = a.m < a.tile_rows ? a.m : a.tile_rows;
   // 8 rows per warp once that leaves 16 warps per SM, else one
   const bool many = tail * col_blocks * rows / 8 >= 148 * 16;
-  const dim3 grid((unsigned)(tail * col_blocks * (many ? 4 : 32))), block(256);
+  const dim3 grid((unsigned)(tail * col_blocks * (a.tile_rows / (many ? 64 : 8)))), block(256);
 #define MOE_JOIN(V, R) launch_kernel(linear_join_kernel<GATED, KEEP, V, R>, grid, block, 0, st, true, a)
   if (many) return a.vec ? MOE_JOIN(true, 8) : MOE_JOIN(false, 8);
   return a.vec ? MOE_JOIN(true, 1) : MOE_JOIN(false, 1);
@@ -950,45 +1012,76 @@ static cudaError_t launch_join(const LinearTileArgs& a, cudaStream_t st) {
 // Tile width and K slices of the last, partial round. Cycles per 64 of K and
 // pair, measured: 2.1 NT for a pair alone (the MMA), 174 + 2.3 NT with all pairs
 // at work (758 at NT = 256, 590 at 192, 466 at 128), and no less than the
-// operands' way from HBM (3.4 KB per cycle); 800 for a change of tile. A tile's epilogue hides behind the
-// next tile's products except for the last one. Slices are at least 4 K-blocks
-// deep; joining them costs a launch and moves 8 bytes per value and slice
-// through L2 (about 3 KB per cycle).
-LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gated, bool keep, bool b_mn, bool direct,
-                                int pairs) {
+// operands' way from HBM (3.4 KB per cycle); 800 for a change of tile. A tile's
+// epilogue hides behind the next tile's products except for the last one, which
+// is long where rows are written element-wise. (Joining the one tile of a small
+// product whose pre-activation is kept, 64 x 256 x 256 with gelu, takes 9.1 instead
+// of 14.5 us on the device, but one launch more costs a host-bound step more: 25.7
+// instead of 21.7 us with the checkpoint and both restores.)
+// Slices are at least 4 K-blocks deep; joining them costs a launch and moves 8
+// bytes per value and slice through L2 (about 3 KB per cycle).
+LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gated, bool grad, bool vec,
+                                const LinearEpilogue& ep, int pairs) {
   LinearTilePlan best{};
   double best_cost = 1e300;
+  const bool keep = ep.z8 != nullptr;
   const int64_t mt = (m + 255) / 256;
   const double hbm = 128.0 * k_blocks * (m + (gated ? 2 : 1) * n) / 3400;
+  // the last tile's epilogue, cycles per column of the tile
+  const double last = keep ? 20 : vec ? 12 : ep.residual ? 80 : ep.y_f32 ? 45 : 20;
   static const int widths[] = {256, 192, 128, 64};
   for (int nt : widths) {
     if (keep && nt != 256) continue;
-    if ((gated || b_mn) && nt % 128) continue;       // epilogue warps take 32 columns; boxes of 64
+    if ((gated || grad) && nt % 128) continue;       // epilogue warps take 32 columns; boxes of 64
     const int64_t cols = gated ? nt / 2 : nt;
-    const int64_t tiles = mt * ((n + cols - 1) / cols), tail = direct ? tiles % pairs : tiles, full = tiles - tail;
+    const int64_t tiles = mt * ((n + cols - 1) / cols);
     const double alone = 2.1 * nt, crowded = 174 + 2.3 * nt;
     const double rows = m < 256 ? m : 256;
-    for (int s = 1; s <= 16; ++s) {
-      if (s > 1 && (tail == 0 || k_blocks < 4 * s)) break;
-      const int64_t units = tail * s, rounds = (units + pairs - 1) / pairs;
+    for (int s = 0; s <= 16; ++s) {                  // 0: every tile whole
+      if (s == 0 && keep && !vec) continue;
+      const int64_t tail = s == 0 ? tiles % pairs : keep && !vec ? tiles : tiles % pairs, full = tiles - tail;
+      const int slices = s ? s : 1;
+      if (s > 0 && tail == 0) break;
+      if (s > 1 && k_blocks < 4 * s) break;
+      const int64_t units = tail * slices, rounds = (units + pairs - 1) / pairs;
       const double busy = units < pairs ? (double)units / pairs : 1.0;
       double cost = (double)(full / pairs) * (k_blocks * crowded + 800) +
-                    (double)rounds * ((k_blocks + s - 1) / s * (alone + busy * (crowded - alone)) + 800);
-      const bool join = s > 1 || !direct;
-      cost = (cost > hbm ? cost : hbm) + 1500 + 12.0 * nt + (join ? 4000 + 8.0 * s * tail * rows * nt / 3000 : 0);
+                    (double)rounds * ((k_blocks + slices - 1) / slices * (alone + busy * (crowded - alone)) + 800);
+      cost = (cost > hbm ? cost : hbm) + 1500 + (s ? 12 * nt + 4000 + 8.0 * s * tail * rows * nt / 3000 : last * nt);
       if (cost < best_cost) {
         best_cost = cost;
-        best = {nt, s, join ? full : tiles, join ? tail : 0};
+        best = {nt, slices, 0, s ? full : tiles, s ? tail : 0};
+      }
+    }
+  }
+  // Few tokens and a long contraction: the weights' rows become the tile's, which pads 64 or 128 columns instead of 256
+  // rows. At 64 (128) tokens and K = 7168 18.4 (18.5) instead of 19.6 (22.8) us for N = 4096 gated, 26.5 (27.8) instead
+  // of 29.2 (29.5) for N = 7168, 10.4 (11.1) instead of 12.1 (11.9) for N = 256 in fp32; at K = 4096 equal, at
+  // K = 2048 14.1 instead of 11.5, because a flipped tile always needs the join.
+  if (m <= 128 && k_blocks >= 96 && !keep && !grad) {
+    best_cost = 1e300;
+    const int nt = m <= 64 ? 64 : 128;
+    const int64_t tail = (n + (gated ? 127 : 255)) / (gated ? 128 : 256);
+    for (int s = 1; s <= 16; ++s) {
+      const int64_t depth = (k_blocks + s - 1) / s;
+      if (s > 1 && k_blocks < 4 * s) break;
+      if (ep.y_f32 && depth > linear_chain(gated, true)) continue;               // longer chains drift
+      const int64_t units = tail * s, rounds = (units + pairs - 1) / pairs;
+      double cost = (double)rounds * (depth * (200.0 + 1.4 * nt) + 800);
+      cost = (cost > hbm ? cost : hbm) + 1500 + 12.0 * nt + 4000 + 8.0 * s * tail * m * 256 / 3000;
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = {nt, s, 1, 0, tail};
       }
     }
   }
   return best;
 }
 
-template <bool A_MN, bool B_MN, bool GATED, bool KEEP, bool CHAIN>
+template <bool A_MN, bool B_MN, bool GATED, bool KEEP, bool CHAIN, bool FLIP = false>
 static cudaError_t launch_c(const LinearTileMaps& maps, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
   static int clusters_of[64];
-  auto kern = linear_tile_kernel<A_MN, B_MN, GATED, KEEP, CHAIN>;
+  auto kern = linear_tile_kernel<A_MN, B_MN, GATED, KEEP, CHAIN, FLIP>;
   int dev = 0;
   cudaGetDevice(&dev);
   cudaLaunchConfig_t cfg = {};
@@ -1030,6 +1123,8 @@ static cudaError_t launch_t(const LinearTileMaps& maps, const LinearTileArgs& a,
 
 static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
                                   const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+  if (a.flip) return gated ? launch_c<false, false, true, false, false, true>(maps, a, num_sms, st)
+                           : launch_c<false, false, false, false, false, true>(maps, a, num_sms, st);
   if (a_mn && b_mn) return launch_t<true, true, false, false>(maps, a, num_sms, st);
   if (b_mn) return launch_t<false, true, false, false>(maps, a, num_sms, st);
   if (gated) return keep ? launch_t<false, false, true, true>(maps, a, num_sms, st)
@@ -1040,8 +1135,11 @@ static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, c
 
 cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
                                const LinearTileArgs& a, int num_sms, cudaStream_t st) {
-  cudaError_t e = launch_product(a_mn, b_mn, gated, keep, maps, a, num_sms, st);
-  if (e != cudaSuccess || a.units == a.full_tiles) return e;
+  return launch_product(a_mn, b_mn, gated, keep, maps, a, num_sms, st);
+}
+
+cudaError_t launch_linear_join(bool gated, bool keep, const LinearTileArgs& a, cudaStream_t st) {
+  if (a.units == a.full_tiles) return cudaSuccess;
   if (gated) return keep ? launch_join<true, true>(a, st) : launch_join<true, false>(a, st);
   return keep ? launch_join<false, true>(a, st) : launch_join<false, false>(a, st);
 }

@@ -51,54 +51,63 @@ bool tma_ready(const void* p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0
 // One tensor-core product: its tile plan and the workspace of its K slices.
 struct Product {
   moe::LinearTilePlan plan;
-  bool direct;
+  bool vec;
   int64_t term_blocks;
   int terms;
   size_t partial;      // bytes
 };
 // Whether 16-byte accesses reach every row of y, the residual and the kept z.
-bool direct_rows(const moe::LinearEpilogue& ep, int64_t out_cols) {
+bool vec_rows(const moe::LinearEpilogue& ep, int64_t out_cols) {
   return aligned(ep.y, 16) && ep.ldy * (ep.y_f32 ? 4 : 2) % 16 == 0 &&
          (!ep.residual || (aligned(ep.residual, 16) && ep.ldr % 8 == 0 && ep.ldr > 0)) &&
          (!ep.z8 || (aligned(ep.z8, 16) && out_cols % 16 == 0));
 }
-Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gated, const moe::LinearEpilogue& ep, bool b_mn) {
+Product plan_product(int64_t m, int64_t out_cols, int64_t k, int terms, bool gated, const moe::LinearEpilogue& ep, bool grad) {
   Product p{};
-  p.direct = direct_rows(ep, out_cols);
+  p.vec = vec_rows(ep, out_cols);
   p.term_blocks = (k + 63) / 64;
   p.terms = terms;
-  p.plan = moe::plan_linear_tile(m, out_cols, p.term_blocks * terms, gated, ep.z8 != nullptr, b_mn, p.direct, pairs());
+  p.plan = moe::plan_linear_tile(m, out_cols, p.term_blocks * terms, gated, grad, p.vec, ep, pairs());
   p.partial = (size_t)p.plan.tail * p.plan.splits * 256 * p.plan.n_tile * sizeof(float);
   return p;
 }
-// A: [terms][rows][..], term stride in elements.
+// A: [terms][rows][..], term stride in elements. `t` is left for the join.
 int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, int64_t m, int64_t out_cols, int64_t k,
                 const void* A, int64_t lda, int64_t term_stride, const void* B, int64_t ldb, int64_t b_rows,
-                const moe::LinearEpilogue& ep, uint8_t* partial, cudaStream_t st, const char* what) {
-  moe::LinearTileArgs t{};
+                const moe::LinearEpilogue& ep, uint8_t* partial, bool early, cudaStream_t st, const char* what,
+                moe::LinearTileArgs& t) {
+  t = {};
+  t.early = early;
   t.m = m;
   t.out_cols = out_cols;
   t.gate_rows = gated ? (int)out_cols : 0;
   t.n_tile = p.plan.n_tile;
-  const int cols = gated ? t.n_tile / 2 : t.n_tile;
-  t.m_tiles = moe::ceil_div(m, 256);
+  t.flip = p.plan.flip;
+  t.tile_rows = t.flip ? t.n_tile : 256;
+  const int width = t.flip ? 256 : t.n_tile, cols = gated ? width / 2 : width;
+  t.m_tiles = moe::ceil_div(m, t.tile_rows);
   t.n_tiles = moe::ceil_div(out_cols, cols);
   t.term_blocks = (int)p.term_blocks;
   t.terms = p.terms;
   t.k_blocks = t.term_blocks * p.terms;
   t.splits = p.plan.splits;
-  t.chain = ep.y_f32 ? 16 : 24;
+  t.chain = moe::linear_chain(gated, ep.y_f32);
   t.full_tiles = p.plan.full;
   t.units = p.plan.full + p.plan.tail * t.splits;
   t.ep = ep;
-  t.vec = p.direct;
+  t.vec = p.vec;
   t.partial = reinterpret_cast<float*>(partial);
   moe::LinearTileMaps maps{};
   const uint32_t half = (uint32_t)t.n_tile / 2;
-  bool ok = (a_mn ? moe::encode_bf16(&maps.a, A, m, k, lda, p.terms, term_stride, 64, 64)
-                  : moe::encode_bf16(&maps.a, A, k, m, lda, p.terms, term_stride, 64, 128)) &&
-            (b_mn ? moe::encode_bf16(&maps.b, B, out_cols, k, ldb, 0, 0, 64, 64)
-                  : moe::encode_bf16(&maps.b, B, k, b_rows, ldb, 0, 0, 64, half));
+  bool ok;
+  if (t.flip)      // the weights' rows are the tile's, the tokens its columns
+    ok = moe::encode_bf16(&maps.a, B, k, b_rows, ldb, 1, b_rows * ldb, 64, 128) &&
+         moe::encode_bf16(&maps.b, A, k, m, lda, 0, 0, 64, half);
+  else
+    ok = (a_mn ? moe::encode_bf16(&maps.a, A, m, k, lda, p.terms, term_stride, 64, 64)
+               : moe::encode_bf16(&maps.a, A, k, m, lda, p.terms, term_stride, 64, 128)) &&
+         (b_mn ? moe::encode_bf16(&maps.b, B, out_cols, k, ldb, 0, 0, 64, 64)
+               : moe::encode_bf16(&maps.b, B, k, b_rows, ldb, 0, 0, 64, half));
   if (t.vec && !ep.y_f32 && t.full_tiles > 0) {
     ok = ok && moe::encode_bf16(&maps.out, ep.y, out_cols, m, ep.ldy, 0, 0, 32, 32);
     if (ep.residual) ok = ok && moe::encode_bf16(&maps.res, ep.residual, out_cols, m, ep.ldr, 0, 0, 32, 32);
@@ -126,7 +135,7 @@ moe::LinearEpilogue plain_epilogue(void* y, int64_t ldy, int f32) {
 }
 LinearPlan linear_plan(const MoeLinearArgs& a) {
   LinearPlan p{};
-  p.small = a.m <= moe::kSmallTokens && a.z8 == nullptr;
+  p.small = a.z8 == nullptr && moe::small_product(a.m, a.k, a.n);
   if (p.small) return p;
   const bool gated = a.activation == MOE_ACT_SWIGLU;
   p.prod = plan_product(a.m, gated ? a.n / 2 : a.n, a.k, 1, gated, epilogue_of(a), false);
@@ -142,13 +151,13 @@ LinearPlan linear_plan(const MoeLinearArgs& a) {
   return p;
 }
 
-// Workspace of the gradient entry: K-slice partials (shared by the products), dz, x^, the padded weights, column sums.
+// Workspace of the gradient entry: the products' K-slice partials, dz, x^, the padded weights, column sums.
 struct GradPlan {
   bool need_dz, direct, pad_w;
   int terms, chunks;
   int64_t ldz, ldk;
   Product px, pw;
-  size_t dz, xhat, w, colsum, total;      // the partials come first
+  size_t part_w, dz, xhat, w, colsum, total;      // the input gradient's partials come first
 };
 GradPlan grad_plan(const MoeLinearGradArgs& a) {
   GradPlan p{};
@@ -159,17 +168,17 @@ GradPlan grad_plan(const MoeLinearGradArgs& a) {
   p.direct = a.activation == MOE_ACT_NONE && !a.grad_y_f32 && tma_ready(a.grad_y, a.ldg) && a.ldg >= a.n;
   p.need_dz = (a.grad_x || a.grad_weight) && !p.direct;
   p.chunks = moe::act_grad_chunks(a.m, a.n);
-  size_t partial = 0;
+  size_t o = 0;
   if (a.grad_x) {
     p.px = plan_product(a.m, a.k, a.n, p.terms, false, plain_epilogue(a.grad_x, a.k, a.grad_f32), true);
-    partial = p.px.partial;
+    o = up256(p.px.partial);
     p.pad_w = !tma_ready(a.weight, a.ldw);
   }
+  p.part_w = o;
   if (a.grad_weight) {
     p.pw = plan_product(a.n, a.k, a.m, p.terms, false, plain_epilogue(a.grad_weight, a.k, a.grad_f32), true);
-    if (p.pw.partial > partial) partial = p.pw.partial;
+    o += up256(p.pw.partial);
   }
-  size_t o = up256(partial);
   p.dz = o;
   if (p.need_dz) o += up256((size_t)a.m * p.ldz * 2 * p.terms);
   p.xhat = o;
@@ -220,8 +229,12 @@ int moe_linear_run(const MoeLinearArgs* a, void* stream) {
   const void* x = p.pad_x ? ws + p.x : a->x;
   const void* w = p.pad_w ? ws + p.w : a->weight;
   const int64_t ldx = p.pad_x ? p.ldp : a->ldx;
-  return run_product(p.prod, false, false, a->activation == MOE_ACT_SWIGLU, a->z8 != nullptr, a->m, O, a->k, x, ldx,
-                     a->m * ldx, w, p.pad_w ? p.ldp : a->ldw, a->n, ep, ws, st, "linear product");
+  const bool gated = a->activation == MOE_ACT_SWIGLU, keep = a->z8 != nullptr;
+  moe::LinearTileArgs t;
+  if (int rc = run_product(p.prod, false, false, gated, keep, a->m, O, a->k, x, ldx, a->m * ldx, w,
+                           p.pad_w ? p.ldp : a->ldw, a->n, ep, ws, false, st, "linear product", t))
+    return rc;
+  return done(moe::launch_linear_join(gated, keep, t, st), "linear product");
 }
 
 size_t moe_linear_grad_workspace_bytes(const MoeLinearGradArgs* a) {
@@ -255,11 +268,10 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
   if (p.total && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < p.total))
     return workspace_error("linear gradient", p.total, a->workspace_bytes);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  // Three steps: what the products need, the products, what finishes them. A step's kernels run side by side (the
+  // first of them waits for the step before, see train_kernels.h).
   cudaError_t e = cudaSuccess;
-  moe::PadArgs pads{};
-  if (p.pad_w) pads.add(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldk);
-  e = moe::launch_pad(pads, st);
-  if (e != cudaSuccess) return done(e, "linear gradient: preparing the operands");
+  bool begun = false;
   if (p.need_dz || a->grad_bias) {
     moe::ActGradArgs g{};
     g.dy = a->grad_y;
@@ -275,29 +287,47 @@ int moe_linear_grad(const MoeLinearGradArgs* a, void* stream) {
     g.dy_f32 = a->grad_y_f32;
     g.terms = p.terms;
     e = moe::launch_act_grad(g, st);
-    if (e == cudaSuccess && a->grad_bias)
-      e = moe::launch_colsum_finish(g.colsum, p.chunks, a->n, a->grad_bias, a->grad_f32 != 0, st);
     if (e != cudaSuccess) return done(e, "activation gradient");
+    begun = true;
+  }
+  if (a->grad_weight) {
+    e = moe::launch_restore_rows(static_cast<const uint8_t*>(a->x8), static_cast<const uint8_t*>(a->x_scale), a->m, a->k,
+                                 ws + p.xhat, p.ldk, begun, st);
+    if (e != cudaSuccess) return done(e, "restoring the input checkpoint");
+    begun = true;
+  }
+  if (p.pad_w) {
+    moe::PadArgs pads{};
+    pads.early = begun;
+    pads.add(a->weight, a->ldw, a->n, a->k, ws + p.w, p.ldk);
+    e = moe::launch_pad(pads, st);
+    if (e != cudaSuccess) return done(e, "linear gradient: preparing the operands");
   }
   const void* dz = p.direct ? a->grad_y : ws + p.dz;
   const int64_t ldz = p.direct ? a->ldg : p.ldz, term_stride = a->m * ldz;
+  moe::LinearTileArgs tx{}, tw{};
   if (a->grad_x) {
     const void* w = p.pad_w ? ws + p.w : a->weight;
     const int64_t ldw = p.pad_w ? p.ldk : a->ldw;
     const moe::LinearEpilogue ep = plain_epilogue(a->grad_x, a->k, a->grad_f32);
     if (int rc = run_product(p.px, false, true, false, false, a->m, a->k, a->n, dz, ldz, term_stride, w, ldw, a->n, ep,
-                             ws, st, "input gradient"))
+                             ws, false, st, "input gradient", tx))
       return rc;
   }
   if (a->grad_weight) {
-    e = moe::launch_restore(static_cast<const uint8_t*>(a->x8), static_cast<const uint8_t*>(a->x_scale), 1, a->m, a->k,
-                            ws + p.xhat, false, p.ldk, st);
-    if (e != cudaSuccess) return done(e, "restoring the input checkpoint");
     const moe::LinearEpilogue ep = plain_epilogue(a->grad_weight, a->k, a->grad_f32);
     if (int rc = run_product(p.pw, true, true, false, false, a->n, a->k, a->m, dz, ldz, term_stride, ws + p.xhat, p.ldk,
-                             a->m, ep, ws, st, "weight gradient"))
+                             a->m, ep, ws + p.part_w, a->grad_x != nullptr, st, "weight gradient", tw))
       return rc;
   }
+  if (a->grad_bias) {
+    e = moe::launch_colsum_finish(reinterpret_cast<float*>(ws + p.colsum), p.chunks, a->n, a->grad_bias,
+                                  a->grad_f32 != 0, a->grad_x || a->grad_weight, st);
+    if (e != cudaSuccess) return done(e, "bias gradient");
+  }
+  if (a->grad_x && (e = moe::launch_linear_join(false, false, tx, st)) != cudaSuccess) return done(e, "input gradient");
+  tw.join_early = a->grad_x && tx.units != tx.full_tiles;
+  if (a->grad_weight && (e = moe::launch_linear_join(false, false, tw, st)) != cudaSuccess) return done(e, "weight gradient");
   return MOE_OK;
 }
 
@@ -320,7 +350,7 @@ int moe_restore_activations(const void* q, const void* scale, int64_t batch, int
   if (batch == 0 || rows == 0 || cols == 0) return MOE_OK;
   if (!q || !scale || !out || !aligned(out, out_f32 ? 4 : 2)) return bad("restore: NULL or misaligned pointer");
   return done(moe::launch_restore(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), batch, rows, cols,
-                                  out, out_f32 != 0, cols, static_cast<cudaStream_t>(stream)),
+                                  out, out_f32 != 0, static_cast<cudaStream_t>(stream)),
               "restore");
 }
 
@@ -364,8 +394,8 @@ int moe_balance_loss_grad(const MoeBalanceGradArgs* a, void* stream) {
       !aligned(a->cu_seqlens, 4) || !aligned(a->counts, 4) || !aligned(a->tokens, 4) || !aligned(a->sequences, 4) ||
       !aligned(a->grad_loss, 4))
     return bad("balance gradient: NULL or misaligned pointer");
-  if (a->grad_loss && (!a->counts || !a->tokens || !a->sequences))
-    return bad("balance gradient: grad_loss needs counts, tokens and sequences");
+  if ((a->grad_loss || a->counts || a->tokens || a->sequences) && (!a->counts || !a->tokens || !a->sequences))
+    return bad("balance gradient: the loss's part needs counts, tokens and sequences");
   if (!a->cu_seqlens && a->num_sequences != 1) return bad("balance gradient: one sequence without cu_seqlens");
   moe::BalanceGradArgs b{a->routing_logits, a->topk_idx, a->cu_seqlens, a->num_tokens, a->num_experts, a->top_k,
                          a->num_sequences, a->scoring, a->alpha, a->routed_scaling_factor, a->counts, a->tokens,

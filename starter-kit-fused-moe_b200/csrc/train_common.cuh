@@ -59,6 +59,22 @@ __device__ __forceinline__ float2 unpack_bf16(uint32_t v) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
+// Read-only load through L1, or through L2 alone in an early launch (train_kernels.h).
+template <bool EARLY, typename T>
+__device__ __forceinline__ T load_input(const T* p) {
+  return EARLY ? __ldcg(p) : __ldg(p);
+}
+// Elements `at`, at + 1 of a row of 16-bit values, which start at an even address;
+// those outside [begin, end) are 0 and not read.
+template <bool EARLY>
+__device__ __forceinline__ uint32_t load_pair(const uint16_t* row, int at, int begin, int end) {
+  if (at >= begin && at + 1 < end) return load_input<EARLY>(reinterpret_cast<const uint32_t*>(row + at));
+  uint32_t v = 0;
+  if (at >= begin && at < end) v = load_input<EARLY>(row + at);
+  if (at + 1 >= begin && at + 1 < end) v |= (uint32_t)load_input<EARLY>(row + at + 1) << 16;
+  return v;
+}
+
 __device__ __forceinline__ float sigmoid_f(float z) { return 1.0f / (1.0f + expf(-z)); }
 
 // Single-input activations (codes 0..3); SwiGLU is first * silu(second).

@@ -29,14 +29,29 @@ struct LinearEpilogue {
 // Every kernel here is launched with programmatic stream serialization: its
 // blocks may become resident while the preceding kernel of the stream ends, and
 // wait for that kernel's completion before they touch global memory.
+//
+// Kernels of one call that do not need each other's results run side by side:
+// one launched `early` does not wait at its start but before it exits. It starts
+// when every block of its predecessor has run launch_dependents, which blocks do
+// after their own wait (or, early ones, at once), so whatever that wait stood for
+// is complete; and as no block leaves before its predecessor has completed, a
+// later kernel's wait covers the whole chain. An early kernel reads what other
+// kernels wrote through L2 only (TMA, ld.cg): it has not run the wait that would
+// order its L1.
 cudaError_t launch_checkpoint(const void* x, bool bf16, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q,
                               uint8_t* scale, cudaStream_t st);
 cudaError_t launch_restore(const uint8_t* q, const uint8_t* scale, int64_t batch, int64_t rows, int64_t cols, void* out,
-                           bool f32, int64_t ldo, cudaStream_t st);
+                           bool f32, cudaStream_t st);
+// To bf16 rows of stride ldo (out 16-byte aligned, ldo a multiple of 8, what lies between cols and ldo is overwritten).
+cudaError_t launch_restore_rows(const uint8_t* q, const uint8_t* scale, int64_t rows, int64_t cols, void* out, int64_t ldo,
+                                bool early, cudaStream_t st);
 
-// Products of at most kSmallTokens tokens without a kept pre-activation
-// (linear_small.cu); larger ones run on linear_tile.cu.
-constexpr int kSmallTokens = 32;
+// Products of few tokens without a kept pre-activation run on linear_small.cu,
+// the others on linear_tile.cu. Up to 16 tokens the small kernel wins throughout
+// (16 tokens: 5.2 against 9.9 us at K, N = 7168, 256; 17.5 against 18.1 at 7168,
+// 4096 gated; 10.9 against 12.5 at 2048, 7168); beyond, it loads the tokens' values too
+// often unless the weights are small (32 tokens: 7.9 against 10.0, 37 against 18, 19.3 against 11.3).
+constexpr bool small_product(int64_t m, int64_t k, int64_t n) { return m <= 16 || (m <= 32 && k * n <= 1 << 22); }
 cudaError_t launch_linear_small(const void* x, int64_t ldx, const void* w, int64_t ldw, int m, int k, int n,
                                 const LinearEpilogue& ep, cudaStream_t st);
 
@@ -53,7 +68,7 @@ struct ActGradArgs {
 };
 int act_grad_chunks(int m, int n);
 cudaError_t launch_act_grad(const ActGradArgs& a, cudaStream_t st);
-cudaError_t launch_colsum_finish(const float* colsum, int chunks, int n, void* out, bool f32, cudaStream_t st);
+cudaError_t launch_colsum_finish(const float* colsum, int chunks, int n, void* out, bool f32, bool early, cudaStream_t st);
 
 struct BalanceArgs {
   const float* logits;     // [t, e]
@@ -72,7 +87,7 @@ struct BalanceGradArgs {
   int t, e, k, s, scoring;
   float alpha, route_scale;
   const int32_t* counts; const int32_t* tokens; const int32_t* live;
-  const float* grad_loss;      // device scalar or NULL (0: no balance part)
+  const float* grad_loss;      // device scalar or NULL (1); counts NULL: no balance part
   const float* grad_weights;   // [t, k] or NULL
   float* grad_logits;          // [t, e]
 };

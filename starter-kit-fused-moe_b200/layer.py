@@ -137,10 +137,8 @@ def linear(x, weight, bias=None, residual=None, activation="none", out_dtype=tor
 def linear_checkpointed(x, weight, bias=None, residual=None, activation="none", out_dtype=torch.bfloat16, output=None):
     """`linear` for a training step: returns (y, LinearCheckpoint). The checkpoint keeps
     x and, with an activation, the pre-activation z = x W^T + bias in 8 bits each."""
-    n = _native()
-    y, z, z_scale = n.linear(x, weight, bias, residual, activation, out_dtype, output, True)
-    q, s = n.checkpoint(x)
-    return y, LinearCheckpoint(q, s, z, z_scale, activation)
+    y, *kept = _native().linear_checkpointed(x, weight, bias, residual, activation, out_dtype, output)
+    return y, LinearCheckpoint(*kept, activation)
 
 
 def linear_backward(grad_output, checkpoint, weight, need_x=True, need_weight=True, need_bias=False,
@@ -206,8 +204,8 @@ def balance_loss_backward(routing_logits, topk_idx, balance, cu_seqlens=None, gr
     counts = tokens = sequences = None
     if balance is not None:
         counts, tokens, sequences = balance.counts, balance.tokens, balance.sequences
-        if not isinstance(grad_loss, torch.Tensor):
-            grad_loss = torch.full((), 1.0 if grad_loss is None else float(grad_loss), device=routing_logits.device)
+        if grad_loss is not None and not isinstance(grad_loss, torch.Tensor):
+            alpha, grad_loss = alpha * float(grad_loss), None
     elif grad_loss is not None:
         raise ValueError("grad_loss needs what balance_loss returned")
     return _native().balance_loss_backward(routing_logits, topk_idx, counts, tokens, sequences, cu_seqlens, grad_loss,

@@ -93,6 +93,13 @@ def test_linear_sizes(pkg, m, k, n, act):
     linear_case(pkg, m, k, n, act)
 
 
+@pytest.mark.parametrize("m", [33, 64, 65, 97, 128])
+@pytest.mark.parametrize("k, n, act, dtype", [(7168, 1030, "swiglu", BF), (2048, 7168, "none", BF), (7168, 300, "none", F32),
+                                              (520, 515, "gelu", BF), (20000, 130, "silu", F32)])
+def test_linear_few_tokens(pkg, m, k, n, act, dtype):
+    linear_case(pkg, m, k, n, act, True, True, dtype)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("m, k, n", [(5, 96, 80), (40, 96, 80), (300, 520, 390), (520, 1024, 768)])
 def test_linear_epilogues(pkg, m, k, n, act):
