@@ -575,6 +575,78 @@ def test_wait_that_runs_out_with_residual_and_checkpoint(pkg, m, k, n, act):
     assert torch.equal(pkg.linear(x, w, residual=r, activation=act), want)
 
 
+def bits(t):
+    return t.view(torch.uint8) if t.element_size() == 1 else t
+
+
+@pytest.mark.parametrize("t, k", [(9, 8), (9, 127), (30, 129), (7, 1001), (40, 3), (5, 1)])
+def test_restore_at_any_offset(pkg, t, k):
+    """Rows cut out of a checkpoint start anywhere in memory."""
+    x = randn(t, k, seed=8, scale=3.0)
+    q, s = pkg.checkpoint_activations(x)
+    for dtype in (BF, F32):
+        whole = pkg.restore_activations(q, s, dtype)
+        for a, b in ((0, t), (1, t), (2, t - 1), (3, 4)):
+            assert torch.equal(pkg.restore_activations(q[a:b], s[:, a:b], dtype), whole[a:b])
+        both = pkg.restore_activations(torch.stack([q, q.flip(0)]), torch.stack([s, s.flip(1)]), dtype)
+        assert torch.equal(both[0], whole) and torch.equal(both[1], whole.flip(0))
+    w, dy = randn(16, k, seed=9), randn(t, 16, seed=10)
+    ck = pkg.LinearCheckpoint(q, s, None, None, "none")
+    cut = pkg.LinearCheckpoint(q[1:], s[:, 1:], None, None, "none")
+    again = pkg.LinearCheckpoint(q[1:].clone(), s[:, 1:].clone(), None, None, "none")
+    assert torch.equal(pkg.linear_backward(dy[1:], cut, w).weight, pkg.linear_backward(dy[1:], again, w).weight)
+    assert torch.equal(pkg.linear_backward(dy, ck, w).x[1:], pkg.linear_backward(dy[1:], cut, w).x)
+
+
+@pytest.mark.parametrize("dtype, t", [(BF, 33), (F32, 8)])
+@pytest.mark.parametrize("k", [128, 136, 131, 258])
+def test_checkpoint_rows_at_any_offset(pkg, dtype, t, k):
+    """Rows of a wider buffer, starting at any element: the same bytes as from a copy."""
+    wide = randn(t, 700, seed=11, dtype=dtype)
+    for c in (0, 1, 2, 3, 4, 7):
+        q, s = pkg.checkpoint_activations(wide[:, c:c + k])
+        q2, s2 = pkg.checkpoint_activations(wide[:, c:c + k].clone())
+        assert torch.equal(bits(q), bits(q2)) and torch.equal(bits(s), bits(s2))
+
+
+@pytest.mark.parametrize("m, k, n, act, grad", [(40, 64, 48, "gelu", BF), (300, 333, 130, "swiglu", F32), (600, 512, 1024, "none", BF),
+                                                (5, 2000, 777, "relu", F32)])
+def test_backward_reads_inputs_written_just_before(pkg, m, k, n, act, grad):
+    """The kernels of a gradient call overlap, but none runs ahead of what was launched before the call."""
+    o = n // 2 if act == "swiglu" else n
+    cases, want = [], []
+    for i in range(3):
+        x, w, dy = randn(m, k, seed=20 + i), randn(n, k, seed=30 + i, scale=0.1), randn(m, o, seed=40 + i)
+        _, ck = pkg.linear_checkpointed(x, w, activation=act)
+        cases.append((dy, w, ck))
+        g = pkg.linear_backward(dy, ck, w, need_bias=True, grad_dtype=grad)
+        torch.cuda.synchronize()
+        want.append(g)
+    dy, w, ck = (cases[0][0].clone(), cases[0][1].clone(), pkg.LinearCheckpoint(*[v.clone() if torch.is_tensor(v) else v for v in cases[0][2]]))
+    got = []
+    for r in range(60):
+        for live, src in zip((dy, w, *ck[:4]), (cases[r % 3][0], cases[r % 3][1], *cases[r % 3][2][:4])):
+            if live is not None:
+                bits(live).copy_(bits(src))
+        got.append(pkg.linear_backward(dy, ck, w, need_bias=True, grad_dtype=grad))
+    for r, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[r % 3]))
+
+
+def test_restore_past_32_bits(pkg):
+    """More than 2^32 values in rows of odd width."""
+    t, k = 1_050_000, 4099
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    q = torch.zeros(t, k, dtype=torch.uint8, device="cuda")
+    q[-20:] = torch.randint(0, 120, (20, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(torch.uint8)
+    s = torch.randint(100, 150, ((k + 127) // 128, t), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(torch.uint8)
+    q, s = q.view(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu)
+    r = pkg.restore_activations(q, s)
+    assert torch.equal(r[-20:], pkg.restore_activations(q[-20:].clone(), s[:, -20:]))
+    assert not r[:1000].any() and not r[-1000:-20].any()
+
+
 def test_offsets_past_32_bits(pkg):
     """More than 2^31 elements: the last rows of a product and of a checkpoint are those of the rows alone."""
     m, k, n = 300_100, 64, 7168
