@@ -10,7 +10,7 @@
 // matrices, which together hold dz's 24 bits, so that fp32 gradients are as
 // exact as an fp32 product (two terms left 2.5e-6 of the result's norm).
 //
-// Bound by HBM: dy, one byte per z value, two (or four) written per dz value.
+// Bound by HBM: dy, one byte per z value, two (or six) written per dz value.
 // 32 threads take 256 columns (8 neighbouring ones each, 16-byte accesses) and
 // 8 thread rows walk a chunk of 64 rows, so a column's sum is in registers until
 // the chunk ends; the chunks' sums are added in order by a second kernel, hence
