@@ -916,7 +916,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearTileArgs a) {
       for (int h = 0; h < HALVES; ++h)
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[u][h][j] = 0.f;
-#pragma unroll 2
+#pragma unroll(R == 1 ? 4 : 2)
     for (int s = 0; s < a.splits; ++s)
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -1061,8 +1061,8 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
     }
   }
   // Few tokens and a long contraction: the weights' rows become the tile's, which pads 64 or 128 columns instead of 256
-  // rows. At 64 (128) tokens and K = 7168 18.4 (18.5) instead of 19.6 (22.8) us for N = 4096 gated, 26.5 (27.8) instead
-  // of 29.2 (29.5) for N = 7168, 10.4 (11.1) instead of 12.1 (11.9) for N = 256 in fp32; at K = 4096 equal, at
+  // rows. At 64 (128) tokens and K = 7168 16.1 (18.3) instead of 19.6 (22.8) us for N = 4096 gated, 25.1 (27.4) instead
+  // of 29.2 (29.5) for N = 7168, 9.6 (10.3) instead of 12.1 (11.9) for N = 256 in fp32; at K = 4096 equal, at
   // K = 2048 14.1 instead of 11.5, because a flipped tile always needs the join.
   if (m <= 128 && k_blocks >= 96 && !keep && !grad) {
     best_cost = 1e300;
@@ -1073,8 +1073,12 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
       if (s > 1 && k_blocks < 4 * s) break;
       if (ep.y_f32 && depth > linear_chain(gated, true)) continue;               // longer chains drift
       const int64_t units = tail * s, rounds = (units + pairs - 1) / pairs;
+      // 52 pairs reach what HBM gives (32 of them 5 of 6.5 TB/s), fewer a part of it, those of the last round too; a
+      // slice more is also a load more, one after the other, in the join
+      const int64_t rest = units % pairs;
+      const double stream = hbm / units * (units - rest + (rest > 52 ? rest : rest ? 52 : 0));
       double cost = (double)rounds * (depth * (200.0 + 1.4 * nt) + 800);
-      cost = (cost > hbm ? cost : hbm) + 1500 + 12.0 * nt + 4000 + 8.0 * s * tail * m * 256 / 3000;
+      cost = (cost > stream ? cost : stream) + 1500 + 12.0 * nt + 4000 + 500.0 * s + 8.0 * s * tail * m * 256 / 3000;
       if (cost < best_cost) {
         best_cost = cost;
         best = {nt, s, 1, 0, tail};

@@ -47,10 +47,10 @@ cudaError_t launch_restore_rows(const uint8_t* q, const uint8_t* scale, int64_t 
                                 bool early, cudaStream_t st);
 
 // Products of few tokens without a kept pre-activation run on linear_small.cu,
-// the others on linear_tile.cu. Up to 16 tokens the small kernel wins throughout
-// (16 tokens: 5.2 against 9.9 us at K, N = 7168, 256; 17.5 against 18.1 at 7168,
-// 4096 gated; 10.9 against 12.5 at 2048, 7168); beyond, it loads the tokens' values too
-// often unless the weights are small (32 tokens: 7.9 against 10.0, 37 against 18, 19.3 against 11.3).
+// the others on linear_tile.cu. Up to 16 tokens the small kernel wins
+// (16 tokens: 5.2 against 9 us at K, N = 7168, 256; 10.9 against 12.5 at 2048, 7168;
+// 17.5 against 16 at 7168, 4096 gated, the one size tried where it does not); beyond, it loads the tokens' values too
+// often unless the weights are small (32 tokens: 7.9 against 9.1, 37 against 16, 19.3 against 11.3).
 constexpr bool small_product(int64_t m, int64_t k, int64_t n) { return m <= 16 || (m <= 32 && k * n <= 1 << 22); }
 cudaError_t launch_linear_small(const void* x, int64_t ldx, const void* w, int64_t ldw, int m, int k, int n,
                                 const LinearEpilogue& ep, cudaStream_t st);
