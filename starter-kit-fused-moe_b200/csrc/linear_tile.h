@@ -31,7 +31,7 @@ struct LinearTileMaps {
   CUtensorMap out, res;   // bf16 y and its residual in 32 x 32 boxes (vec)
 };
 // K-blocks per accumulator where long sums are cut: see the kernel's comment on sums.
-constexpr int linear_chain(bool gated, bool f32) { return f32 ? (gated ? 6 : 16) : 12; }
+constexpr int linear_chain(bool gated, bool f32) { return f32 ? (gated ? 6 : 16) : 8; }
 struct LinearTilePlan {
   int n_tile, splits, flip;
   int64_t full, tail;     // whole tiles, tiles left to the join
