@@ -529,6 +529,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
     bool ok = true, res_ok = true;
     int tt = 0;
     uint32_t res_count = 0;                              // residual boxes waited for
+    uint32_t out_box = 0;                                // without a residual: the box of the next store, across tiles
     for (int64_t u = wid; u < a.units; u += G) {
       const LtUnit x = lt_unit<FLIP>(a, u);
       const int64_t row0 = (int64_t)x.mt * 256 + crank * 128 + 32 * q, row = row0 + lane;
@@ -668,7 +669,9 @@ __global__ void __launch_bounds__(kLtThreads, 1)
           lt_stage_f32(stage, v, lane);
           lt_copy_f32(stage, static_cast<float*>(ep.y) + row0 * ep.ldy + c, ep.ldy, warp_rows, O - c, lane);
         } else {
-          uint8_t* box = stage + (j & 1) * 2048;
+          // without a residual the boxes alternate over all of the warp's stores: a tile may end on either one (NT of
+          // 192, one chunk per tile, a cut-off last column tile), and the wait below leaves the last store reading
+          uint8_t* box = stage + (res_boxes ? j & 1 : out_box) * 2048;
           if (res_boxes) {
             // waited for in a failed call too: a box that arrives later would cover the NaN staged here
             if (res_ok && !mbar_wait(smem_u32(&S.res[ew][j & 1]), (res_count >> (j & 1)) & 1)) {
@@ -693,6 +696,7 @@ __global__ void __launch_bounds__(kLtThreads, 1)
             }
           } else {
             lt_boxes_free<1>(lane);
+            out_box ^= 1;
           }
           lt_stage_bf16(box, v, lane);
           lt_box_out(&maps.out, box, (int)c, row0, lane);
