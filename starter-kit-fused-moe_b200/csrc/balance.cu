@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_gr
         for (int j = 0; j < ITEMS; ++j) dx[j] += scatter[warp][expert_of<VEC>(lane, j)];
         __syncwarp();
         if (first) scatter[warp][id] = 0.f;
+        __syncwarp();                                        // the warp's next token may pick it in another lane
       }
       float* out = a.grad_logits + (int64_t)t * a.e;
       if constexpr (VEC) {

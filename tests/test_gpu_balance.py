@@ -234,3 +234,18 @@ def test_layer_around_the_routed_experts(pkg, oracle):
     s = torch.sigmoid(logits.double()).gather(1, idx.long())
     w64 = s / (s.sum(1, keepdim=True) + 1e-20) * 2.5
     assert ((weights.double() - w64).abs() <= 2.0 ** -18 * w64).all()
+
+
+@pytest.mark.parametrize("e, k, stride", [(8, 8, 1), (16, 8, 3), (256, 8, 5), (64, 32, 7)])
+def test_same_experts_in_other_pick_positions(pkg, e, k, stride):
+    """Tokens one after the other pick the same experts, each in another position than the token before."""
+    t = 20000
+    x, _, _ = inputs(t, e, 1, seed=12)
+    turn = (torch.arange(t, device="cuda") * stride)[:, None] + torch.arange(k, device="cuda")
+    idx = ((turn % k) * (e // k)).to(torch.int32)
+    dw = 0.01 * torch.randn(t, k, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    g = pkg.balance_loss_backward(x, idx, None, grad_topk_weights=dw)
+    want = ref64(x, idx, None, 0.1, "sigmoid", None, dw)[4]
+    assert ((g.double() - want).abs() <= 2.0 ** -16 * 2.5 * dw.double().abs().sum(1, keepdim=True)).all()
+    for _ in range(10):
+        assert torch.equal(pkg.balance_loss_backward(x, idx, None, grad_topk_weights=dw), g)
