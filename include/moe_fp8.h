@@ -354,8 +354,9 @@ int moe_restore_activations(const void* q, const void* scale, int64_t batch, int
  *   p_te = s_te / (sum_j s_tj + 1e-20), s = sigmoid(logit)   (scoring 0), or softmax (scoring 1).
  * A pick outside [0, E) selects nothing, and a token with no other picks is
  * padding: it counts in no T_q and no sum. Tokens outside every sequence count
- * nowhere. Boundaries that decrease or leave [0, T] give a NaN loss, -1 for
- * `sequences` and a NaN gradient. The gradient treats f as constant. grad_topk_weights adds the gradient of the combine
+ * nowhere. Boundaries that decrease or leave [0, T], one or several, give a NaN
+ * loss, -1 for `sequences` and every T_q, no counts, NaN mean scores and a NaN
+ * gradient. The gradient treats f as constant. grad_topk_weights adds the gradient of the combine
  * weights of moe_fp8_route, w_k = s_k / (sum of the picked s + 1e-20) * scale
  * with s = sigmoid(logit), for every token. Both sums run in a fixed order. */
 typedef struct MoeBalanceArgs {
@@ -364,7 +365,7 @@ typedef struct MoeBalanceArgs {
   const int32_t* cu_seqlens;     /* [S + 1] device, or NULL (S = 1) */
   float* loss;                   /* [1] */
   int32_t* counts;               /* [S, E] */
-  int32_t* tokens;               /* [S]: T_q; -1 between wrong boundaries */
+  int32_t* tokens;               /* [S]: T_q; -1: wrong boundaries */
   float* mean_scores;            /* [S, E]: P */
   int32_t* sequences;            /* [1]: sequences with T_q > 0; -1: wrong boundaries */
   void* workspace;               /* >= moe_balance_workspace_bytes(T, E, S) */

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
   const int e = 32 * g + tx;
   int qa, qb;
   seq_bounds(a.cu, q, a.t, qa, qb);
-  // a decreasing or out-of-range boundary is reported as a NaN loss
+  // a decreasing or out-of-range boundary: a NaN loss, no tokens and no counts anywhere (see the last block below)
   bool bad = false;
   if (a.cu != nullptr) {
     const int c0 = __ldg(a.cu + q), c1 = __ldg(a.cu + q + 1);
@@ -276,6 +276,7 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) term += __shfl_xor_sync(0xffffffffu, term, d);
+    __syncwarp();                                            // the warp's outputs come before lane 0's fence
     if (tx == 0) {
       w.loss[(int64_t)q * groups + g] = bad ? (double)NAN : term;
       if (g == 0) a.tokens[q] = bad ? -1 : tq;
@@ -312,18 +313,31 @@ __global__ void __launch_bounds__(256) balance_reduce_kernel(BalanceArgs a, Bala
     *a.loss = (float)(live > 0 ? (double)a.alpha * l / live : l);   // l is 0 (or NaN) without sequences
     *a.live = any_wrong ? -1 : live;
   }
+  // One wrong boundary leaves the tokens of others unassigned too (the search for a block's first sequence expects
+  // them in order), so no sequence of the call has counts.
+  if (any_wrong) {
+    for (int64_t i = threadIdx.x; i < (int64_t)a.s * a.e; i += 256) {
+      a.counts[i] = 0;
+      a.mean_scores[i] = NAN;
+    }
+    for (int i = threadIdx.x; i < a.s; i += 256) a.tokens[i] = -1;
+  }
 }
 
-// t = 0: no tokens anywhere.
+// t = 0: no tokens anywhere, and every boundary has to be 0.
 __global__ void balance_empty_kernel(BalanceArgs a) {
+  bool wrong = false;
+  if (a.cu != nullptr)
+    for (int i = threadIdx.x; i <= a.s; i += blockDim.x) wrong |= a.cu[i] != 0;
+  wrong = __syncthreads_or(wrong);
   for (int64_t i = threadIdx.x; i < (int64_t)a.s * a.e; i += blockDim.x) {
     a.counts[i] = 0;
-    a.mean_scores[i] = 0.f;
+    a.mean_scores[i] = wrong ? NAN : 0.f;
   }
-  for (int i = threadIdx.x; i < a.s; i += blockDim.x) a.tokens[i] = 0;
+  for (int i = threadIdx.x; i < a.s; i += blockDim.x) a.tokens[i] = wrong ? -1 : 0;
   if (threadIdx.x == 0) {
-    *a.loss = 0.f;
-    *a.live = 0;
+    *a.loss = wrong ? NAN : 0.f;
+    *a.live = wrong ? -1 : 0;
   }
 }
 

@@ -184,8 +184,9 @@ def balance_loss(routing_logits, topk_idx, cu_seqlens=None, alpha=1e-4, scoring=
         f_qe = E / (k T_q) * counts_qe,  P_qe = mean over the sequence of p_te.
 
     A pick outside [0, E) selects nothing and a token without picks is padding:
-    it counts nowhere. Boundaries that decrease or leave [0, T] give a NaN loss,
-    `sequences` -1 and NaN gradients.
+    it counts nowhere. Boundaries that decrease or leave [0, T], one or several, give
+    a NaN loss, -1 for `sequences` and all `tokens`, counts of 0, NaN mean scores and
+    NaN gradients.
     """
     return BalanceLoss(*_native().balance_loss(routing_logits, topk_idx, cu_seqlens, alpha, scoring))
 

@@ -249,3 +249,38 @@ def test_same_experts_in_other_pick_positions(pkg, e, k, stride):
     assert ((g.double() - want).abs() <= 2.0 ** -16 * 2.5 * dw.double().abs().sum(1, keepdim=True)).all()
     for _ in range(10):
         assert torch.equal(pkg.balance_loss_backward(x, idx, None, grad_topk_weights=dw), g)
+
+
+@pytest.mark.parametrize("cuts", [[0, 30, 20, 40], [-5, 10, 40], [0, 10, 41], [10, 5], [0, 5, 10, 39, 7, 12, 40], [0, 8, 16, 24, 50]])
+def test_bad_boundaries_leave_no_counts_behind(pkg, cuts):
+    """Wrong boundaries give the same outputs for every sequence, whatever the workspace and the outputs held before."""
+    import ctypes
+    import sys
+    layer = sys.modules[pkg.__name__ + ".layer"]
+    lib = layer._library()
+    t, e, k, s = 40, 96, 2, len(cuts) - 1
+    x, idx, _ = inputs(t, e, k)
+    cu = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    need = lib.moe_balance_workspace_bytes(t, e, s)
+    for fill in (0, 1, 127):
+        ws = torch.full((need,), fill, dtype=torch.uint8, device="cuda")
+        out = torch.full((2 + s + 2 * s * e,), fill, dtype=torch.int32, device="cuda")
+        loss, live, tokens, counts, mean = out[:1].view(torch.float32), out[1:2], out[2:2 + s], out[2 + s:2 + s + s * e], out[2 + s + s * e:].view(torch.float32)
+        a = layer.MoeBalanceArgs(x.data_ptr(), idx.data_ptr(), cu.data_ptr(), loss.data_ptr(), counts.data_ptr(), tokens.data_ptr(),
+                                 mean.data_ptr(), live.data_ptr(), ws.data_ptr(), need, t, e, k, s, 0, 0.1)
+        assert lib.moe_balance_loss(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert torch.isnan(loss).all() and torch.isnan(mean).all() and not counts.any()
+        assert (tokens == -1).all() and int(live) == -1
+
+
+def test_boundaries_of_no_tokens(pkg):
+    """Without tokens the only right boundaries are zeros."""
+    x, idx, _ = inputs(4, 32, 2)
+    for cuts, ok in (([0, 0, 0], True), ([0, 3], False), ([0, 0, -1], False), ([2, 2], False)):
+        b = pkg.balance_loss(x[:0], idx[:0], cu_seqlens=torch.tensor(cuts, dtype=torch.int32, device="cuda"))
+        assert not b.counts.any()
+        if ok:
+            assert float(b.loss) == 0 and int(b.sequences) == 0 and not b.tokens.any() and not b.mean_scores.any()
+        else:
+            assert torch.isnan(b.loss) and int(b.sequences) == -1 and (b.tokens == -1).all() and torch.isnan(b.mean_scores).all()
