@@ -1,7 +1,8 @@
 // Gradient of a dense product's pre-activation, dz = dy * act'(z^) with z^ the
 // 8-bit checkpoint of z, and its column sums (the bias gradient).
 //
-//   relu'(z) = [z > 0], silu'(z) = s (1 + z (1 - s)), gelu'(z) = Phi(z) + z phi(z),
+//   relu'(z) = [z > 0] (NaN for NaN: a block that overflowed does not leave the
+//   gradients in silence), silu'(z) = s (1 + z (1 - s)), gelu'(z) = Phi(z) + z phi(z),
 //   SwiGLU y = a silu(b): da = dy silu(b), db = dy a silu'(b), stored as [da | db].
 //
 // dz is computed in fp32 and written in bf16, the operand type of the two

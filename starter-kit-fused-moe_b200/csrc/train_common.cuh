@@ -91,7 +91,7 @@ __device__ __forceinline__ float sigmoid_fast(float z) { return __fdividef(1.0f,
 template <bool FAST>
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
-    case kActRelu: return z > 0.f ? 1.f : 0.f;
+    case kActRelu: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;      // NaN stays, as in the value
     case kActGelu:
       return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * (FAST ? __expf(-0.5f * z * z) : expf(-0.5f * z * z));
     case kActSilu: {

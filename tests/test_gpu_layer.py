@@ -670,3 +670,51 @@ def test_offsets_past_32_bits(pkg):
     check(g.x[-40:], ref, ref.abs() * 2.0 ** -20 + 1e-4, "grad_x of the last rows")
     want = dy[:, 0].double().sum()
     assert abs(float(g.bias[0].double() - want)) <= 2.0 ** -16 * float(dy[:, 0].double().abs().sum())
+
+
+# --------------------------------------------------------------------------------- far and non-finite values
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("gin, gout", [(BF, BF), (F32, F32)])
+@pytest.mark.parametrize("m, k, n", [(40, 64, 512), (300, 130, 390)])
+def test_backward_non_finite(pkg, act, gin, gout, m, k, n):
+    """A NaN or infinity in grad_output or in a kept block reaches the gradients it is part of, and no others."""
+    x, w = randn(m, k, seed=1), randn(n, k, seed=2, scale=k ** -0.5)
+    y, ck = pkg.linear_checkpointed(x, w, activation=act)
+    o = y.shape[1]
+    dy = randn(m, o, seed=5, dtype=gin)
+    clean = pkg.linear_backward(dy, ck, w, need_bias=True, grad_dtype=gout)
+    rows = torch.arange(m, device="cuda")
+
+    def compare(g, row, cols):
+        out = torch.zeros(n, dtype=torch.bool, device="cuda")
+        for c in cols:
+            out[c] = True
+        assert not torch.isfinite(g.x[row]).any() and torch.equal(g.x[rows != row], clean.x[rows != row])
+        assert not torch.isfinite(g.weight[out]).any() and torch.equal(g.weight[~out], clean.weight[~out])
+        assert not torch.isfinite(g.bias[out]).any() and torch.equal(g.bias[~out], clean.bias[~out])
+
+    halves = (0, o) if act == "swiglu" else (0,)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        d = dy.clone()
+        row, col = m // 2, 3
+        if act == "relu":                                      # an infinity times a slope of 0 is a NaN too
+            col = int(torch.nonzero(y[row] > 0)[0])
+        d[row, col] = bad
+        compare(pkg.linear_backward(d, ck, w, need_bias=True, grad_dtype=gout), row, [h + col for h in halves])
+    if act == "none":
+        return
+    z = ck.z.clone().view(torch.uint8)
+    s = ck.z_scale.clone().view(torch.uint8)
+    row = m - 1
+    for h in range(len(halves)):                               # the NaN scale of one block, as an overflow leaves it
+        zs = s.clone()
+        (zs[h] if act == "swiglu" else zs)[1, row] = 255
+        c = ck._replace(z_scale=zs.view(torch.float8_e8m0fnu))
+        cols = slice(128, min(256, o))
+        # d/da = dy silu(b) does not see a; d/db = dy a silu'(b) sees both
+        hit = [cols] if act != "swiglu" else [slice(o + cols.start, o + cols.stop)] + ([cols] if h == 1 else [])
+        compare(pkg.linear_backward(dy, c, w, need_bias=True, grad_dtype=gout), row, hit)
+    zq = z.clone()                                             # a NaN byte
+    (zq[0] if act == "swiglu" else zq)[row, 5] = 0x7f
+    c = ck._replace(z=zq.view(torch.float8_e4m3fn))
+    compare(pkg.linear_backward(dy, c, w, need_bias=True, grad_dtype=gout), row, [5] if act != "swiglu" else [o + 5])
