@@ -215,9 +215,9 @@ __device__ __forceinline__ void lt_bias32(const __nv_bfloat16* bias, int64_t c, 
   lt_bias16(bias, c, end, v);
   lt_bias16(bias, c + 16, end, v + 16);
 }
-// bf16 results take silu from the hardware exponential and reciprocal (2^-20 of
+// bf16 results take silu and gelu from the hardware exponential and reciprocal (2^-20 of
 // 1 + |z|), fp32 ones from the exact ones: the epilogue is bound by its
-// instructions, and the exact quotient is half of them.
+// instructions, and silu's exact quotient is half of them.
 __device__ __forceinline__ float lt_silu(float z, bool exact) {
   return exact ? act_value(z, kActSilu) : z * sigmoid_fast(z);
 }
@@ -227,8 +227,13 @@ __device__ __forceinline__ void lt_act32(float* v, int act, bool exact) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActRelu);
   } else if (act == kActGelu) {
+    if (exact) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActGelu);
+      for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], kActGelu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] *= normal_cdf<true>(v[i]);
+    }
   } else if (exact) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = lt_silu(v[i], true);

@@ -77,23 +77,44 @@ __device__ __forceinline__ uint32_t load_pair(const uint16_t* row, int at, int b
 
 __device__ __forceinline__ float sigmoid_f(float z) { return 1.0f / (1.0f + expf(-z)); }
 
+// 1 / (1 + e^-z) with the hardware exponential and reciprocal.
+__device__ __forceinline__ float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+// Phi(z), good to z^2 + 8 units of 2^-23 of itself down to the least normal number: as 1 + erf(z / sqrt 2) the lower
+// tail cancels (4 % off at z = -5, zero below -5.6). With a = |z| and t = 1 / (1 + 0.3 a), e^(a^2 / 2) Phi(-a) is t times
+// a smooth function of t on (0, 1]; the polynomial is its least relative maximum error of degree 7 (1.5e-7), fitted by
+// Lawson's reweighted least squares in 64 bits for a up to 14. FAST: the hardware exponential (another z^2 / 2 units),
+// for results in bf16. gelu of 4096 x 7168 values, K = 256: 53 us in bf16, 56 with erff, 92 with erfcf.
+template <bool FAST>
+__device__ __forceinline__ float normal_cdf(float z) {
+  const float a = fabsf(z), t = __fdividef(1.0f, fmaf(0.3f, a, 1.0f));
+  float p = 0.0356747732f;
+  p = fmaf(p, t, -0.157203078f);
+  p = fmaf(p, t, 0.20635349f);
+  p = fmaf(p, t, -0.05368363f);
+  p = fmaf(p, t, 0.12856162f);
+  p = fmaf(p, t, 0.09991349f);
+  p = fmaf(p, t, 0.12075396f);
+  p = fmaf(p, t, 0.1196293f);
+  const float e = -0.5f * z * z, q = p * t * (FAST ? __expf(e) : expf(e));      // Phi(-a); NaN stays
+  return z > 0.f ? 1.0f - q : q;
+}
+
 // Single-input activations (codes 0..3); SwiGLU is first * silu(second).
 __device__ __forceinline__ float act_value(float z, int act) {
   switch (act) {
     case kActRelu: return z < 0.f ? 0.f : z;              // NaN stays
-    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case kActGelu: return z * normal_cdf<false>(z);
     case kActSilu: return z / (1.0f + expf(-z));
     default: return z;
   }
 }
-// 1 / (1 + e^-z) with the hardware exponential and reciprocal.
-__device__ __forceinline__ float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
 template <bool FAST>
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case kActRelu: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;      // NaN stays, as in the value
     case kActGelu:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * (FAST ? __expf(-0.5f * z * z) : expf(-0.5f * z * z));
+      return normal_cdf<FAST>(z) + z * 0.39894228040143268f * (FAST ? __expf(-0.5f * z * z) : expf(-0.5f * z * z));
     case kActSilu: {
       const float s = FAST ? sigmoid_fast(z) : sigmoid_f(z);
       return s * (1.0f + z * (1.0f - s));

@@ -400,6 +400,49 @@ def test_linear_backward(pkg, m, k, n, act, gin, gout):
     assert torch.equal(pkg.linear_backward(dy, ck, w, need_x=False, grad_dtype=gout).weight, g.weight)
 
 
+@pytest.mark.parametrize("m, n", [(4, 1), (40, 1), (300, 96), (300, 97)])
+@pytest.mark.parametrize("keep", [False, True])
+def test_gelu_far_below_zero(pkg, m, n, keep):
+    """gelu(z) = z Phi(z) keeps its value down to where Phi leaves the normal numbers. In fp32 a value is
+    off by the rounding of z^2 / 2, whose exponential multiplies it (z^2 / 4 units of 2^-23), and by a few units of the
+    exponential, a reciprocal and a product of polynomials: z^2 + 8 together."""
+    z = torch.linspace(-13, 1, m * n, device="cuda").view(m, n)
+    x = torch.zeros(m, 128, device="cuda", dtype=BF)
+    w = torch.zeros(n, 128, device="cuda", dtype=BF)
+    x[:, 0] = 1                                                # z = bias + x_1: both in bf16
+    x[:, 1] = z[:, 0].to(BF)
+    w[:, 1] = 1
+    b = (z[0] - z[0, 0]).to(BF)
+    z = x[:, 1:2].double() + b.double()
+    z32 = z.float().double()                                   # what fp32 holds of it
+    f = pkg.linear_checkpointed if keep else pkg.linear
+    y = f(x, w, bias=b, activation="gelu", out_dtype=F32)
+    y = y[0] if keep else y
+    ref = act64(z32, "gelu")
+    assert ((y.double() - ref).abs() <= ref.abs() * (z32 * z32 + 8) * 2.0 ** -23 + 1e-37).all()
+    yb = f(x, w, bias=b, activation="gelu")
+    yb = yb[0] if keep else yb
+    assert ((yb.double() - ref).abs() <= ref.abs() * (2.0 ** -8 + (z32 * z32 + 8) * 2.0 ** -22) + 1e-37).all()
+
+
+@pytest.mark.parametrize("gout", [BF, F32])
+@pytest.mark.parametrize("n", [8, 9])
+def test_gelu_slope_far_below_zero(pkg, gout, n):
+    """Phi(z) + z phi(z) at values that the checkpoint holds exactly; for bf16 gradients the exponential is the hardware's,
+    2^-21 of the larger of 1 and its exponent z^2 / 2."""
+    z = torch.tensor([-12.0, -11, -10, -9, -8, -7.5, -7, -6.5, -6, -5.5, -5, -4, -3.5, -3, -2, -1, -0.5, 0, 0.5, 1, 3, 8], device="cuda")
+    z8, zs = pkg.checkpoint_activations(z[:, None].expand(-1, n).contiguous())
+    assert torch.equal(pkg.restore_activations(z8, zs, F32)[:, 0], z)
+    x8, xs = pkg.checkpoint_activations(torch.ones(z.numel(), n, device="cuda"))
+    g = pkg.linear_backward(torch.ones(z.numel(), n, device="cuda"), pkg.LinearCheckpoint(x8, xs, z8, zs, "gelu"),
+                            torch.eye(n, device="cuda").to(BF), grad_dtype=gout)
+    zz = z.double()
+    phi, cdf = zz * torch.exp(-zz * zz / 2) / math.sqrt(2 * math.pi), 0.5 * torch.erfc(-zz / math.sqrt(2))
+    tol = (cdf + phi.abs()) * (zz * zz + 8) * (2.0 ** -20 if gout == BF else 2.0 ** -22)
+    tol = tol + ((cdf + phi).abs() + tol) * (2.0 ** -8 if gout == BF else 2.0 ** -23) + 1e-36
+    assert ((g.x.double() - (cdf + phi)[:, None]).abs() <= tol[:, None]).all()
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_backward_against_differences(pkg, act):
     """The gradients are those of the forward: with inputs whose checkpoints are exact (few-bit values, one
