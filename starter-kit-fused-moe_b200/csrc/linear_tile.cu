@@ -22,7 +22,7 @@
 // an fp32 one does, and so does a kept pre-activation (one value in 10^4 moves to
 // the next e4m3 step). For those (CHAIN) the chain is cut every 16 K-blocks of 64
 // (fp32), 6 (fp32 gated, where both factors drift the same way: 1.7e-6 at K = 768
-// with 16, 9e-7 with 8) or 8 (kept): the epilogue warps add each partial
+// with 16, 9e-7 with 8) or 8 (kept, whatever y's type): the epilogue warps add each partial
 // accumulator to fp32 registers, rounding to nearest, while the tensor core fills
 // the other one. The reads of TMEM cost the tensor core about a K-block each: 218
 // us for the checkpointed product of 4096 x 7168 x 4096 instead of 214 with 12 and
@@ -1082,7 +1082,7 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
     for (int s = 1; s <= 16; ++s) {
       const int64_t depth = (k_blocks + s - 1) / s;
       if (s > 1 && k_blocks < 4 * s) break;
-      if (ep.y_f32 && depth > linear_chain(gated, true)) continue;               // longer chains drift
+      if (ep.y_f32 && depth > linear_chain(gated, false)) continue;               // longer chains drift
       const int64_t units = tail * s, rounds = (units + pairs - 1) / pairs;
       // 52 pairs reach what HBM gives (32 of them 5 of 6.5 TB/s), fewer a part of it, those of the last round too; a
       // slice more is also a load more, one after the other, in the join

@@ -31,7 +31,8 @@ struct LinearTileMaps {
   CUtensorMap out, res;   // bf16 y and its residual in 32 x 32 boxes (vec)
 };
 // K-blocks per accumulator where long sums are cut: see the kernel's comment on sums.
-constexpr int linear_chain(bool gated, bool f32) { return f32 ? (gated ? 6 : 16) : 8; }
+// Kept pre-activations have one length, so that their bytes do not depend on y's type.
+constexpr int linear_chain(bool gated, bool keep) { return keep ? 8 : gated ? 6 : 16; }
 struct LinearTilePlan {
   int n_tile, splits, flip;
   int64_t full, tail;     // whole tiles, tiles left to the join
