@@ -18,9 +18,11 @@
 //
 // Sums. The tensor core adds to its fp32 accumulator by truncation, so a long
 // chain drifts: 8e-6 of the result's norm at K = 7168, 2e-6 at 2048, 5e-7 at
-// 512, where an fp32 product has 9e-7. A bf16 result (2^-8) does not show that,
-// an fp32 one does, and so does a kept pre-activation (one value in 10^4 moves to
-// the next e4m3 step). For those (CHAIN) the chain is cut every 16 K-blocks of 64
+// 512 for values of both signs, 3.7e-7 per 64 of K for values of one sign, which is
+// 1.5e-3 of a bf16 result at K = 262144. So the chain is cut (CHAIN) every 256 K-blocks
+// of 64, which costs nothing that can be seen (1e-4 of a bf16 result at most); an
+// fp32 result and a kept pre-activation (one value in 10^4 moves to
+// the next e4m3 step) show less, and there it is cut every 16
 // (fp32), 6 (fp32 gated, where both factors drift the same way: 1.7e-6 at K = 768
 // with 16, 9e-7 with 8) or 8 (kept, whatever y's type): the epilogue warps add each partial
 // accumulator to fp32 registers, rounding to nearest, while the tensor core fills
@@ -1082,7 +1084,7 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
     for (int s = 1; s <= 16; ++s) {
       const int64_t depth = (k_blocks + s - 1) / s;
       if (s > 1 && k_blocks < 4 * s) break;
-      if (ep.y_f32 && depth > linear_chain(gated, false)) continue;               // longer chains drift
+      if (depth > linear_chain(gated, ep.y_f32, false)) continue;                // longer chains drift
       const int64_t units = tail * s, rounds = (units + pairs - 1) / pairs;
       // 52 pairs reach what HBM gives (32 of them 5 of 6.5 TB/s), fewer a part of it, those of the last round too; a
       // slice more is also a load more, one after the other, in the join
@@ -1136,9 +1138,9 @@ static cudaError_t launch_c(const LinearTileMaps& maps, const LinearTileArgs& a,
 
 template <bool A_MN, bool B_MN, bool GATED, bool KEEP>
 static cudaError_t launch_t(const LinearTileMaps& maps, const LinearTileArgs& a, int num_sms, cudaStream_t st) {
-  // cut the chain where the result shows its drift and a unit is longer than one piece
+  // cut the chain where a unit is longer than one piece
   const int unit = a.full_tiles > 0 ? a.k_blocks : (a.k_blocks + a.splits - 1) / a.splits;
-  if ((KEEP || a.ep.y_f32) && unit > a.chain) return launch_c<A_MN, B_MN, GATED, KEEP, true>(maps, a, num_sms, st);
+  if (unit > a.chain) return launch_c<A_MN, B_MN, GATED, KEEP, true>(maps, a, num_sms, st);
   return launch_c<A_MN, B_MN, GATED, KEEP, false>(maps, a, num_sms, st);
 }
 

@@ -18,7 +18,7 @@ struct LinearTileArgs {
   int term_blocks;        // of one term
   int terms;
   int splits;
-  int chain;              // K-blocks per accumulator where long sums are cut (fp32 y, kept pre-activations)
+  int chain;              // K-blocks per accumulator, where a unit is longer
   int64_t full_tiles;     // tiles done whole; the others leave `splits` K slices to the join
   int64_t units;          // full_tiles + splits * (number of the others)
   int early, join_early;  // see train_kernels.h
@@ -32,7 +32,7 @@ struct LinearTileMaps {
 };
 // K-blocks per accumulator where long sums are cut: see the kernel's comment on sums.
 // Kept pre-activations have one length, so that their bytes do not depend on y's type.
-constexpr int linear_chain(bool gated, bool keep) { return keep ? 8 : gated ? 6 : 16; }
+constexpr int linear_chain(bool gated, bool f32, bool keep) { return keep ? 8 : !f32 ? 256 : gated ? 6 : 16; }
 struct LinearTilePlan {
   int n_tile, splits, flip;
   int64_t full, tail;     // whole tiles, tiles left to the join

@@ -100,3 +100,56 @@ def test_kept_bytes_do_not_depend_on_the_output_type(pkg, m, k, n, act):
     b = pkg.linear_checkpointed(x, w, activation=act, out_dtype=F32)[1]
     assert torch.equal(a.z.view(torch.uint8), b.z.view(torch.uint8))
     assert torch.equal(a.z_scale.view(torch.uint8), b.z_scale.view(torch.uint8))
+
+
+def positive(rows, cols, seed):
+    """Values of one sign, rows at different scales so that sums of the same size round everywhere between two steps."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.rand(rows, cols, generator=g, device="cuda") + 0.5
+    return (x * (1 + torch.rand(rows, 1, generator=g, device="cuda"))).to(BF)
+
+
+def product64(x, w):
+    """x w^T in 64 bits, a piece of K at a time."""
+    z = torch.zeros(x.shape[0], w.shape[0], dtype=torch.float64, device="cuda")
+    for i in range(0, x.shape[1], 32768):
+        z.addmm_(x[:, i:i + 32768].double(), w[:, i:i + 32768].double().t())
+    return z
+
+
+def drift(got, want):
+    """Mean relative error, with its sign: roundings to nearest cancel in it, truncation does not."""
+    return float(((got.double() - want) / want).mean())
+
+
+@pytest.fixture
+def room():
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    yield
+    torch.cuda.empty_cache()
+
+
+# A bf16 rounding is off by 2^-9 of the value at the most typical, either way: over 16384 values and more the mean is below
+# 2^-9 / sqrt(16384) = 1.5e-5. The tensor core cuts the 16 products of an addition and the running sum at one place before
+# it adds them, so terms of one sign lose more than the sum's own half unit: 3.7e-7 per K-block of 64 (measured), 9.5e-5 in a
+# chain of 256. Together 1.1e-4, under the bound of 1.18e-4; uncut chains of 4096 K-blocks lose 1.5e-3.
+LONG = 0.18 * 4096 * 2.0 ** -23 + 3e-5
+
+
+@pytest.mark.parametrize("m, k, n", [(2560, 262144, 2048), (64, 4194304, 256)])
+def test_bf16_products_of_a_long_contraction(pkg, room, m, k, n):
+    x, w = positive(m, k, 1), positive(n, k, 2)
+    assert abs(drift(pkg.linear(x, w), product64(x, w))) <= LONG
+
+
+def test_bf16_weight_gradient_of_many_tokens(pkg, room):
+    m, k, n = 262144, 4096, 4096
+    x = positive(k, m, 1).t().contiguous()
+    dy = positive(n, m, 2).t().contiguous()
+    x8, xs = pkg.checkpoint_activations(x)
+    del x
+    g = pkg.linear_backward(dy, pkg.LinearCheckpoint(x8, xs, None, None, "none"), randn(n, k), need_x=False)
+    xr = pkg.restore_activations(x8, xs)
+    assert abs(drift(g.weight, product64(dy.t(), xr.t()))) <= LONG
