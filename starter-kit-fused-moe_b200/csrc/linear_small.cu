@@ -10,7 +10,10 @@
 // a chunk cancels and nothing passes through shared memory. (A tcgen05 tile would
 // spend its rows on padding; the tensor work is not what bounds this.) The partial
 // sums meet in shared memory, then across the cluster in distributed shared memory,
-// both in a fixed order.
+// both in a fixed order. The tensor core's additions truncate, so a chain of more
+// than 64 of them per warp (K > 8192, or more with a cluster) is cut (CUT): rounded to
+// nearest after every 16 or 8. Uncut, K = 262144 lost 1.7e-4 of a sum of one sign. Everywhere, it
+// would cost registers and with them an SM's fourth CTA (16 x 2048 x 7168: 14.3 us, not 10.9).
 #include "cta_pair.cuh"
 #include "train_common.cuh"
 
@@ -54,10 +57,12 @@ __device__ __forceinline__ uint4 ls_load(const __nv_bfloat16* row, int c, int k)
   }
 }
 
-template <int NT8, bool GATED, bool VEC>
+constexpr int ls_unroll(int nt8, bool vec) { return nt8 == 1 && vec ? 4 : 2; }     // chunks in flight
+
+template <int NT8, bool GATED, bool VEC, bool CUT>
 __global__ void __launch_bounds__(kLsWarps * 32) linear_small_kernel(LinearSmallArgs a) {
   constexpr int TOK = 8 * NT8, OUT = GATED ? 8 : 16;
-  constexpr int U = NT8 == 1 && VEC ? 4 : 2;       // chunks in flight
+  constexpr int U = ls_unroll(NT8, VEC);
   __shared__ float red[kLsWarps][16][TOK + 1];
   __shared__ float part[16][TOK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -70,11 +75,14 @@ __global__ void __launch_bounds__(kLsWarps * 32) linear_small_kernel(LinearSmall
   const int64_t r1 = GATED ? a.out_cols + r0 : min(j0 + 8 + g, a.out_cols - 1);
   const __nv_bfloat16* w0 = a.w + r0 * a.ldw;
   const __nv_bfloat16* w1 = a.w + r1 * a.ldw;
-  float acc[NT8][4];
+  float acc[NT8][4], sum[CUT ? NT8 : 1][4];
 #pragma unroll
   for (int i = 0; i < NT8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) {
+      acc[i][j] = 0.f;
+      if constexpr (CUT) sum[i][j] = 0.f;
+    }
   const int chunks = (a.k + 63) / 64, step = kLsWarps * cl;
   for (int c0 = crank * kLsWarps + warp; c0 < chunks; c0 += U * step) {
     uint4 wa[U][2], wb[U][2];
@@ -100,9 +108,20 @@ __global__ void __launch_bounds__(kLsWarps * 32) linear_small_kernel(LinearSmall
           mma_16816(acc[i], wa[u][h].z, wb[u][h].z, wa[u][h].w, wb[u][h].w, xv.z, xv.w);
         }
       }
+    if constexpr (CUT)
+#pragma unroll
+      for (int i = 0; i < NT8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sum[i][j] += acc[i][j];
+          acc[i][j] = 0.f;
+        }
   }
 #pragma unroll
   for (int i = 0; i < NT8; ++i) {
+    if constexpr (CUT)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = sum[i][j];
     red[warp][g][8 * i + 2 * t] = acc[i][0];
     red[warp][g][8 * i + 2 * t + 1] = acc[i][1];
     red[warp][g + 8][8 * i + 2 * t] = acc[i][2];
@@ -165,8 +184,14 @@ static cudaError_t launch_ls(const LinearSmallArgs& a, bool vec, cudaStream_t st
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return vec ? cudaLaunchKernelEx(&cfg, linear_small_kernel<NT8, GATED, true>, a)
-             : cudaLaunchKernelEx(&cfg, linear_small_kernel<NT8, GATED, false>, a);
+  // additions of a warp's chain: 4 per chunk, whole rounds
+  const int u = ls_unroll(NT8, vec), round = kLsWarps * cl * u;
+  const bool cut = 4 * u * ((chunks + round - 1) / round) > 64;
+  if (vec)
+    return cut ? cudaLaunchKernelEx(&cfg, linear_small_kernel<NT8, GATED, true, true>, a)
+               : cudaLaunchKernelEx(&cfg, linear_small_kernel<NT8, GATED, true, false>, a);
+  return cut ? cudaLaunchKernelEx(&cfg, linear_small_kernel<NT8, GATED, false, true>, a)
+             : cudaLaunchKernelEx(&cfg, linear_small_kernel<NT8, GATED, false, false>, a);
 }
 
 cudaError_t launch_linear_small(const void* x, int64_t ldx, const void* w, int64_t ldw, int m, int k, int n,

@@ -153,3 +153,10 @@ def test_bf16_weight_gradient_of_many_tokens(pkg, room):
     g = pkg.linear_backward(dy, pkg.LinearCheckpoint(x8, xs, None, None, "none"), randn(n, k), need_x=False)
     xr = pkg.restore_activations(x8, xs)
     assert abs(drift(g.weight, product64(dy.t(), xr.t()))) <= LONG
+
+
+def test_fp32_product_of_few_tokens_and_a_long_contraction(pkg, room):
+    """A warp's chain is joined after 16 additions of terms of one sign or fewer, each of which loses up to 9e-8 of the running
+    sum (see LONG); half of that on average, and the fp32 joins round to nearest."""
+    x, w = positive(8, 262144, 1), positive(7168, 262144, 2)
+    assert abs(drift(pkg.linear(x, w, out_dtype=F32), product64(x, w))) <= 0.18 * 64 * 2.0 ** -23 + 2.0 ** -23
