@@ -761,3 +761,69 @@ def test_backward_non_finite(pkg, act, gin, gout, m, k, n):
     (zq[0] if act == "swiglu" else zq)[row, 5] = 0x7f
     c = ck._replace(z=zq.view(torch.float8_e4m3fn))
     compare(pkg.linear_backward(dy, c, w, need_bias=True, grad_dtype=gout), row, [5] if act != "swiglu" else [o + 5])
+
+
+# --------------------------------------------------------------------------------- aligned slices of wider buffers
+@pytest.mark.parametrize("m, k, n", [(9, 128, 72), (60, 192, 104), (300, 520, 264), (1500, 192, 1096), (9000, 64, 328), (64, 7168, 520)])
+@pytest.mark.parametrize("act", ["none", "silu", "swiglu"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_linear_aligned_slices(pkg, m, k, n, act, dtype):
+    """x, weight, residual and output as slices of wider buffers whose rows bulk copies reach (strides of multiples of 16 bytes
+    beyond the width), the last box cut off beside live neighbours: the same bits as from tensors of their own, and nothing
+    else is written."""
+    o = n // 2 if act == "swiglu" else n
+    xb, wb = randn(m + 2, k + 72, seed=1), randn(n + 3, k + 40, seed=2, scale=k ** -0.5)
+    x, w, b = xb[1:m + 1, 8:8 + k], wb[2:2 + n, 32:32 + k], randn(n, seed=3)
+    rb, ob = randn(m, o + 56, seed=4), randn(m + 2, o + 80, seed=6, dtype=dtype)
+    for r in (None, rb[:, 24:24 + o]):
+        want = pkg.linear(x.contiguous(), w.contiguous(), bias=b, residual=None if r is None else r.contiguous(), activation=act, out_dtype=dtype)
+        z, tz = dense64(x, w, b)
+        ref, tol = act64(z, act), tol_act(z, tz, act)
+        if r is not None:
+            ref = ref + r.double()
+            tol = tol + ref.abs() * 2.0 ** -23
+        check(want, ref, rounded(ref, tol, dtype), "own tensors")
+        for c0 in (16, 4 if dtype == F32 else 8):
+            out = ob.clone()
+            y = out[1:m + 1, c0:c0 + o]
+            got = pkg.linear(x, w, bias=b, residual=r, activation=act, out_dtype=dtype, output=y)
+            assert got is y
+            if o % 8 == 0:                                     # else the contiguous rows go another way
+                assert torch.equal(y, want)
+            check(y, ref, rounded(ref, tol, dtype), "slices")
+            out[1:m + 1, c0:c0 + o] = ob[1:m + 1, c0:c0 + o]
+            assert torch.equal(out, ob)
+    if dtype == BF:                                            # in place, in the residual's wider rows
+        out = rb.clone()
+        r = out[:, 24:24 + o]
+        want = pkg.linear(x, w, bias=b, residual=r.clone(), activation=act)
+        pkg.linear(x, w, bias=b, residual=r, activation=act, output=r)
+        if o % 8 == 0:
+            assert torch.equal(r, want)
+        out[:, 24:24 + o] = rb[:, 24:24 + o]
+        assert torch.equal(out, rb)
+
+
+@pytest.mark.parametrize("m, k, n", [(40, 128, 96), (300, 520, 288), (1500, 192, 1120), (300, 136, 264)])
+@pytest.mark.parametrize("act", ["none", "gelu", "swiglu"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_training_step_on_aligned_slices(pkg, m, k, n, act, dtype):
+    """The same for a checkpointed product and its gradients."""
+    o = n // 2 if act == "swiglu" else n
+    x = randn(m + 2, k + 72, seed=1)[1:m + 1, 8:8 + k]
+    w = randn(n + 3, k + 40, seed=2, scale=k ** -0.5)[2:2 + n, 32:32 + k]
+    ob = randn(m, o + 80, seed=6, dtype=dtype)
+    out = ob.clone()
+    y, ck = pkg.linear_checkpointed(x, w, activation=act, out_dtype=dtype, output=out[:, 16:16 + o])
+    yc, cc = pkg.linear_checkpointed(x.contiguous(), w.contiguous(), activation=act, out_dtype=dtype)
+    if o % 8 == 0:
+        assert torch.equal(y, yc)
+    for a, c in zip(ck[:4], cc[:4]):
+        assert (a is None and c is None) or torch.equal(bits(a), bits(c))
+    out[:, 16:16 + o] = ob[:, 16:16 + o]
+    assert torch.equal(out, ob)
+    dy = randn(m + 1, o + 64, seed=7, dtype=dtype)[1:, 16:16 + o]
+    for need in (dict(), dict(need_weight=False), dict(need_x=False, need_bias=True)):
+        g = pkg.linear_backward(dy, ck, w, grad_dtype=dtype, **need)
+        gc = pkg.linear_backward(dy.contiguous(), cc, w.contiguous(), grad_dtype=dtype, **need)
+        assert all((a is None and c is None) or torch.equal(a, c) for a, c in zip(g, gc))
