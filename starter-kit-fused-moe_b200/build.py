@@ -2,7 +2,7 @@
 
     python starter-kit-fused-moe_b200/build.py [-v] [--debug]
 
-Every .cu file under csrc/ is compiled for sm_100a only
+Every .cu file of csrc/ and csrc/layer/ is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a) and linked into one shared library
 next to this file, so it travels with the source tree.
 """
@@ -18,6 +18,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = pathlib.Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
+LAYER = CSRC / "layer"          # the operators around the routed experts; they use csrc/, not the other way round
 INCLUDE = HERE.parent / "include"
 LIB = HERE / "libmoe_b200.so"
 OBJ = HERE / "_build"
@@ -36,7 +37,7 @@ def nvcc() -> str:
 
 
 def _deps():
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.cuh")) + \
+    return [p for d in (CSRC, LAYER) for p in sorted(d.iterdir()) if p.suffix in (".cu", ".h", ".cuh")] + \
         sorted(INCLUDE.glob("*.h"))
 
 
@@ -51,12 +52,12 @@ def build(debug: bool = False, verbose: bool = False, force: bool = False) -> pa
         return lib_path
     obj_dir.mkdir(exist_ok=True)
     flags = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
-             "-O3", "--expt-relaxed-constexpr", "-I", str(INCLUDE)]
+             "-O3", "--expt-relaxed-constexpr", "-I", str(INCLUDE), "-I", str(CSRC)]
     if debug:
         flags += ["-DMOE_DEBUG"]
     if verbose:
         flags += ["-Xptxas", "-v"]
-    srcs = sorted(CSRC.glob("*.cu"))
+    srcs = sorted(CSRC.glob("*.cu")) + sorted(LAYER.glob("*.cu"))
 
     def compile_one(s):
         o = obj_dir / (s.stem + ".o")

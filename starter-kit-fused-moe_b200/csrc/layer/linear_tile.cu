@@ -51,6 +51,7 @@
 // block then gives its copies in flight a millisecond before it leaves.
 #include "cta_pair.cuh"
 #include "linear_tile.h"
+#include "moe_kernels.h"
 #include "train_common.cuh"
 
 namespace moe {
@@ -1167,8 +1168,6 @@ cudaError_t launch_linear_join(bool gated, bool keep, const LinearTileArgs& a, c
   return keep ? launch_join<false, true>(a, st) : launch_join<false, false>(a, st);
 }
 
-cudaError_t set_debug_waits_linear(unsigned long long limit_ns, int gate_extra) {
-  return set_debug_waits_here(limit_ns, gate_extra);
-}
+static const bool g_debug_waits_added = (add_debug_waits(set_debug_waits_here), true);
 
 }  // namespace moe

@@ -94,6 +94,11 @@ int check_workspace(void* ws, size_t bytes, int T, int E) {
 
 void moe::set_last_error(const char* msg) { g_last_error = msg; }
 
+// Zero before any static initialiser runs, so the order of the sources does not matter.
+static cudaError_t (*g_debug_hook[4])(unsigned long long, int);
+static int g_debug_hooks;
+void moe::add_debug_waits(cudaError_t (*hook)(unsigned long long, int)) { g_debug_hook[g_debug_hooks++] = hook; }
+
 int moe::current_device_sms() { return num_sms_of_current_device(); }
 
 bool moe::encode_bf16(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride,
@@ -498,7 +503,7 @@ int moe_fp8_debug_set_waits(uint64_t wait_limit_ns, int32_t gate_extra) {
   cudaError_t e = moe::set_debug_waits_stream(wait_limit_ns, gate_extra);
   if (e == cudaSuccess) e = moe::set_debug_waits_tile(wait_limit_ns, gate_extra);
   if (e == cudaSuccess) e = moe::set_debug_waits_ep(wait_limit_ns, gate_extra);
-  if (e == cudaSuccess) e = moe::set_debug_waits_linear(wait_limit_ns, gate_extra);
+  for (int i = 0; i < g_debug_hooks && e == cudaSuccess; ++i) e = g_debug_hook[i](wait_limit_ns, gate_extra);
   return e == cudaSuccess ? MOE_OK : cuda_fail(e, "debug_set_waits");
 }
 

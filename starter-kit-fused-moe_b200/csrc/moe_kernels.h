@@ -79,7 +79,9 @@ cudaError_t launch_quantize(const void* x, bool bf16, int T, uint8_t* q, float* 
 cudaError_t set_debug_waits_stream(unsigned long long limit_ns, int gate_extra);
 cudaError_t set_debug_waits_tile(unsigned long long limit_ns, int gate_extra);
 cudaError_t set_debug_waits_ep(unsigned long long limit_ns, int gate_extra);
-cudaError_t set_debug_waits_linear(unsigned long long limit_ns, int gate_extra);
+// Adds a hook that moe_fp8_debug_set_waits calls too; for sources that csrc/ does not link against (csrc/layer/), during
+// their static initialisation.
+void add_debug_waits(cudaError_t (*hook)(unsigned long long limit_ns, int gate_extra));
 // SMs of the current device (0 without one).
 int current_device_sms();
 // Tensor map of a bf16 matrix [planes][rows][cols] (rank 2 when planes is 0;

@@ -4,8 +4,10 @@ The reference submits its kernels to the FlashInfer-Bench harness as a
 Solution document (``scripts/pack_solution.py:34-84``, format in
 ``README.md:227-279``): name, definition, author, a build spec and the source
 files. This writes the same document for this package: every CUDA source and
-header of the library, the C-ABI header, and the TVM-FFI binding as
-``main.cpp`` whose ``run`` has the reference's destination-passing signature.
+header of the routed operator (csrc/ without csrc/layer/, which ``run`` cannot
+reach and which takes most of the library's compile time), the C-ABI header,
+and the TVM-FFI binding as ``main.cpp`` whose ``run`` has the reference's
+destination-passing signature.
 All includes are by file name, so the flat source list compiles as one
 directory. The tcgen05 kernels need the harness to compile for sm_100a.
 

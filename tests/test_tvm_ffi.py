@@ -110,3 +110,22 @@ def test_packed_sources_compile_as_one_flat_directory(tmp_path):
     for name, proc in jobs:
         out, _ = proc.communicate(timeout=600)
         assert proc.returncode == 0, f"{name} does not compile in the flat layout:\n{out[-2000:]}"
+
+
+def test_packed_sources_are_the_routed_operator_alone(tmp_path):
+    """The operators around the routed experts are not packed, and what is packed links without them."""
+    import shutil
+    import subprocess
+    b = _module("_moe_build_pack", PKG / "build.py")
+    p = _module("_moe_pack3", PKG / "pack_solution.py")
+    files = [f for _, f in p.source_files()]
+    assert not [f for f in files if f.parent.name == "layer"]
+    layer = {f.name for f in (PKG / "csrc" / "layer").iterdir()}
+    assert layer and not layer & {n for n, _ in p.source_files()}
+    objs = [b.OBJ / (f.stem + ".o") for f in files if f.suffix == ".cu"]
+    if not b.up_to_date() or not all(o.exists() for o in objs):
+        b.build(force=True)
+    cuda = pathlib.Path(b.nvcc()).parent.parent
+    r = subprocess.run([shutil.which("g++") or "g++", "-shared", "-o", str(tmp_path / "run.so"), *map(str, objs), "-Wl,--no-undefined",
+                        "-L", str(cuda / "lib64"), "-lcudart"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
