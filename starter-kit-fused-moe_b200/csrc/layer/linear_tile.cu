@@ -1145,8 +1145,8 @@ static cudaError_t launch_t(const LinearTileMaps& maps, const LinearTileArgs& a,
   return launch_c<A_MN, B_MN, GATED, KEEP, false>(maps, a, num_sms, st);
 }
 
-static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
-                                  const LinearTileArgs& a, int num_sms, cudaStream_t st) {
+cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
+                               const LinearTileArgs& a, int num_sms, cudaStream_t st) {
   if (a.flip) return gated ? launch_c<false, false, true, false, false, true>(maps, a, num_sms, st)
                            : launch_c<false, false, false, false, false, true>(maps, a, num_sms, st);
   if (a_mn && b_mn) return launch_t<true, true, false, false>(maps, a, num_sms, st);
@@ -1155,11 +1155,6 @@ static cudaError_t launch_product(bool a_mn, bool b_mn, bool gated, bool keep, c
                          : launch_t<false, false, true, false>(maps, a, num_sms, st);
   return keep ? launch_t<false, false, false, true>(maps, a, num_sms, st)
               : launch_t<false, false, false, false>(maps, a, num_sms, st);
-}
-
-cudaError_t launch_linear_tile(bool a_mn, bool b_mn, bool gated, bool keep, const LinearTileMaps& maps,
-                               const LinearTileArgs& a, int num_sms, cudaStream_t st) {
-  return launch_product(a_mn, b_mn, gated, keep, maps, a, num_sms, st);
 }
 
 cudaError_t launch_linear_join(bool gated, bool keep, const LinearTileArgs& a, cudaStream_t st) {

@@ -23,8 +23,6 @@ from typing import NamedTuple, Optional
 
 import torch
 
-ACTIVATIONS = ("none", "relu", "gelu", "silu", "swiglu")     # in the order of MOE_ACT_*
-SCORINGS = ("sigmoid", "softmax")
 BINDING_PATH = pathlib.Path(__file__).resolve().parent / "moe_b200_layer.so"
 
 _vp, _i32, _i64, _sz, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
