@@ -17,19 +17,21 @@
 // coordinates repeating.
 //
 // Sums. The tensor core adds to its fp32 accumulator by truncation, so a long
-// chain drifts: 8e-6 of the result's norm at K = 7168, 2e-6 at 2048, 5e-7 at
-// 512 for values of both signs, 3.7e-7 per 64 of K for values of one sign, which is
-// 1.5e-3 of a bf16 result at K = 262144. So the chain is cut (CHAIN) every 256 K-blocks
-// of 64, which costs nothing that can be seen (1e-4 of a bf16 result at most); an
-// fp32 result and a kept pre-activation (one value in 10^4 moves to
-// the next e4m3 step) show less, and there it is cut every 16
-// (fp32), 6 (fp32 gated, where both factors drift the same way: 1.7e-6 at K = 768
-// with 16, 9e-7 with 8) or 8 (kept, whatever y's type): the epilogue warps add each partial
+// chain drifts: 8e-6 of the result's norm at K = 7168, 2e-6 at 2048, 5e-7 at 512 for
+// values of both signs (an fp32 product with rounding: 1.0e-6, 4.5e-7, 1.9e-7), and
+// 3.7e-7 per 64 of K for values of one sign, which is 1.5e-3 of a bf16 result at
+// K = 262144. So the chain is cut (CHAIN): the epilogue warps add each partial
 // accumulator to fp32 registers, rounding to nearest, while the tensor core fills
-// the other one. The reads of TMEM cost the tensor core about a K-block each: 218
-// us for the checkpointed product of 4096 x 7168 x 4096 instead of 214 with 12 and
-// 210 with 24, for 2.3e-4 of the norm in values that fall on the next e4m3 step
-// instead of 2.7e-4 and 3.4e-4 (an fp32 product has 2.0e-4).
+// the other one. The reads of TMEM cost the tensor core about a K-block each.
+//  - bf16 results: every 256 K-blocks of 64, which costs nothing that can be seen and
+//    leaves 1e-4 of a result at most.
+//  - fp32 results: every 16, gated ones every 6, as both factors drift the same way (1.7e-6
+//    at K = 768 with 16, 9e-7 with 8). Up to K = 1024 (384) that is no cut at all: 5e-7.
+//  - kept pre-activations, of which an error moves some to the next e4m3 step: every
+//    c K-blocks, c the root of their number (8 at most), because the drift grows with c and
+//    the error of an fp32 product with the root of K. At 8192 x 512 x 2048 (silu) 1.3e-4 of the norm in
+//    such steps and 52 us, uncut 2.0e-4 and 43 us (fp32 1.2e-4); at K = 1024 1.7e-4 and 62 us,
+//    with 8 2.3e-4 and 55 us (1.6e-4); at K = 7168 2.5e-4 (2.5e-4).
 //
 // Warps: 0 TMA producer, 1 MMA issuer (the leader CTA's), 4-11 epilogue. The two
 // accumulators of NT columns in TMEM also let a tile's epilogue overlap the next
@@ -1085,7 +1087,7 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
     for (int s = 1; s <= 16; ++s) {
       const int64_t depth = (k_blocks + s - 1) / s;
       if (s > 1 && k_blocks < 4 * s) break;
-      if (depth > linear_chain(gated, ep.y_f32, false)) continue;                // longer chains drift
+      if (depth > linear_chain(gated, ep.y_f32, false, k_blocks)) continue;                // longer chains drift
       const int64_t units = tail * s, rounds = (units + pairs - 1) / pairs;
       // 52 pairs reach what HBM gives (32 of them 5 of 6.5 TB/s), fewer a part of it, those of the last round too; a
       // slice more is also a load more, one after the other, in the join

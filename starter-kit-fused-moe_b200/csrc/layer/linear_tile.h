@@ -30,9 +30,14 @@ struct LinearTileMaps {
   CUtensorMap a, b;       // operands
   CUtensorMap out, res;   // bf16 y and its residual in 32 x 32 boxes (vec)
 };
-// K-blocks per accumulator where long sums are cut: see the kernel's comment on sums.
-// Kept pre-activations have one length, so that their bytes do not depend on y's type.
-constexpr int linear_chain(bool gated, bool f32, bool keep) { return keep ? 8 : !f32 ? 256 : gated ? 6 : 16; }
+// K-blocks per accumulator where long sums are cut: see the kernel's comment on sums. Kept pre-activations have a length that
+// y's type does not change, so that their bytes do not depend on it: the root of the K-blocks, 8 at most.
+constexpr int linear_chain(bool gated, bool f32, bool keep, int64_t k_blocks) {
+  if (!keep) return !f32 ? 256 : gated ? 6 : 16;
+  int c = 1;
+  while (c < 8 && (c + 1) * c < k_blocks) ++c;
+  return c;
+}
 struct LinearTilePlan {
   int n_tile, splits, flip;
   int64_t full, tail;     // whole tiles, tiles left to the join

@@ -91,7 +91,7 @@ int run_product(const Product& p, bool a_mn, bool b_mn, bool gated, bool keep, i
   t.terms = p.terms;
   t.k_blocks = t.term_blocks * p.terms;
   t.splits = p.plan.splits;
-  t.chain = moe::linear_chain(gated, ep.y_f32, keep);
+  t.chain = moe::linear_chain(gated, ep.y_f32, keep, t.k_blocks);
   t.full_tiles = p.plan.full;
   t.units = p.plan.full + p.plan.tail * t.splits;
   t.ep = ep;

@@ -92,6 +92,23 @@ def test_kept_values(pkg, m, k, n, act, dtype):
     assert off(got, want) <= 1.1 * math.sqrt(0.07 * 1.1 * 0.24 * 32 * 2.0 ** -23)
 
 
+@pytest.mark.parametrize("k", [64, 128, 256, 400, 512, 832, 1024, 1536, 2048, 3283, 4096])
+@pytest.mark.parametrize("act", ["silu", "swiglu"])
+def test_kept_values_like_those_of_an_fp32_product(pkg, k, act):
+    """Chains of sqrt(K / 64) K-blocks drift like the roundings of an fp32 product, so about as many values fall on another
+    step: some 30 of the 2^24 here, which makes the ratio of the two norms good to 18 % (30^-1/2)."""
+    m, n = 8192, 2048
+    x, w = randn(m, k, seed=1), randn(n, k, seed=2, scale=k ** -0.5)
+    z, z32 = x.double() @ w.double().t(), x.float() @ w.float().t()
+    if act == "swiglu":
+        cut = lambda v: torch.stack([kept64(h.double()) for h in v.chunk(2, 1)])  # noqa: E731
+    else:
+        cut = lambda v: kept64(v.double())  # noqa: E731
+    _, ck = pkg.linear_checkpointed(x, w, activation=act)
+    got = pkg.restore_activations(ck.z, ck.z_scale, F32).double()
+    assert off(got, cut(z)) <= 1.5 * off(cut(z32), cut(z))
+
+
 @pytest.mark.parametrize("m, k, n", [(300, 768, 512), (700, 2048, 512), (2048, 7168, 1024), (513, 1100, 1040)])
 @pytest.mark.parametrize("act", ["gelu", "swiglu"])
 def test_kept_bytes_do_not_depend_on_the_output_type(pkg, m, k, n, act):
