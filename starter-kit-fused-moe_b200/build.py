@@ -124,16 +124,28 @@ LAYER_SRC = HERE / "binding" / "layer_binding.cc"
 LAYER_LIB = HERE / "moe_b200_layer.so"
 
 
-def build_layer_binding(force: bool = False) -> pathlib.Path:
-    """Build the Python binding of the layer operators (layer.py) over libmoe_b200.so."""
+def torch_root() -> pathlib.Path | None:
+    """Directory of an installed torch with its C++ headers, or None."""
+    import torch
+    root = pathlib.Path(torch.__file__).parent
+    return root if (root / "include" / "torch" / "csrc" / "utils" / "pybind.h").exists() else None
+
+
+def build_layer_binding(force: bool = False) -> pathlib.Path | None:
+    """Build the Python binding of the layer operators (layer.py) over libmoe_b200.so.
+    Returns None, and says so, where torch comes without its C++ headers: the routed
+    operator needs no binding, and the layer operators raise without theirs."""
     build()
+    root = torch_root()
+    if root is None:
+        sys.stderr.write("torch has no C++ headers here: the binding of the layer operators is not built\n")
+        return None
     if not force and LAYER_LIB.exists() and \
             LAYER_LIB.stat().st_mtime >= max(LAYER_SRC.stat().st_mtime, (INCLUDE / "moe_fp8.h").stat().st_mtime):
         return LAYER_LIB
     import sysconfig
 
     import torch
-    root = pathlib.Path(torch.__file__).parent
     cuda = pathlib.Path(nvcc()).parent.parent
     tmp = LAYER_LIB.with_name(LAYER_LIB.name + ".tmp")
     cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", str(LAYER_SRC), "-o", str(tmp),

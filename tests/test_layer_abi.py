@@ -172,3 +172,19 @@ def test_python_refusals_without_a_gpu(pkg):
         pkg.balance_loss(torch.zeros(2, 8), torch.zeros(2, 2, dtype=torch.int32))
     with pytest.raises(ValueError, match="float32"):
         pkg.balance_loss(x, torch.zeros(2, 2, dtype=torch.int32))
+
+
+def test_build_without_torch_headers(monkeypatch, tmp_path, capsys):
+    """Where torch has no C++ headers the binding is left out and the build goes on."""
+    import importlib.util
+    import pathlib
+    path = pathlib.Path(__file__).resolve().parents[1] / "starter-kit-fused-moe_b200" / "build.py"
+    spec = importlib.util.spec_from_file_location("_moe_build_layer", path)
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    assert b.torch_root() is not None
+    monkeypatch.setattr(torch, "__file__", str(tmp_path / "torch" / "__init__.py"))
+    assert b.torch_root() is None
+    monkeypatch.setattr(b, "build", lambda *a, **k: None)
+    assert b.build_layer_binding(force=True) is None
+    assert "headers" in capsys.readouterr().err
