@@ -284,3 +284,24 @@ def test_boundaries_of_no_tokens(pkg):
             assert float(b.loss) == 0 and int(b.sequences) == 0 and not b.tokens.any() and not b.mean_scores.any()
         else:
             assert torch.isnan(b.loss) and int(b.sequences) == -1 and (b.tokens == -1).all() and torch.isnan(b.mean_scores).all()
+
+
+@pytest.mark.parametrize("k", [1, 2, 8])
+@pytest.mark.parametrize("masked", [False, True])
+def test_what_the_weights_have_in_common_has_no_gradient(pkg, k, masked):
+    """A token's combine weights add up to the scale whatever its logits are, so the part of their gradients that is the same for all
+    picks of a token cancels: for one pick that is everything, and it is not a remainder of rounding that is left."""
+    t, e = 3000, 64
+    x, idx, _ = inputs(t, e, k, seed=7)
+    if masked and k > 1:
+        idx[:, 0] = -1
+    common = torch.randn(t, 1, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").expand(t, k).contiguous()
+    g = pkg.balance_loss_backward(x, idx, None, grad_topk_weights=common)
+    # what is left is dw scale 1e-20 / S^2 s (1 - s); S is above 1e-4 here
+    assert (g.abs() <= 2.5 * common.abs().amax(1, keepdim=True) * 1e-20 * 1e8).all()
+    own = common + 0.01 * torch.randn(t, k, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    g = pkg.balance_loss_backward(x, idx, None, grad_topk_weights=own)
+    ok = (idx >= 0)
+    spread = torch.where(ok, own - own[:, -1:], 0.0).double().abs().sum(1, keepdim=True)
+    want = ref64(x, idx, None, 0.1, "sigmoid", None, own, 2.5)[4]
+    assert ((g.double() - want).abs() <= 2.0 ** -16 * 2.5 * spread + 1e-12).all()
