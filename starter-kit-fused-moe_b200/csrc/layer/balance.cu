@@ -364,7 +364,9 @@ __global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_gr
       load_logits<ITEMS, VEC>(a.logits + (int64_t)(pos + warp) * a.e, a.e, lane, next);
       if (lane < a.k) id_next = __ldg(a.idx + (int64_t)(pos + warp) * a.k + lane);
     }
-    float coef[ITEMS];
+    // c_e less the first expert's: p adds up to 1 (sigmoid: 1 - 1e-20 / (sum + 1e-20)), so c_e - sum_j c_j p_j does not
+    // see what all experts have in common but for that share, and balanced counts leave no remainder of rounding
+    float coef[ITEMS], common = 0.f;
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) coef[j] = live < 0 ? NAN : 0.f;        // wrong boundaries: no gradient either
     if (with_loss && live >= 0) {
@@ -377,9 +379,12 @@ __global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_gr
         end = min(qb, b1);
         const int tq = __ldg(a.tokens + q);
         const double f = tq > 0 && live > 0 ? (double)g * a.alpha * a.e / ((double)a.k * live * tq * tq) : 0.0;
+        const int32_t* count = a.counts + (int64_t)q * a.e;
+        const int first = __ldg(count);
+        common = a.scoring == 0 ? (float)(f * first) * kScoreEps : 0.f;
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j)
-          if (VEC || lane + 32 * j < a.e) coef[j] = (float)(f * __ldg(a.counts + (int64_t)q * a.e + expert_of<VEC>(lane, j)));
+          if (VEC || lane + 32 * j < a.e) coef[j] = (float)(f * (__ldg(count + expert_of<VEC>(lane, j)) - first));
       }                                                      // else: behind the last sequence
     }
     for (int t = pos + warp; t < end; t += kBalWarps) {
@@ -416,7 +421,7 @@ __global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_gr
         float inner = 0.f;
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) inner += coef[j] * s[j];
-        inner = warp_sum(inner) * inv;
+        inner = (warp_sum(inner) - common) * inv;
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) dx[j] = (coef[j] - inner) * inv * slope[j];
       }

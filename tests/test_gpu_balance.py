@@ -305,3 +305,27 @@ def test_what_the_weights_have_in_common_has_no_gradient(pkg, k, masked):
     spread = torch.where(ok, own - own[:, -1:], 0.0).double().abs().sum(1, keepdim=True)
     want = ref64(x, idx, None, 0.1, "sigmoid", None, own, 2.5)[4]
     assert ((g.double() - want).abs() <= 2.0 ** -16 * 2.5 * spread + 1e-12).all()
+
+
+@pytest.mark.parametrize("e, k", [(1, 1), (8, 2), (64, 4), (256, 8)])
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_balanced_counts_have_no_gradient(pkg, e, k, scoring):
+    """Where every expert is picked equally often the loss does not depend on the logits; one pick more leaves that pick's part,
+    not a remainder of rounding of the rest."""
+    t = 8 * e // k * 32
+    x, _, _ = inputs(t, e, 1, seed=3)
+    idx = (torch.arange(t * k, device="cuda") % e).view(t, k).to(torch.int32)
+    b = pkg.balance_loss(x, idx, alpha=1.0, scoring=scoring)
+    assert (b.counts == t * k // e).all()
+    g = pkg.balance_loss_backward(x, idx, b, alpha=1.0, scoring=scoring)
+    # what is left of c (1 - sum p): c 1e-20 / S, twice over S, with S above 1e-4 and c = e / (k t^2) t k / e = 1 / t
+    assert (g.abs() <= 1e-20 * 1e8 / t).all()
+    if e > 1:
+        idx[5, 0] = idx[5, k - 1] if k > 1 else (idx[5, 0] + 1) % e
+        b = pkg.balance_loss(x, idx, alpha=1.0, scoring=scoring)
+        g = pkg.balance_loss_backward(x, idx, b, alpha=1.0, scoring=scoring)
+        want = ref64(x, idx, None, 1.0, scoring, 1.0)[4]
+        # two coefficients are off the common one by e / (k t^2); the factors are good to 2^-20
+        s = torch.sigmoid(x.double())
+        factor = (s * (1 - s)).amax(1, keepdim=True) / (s.sum(1, keepdim=True) + 1e-20) if scoring == "sigmoid" else 1.0
+        assert ((g.double() - want).abs() <= 2.0 ** -16 * e / (k * t * t) * factor + 1e-12 / t).all()
