@@ -25,8 +25,10 @@
 // the other one. The reads of TMEM cost the tensor core about a K-block each.
 //  - bf16 results: every 256 K-blocks of 64, which costs nothing that can be seen and
 //    leaves 1e-4 of a result at most.
-//  - fp32 results: every 16, gated ones every 6, as both factors drift the same way (1.7e-6
-//    at K = 768 with 16, 9e-7 with 8). Up to K = 1024 (384) that is no cut at all: 5e-7.
+//  - fp32 results: every 12, gated ones every 6, as both factors drift the same way, which
+//    keeps them within 1e-6 of the norm: 7e-7 both (16: 1.0e-6, where an fp32 product has 2.5e-7 at
+//    K = 1024 and 9e-7 at 7168; 2 % less time at 4096 x 7168 x 4096). Up to K = 768 (384) that is no
+//    cut at all.
 //  - kept pre-activations, of which an error moves some to the next e4m3 step: every
 //    c K-blocks, c the root of their number (8 at most), because the drift grows with c and
 //    the error of an fp32 product with the root of K. At 8192 x 512 x 2048 (silu) 1.3e-4 of the norm in

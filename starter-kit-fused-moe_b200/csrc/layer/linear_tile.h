@@ -33,7 +33,7 @@ struct LinearTileMaps {
 // K-blocks per accumulator where long sums are cut: see the kernel's comment on sums. Kept pre-activations have a length that
 // y's type does not change, so that their bytes do not depend on it: the root of the K-blocks, 8 at most.
 constexpr int linear_chain(bool gated, bool f32, bool keep, int64_t k_blocks) {
-  if (!keep) return !f32 ? 256 : gated ? 6 : 16;
+  if (!keep) return !f32 ? 256 : gated ? 6 : 12;
   int c = 1;
   while (c < 8 && (c + 1) * c < k_blocks) ++c;
   return c;
