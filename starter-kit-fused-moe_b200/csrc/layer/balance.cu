@@ -430,12 +430,12 @@ __global__ void __launch_bounds__(kBalWarps * 32, ITEMS <= 8 ? 4 : 1) balance_gr
         const float e = __expf(-fabsf(xs)), r = __fdividef(1.0f, 1.0f + e);
         const float top = hit ? (xs >= 0.f ? r : e * r) : 0.f;
         const float dw = hit ? __ldg(a.grad_weights + (int64_t)t * a.k + lane) : 0.f;
-        const float total = warp_sum(top) + kScoreEps;
+        const float share = 1.0f / (warp_sum(top) + kScoreEps);
         // dw_k - sum_j dw_j s_j / S from the first pick's dw on (the shares s_j / S add up to 1 - 1e-20 / S): what all picks
         // have in common cancels exactly, all of it with one pick, whose weight does not depend on its logit
         const float c = __shfl_sync(0xffffffffu, dw, __ffs(__ballot_sync(0xffffffffu, hit)) - 1);
         const float dot = warp_sum(hit ? (dw - c) * top : 0.f);
-        const float d = hit ? (dw - c - dot / total + c * (kScoreEps / total)) / total * (e * r * r) * a.route_scale : 0.f;
+        const float d = hit ? ((dw - c) + (c * kScoreEps - dot) * share) * share * (e * r * r) * a.route_scale : 0.f;
         // scattered through shared memory; repeated picks (rare) are added by their first lane in pick order
         const uint32_t same = __match_any_sync(0xffffffffu, hit ? id : -1 - lane);
         float sum = d;
