@@ -1079,9 +1079,10 @@ LinearTilePlan plan_linear_tile(int64_t m, int64_t n, int64_t k_blocks, bool gat
     }
   }
   // Few tokens and a long contraction: the weights' rows become the tile's, which pads 64 or 128 columns instead of 256
-  // rows. At 64 (128) tokens and K = 7168 16.1 (18.3) instead of 19.6 (22.8) us for N = 4096 gated, 25.1 (27.4) instead
-  // of 29.2 (29.5) for N = 7168, 9.6 (10.3) instead of 12.1 (11.9) for N = 256 in fp32; at K = 4096 equal, at
-  // K = 2048 14.1 instead of 11.5, because a flipped tile always needs the join.
+  // rows, but always needs the join. At 64 (128) tokens and K = 7168 16.2 (18.3) instead of 19.2 (22.8) us for N = 4096
+  // gated, 25.8 instead of 29.3 for N = 7168, 10.2 instead of 12.8 for N = 256; at K = 5120 14.0 (15.1) instead of 16.2 (19.0), at
+  // 4096 12.8 (13.9) instead of 16.1 (17.2), at 2048 11.8 (11.4) instead of 12.8 (12.0) but 12.9 instead of 11.8 for
+  // N = 7168 (weights that change, in a graph). The limit was set when the slices left HBM idle below it.
   if (m <= 128 && k_blocks >= 96 && !keep && !grad) {
     best_cost = 1e300;
     const int nt = m <= 64 ? 64 : 128;

@@ -184,7 +184,8 @@ def balance_loss(routing_logits, topk_idx, cu_seqlens=None, alpha=1e-4, scoring=
     A pick outside [0, E) selects nothing and a token without picks is padding:
     it counts nowhere. Boundaries that decrease or leave [0, T], one or several, give
     a NaN loss, -1 for `sequences` and all `tokens`, counts of 0, NaN mean scores and
-    NaN gradients.
+    NaN gradients. The outputs share one allocation: keep `loss.clone()` where losses
+    are kept over many steps.
     """
     return BalanceLoss(*_native().balance_loss(routing_logits, topk_idx, cu_seqlens, alpha, scoring))
 
