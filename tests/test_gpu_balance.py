@@ -329,3 +329,29 @@ def test_balanced_counts_have_no_gradient(pkg, e, k, scoring):
         s = torch.sigmoid(x.double())
         factor = (s * (1 - s)).amax(1, keepdim=True) / (s.sum(1, keepdim=True) + 1e-20) if scoring == "sigmoid" else 1.0
         assert ((g.double() - want).abs() <= 2.0 ** -16 * e / (k * t * t) * factor + 1e-12 / t).all()
+
+
+@pytest.mark.parametrize("t, cuts", [(65534, list(range(65535))), (100, [0] * 30000 + [50] * 30000 + [100])])
+def test_balance_most_sequences(pkg, t, cuts):
+    """A sequence per token, and tens of thousands of empty ones in one place."""
+    e, k, s = 8, 2, len(cuts) - 1
+    x, idx, _ = inputs(t, e, k, seed=5)
+    cu = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    b = pkg.balance_loss(x, idx, cu_seqlens=cu, alpha=0.1)
+    g = pkg.balance_loss_backward(x, idx, b, cu_seqlens=cu, alpha=0.1)
+    tokens = cu.diff().double()[:, None]
+    seq = torch.repeat_interleave(torch.arange(s, device="cuda"), cu.diff().long())
+    counts = torch.zeros(s, e, dtype=torch.float64, device="cuda").index_put_(
+        (seq[:, None].expand(t, k), idx.long()), torch.ones((), dtype=torch.float64, device="cuda"), accumulate=True)
+    sg = torch.sigmoid(x.double())
+    p = sg / (sg.sum(1, keepdim=True) + 1e-20)
+    freq = counts * e / (k * tokens.clamp(min=1))
+    live = int((tokens > 0).sum())
+    mean = torch.zeros_like(counts).index_add_(0, seq, p) / tokens.clamp(min=1)
+    loss = 0.1 * (freq * mean).sum() / live
+    assert torch.equal(b.counts.double(), counts) and torch.equal(b.tokens.double(), tokens[:, 0]) and int(b.sequences) == live
+    assert abs(float(b.loss.double() - loss)) <= 2.0 ** -18 * float(loss)
+    c = (0.1 * freq / (tokens.clamp(min=1) * live))[seq]
+    want = (c - (c * p).sum(1, keepdim=True)) / (sg.sum(1, keepdim=True) + 1e-20) * sg * (1 - sg)
+    top = c.amax(1, keepdim=True) * (sg * (1 - sg)).amax(1, keepdim=True) / sg.sum(1, keepdim=True)
+    assert ((g.double() - want).abs() <= 2.0 ** -16 * top).all()

@@ -827,3 +827,33 @@ def test_training_step_on_aligned_slices(pkg, m, k, n, act, dtype):
         g = pkg.linear_backward(dy, ck, w, grad_dtype=dtype, **need)
         gc = pkg.linear_backward(dy.contiguous(), cc, w.contiguous(), grad_dtype=dtype, **need)
         assert all((a is None and c is None) or torch.equal(a, c) for a, c in zip(g, gc))
+
+
+def test_graph_that_forks_and_joins(pkg):
+    """A capture whose calls run on two streams and wait for one another replays to the eager results."""
+    x, w1, w2 = randn(300, 512, seed=1), randn(512, 512, seed=2, scale=0.05), randn(512, 512, seed=3, scale=0.05)
+    dy, side = randn(300, 512, seed=4), torch.cuda.Stream()
+
+    def step():
+        a = pkg.linear(x, w1)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            b, ck = pkg.linear_checkpointed(a, w2, activation="silu")
+            g = pkg.linear_backward(dy, ck, w2, need_bias=True)
+        c = pkg.linear(a, w1)
+        torch.cuda.current_stream().wait_stream(side)
+        d = pkg.linear(b, w1, residual=c)
+        e, ck = pkg.linear_checkpointed(d, w1, activation="swiglu")
+        return (a, b, c, d, e, *g, *pkg.linear_backward(dy[:, :256], ck, w1, need_bias=True))
+
+    want = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(10):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

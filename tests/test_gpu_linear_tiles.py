@@ -1,4 +1,4 @@
-"""GPU: dense products whose tiles follow one another closely on every pair of SMs.
+"""GPU: dense products whose tiles follow one another closely on every pair of SMs, and whose waits run out.
 
 The inputs are small integers, so every product sum is a whole number below 2^24 and exact in fp32 in any order: y is
 the 64-bit form rounded once, bit for bit."""
@@ -59,3 +59,40 @@ def test_many_short_tiles(pkg, m, k, n, act, keep):
                 assert torch.equal(out[2], stack([bits(v[1]) for v in q]))
         else:
             assert all(torch.equal(a, c) for a, c in zip(out, first))
+
+
+@pytest.mark.parametrize("m, k, n, act, grad", [(300, 512, 512, "none", BF), (600, 2048, 1024, "silu", F32), (4096, 256, 2048, "none", BF)])
+def test_wait_that_runs_out_in_the_gradients(pkg, m, k, n, act, grad):
+    """Gradients whose accumulators never come (a host-set test hook) are NaN after the shortened limit, the bias gradient, which
+    needs none, is not, and the next call is right again. The two products overlap."""
+    x, w, dy = whole(m, k, seed=1), whole(n, k, seed=2), whole(m, n, seed=3)
+    ck = pkg.linear_checkpointed(x, w, activation=act)[1]
+    want = pkg.linear_backward(dy, ck, w, need_bias=True, grad_dtype=grad)
+    lib = pkg.load_library()
+    torch.cuda.synchronize()
+    assert lib.moe_fp8_debug_set_waits(20_000_000, 1) == 0
+    try:
+        bad = pkg.linear_backward(dy, ck, w, need_bias=True, grad_dtype=grad)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.moe_fp8_debug_set_waits(2_000_000_000, 0) == 0
+    assert torch.isnan(bad.x).all() and torch.isnan(bad.weight).all() and torch.equal(bad.bias, want.bias)
+    again = pkg.linear_backward(dy, ck, w, need_bias=True, grad_dtype=grad)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+@pytest.mark.parametrize("m, n, act, dtype", [(64, 512, "none", BF), (128, 4096, "swiglu", BF), (40, 256, "none", F32)])
+def test_wait_that_runs_out_with_few_tokens(pkg, m, n, act, dtype):
+    """The same where the weights' rows are the tile's."""
+    x, w = whole(m, 7168, seed=1, top=1), whole(n, 7168, seed=2, top=1)
+    want = pkg.linear(x, w, activation=act, out_dtype=dtype)
+    lib = pkg.load_library()
+    torch.cuda.synchronize()
+    assert lib.moe_fp8_debug_set_waits(20_000_000, 1) == 0
+    try:
+        bad = pkg.linear(x, w, activation=act, out_dtype=dtype)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.moe_fp8_debug_set_waits(2_000_000_000, 0) == 0
+    assert torch.isnan(bad).all()
+    assert torch.equal(pkg.linear(x, w, activation=act, out_dtype=dtype), want)
